@@ -464,3 +464,58 @@ typedef struct {
     uint8_t * codes;              // [rows][cols] codes too, or NULL
     int rows, cols, nbits;
 } sml_king_pack;
+
+// ------------------------------------------------------------ serve.hip
+// A paged cache as the kernels see it (page_shift: log2 of the page size).
+typedef struct {
+    uint16_t * k, * v;
+    const int32_t * table;
+    size_t page_stride;
+    int n_pages, page_shift, n_seq, seq_pages, n_kv, hd;
+} sml_kpages;
+
+typedef struct {
+    sml_kpages pg;
+    float * qkv;
+    size_t stride;
+    const int32_t * seq, * pos;   // seq NULL: sequence r
+    const float * cos_t, * sin_t;
+    float * q_out;                // NULL: in place
+    int n_rope, n_head;
+} sml_kappend;
+
+typedef struct {
+    sml_kpages pg;
+    const float * q;
+    size_t q_stride;
+    const int32_t * len;
+    float * part, * out;
+    float scale;                  // times log2(e)
+    int n_head, max_len;
+    int nsplit, chunk;            // positions [i * chunk, (i + 1) * chunk) of split i
+} sml_kattend;
+
+typedef struct {
+    const float * logits;
+    float * out;
+    size_t stride, out_stride;
+    const int32_t * hist, * hist_start, * n_prompt;
+    const float * rep, * presence, * frequency;
+    const int32_t * bias_id, * bias_start;
+    const float * bias;
+    const uint32_t * mask;
+    const int32_t * mask_row;
+    int4 * part;                  // per row and block: max, its index, first permitted index, whether that is NaN
+    int32_t * tok;
+    int n_hist, n_bias, n_mask, n_vocab, n_part;
+} sml_klogits;
+
+typedef struct {
+    const uint16_t * a, * b;
+    const float * scale;
+    const int32_t * ranks, * adapter;
+    const float * x, * base;
+    float * y, * work;            // work [row][split][rank]
+    size_t x_stride, y_stride;
+    int n_adapter, rank, n_in, n_out, n_row, nsplit, chunk;
+} sml_klora;

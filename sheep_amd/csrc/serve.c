@@ -1,0 +1,191 @@
+// The operators of a step that serves many requests at once (sml-serve.h):
+// argument checks and launches. The checks come before the device is touched,
+// so they refuse alike on a machine without one.
+#include "ops.h"
+#include "sml-serve.h"
+
+#include <math.h>
+#include <stdio.h>
+#include <string.h>
+
+static int al16(const void * p) { return ((uintptr_t) p & 15u) == 0; }
+static int ceil_div(int a, int b) { return (int) (((long) a + b - 1) / b); }
+
+// The device of sml_hip_init has to be the calling thread's: the stream and
+// the buffers of another one would meet kernels loaded for this one.
+static void on_device(void) {
+    if (!hx.inited) hx_init(0);
+    int d = -1;
+    HX(hipGetDevice(&d));
+    if (d != hx.device) hx_failf("device %d is current, the library runs on device %d", d, hx.device);
+}
+
+static void check_pages(const sml_hip_pages * p, sml_kpages * k) {
+    if (!p || !p->k || !p->v || !p->table) hx_failf("paged cache: missing pools or table");
+    if (p->type != SML_F16 && p->type != SML_BF16) hx_failf("paged cache: type %d", p->type);
+    if (p->hd != 64 && p->hd != 128) hx_failf("paged cache: head_dim %d (64 or 128)", p->hd);
+    if (p->n_kv < 1 || p->n_kv > 4096) hx_failf("paged cache: %d kv heads", p->n_kv);
+    if (p->page_size < 16 || p->page_size > 65536 || (p->page_size & (p->page_size - 1)))
+        hx_failf("paged cache: pages of %d positions (a power of two, 16..65536)", p->page_size);
+    const size_t page = (size_t) p->page_size * p->n_kv * p->hd;
+    if (page > (size_t) 1 << 30) hx_failf("paged cache: pages of %zu values", page);
+    if (p->page_stride && (p->page_stride < page || p->page_stride % 8))
+        hx_failf("paged cache: page stride %zu for pages of %zu values (a multiple of 8)", p->page_stride, page);
+    if (p->n_pages < 1 || p->n_seq < 1 || p->n_seq > 65535 || p->seq_pages < 1)
+        hx_failf("paged cache: %d pages, %d sequences of %d pages", p->n_pages, p->n_seq, p->seq_pages);
+    if ((uint64_t) p->seq_pages * (uint64_t) p->page_size > (uint64_t) 1 << 30)
+        hx_failf("paged cache: %d pages of %d positions a sequence", p->seq_pages, p->page_size);
+    if (!al16(p->k) || !al16(p->v)) hx_failf("paged cache: pools off 16-byte boundaries");
+    memset(k, 0, sizeof *k);
+    k->k = p->k; k->v = p->v; k->table = p->table;
+    k->page_stride = p->page_stride ? p->page_stride : page;
+    k->n_pages = p->n_pages; k->page_shift = __builtin_ctz((unsigned) p->page_size);
+    k->n_seq = p->n_seq; k->seq_pages = p->seq_pages; k->n_kv = p->n_kv; k->hd = p->hd;
+}
+
+static void sv_name(char * s, size_t n, const char * base, int hd, int type) {
+    snprintf(s, n, "%s%s%s", base, hd == 64 ? "_d64" : "", type == SML_BF16 ? "_bf" : "");
+}
+
+int sml_hip_paged_append(const sml_hip_pages * pg, float * qkv, size_t qkv_stride, int n_rows, const int32_t * seq,
+                         const int32_t * pos, const float * cos_t, const float * sin_t, int n_rope, int n_head,
+                         float * q_out, void * stream) {
+    HX_ENTRY(-1);
+    sml_kappend a;
+    memset(&a, 0, sizeof a);
+    check_pages(pg, &a.pg);
+    if (n_rows < 0 || n_rows > 1 << 24 || n_head < 1 || n_head > 65536) hx_failf("append: %d rows of %d heads", n_rows, n_head);
+    const size_t width = ((size_t) n_head + 2 * (size_t) pg->n_kv) * pg->hd;
+    if (!qkv || !pos || !cos_t || !sin_t || n_rope < 1) hx_failf("append: missing rows, positions or rotation tables");
+    if (qkv_stride && qkv_stride < width) hx_failf("append: rows of %zu floats %zu apart", width, qkv_stride);
+    on_device();
+    if (n_rows) {
+        a.qkv = qkv; a.stride = qkv_stride ? qkv_stride : width; a.seq = seq; a.pos = pos;
+        a.cos_t = cos_t; a.sin_t = sin_t; a.q_out = q_out; a.n_rope = n_rope; a.n_head = n_head;
+        char name[40];
+        sv_name(name, sizeof name, "sml_sv_append", pg->hd, pg->type);
+        const int items = (n_head + pg->n_kv) * (pg->hd / 8) + pg->n_kv * (pg->hd / 4);
+        hx_launch(name, (unsigned) n_rows, (unsigned) ceil_div(items, 256), 256, 0, (hipStream_t) stream, &a);
+    }
+    HX_LEAVE();
+    return 0;
+}
+
+size_t sml_hip_paged_part_floats(int n_seq, int n_head, int hd, int max_len) {
+    if (n_seq < 1 || n_head < 1 || hd < 1 || max_len < 1) return 0;
+    const int ns = ceil_div(max_len, 64);
+    return (size_t) n_seq * (size_t) n_head * (size_t) (ns < 256 ? ns : 256) * (size_t) (hd + 2);
+}
+
+int sml_hip_paged_attention(const sml_hip_pages * pg, const float * q, size_t q_stride, const int32_t * len,
+                            int max_len, int n_head, float scale, float * part, float * out, void * stream) {
+    HX_ENTRY(-1);
+    sml_kattend a;
+    memset(&a, 0, sizeof a);
+    check_pages(pg, &a.pg);
+    if (n_head < 1 || n_head % pg->n_kv || n_head / pg->n_kv > 16)
+        hx_failf("paged attention: %d heads over %d kv heads (1 to 16 each)", n_head, pg->n_kv);
+    if (!q || !len || !part || !out || max_len < 0) hx_failf("paged attention: missing buffers, or lengths up to %d", max_len);
+    const size_t width = (size_t) n_head * pg->hd;
+    if (q_stride && q_stride < width) hx_failf("paged attention: rows of %zu floats %zu apart", width, q_stride);
+    on_device();
+    a.q = q; a.q_stride = q_stride ? q_stride : width; a.len = len; a.part = part; a.out = out;
+    a.scale = (scale != 0.0f ? scale : 1.0f / sqrtf((float) pg->hd)) * 1.44269504088896341f;
+    a.n_head = n_head;
+    const long cap = (long) pg->seq_pages * pg->page_size;
+    a.max_len = max_len < cap ? max_len : (int) cap;
+    char name[40];
+    sv_name(name, sizeof name, "sml_sv_attend", pg->hd, pg->type);
+    hx_launch(name, (unsigned) n_head, (unsigned) pg->n_seq, 256, 0, (hipStream_t) stream, &a);
+    HX_LEAVE();
+    return 0;
+}
+
+#define LG_RANGE 4096
+
+size_t sml_hip_logits_part_bytes(int n_row, int n_vocab) {
+    if (n_row < 1 || n_vocab < 1) return 0;
+    return (size_t) n_row * (size_t) ceil_div(n_vocab, 2048) * 16;
+}
+
+int sml_hip_logits_adjust(const float * logits, size_t stride, int n_row, int n_vocab, const sml_hip_rules * rules,
+                          float * out, size_t out_stride, int32_t * tok, void * part, void * stream) {
+    HX_ENTRY(-1);
+    if (n_row < 0 || n_row > 65535 || n_vocab < 1 || n_vocab > 1 << 30)
+        hx_failf("logits: %d rows of %d", n_row, n_vocab);
+    if (!logits || (!out && !tok) || (tok && !part)) hx_failf("logits: missing rows, output or workspace");
+    if ((stride && stride < (size_t) n_vocab) || (out_stride && out_stride < (size_t) n_vocab))
+        hx_failf("logits: rows of %d floats %zu and %zu apart", n_vocab, stride, out_stride);
+    sml_klogits a;
+    memset(&a, 0, sizeof a);
+    a.logits = logits; a.out = out; a.tok = tok; a.part = part; a.n_vocab = n_vocab;
+    a.stride = stride ? stride : (size_t) n_vocab;
+    a.out_stride = out_stride ? out_stride : (size_t) n_vocab;
+    if (out == logits && a.out_stride != a.stride) hx_failf("logits: in place with strides %zu and %zu", a.stride, a.out_stride);
+    if (tok && ((uintptr_t) part & 15u)) hx_failf("logits: workspace off a 16-byte boundary");
+    if (rules) {
+        const sml_hip_rules * r = rules;
+        if (r->n_hist < 0 || r->n_bias < 0 || r->n_mask < 0)
+            hx_failf("logits: %d ids, %d biases, %d masks", r->n_hist, r->n_bias, r->n_mask);
+        if (r->hist && r->n_hist && (r->rep || r->presence || r->frequency)) {
+            if (!r->hist_start) hx_failf("logits: a history without hist_start");
+            a.hist = r->hist; a.hist_start = r->hist_start; a.n_prompt = r->n_prompt; a.n_hist = r->n_hist;
+            a.rep = r->rep; a.presence = r->presence; a.frequency = r->frequency;
+        }
+        if (r->bias && r->n_bias) {
+            if (!r->bias_id || !r->bias_start) hx_failf("logits: biases without bias_id or bias_start");
+            a.bias = r->bias; a.bias_id = r->bias_id; a.bias_start = r->bias_start; a.n_bias = r->n_bias;
+        }
+        if (r->mask) {
+            if (!r->mask_row && r->n_mask < n_row) hx_failf("logits: %d masks for %d rows without mask_row", r->n_mask, n_row);
+            a.mask = r->mask; a.mask_row = r->mask_row; a.n_mask = r->n_mask;
+        }
+    }
+    on_device();
+    if (n_row) {
+        a.n_part = ceil_div(n_vocab, LG_RANGE);
+        hx_launch("sml_sv_logits", (unsigned) a.n_part, (unsigned) n_row, 256, 0, (hipStream_t) stream, &a);
+        if (tok) hx_launch("sml_sv_pick", (unsigned) n_row, 1, 64, 0, (hipStream_t) stream, &a);
+    }
+    HX_LEAVE();
+    return 0;
+}
+
+size_t sml_hip_lora_work_floats(int rank, int n_row) {
+    if (rank < 1 || n_row < 1) return 0;
+    const size_t split = 32 * (size_t) n_row < 8192 ? 32 * (size_t) n_row : 8192;
+    return (size_t) rank * (split > (size_t) n_row ? split : (size_t) n_row);
+}
+
+int sml_hip_lora_add(const sml_hip_adapters * ad, const float * x, size_t x_stride, int n_row, const int32_t * adapter,
+                     const float * base, float * y, size_t y_stride, float * work, void * stream) {
+    HX_ENTRY(-1);
+    if (!ad || !ad->a || !ad->b) hx_failf("adapters: missing pools");
+    if (ad->type != SML_F16 && ad->type != SML_BF16) hx_failf("adapters: type %d", ad->type);
+    if (ad->n_adapter < 1 || ad->rank < 8 || ad->rank > 256 || ad->rank % 8)
+        hx_failf("adapters: %d of rank %d (a multiple of 8 up to 256)", ad->n_adapter, ad->rank);
+    if (ad->n_in < 8 || ad->n_in % 8 || ad->n_in > 1 << 24 || ad->n_out < 1 || ad->n_out > 1 << 24)
+        hx_failf("adapters: %d inputs (a multiple of 8), %d outputs", ad->n_in, ad->n_out);
+    if (!al16(ad->a) || !al16(ad->b)) hx_failf("adapters: pools off 16-byte boundaries");
+    if (n_row < 0 || n_row > 65535) hx_failf("adapters: %d rows", n_row);
+    if (!x || !adapter || !y || !work) hx_failf("adapters: missing rows, ids, output or workspace");
+    if ((x_stride && x_stride < (size_t) ad->n_in) || (y_stride && y_stride < (size_t) ad->n_out))
+        hx_failf("adapters: rows of %d and %d floats %zu and %zu apart", ad->n_in, ad->n_out, x_stride, y_stride);
+    on_device();
+    if (n_row) {
+        sml_klora a;
+        memset(&a, 0, sizeof a);
+        a.a = ad->a; a.b = ad->b; a.scale = ad->scale; a.ranks = ad->ranks; a.adapter = adapter;
+        a.x = x; a.base = base; a.y = y; a.work = work;
+        a.x_stride = x_stride ? x_stride : (size_t) ad->n_in;
+        a.y_stride = y_stride ? y_stride : (size_t) ad->n_out;
+        a.n_adapter = ad->n_adapter; a.rank = ad->rank; a.n_in = ad->n_in; a.n_out = ad->n_out; a.n_row = n_row;
+        const int bf = ad->type == SML_BF16;
+        hx_launch(bf ? "sml_sv_lora_down_bf" : "sml_sv_lora_down", (unsigned) ad->rank, (unsigned) n_row, 64, 0,
+                  (hipStream_t) stream, &a);
+        hx_launch(bf ? "sml_sv_lora_up_bf" : "sml_sv_lora_up", (unsigned) ceil_div(ad->n_out, 256), (unsigned) n_row, 256,
+                  0, (hipStream_t) stream, &a);
+    }
+    HX_LEAVE();
+    return 0;
+}

@@ -1,0 +1,140 @@
+"""A step that serves many requests at once: the ctypes wrappers of
+include/sml-serve.h.
+
+Keys and values live in a paged cache (`Pages`): `append` rotates the new
+tokens' keys and writes them with their values, `attention` lets one new token
+a sequence attend over its pages, `lora` adds each request's adapter beside a
+shared projection (`sheep_amd.gemm`), and `adjust_logits` applies penalties,
+biases and grammar masks and picks greedily. Buffers are DevBuf or anything
+with a device pointer in `.ptr`; workspaces are the caller's, sized by
+`part_floats`, `logits_part_bytes` and `lora_work_floats`. `stream` is a
+hipStream_t as an int (0: the null stream). The reference has no counterpart:
+it keeps one contiguous cache per sequence (sml/sml-run.c:3414-3434) and picks
+greedily (sml/sml-run.c:3539-3544).
+"""
+import ctypes
+
+from . import _chk, lib
+
+TYPES = {"f16": 0, "bf16": 1}
+_vp, _int, _size, _float = ctypes.c_void_p, ctypes.c_int, ctypes.c_size_t, ctypes.c_float
+
+
+class _Pages(ctypes.Structure):
+    """sml_hip_pages."""
+    _fields_ = [("k", _vp), ("v", _vp), ("table", _vp), ("page_stride", _size), ("n_pages", _int),
+                ("page_size", _int), ("n_seq", _int), ("seq_pages", _int), ("n_kv", _int), ("hd", _int),
+                ("type", _int)]
+
+
+class _Rules(ctypes.Structure):
+    """sml_hip_rules."""
+    _fields_ = [("hist", _vp), ("hist_start", _vp), ("n_prompt", _vp), ("n_hist", _int), ("rep", _vp),
+                ("presence", _vp), ("frequency", _vp), ("bias_id", _vp), ("bias", _vp), ("bias_start", _vp),
+                ("n_bias", _int), ("mask", _vp), ("mask_row", _vp), ("n_mask", _int)]
+
+
+class _Adapters(ctypes.Structure):
+    """sml_hip_adapters."""
+    _fields_ = [("a", _vp), ("b", _vp), ("scale", _vp), ("ranks", _vp), ("n_adapter", _int), ("rank", _int),
+                ("n_in", _int), ("n_out", _int), ("type", _int)]
+
+
+_P = ctypes.POINTER
+_SIGS = [
+    ("sml_hip_paged_append", _int, [_P(_Pages), _vp, _size, _int, _vp, _vp, _vp, _vp, _int, _int, _vp, _vp]),
+    ("sml_hip_paged_part_floats", _size, [_int, _int, _int, _int]),
+    ("sml_hip_paged_attention", _int, [_P(_Pages), _vp, _size, _vp, _int, _int, _float, _vp, _vp, _vp]),
+    ("sml_hip_logits_part_bytes", _size, [_int, _int]),
+    ("sml_hip_logits_adjust", _int, [_vp, _size, _int, _int, _P(_Rules), _vp, _size, _vp, _vp, _vp]),
+    ("sml_hip_lora_work_floats", _size, [_int, _int]),
+    ("sml_hip_lora_add", _int, [_P(_Adapters), _vp, _size, _int, _vp, _vp, _vp, _size, _vp, _vp]),
+]
+_fns = None
+
+
+def _fn(name):
+    global _fns
+    if _fns is None:
+        found = {}
+        for n, res, args in _SIGS:
+            f = getattr(lib(), n)
+            f.restype, f.argtypes = res, args
+            found[n] = f
+        _fns = found
+    return _fns[name]
+
+
+def _ptr(b):
+    return b.ptr if b is not None else None
+
+
+class Pages:
+    """One layer's paged cache: pools k and v [n_pages][page_size][n_kv][hd]
+    of 16-bit values, table [n_seq][seq_pages] int32. The buffers stay alive
+    with the object."""
+
+    def __init__(self, k, v, table, n_pages, page_size, n_seq, seq_pages, n_kv, hd, dtype="f16", page_stride=0):
+        self.buffers = (k, v, table)
+        self.n_seq, self.n_kv, self.hd = n_seq, n_kv, hd
+        self.c = _Pages(_ptr(k), _ptr(v), _ptr(table), page_stride, n_pages, page_size, n_seq, seq_pages, n_kv, hd,
+                        TYPES[dtype])
+
+
+def append(pages, qkv, n_rows, pos, cos, sin, n_rope, n_head, seq=None, q_out=None, qkv_stride=0, stream=0):
+    """Rotate n_rows new tokens' q and k by their positions and write their k
+    and v to the cache (sml_hip_paged_append); without q_out the rotated q
+    goes back to qkv."""
+    _chk(_fn("sml_hip_paged_append")(pages.c, _ptr(qkv), qkv_stride, n_rows, _ptr(seq), _ptr(pos), _ptr(cos),
+                                     _ptr(sin), n_rope, n_head, _ptr(q_out), stream), "paged append")
+
+
+def part_floats(n_seq, n_head, hd, max_len):
+    """Floats of attention's workspace."""
+    return _fn("sml_hip_paged_part_floats")(n_seq, n_head, hd, max_len)
+
+
+def attention(pages, q, lens, max_len, n_head, part, out, scale=0.0, q_stride=0, stream=0):
+    """out [n_seq][n_head*hd]: one new token a sequence over its first
+    lens[b] positions (sml_hip_paged_attention)."""
+    _chk(_fn("sml_hip_paged_attention")(pages.c, _ptr(q), q_stride, _ptr(lens), max_len, n_head, scale, _ptr(part),
+                                        _ptr(out), stream), "paged attention")
+
+
+def logits_part_bytes(n_row, n_vocab):
+    """Bytes of adjust_logits' workspace (with tok)."""
+    return _fn("sml_hip_logits_part_bytes")(n_row, n_vocab)
+
+
+def adjust_logits(logits, n_row, n_vocab, out=None, tok=None, part=None, hist=None, n_hist=0, hist_start=None,
+                  n_prompt=None, rep=None, presence=None, frequency=None, bias_id=None, bias=None, n_bias=0,
+                  bias_start=None, mask=None, n_mask=0, mask_row=None, stride=0, out_stride=0, stream=0):
+    """Penalties, biases and masks on n_row rows of logits into out (which may
+    be logits), and each row's greedy pick into tok (sml_hip_logits_adjust)."""
+    r = _Rules(_ptr(hist), _ptr(hist_start), _ptr(n_prompt), n_hist, _ptr(rep), _ptr(presence), _ptr(frequency),
+               _ptr(bias_id), _ptr(bias), _ptr(bias_start), n_bias, _ptr(mask), _ptr(mask_row), n_mask)
+    _chk(_fn("sml_hip_logits_adjust")(_ptr(logits), stride, n_row, n_vocab, r, _ptr(out), out_stride, _ptr(tok),
+                                      _ptr(part), stream), "logits")
+
+
+class Adapters:
+    """Low-rank adapters of one projection: a [n_adapter][rank][n_in] and
+    b [n_adapter][n_out][rank] of one 16-bit type, scale [n_adapter] floats
+    and ranks [n_adapter] int32 (None: 1 and rank). The buffers stay alive
+    with the object."""
+
+    def __init__(self, a, b, n_adapter, rank, n_in, n_out, dtype="f16", scale=None, ranks=None):
+        self.buffers = (a, b, scale, ranks)
+        self.c = _Adapters(_ptr(a), _ptr(b), _ptr(scale), _ptr(ranks), n_adapter, rank, n_in, n_out, TYPES[dtype])
+
+
+def lora_work_floats(rank, n_row):
+    """Floats of lora's workspace."""
+    return _fn("sml_hip_lora_work_floats")(rank, n_row)
+
+
+def lora(adapters, x, n_row, adapter, y, work, base=None, x_stride=0, y_stride=0, stream=0):
+    """y[r] = base[r] + scale * B (A x[r]) with row r's adapter, -1 for none
+    (sml_hip_lora_add); base may be y."""
+    _chk(_fn("sml_hip_lora_add")(adapters.c, _ptr(x), x_stride, n_row, _ptr(adapter), _ptr(base), _ptr(y), y_stride,
+                                 _ptr(work), stream), "lora")
