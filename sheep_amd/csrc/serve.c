@@ -77,6 +77,20 @@ size_t sml_hip_paged_part_floats(int n_seq, int n_head, int hd, int max_len) {
     return (size_t) n_seq * (size_t) n_head * (size_t) (ns < 256 ? ns : 256) * (size_t) (hd + 2);
 }
 
+// Positions of a split: a multiple of the 128 that a workgroup's waves take at
+// once, as few as keep at most 256 splits of the longest sequence (the
+// workspace's count) and about 4096 workgroups, but no more than 512 while
+// 256 splits of those suffice: lengths are ragged, and a workgroup with a long
+// sequence to itself would outlast the rest.
+static void attend_split(sml_kattend * a, int n_seq) {
+    const int n = a->max_len > 0 ? a->max_len : 1;
+    int chunk = 128;
+    while (chunk < 512 && (long) n_seq * a->pg.n_kv * ceil_div(n, chunk) > 4096) chunk += 128;
+    while (ceil_div(n, chunk) > 256) chunk += 128;
+    a->chunk = chunk;
+    a->nsplit = ceil_div(n, chunk);
+}
+
 int sml_hip_paged_attention(const sml_hip_pages * pg, const float * q, size_t q_stride, const int32_t * len,
                             int max_len, int n_head, float scale, float * part, float * out, void * stream) {
     HX_ENTRY(-1);
@@ -86,6 +100,7 @@ int sml_hip_paged_attention(const sml_hip_pages * pg, const float * q, size_t q_
     if (n_head < 1 || n_head % pg->n_kv || n_head / pg->n_kv > 16)
         hx_failf("paged attention: %d heads over %d kv heads (1 to 16 each)", n_head, pg->n_kv);
     if (!q || !len || !part || !out || max_len < 0) hx_failf("paged attention: missing buffers, or lengths up to %d", max_len);
+    if (!al16(part)) hx_failf("paged attention: workspace off a 16-byte boundary");
     const size_t width = (size_t) n_head * pg->hd;
     if (q_stride && q_stride < width) hx_failf("paged attention: rows of %zu floats %zu apart", width, q_stride);
     on_device();
@@ -94,9 +109,13 @@ int sml_hip_paged_attention(const sml_hip_pages * pg, const float * q, size_t q_
     a.n_head = n_head;
     const long cap = (long) pg->seq_pages * pg->page_size;
     a.max_len = max_len < cap ? max_len : (int) cap;
+    attend_split(&a, pg->n_seq);
     char name[40];
     sv_name(name, sizeof name, "sml_sv_attend", pg->hd, pg->type);
-    hx_launch(name, (unsigned) n_head, (unsigned) pg->n_seq, 256, 0, (hipStream_t) stream, &a);
+    hx_launch3(name, (unsigned) pg->n_kv, (unsigned) a.nsplit, (unsigned) pg->n_seq, 256, 0, (hipStream_t) stream, &a);
+    if (a.nsplit > 1)
+        hx_launch(pg->hd == 64 ? "sml_sv_merge_d64" : "sml_sv_merge", (unsigned) n_head, (unsigned) pg->n_seq, 256, 0,
+                  (hipStream_t) stream, &a);
     HX_LEAVE();
     return 0;
 }

@@ -80,51 +80,302 @@ APPEND(64, 1, sml_sv_append_d64_bf)
 
 // ---------------------------------------------------------------- attention
 //
-// One workgroup a query head, a wave every fourth position.
+// out = sum_i 2^(s_i - m) v_i / sum_i 2^(s_i - m), s_i = scale log2(e) q.k_i,
+// in one pass over the cache with a running base m. Nothing is read twice and
+// the arithmetic is 4 operations a value of up to 16 heads, so the cache's
+// bytes bound it: everything else is arranged to keep loads in flight.
+//
+// A workgroup takes a split of a sequence's positions for one KV head, its
+// waves alternate tiles of 32 positions, and a wave keeps all of a tile in
+// registers (no LDS until the waves' sums are joined). The matrix cores take
+// S^T = K Q^T and O^T = V^T P^T, heads in the columns (the unused of the 16
+// are zero). With the lane's c = lane % 16, g = lane / 16:
+// - K is the first operand as the cache stores it: lane (c, g) loads 16 bytes
+//   of position c's row, dims 32j + 8g.. for product j.
+// - S comes back as positions 4g + r of head c, which is just what the second
+//   product takes as its P^T operand if its inner index 8g + i stands for
+//   position 4g + i of the first 16 positions (i < 4) or of the second: P
+//   never crosses lanes.
+// - V's rows of those 8 positions are loaded whole, 16 lanes a row, dims
+//   (D/16)c.. each; the product u takes dim (D/16)c + u of every lane, so V^T
+//   is 4 D/16 byte permutes in the lane, and lane (c, g) ends with dims
+//   (D/4)g.. of head c: the base's rescaling is a lane's own too.
+// q and the weights are split into parts of the cache's type (two of fp16,
+// three of bf16: 22 and 24 bits), a matrix instruction each; q's row is scaled
+// by a power of two to below 2^11 first so that fp16 holds it. The base
+// starts 10 below the first maximum and moves when a score passes it by 15:
+// weights then lie up to 2^15, fp16's range, and those that its smallest
+// steps round are 2^-34 of the largest.
+//
+// Pages are looked up a tile ahead, once per 16 positions (a page is a
+// multiple of 16). Positions past the length or on absent pages are loaded
+// from where memory is (the rest of the page, or page 0), their scores
+// replaced by -infinity and their V rows by zeros; tiles of absent pages alone
+// are passed over.
+#define AT_WAVES 4
+
+template <int BF> struct Mx;
+template <> struct Mx<0> {
+    typedef _Float16 t;
+    typedef t v8 __attribute__((ext_vector_type(8)));
+    static constexpr int parts = 2;
+    static __device__ __forceinline__ v4f mul(v8 a, v8 b, v4f c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+};
+template <> struct Mx<1> {
+    typedef __bf16 t;
+    typedef t v8 __attribute__((ext_vector_type(8)));
+    static constexpr int parts = 3;
+    static __device__ __forceinline__ v4f mul(v8 a, v8 b, v4f c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+};
+
+// element e of the parts of x: each part the rounding of what is left
+template <int BF>
+__device__ __forceinline__ void parts_of(float x, typename Mx<BF>::v8 (&p)[Mx<BF>::parts], int e) {
+    #pragma unroll
+    for (int k = 0; k < Mx<BF>::parts; k++) {
+        const typename Mx<BF>::t h = (typename Mx<BF>::t) x;
+        p[k][e] = h;
+        x -= (float) h;
+    }
+}
+
 template <int D, int BF>
 __device__ __forceinline__ void attend_body(const sml_kattend & a) {
-    constexpr int E = D / 64;
-    __shared__ float so[4][D], sm[4], sl[4];
-    const int h = blockIdx.x, b = blockIdx.y, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    const int n = min(a.len[b], a.max_len), kh = h / (a.n_head / a.pg.n_kv);
-    float q[E], o[E], m = -INFINITY, l = 0.0f;
-    #pragma unroll
-    for (int e = 0; e < E; e++) {
-        q[e] = a.q[(size_t) b * a.q_stride + (size_t) h * D + lane * E + e] * a.scale;
-        o[e] = 0.0f;
-    }
-    for (int p = w; p < n; p += 4) {
-        const int page = page_of(a.pg, b, p >> a.pg.page_shift);
-        if (page < 0) continue;
-        const size_t at = (size_t) page * a.pg.page_stride +
-                          (size_t) (p & ((1 << a.pg.page_shift) - 1)) * (a.pg.n_kv * D) + (size_t) kh * D + lane * E;
-        float s = 0.0f;
+    using M = Mx<BF>;
+    typedef typename M::v8 v8;
+    constexpr int NJ = D / 32, E = D / 16, NP = M::parts, W = AT_WAVES;
+    typedef unsigned vrow __attribute__((ext_vector_type(E / 2)));
+    __shared__ float so[W][16][D + 4], sm[W][16], sl[W][16];
+    const int kh = blockIdx.x, split = blockIdx.y, b = blockIdx.z, tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, g = lane >> 4;
+    const int n = min(a.len[b], a.max_len), t0 = split * a.chunk, t1 = min(n, t0 + a.chunk);
+    if (t0 >= t1 && a.nsplit > 1) return;             // the merge takes the splits below the length only
+    const int rep = a.n_head / a.pg.n_kv, kvd = a.pg.n_kv * D;
+    const int sh = a.pg.page_shift, pmask = (1 << sh) - 1;
+    const int32_t * const tab = a.pg.table + (size_t) b * a.pg.seq_pages;
+
+    // the query: lane (c, g) holds dims 32j + 8g.. of head c, in parts
+    v8 q[NJ][NP];
+    float back;                                       // what a product of the scaled q is multiplied by
+    {
+        float x[NJ][8], mx = 0.0f;
+        const float * qp = a.q + (size_t) b * a.q_stride + (size_t) (kh * rep + min(c, rep - 1)) * D + 8 * g;
         #pragma unroll
-        for (int e = 0; e < E; e++) s += q[e] * of16<BF>(a.pg.k[at + e]);
-        s = wave_sum(s);
-        const float mn = fmaxf(m, s), mu = mn == -INFINITY ? 0.0f : mn;
-        const float al = __builtin_amdgcn_exp2f(m - mu), pr = __builtin_amdgcn_exp2f(s - mu);
-        l = l * al + pr;
+        for (int j = 0; j < NJ; j++)
+            #pragma unroll
+            for (int e = 0; e < 8; e += 4) {
+                const v4f v = *(const v4fu *) (qp + 32 * j + e);
+                #pragma unroll
+                for (int i = 0; i < 4; i++) { x[j][e + i] = c < rep ? v[i] : 0.0f; mx = fmaxf(mx, fabsf(x[j][e + i])); }
+            }
+        mx = fmaxf(mx, __shfl_xor(mx, 16));
+        mx = fmaxf(mx, __shfl_xor(mx, 32));
+        const int ex = mx > 0.0f && mx < INFINITY ? __builtin_amdgcn_frexp_expf(mx) - 11 : 0;
         #pragma unroll
-        for (int e = 0; e < E; e++) o[e] = o[e] * al + pr * of16<BF>(a.pg.v[at + e]);
-        m = mn;
+        for (int j = 0; j < NJ; j++)
+            #pragma unroll
+            for (int e = 0; e < 8; e++) parts_of<BF>(__builtin_amdgcn_ldexpf(x[j][e], -ex), q[j], e);
+        back = __builtin_amdgcn_ldexpf(a.scale, ex);
     }
+
+    v4f o[E];
     #pragma unroll
-    for (int e = 0; e < E; e++) so[w][lane * E + e] = o[e];
-    if (!lane) { sm[w] = m; sl[w] = l; }
+    for (int u = 0; u < E; u++) o[u] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+    float base = -INFINITY, l = 0.0f;
+
+    // the next tile at or after t (this wave's) that has a page, and its two
+    // pages (-1: absent)
+    int pa = -1, pb = -1;
+    auto seek = [&](int t) {
+        for (; t < t1; t += 32 * W) {
+            pa = tab[t >> sh];
+            pb = t + 16 < t1 ? tab[(t + 16) >> sh] : -1;
+            pa = pa >= 0 && pa < a.pg.n_pages ? pa : -1;
+            pb = pb >= 0 && pb < a.pg.n_pages ? pb : -1;
+            if (pa >= 0 || pb >= 0) break;
+        }
+        return t;
+    };
+    v4u kr[2][NJ];
+    vrow vr[8];
+    const uint32_t koff = 2u * (uint32_t) (c * kvd + 8 * g);
+    uint32_t voff[4];
+    #pragma unroll
+    for (int i = 0; i < 4; i++) voff[i] = 2u * (uint32_t) ((4 * g + i) * kvd + E * c);
+    // the places of a tile's two halves in a pool
+    auto place = [&](int page, int t) {
+        return (size_t) max(page, 0) * a.pg.page_stride + (size_t) (t & pmask) * kvd + (size_t) kh * D;
+    };
+    auto load_k = [&](size_t xa, size_t xb) {
+        #pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const GLOBAL char * p = (const GLOBAL char *) (a.pg.k + (h ? xb : xa));
+            #pragma unroll
+            for (int j = 0; j < NJ; j++) kr[h][j] = *(const GLOBAL v4u *) (p + koff + 64 * j);
+        }
+    };
+    auto load_v = [&](size_t xa, size_t xb) {
+        #pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const GLOBAL char * p = (const GLOBAL char *) (a.pg.v + (h ? xb : xa));
+            #pragma unroll
+            for (int i = 0; i < 4; i++) vr[4 * h + i] = *(const GLOBAL vrow *) (p + voff[i]);
+        }
+    };
+
+    int t = seek(t0 + 32 * wave);
+    if (t < t1) {
+        const size_t xa = place(pa, t), xb = place(pb, t + 16);
+        load_k(xa, xb);
+        load_v(xa, xb);
+    }
+    while (t < t1) {
+        const bool ha = pa >= 0, hb = pb >= 0, whole = ha && hb && t + 32 <= t1;
+        const int tn = seek(t + 32 * W);
+        const size_t xa = place(pa, tn), xb = place(pb, tn + 16);
+        v4f s[2];
+        #pragma unroll
+        for (int h = 0; h < 2; h++) {
+            s[h] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+            #pragma unroll
+            for (int j = 0; j < NJ; j++)
+                #pragma unroll
+                for (int k = 0; k < NP; k++) s[h] = M::mul(__builtin_bit_cast(v8, kr[h][j]), q[j][k], s[h]);
+        }
+        if (tn < t1) load_k(xa, xb);
+        // the lane's scores: positions 4g + r of either half
+        float mx = -INFINITY;
+        #pragma unroll
+        for (int h = 0; h < 2; h++)
+            #pragma unroll
+            for (int r = 0; r < 4; r++) s[h][r] *= back;
+        if (!whole) {
+            #pragma unroll
+            for (int h = 0; h < 2; h++)
+                #pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const bool in = (h ? hb : ha) && t + 16 * h + 4 * g + r < t1;
+                    s[h][r] = in ? s[h][r] : -INFINITY;
+                    if (!in) vr[4 * h + r] = vrow(0u);
+                }
+        }
+        #pragma unroll
+        for (int h = 0; h < 2; h++)
+            #pragma unroll
+            for (int r = 0; r < 4; r++) mx = fmaxf(mx, s[h][r]);
+        if (__any(mx > base + 15.0f)) {
+            mx = fmaxf(mx, __shfl_xor(mx, 16));
+            mx = fmaxf(mx, __shfl_xor(mx, 32));
+            const float to = mx > base + 15.0f ? mx - 10.0f : base;
+            const float al = __builtin_amdgcn_exp2f(base - (to == -INFINITY ? 0.0f : to));
+            l *= al;
+            #pragma unroll
+            for (int u = 0; u < E; u++)
+                #pragma unroll
+                for (int r = 0; r < 4; r++) o[u][r] *= al;
+            base = to;
+        }
+        const float bu = base == -INFINITY ? 0.0f : base;
+        v8 p[NP];
+        #pragma unroll
+        for (int h = 0; h < 2; h++)
+            #pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const float w = __builtin_amdgcn_exp2f(s[h][r] - bu);
+                l += w;
+                parts_of<BF>(w, p, 4 * h + r);
+            }
+        #pragma unroll
+        for (int u = 0; u < E; u++) {
+            v4u w;
+            #pragma unroll
+            for (int i = 0; i < 4; i++)
+                w[i] = __builtin_amdgcn_perm(vr[2 * i + 1][u / 2], vr[2 * i][u / 2], u & 1 ? 0x07060302u : 0x05040100u);
+            #pragma unroll
+            for (int k = 0; k < NP; k++) o[u] = M::mul(__builtin_bit_cast(v8, w), p[k], o[u]);
+        }
+        if (tn < t1) load_v(xa, xb);
+        t = tn;
+    }
+
+    // the waves' sums joined: wave w's head c, dims (D/4)g + Er + u
+    l += __shfl_xor(l, 16);
+    l += __shfl_xor(l, 32);
+    if (c < rep) {
+        #pragma unroll
+        for (int r = 0; r < 4; r++)
+            #pragma unroll
+            for (int u = 0; u < E; u++) so[wave][c][(D / 4) * g + E * r + u] = o[u][r];
+        if (!g) { sm[wave][c] = base; sl[wave][c] = l; }
+    }
     __syncthreads();
-    if ((int) threadIdx.x >= D) return;
-    float mm = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3])), ll = 0.0f, oo = 0.0f;
-    if (mm == -INFINITY) mm = 0.0f;
-    for (int i = 0; i < 4; i++) {
-        const float e = __builtin_amdgcn_exp2f(sm[i] - mm);
-        ll += e * sl[i];
-        oo += e * so[i][threadIdx.x];
+    const size_t row0 = (size_t) b * a.n_head + (size_t) kh * rep;
+    for (int i = tid; i < rep * D; i += 64 * W) {
+        const int h = i / D, d = i % D;
+        float m = sm[0][h];
+        #pragma unroll
+        for (int w = 1; w < W; w++) m = fmaxf(m, sm[w][h]);
+        const float mu = m == -INFINITY ? 0.0f : m;
+        float os = 0.0f, ls = 0.0f;
+        #pragma unroll
+        for (int w = 0; w < W; w++) {
+            const float f = __builtin_amdgcn_exp2f(sm[w][h] - mu);
+            os += f * so[w][h][d];
+            ls += f * sl[w][h];
+        }
+        if (a.nsplit == 1) {
+            a.out[(row0 + h) * D + d] = ls == 0.0f ? 0.0f : os / ls;
+        } else {
+            const size_t at = (row0 + h) * a.nsplit + split;
+            a.part[at * D + d] = os;
+            if (!d) *(float2 *) (a.part + (size_t) a.pg.n_seq * a.n_head * a.nsplit * D + 2 * at) = make_float2(m, ls);
+        }
     }
-    a.out[((size_t) b * a.n_head + h) * D + threadIdx.x] = ll == 0.0f ? 0.0f : oo / ll;
 }
+
+// The splits of a row joined: a workgroup a (sequence, head), D threads a
+// share of its splits.
+#define AM_THREADS 256
+template <int D>
+__device__ __forceinline__ void attend_merge_body(const sml_kattend & a) {
+    constexpr int S = AM_THREADS / D;                 // shares
+    __shared__ float f[256], red[S][D], sred[AM_THREADS / 64];
+    const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
+    const int n = min(a.len[b], a.max_len), ns = n > 0 ? (n + a.chunk - 1) / a.chunk : 0;
+    const size_t row = (size_t) b * a.n_head + h;
+    const float * po = a.part + row * a.nsplit * D;
+    const float2 * pm = (const float2 *) (a.part + (size_t) a.pg.n_seq * a.n_head * a.nsplit * D) + row * a.nsplit;
+    const float2 ml = tid < ns ? pm[tid] : make_float2(-INFINITY, 0.0f);
+    float m = wave_max(ml.x);
+    if (!(tid & 63)) sred[tid >> 6] = m;
+    __syncthreads();
+    m = sred[0];
+    #pragma unroll
+    for (int w = 1; w < AM_THREADS / 64; w++) m = fmaxf(m, sred[w]);
+    const float e = __builtin_amdgcn_exp2f(ml.x - (m == -INFINITY ? 0.0f : m));
+    f[tid] = e;
+    __syncthreads();                                  // f is whole, and sred read by all
+    const float lw = wave_sum(e * ml.y);
+    if (!(tid & 63)) sred[tid >> 6] = lw;
+    const int d = tid % D, s0 = tid / D;
+    float o = 0.0f;
+    #pragma unroll 8
+    for (int i = s0; i < ns; i += S) o += f[i] * po[(size_t) i * D + d];
+    red[s0][d] = o;
+    __syncthreads();
+    if (tid >= D) return;
+    float l = 0.0f;
+    #pragma unroll
+    for (int w = 0; w < AM_THREADS / 64; w++) l += sred[w];
+    #pragma unroll
+    for (int s = 1; s < S; s++) o += red[s][d];
+    a.out[row * D + d] = l == 0.0f ? 0.0f : o / l;
+}
+extern "C" __global__ __launch_bounds__(AM_THREADS) void sml_sv_merge(const sml_kattend a) { attend_merge_body<128>(a); }
+extern "C" __global__ __launch_bounds__(AM_THREADS) void sml_sv_merge_d64(const sml_kattend a) { attend_merge_body<64>(a); }
+
 #define ATTEND(D, BF, name) \
-    extern "C" __global__ __launch_bounds__(256) void name(const sml_kattend a) { attend_body<D, BF>(a); }
+    extern "C" __global__ __launch_bounds__(64 * AT_WAVES) void name(const sml_kattend a) { attend_body<D, BF>(a); }
 ATTEND(128, 0, sml_sv_attend)
 ATTEND(128, 1, sml_sv_attend_bf)
 ATTEND(64, 0, sml_sv_attend_d64)
