@@ -176,6 +176,34 @@ size_t sml_hip_lora_work_floats(int rank, int n_row) {
     return (size_t) rank * (split > (size_t) n_row ? split : (size_t) n_row);
 }
 
+// Inputs a workgroup of the first product takes at once, and the rows of its tile.
+#define LD_TILE 1024
+#define LD_ROWS 16
+
+static void lora_launch(sml_klora * a, int bf, hipStream_t st) {
+    char name[40];
+    // the inputs split LD_TILE apiece, less finely where the rows give 256
+    // workgroups already or the workspace holds no more
+    const int ntile = ceil_div(a->n_row, LD_ROWS);
+    int most = 8192 / a->n_row < 32 ? 8192 / a->n_row : 32;
+    if (most > ceil_div(256, ntile)) most = ceil_div(256, ntile);
+    if (most < 1) most = 1;
+    a->chunk = LD_TILE;
+    while (ceil_div(a->n_in, a->chunk) > most) a->chunk += LD_TILE;
+    a->nsplit = ceil_div(a->n_in, a->chunk);
+    // a tile's distinct adapters side by side for a step's few rows; the rows
+    // of prompts come in runs, a tile mostly of one
+    const int few = a->n_row <= 128, nz = !few ? 1 : a->n_row < 16 ? a->n_row : 16;
+    const int rt = a->rank <= 16 ? 1 : 4, ngroup = ceil_div(a->rank, 16 * rt);
+    snprintf(name, sizeof name, "sml_sv_lora_down_t%d%s", rt, bf ? "_bf" : "");
+    hx_launch3(name, (unsigned) ntile, (unsigned) a->nsplit, (unsigned) (nz * ngroup), 512, 0, st, a);
+    const int rb = few ? 1 : 4, ot = few ? 1 : 2;
+    snprintf(name, sizeof name, "sml_sv_lora_up_b%d%s", rb, bf ? "_bf" : "");
+    const size_t lds = (size_t) (bf ? 3 : 2) * 16 * rb * (size_t) (a->rank + 8) * 2 + (size_t) 16 * rb * 4;
+    hx_launch3(name, (unsigned) ceil_div(a->n_out, 64 * ot), (unsigned) ceil_div(a->n_row, 16 * rb), (unsigned) nz, 256,
+               lds, st, a);
+}
+
 int sml_hip_lora_add(const sml_hip_adapters * ad, const float * x, size_t x_stride, int n_row, const int32_t * adapter,
                      const float * base, float * y, size_t y_stride, float * work, void * stream) {
     HX_ENTRY(-1);
@@ -199,11 +227,7 @@ int sml_hip_lora_add(const sml_hip_adapters * ad, const float * x, size_t x_stri
         a.x_stride = x_stride ? x_stride : (size_t) ad->n_in;
         a.y_stride = y_stride ? y_stride : (size_t) ad->n_out;
         a.n_adapter = ad->n_adapter; a.rank = ad->rank; a.n_in = ad->n_in; a.n_out = ad->n_out; a.n_row = n_row;
-        const int bf = ad->type == SML_BF16;
-        hx_launch(bf ? "sml_sv_lora_down_bf" : "sml_sv_lora_down", (unsigned) ad->rank, (unsigned) n_row, 64, 0,
-                  (hipStream_t) stream, &a);
-        hx_launch(bf ? "sml_sv_lora_up_bf" : "sml_sv_lora_up", (unsigned) ceil_div(ad->n_out, 256), (unsigned) n_row, 256,
-                  0, (hipStream_t) stream, &a);
+        lora_launch(&a, ad->type == SML_BF16, (hipStream_t) stream);
     }
     HX_LEAVE();
     return 0;

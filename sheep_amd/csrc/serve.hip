@@ -128,6 +128,11 @@ template <> struct Mx<1> {
     static __device__ __forceinline__ v4f mul(v8 a, v8 b, v4f c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 };
 
+// Powers of two: the one that brings values up to mx below 2^11, and back.
+__device__ __forceinline__ int scale_of(float mx) {
+    return mx > 0.0f && mx < INFINITY ? __builtin_amdgcn_frexp_expf(mx) - 11 : 0;
+}
+
 // element e of the parts of x: each part the rounding of what is left
 template <int BF>
 __device__ __forceinline__ void parts_of(float x, typename Mx<BF>::v8 (&p)[Mx<BF>::parts], int e) {
@@ -170,7 +175,7 @@ __device__ __forceinline__ void attend_body(const sml_kattend & a) {
             }
         mx = fmaxf(mx, __shfl_xor(mx, 16));
         mx = fmaxf(mx, __shfl_xor(mx, 32));
-        const int ex = mx > 0.0f && mx < INFINITY ? __builtin_amdgcn_frexp_expf(mx) - 11 : 0;
+        const int ex = scale_of(mx);
         #pragma unroll
         for (int j = 0; j < NJ; j++)
             #pragma unroll
@@ -490,35 +495,245 @@ extern "C" __global__ __launch_bounds__(64) void sml_sv_pick(const sml_klogits a
 
 // ---------------------------------------------------------------- adapters
 //
-// Two launches: t = A x of a row's adapter, then y = base + scale * B t.
-template <int BF>
+// y = base + scale B (A x), two launches: t = A x of every row under its own
+// adapter (split over the inputs, joined by the second launch's prologue), then
+// y. Rows come in tiles of 16, the matrix cores' columns: a workgroup takes the
+// distinct adapters among its tile's rows one by one, computes all columns
+// with each and stores those of its rows. Columns never mix, so a row sees
+// nothing of the others, and no sorting of requests is needed: requests that
+// share an adapter in a tile read it once, those that do not read each their
+// own, which is the least there is to read.
+//
+// fp32 x and t meet the 16-bit matrices as parts of their type (fp16: two, and
+// each row scaled by a power of two to below 2^11 first; bf16: three), 22 or 24
+// bits, summed in fp32.
+#define LD_WAVES 8
+#define LD_STEPS 4                                    // inner products of 32 a wave holds at once
+#define LD_TILE (LD_WAVES * LD_STEPS * 32)            // inputs a workgroup takes at once
+
+// The valid adapter id of a row, or -1.
+__device__ __forceinline__ int adapter_of(const sml_klora & a, int row) {
+    const int id = row < a.n_row ? a.adapter[row] : -1;
+    return id >= 0 && id < a.n_adapter ? id : -1;
+}
+__device__ __forceinline__ int rank_of(const sml_klora & a, int id) {
+    return a.ranks ? min(max(a.ranks[id], 0), a.rank) : a.rank;
+}
+
+template <int BF, int RT>
 __device__ __forceinline__ void lora_down_body(const sml_klora & a) {
-    const int j = blockIdx.x, r = blockIdx.y, ad = a.adapter[r];
-    if (ad < 0 || ad >= a.n_adapter || (a.ranks && j >= a.ranks[ad])) return;
-    const uint16_t * w = a.a + ((size_t) ad * a.rank + j) * a.n_in;
-    const float * x = a.x + (size_t) r * a.x_stride;
-    float s = 0.0f;
-    for (int i = threadIdx.x; i < a.n_in; i += 64) s += x[i] * of16<BF>(w[i]);
-    s = wave_sum(s);
-    if (!threadIdx.x) a.work[(size_t) r * a.rank + j] = s;
-}
-template <int BF>
-__device__ __forceinline__ void lora_up_body(const sml_klora & a) {
-    const int o = blockIdx.x * 256 + threadIdx.x, r = blockIdx.y, ad = a.adapter[r];
-    if (o >= a.n_out) return;
-    const size_t at = (size_t) r * a.y_stride + o;
-    float y = a.base ? a.base[at] : 0.0f;
-    if (ad >= 0 && ad < a.n_adapter) {
-        const int rk = a.ranks ? min(a.ranks[ad], a.rank) : a.rank;
-        const uint16_t * w = a.b + ((size_t) ad * a.n_out + o) * a.rank;
-        const float * t = a.work + (size_t) r * a.rank;
-        float s = 0.0f;
-        for (int j = 0; j < rk; j++) s += t[j] * of16<BF>(w[j]);
-        y += (a.scale ? a.scale[ad] : 1.0f) * s;
+    using M = Mx<BF>;
+    typedef typename M::v8 v8;
+    __shared__ float red[LD_WAVES][16][16 * RT + 1];
+    const int row0 = blockIdx.x * 16, split = blockIdx.y, tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int ngroup = (a.rank + 16 * RT - 1) / (16 * RT), nz = gridDim.z / ngroup;
+    const int j0 = (blockIdx.z % ngroup) * 16 * RT, z = blockIdx.z / ngroup;
+    const int k0 = split * a.chunk, k1 = min(a.n_in, k0 + a.chunk);
+    const int id = adapter_of(a, row0 + c);
+    const float * x = a.x + (size_t) min(row0 + c, a.n_row - 1) * a.x_stride;
+
+    unsigned left = (unsigned) (__ballot(id >= 0) & 0xFFFFu);
+    for (int k = 0; left; k++) {
+        const int cur = __builtin_amdgcn_readlane(id, __builtin_ctz(left));
+        const unsigned mine = (unsigned) (__ballot(id == cur) & 0xFFFFu);
+        left &= ~mine;
+        if (k % nz != z) continue;
+        const int rk = rank_of(a, cur);
+        if (j0 >= rk) continue;
+        const int nt = min(RT, (rk - j0 + 15) / 16);
+        const uint16_t * w = a.a + (size_t) cur * a.rank * a.n_in;
+        v4f tot[RT];
+        #pragma unroll
+        for (int t = 0; t < RT; t++) tot[t] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int kb = k0 + wave * 32 * LD_STEPS; kb < k1; kb += LD_TILE) {
+            float xv[LD_STEPS][8], mx = 0.0f;
+            v4u wv[RT][LD_STEPS];
+            #pragma unroll
+            for (int s = 0; s < LD_STEPS; s++) {
+                const int kk = kb + 32 * s + 8 * g;
+                #pragma unroll
+                for (int e = 0; e < 8; e += 4) {
+                    const v4f v = *(const GLOBAL v4fu *) (x + (kk < k1 ? kk + e : 0));
+                    #pragma unroll
+                    for (int i = 0; i < 4; i++) xv[s][e + i] = kk < k1 ? v[i] : 0.0f;
+                }
+            }
+            #pragma unroll
+            for (int t = 0; t < RT; t++)
+                if (t < nt) {
+                    const uint16_t * wr = w + (size_t) min(j0 + 16 * t + c, rk - 1) * a.n_in;
+                    #pragma unroll
+                    for (int s = 0; s < LD_STEPS; s++) {
+                        const int kk = kb + 32 * s + 8 * g;
+                        wv[t][s] = *(const GLOBAL v4u *) (wr + (kk < k1 ? kk : 0));
+                        if (kk >= k1) wv[t][s] = v4u(0u);
+                    }
+                }
+            #pragma unroll
+            for (int s = 0; s < LD_STEPS; s++)
+                #pragma unroll
+                for (int e = 0; e < 8; e++) mx = fmaxf(mx, fabsf(xv[s][e]));
+            mx = fmaxf(mx, __shfl_xor(mx, 16));
+            mx = fmaxf(mx, __shfl_xor(mx, 32));
+            const int ex = BF ? 0 : scale_of(mx);
+            v8 p[LD_STEPS][M::parts];
+            #pragma unroll
+            for (int s = 0; s < LD_STEPS; s++)
+                #pragma unroll
+                for (int e = 0; e < 8; e++) parts_of<BF>(__builtin_amdgcn_ldexpf(xv[s][e], -ex), p[s], e);
+            #pragma unroll
+            for (int t = 0; t < RT; t++)
+                if (t < nt) {
+                    v4f acc = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+                    #pragma unroll
+                    for (int s = 0; s < LD_STEPS; s++)
+                        #pragma unroll
+                        for (int i = 0; i < M::parts; i++) acc = M::mul(__builtin_bit_cast(v8, wv[t][s]), p[s][i], acc);
+                    #pragma unroll
+                    for (int r = 0; r < 4; r++) tot[t][r] += __builtin_amdgcn_ldexpf(acc[r], ex);
+                }
+        }
+        #pragma unroll
+        for (int t = 0; t < RT; t++)
+            #pragma unroll
+            for (int r = 0; r < 4; r++) red[wave][c][16 * t + 4 * g + r] = tot[t][r];
+        __syncthreads();
+        for (int i = tid; i < 256 * RT; i += 64 * LD_WAVES) {
+            const int rw = i / (16 * RT), j = i % (16 * RT);
+            float s = 0.0f;
+            #pragma unroll
+            for (int v = 0; v < LD_WAVES; v++) s += red[v][rw][j];
+            if ((mine >> rw & 1) && j0 + j < rk)
+                a.work[((size_t) (row0 + rw) * a.nsplit + split) * a.rank + j0 + j] = s;
+        }
+        __syncthreads();
     }
-    a.y[at] = y;
 }
-extern "C" __global__ __launch_bounds__(64) void sml_sv_lora_down(const sml_klora a) { lora_down_body<0>(a); }
-extern "C" __global__ __launch_bounds__(64) void sml_sv_lora_down_bf(const sml_klora a) { lora_down_body<1>(a); }
-extern "C" __global__ __launch_bounds__(256) void sml_sv_lora_up(const sml_klora a) { lora_up_body<0>(a); }
-extern "C" __global__ __launch_bounds__(256) void sml_sv_lora_up_bf(const sml_klora a) { lora_up_body<1>(a); }
+
+// RB tiles of 16 rows and 4 waves of OT tiles of 16 outputs a workgroup.
+template <int BF, int RB, int OT>
+__device__ __forceinline__ void lora_up_body(const sml_klora & a) {
+    using M = Mx<BF>;
+    typedef typename M::v8 v8;
+    typedef typename M::t T;
+    extern __shared__ __align__(16) uint8_t lds[];
+    constexpr int NR = 16 * RB, NP = M::parts;
+    const int ld = a.rank + 8;                        // values of a row of t's parts in LDS
+    T * const tp = (T *) lds;                         // [part][row][ld]
+    int * const ex_s = (int *) (lds + (size_t) NP * NR * ld * 2);
+    const int row0 = blockIdx.y * NR, tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), nz = gridDim.z, z = blockIdx.z;
+    const int o0 = (blockIdx.x * 4 + wave) * 16 * OT;
+
+    // t: the splits' sums, scaled, in parts; lr lanes of 4 values a row
+    {
+        int lr = 2;
+        while (4 * lr < a.rank) lr *= 2;
+        const int q = tid & (lr - 1), step = 256 / lr;
+        for (int r = tid / lr; r < NR; r += step) {
+            const int row = min(row0 + r, a.n_row - 1), id = adapter_of(a, row), rk = id < 0 ? 0 : rank_of(a, id);
+            const float sc = id < 0 ? 0.0f : a.scale ? a.scale[id] : 1.0f;
+            const float * t = a.work + (size_t) row * a.nsplit * a.rank + 4 * q;
+            v4f v = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+            if (4 * q < rk)
+                for (int s = 0; s < a.nsplit; s++) v += *(const v4fu *) (t + (size_t) s * a.rank);
+            float mx = 0.0f;
+            #pragma unroll
+            for (int e = 0; e < 4; e++) { v[e] = 4 * q + e < rk ? v[e] * sc : 0.0f; mx = fmaxf(mx, fabsf(v[e])); }
+            for (int o = 1; o < lr; o *= 2) mx = fmaxf(mx, __shfl_xor(mx, o));
+            const int ex = BF ? 0 : scale_of(mx);
+            if (4 * q < a.rank) {
+                v8 p[NP];
+                #pragma unroll
+                for (int e = 0; e < 4; e++) parts_of<BF>(__builtin_amdgcn_ldexpf(v[e], -ex), p, e);
+                #pragma unroll
+                for (int k = 0; k < NP; k++)
+                    #pragma unroll
+                    for (int e = 0; e < 4; e++) tp[((size_t) k * NR + r) * ld + 4 * q + e] = p[k][e];
+            }
+            if (!q) ex_s[r] = ex;
+        }
+    }
+    __syncthreads();
+    const int id = lane < NR ? adapter_of(a, row0 + lane) : -1;
+    unsigned long long left = __ballot(id >= 0), none = ~left;
+    for (int k = 0; left || none; k++) {
+        // the rows without an adapter are taken like those of one more
+        int cur = -1;
+        unsigned long long mine = none;
+        if (left) {
+            cur = __builtin_amdgcn_readlane(id, __builtin_ctzll(left));
+            mine = __ballot(id == cur);
+            left &= ~mine;
+        } else {
+            none = 0;
+        }
+        if (k % nz != z || (cur < 0 && a.base == a.y)) continue;
+        const int rk = cur < 0 ? 0 : rank_of(a, cur);
+        const uint16_t * w = a.b + (size_t) max(cur, 0) * a.n_out * a.rank;
+        v4f acc[RB][OT];
+        #pragma unroll
+        for (int b = 0; b < RB; b++)
+            #pragma unroll
+            for (int u = 0; u < OT; u++) acc[b][u] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int k0 = 0; k0 < rk; k0 += 32) {
+            const int kk = k0 + 8 * g, at = kk < a.rank ? kk : 0;
+            v4u wv[OT];
+            #pragma unroll
+            for (int u = 0; u < OT; u++) {
+                wv[u] = *(const GLOBAL v4u *) (w + (size_t) min(o0 + 16 * u + c, a.n_out - 1) * a.rank + at);
+                if (k0 + 32 > rk) {
+                    #pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const int j = kk + 2 * i;
+                        wv[u][i] = j + 1 < rk ? wv[u][i] : j < rk ? wv[u][i] & 0xFFFFu : 0u;
+                    }
+                }
+            }
+            #pragma unroll
+            for (int b = 0; b < RB; b++)
+                #pragma unroll
+                for (int i = 0; i < NP; i++) {
+                    v8 tv = *(const v8 *) (tp + ((size_t) i * NR + 16 * b + c) * ld + at);
+                    if (kk >= a.rank) tv = __builtin_bit_cast(v8, v4u(0u));
+                    #pragma unroll
+                    for (int u = 0; u < OT; u++) acc[b][u] = M::mul(__builtin_bit_cast(v8, wv[u]), tv, acc[b][u]);
+                }
+        }
+        #pragma unroll
+        for (int b = 0; b < RB; b++) {
+            const int row = row0 + 16 * b + c;
+            if (!(mine >> (16 * b + c) & 1) || row >= a.n_row) continue;
+            const int ex = ex_s[16 * b + c];
+            #pragma unroll
+            for (int u = 0; u < OT; u++) {
+                const int o = o0 + 16 * u + 4 * g;
+                const size_t at = (size_t) row * a.y_stride + o;
+                v4f d;
+                #pragma unroll
+                for (int r = 0; r < 4; r++) d[r] = __builtin_amdgcn_ldexpf(acc[b][u][r], ex);
+                if (o + 4 <= a.n_out) {
+                    if (a.base) d += *(const v4fu *) (a.base + at);
+                    *(v4fu *) (a.y + at) = d;
+                } else {
+                    #pragma unroll
+                    for (int r = 0; r < 4; r++)
+                        if (o + r < a.n_out) a.y[at + r] = (a.base ? a.base[at + r] : 0.0f) + d[r];
+                }
+            }
+        }
+    }
+}
+#define LORA_DOWN(BF, RT, name) \
+    extern "C" __global__ __launch_bounds__(64 * LD_WAVES) void name(const sml_klora a) { lora_down_body<BF, RT>(a); }
+LORA_DOWN(0, 1, sml_sv_lora_down_t1)
+LORA_DOWN(1, 1, sml_sv_lora_down_t1_bf)
+LORA_DOWN(0, 4, sml_sv_lora_down_t4)
+LORA_DOWN(1, 4, sml_sv_lora_down_t4_bf)
+#define LORA_UP(BF, RB, OT, name) \
+    extern "C" __global__ __launch_bounds__(256) void name(const sml_klora a) { lora_up_body<BF, RB, OT>(a); }
+LORA_UP(0, 1, 1, sml_sv_lora_up_b1)
+LORA_UP(1, 1, 1, sml_sv_lora_up_b1_bf)
+LORA_UP(0, 4, 2, sml_sv_lora_up_b4)
+LORA_UP(1, 4, 2, sml_sv_lora_up_b4_bf)
