@@ -82,7 +82,7 @@ int sml_hip_paged_attention(const sml_hip_pages * pg, const float * q, size_t q_
 typedef struct {
     // the row's tokens so far: ids hist[hist_start[b] .. hist_start[b+1]), the
     // first n_prompt[b] of them (NULL: none) its prompt, the rest generated
-    const int32_t * hist;         // [n_hist]
+    const int32_t * hist;         // [n_hist], at most 2^30
     const int32_t * hist_start;   // [n_row + 1], clamped to 0..n_hist
     const int32_t * n_prompt;     // [n_row]
     int n_hist;
@@ -92,7 +92,7 @@ typedef struct {
     const float * rep, * presence, * frequency;
     // then bias[i] is added to token bias_id[i], i in bias_start[b] ..
     // bias_start[b+1]; of a token listed twice the last entry counts
-    const int32_t * bias_id;      // [n_bias]
+    const int32_t * bias_id;      // [n_bias], at most 2^30
     const float * bias;
     const int32_t * bias_start;   // [n_row + 1], clamped to 0..n_bias
     int n_bias;

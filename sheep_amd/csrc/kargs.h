@@ -495,6 +495,7 @@ typedef struct {
     int nsplit, chunk;            // positions [i * chunk, (i + 1) * chunk) of split i
 } sml_kattend;
 
+#define LG_RANGE 2048             // tokens of a row a workgroup takes
 typedef struct {
     const float * logits;
     float * out;
@@ -505,11 +506,21 @@ typedef struct {
     const float * bias;
     const uint32_t * mask;
     const int32_t * mask_row;
-    int4 * part;                  // per row and block: max, its index, first permitted index, whether that is NaN
+    int4 * part;                  // per row and block: max, its index, twice the first permitted index (+ 1: it is NaN)
     int32_t * tok;
     int n_hist, n_bias, n_mask, n_vocab, n_part;
 } sml_klogits;
 
+#define LD_WAVES 8                // waves of a workgroup of A x
+#define LD_TILE (LD_WAVES * 64)   // inputs they take at once
+#define LD_ROW 144                // bytes of 64 16-bit values in LDS: 16 rows fall on different banks
+#define LF_WAVES 16               // waves of the one launch of a few rows
+#define LF_OUT (16 * LF_WAVES)    // outputs of its workgroup
+#define LF_RANK 64                // its highest rank
+#define LF_LD (LF_RANK + 16)      // values of a row of t's parts in LDS
+#define LF_SLICE 512              // inputs of a wave's round (8 ranks)
+#define LU_OUT 64                 // outputs of a wave's block of y
+#define LD_WAVE_LDS(parts) ((64 + 16 * (parts)) * LD_ROW + 64)
 typedef struct {
     const uint16_t * a, * b;
     const float * scale;

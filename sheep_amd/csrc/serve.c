@@ -120,11 +120,9 @@ int sml_hip_paged_attention(const sml_hip_pages * pg, const float * q, size_t q_
     return 0;
 }
 
-#define LG_RANGE 4096
-
 size_t sml_hip_logits_part_bytes(int n_row, int n_vocab) {
     if (n_row < 1 || n_vocab < 1) return 0;
-    return (size_t) n_row * (size_t) ceil_div(n_vocab, 2048) * 16;
+    return (size_t) n_row * (size_t) ceil_div(n_vocab, LG_RANGE) * sizeof(int4);
 }
 
 int sml_hip_logits_adjust(const float * logits, size_t stride, int n_row, int n_vocab, const sml_hip_rules * rules,
@@ -144,7 +142,7 @@ int sml_hip_logits_adjust(const float * logits, size_t stride, int n_row, int n_
     if (tok && ((uintptr_t) part & 15u)) hx_failf("logits: workspace off a 16-byte boundary");
     if (rules) {
         const sml_hip_rules * r = rules;
-        if (r->n_hist < 0 || r->n_bias < 0 || r->n_mask < 0)
+        if (r->n_hist < 0 || r->n_hist > 1 << 30 || r->n_bias < 0 || r->n_bias > 1 << 30 || r->n_mask < 0)
             hx_failf("logits: %d ids, %d biases, %d masks", r->n_hist, r->n_bias, r->n_mask);
         if (r->hist && r->n_hist && (r->rep || r->presence || r->frequency)) {
             if (!r->hist_start) hx_failf("logits: a history without hist_start");
@@ -163,7 +161,11 @@ int sml_hip_logits_adjust(const float * logits, size_t stride, int n_row, int n_
     on_device();
     if (n_row) {
         a.n_part = ceil_div(n_vocab, LG_RANGE);
-        hx_launch("sml_sv_logits", (unsigned) a.n_part, (unsigned) n_row, 256, 0, (hipStream_t) stream, &a);
+        // one word a thread while the workgroups are at most 4 a CU (a call of
+        // latencies), else half the threads with two (measured beside the kernel)
+        const int wide = (long) a.n_part * n_row <= 4L * hx.ncu;
+        hx_launch(wide ? "sml_sv_logits_512_1" : "sml_sv_logits_256_2", (unsigned) a.n_part, (unsigned) n_row,
+                  wide ? 512 : 256, 0, (hipStream_t) stream, &a);
         if (tok) hx_launch("sml_sv_pick", (unsigned) n_row, 1, 64, 0, (hipStream_t) stream, &a);
     }
     HX_LEAVE();
@@ -176,32 +178,47 @@ size_t sml_hip_lora_work_floats(int rank, int n_row) {
     return (size_t) rank * (split > (size_t) n_row ? split : (size_t) n_row);
 }
 
-// Inputs a workgroup of the first product takes at once, and the rows of its tile.
-#define LD_TILE 1024
-#define LD_ROWS 16
+#define LD_ROWS 16                                    // rows of a tile
 
+// One launch or two, as measured beside the kernels. One: up to 16 rows of rank
+// up to 64, at most 16 row products a wave and 256 workgroups, and sums that
+// fit LDS.
 static void lora_launch(sml_klora * a, int bf, hipStream_t st) {
-    char name[40];
-    // the inputs split LD_TILE apiece, less finely where the rows give 256
-    // workgroups already or the workspace holds no more
-    const int ntile = ceil_div(a->n_row, LD_ROWS);
+    const int parts = bf ? 3 : 2, nslice = ceil_div(a->n_in, LF_SLICE), few = a->n_row < 16 ? a->n_row : 16;
+    const size_t sums = (size_t) nslice * 16 * (size_t) a->rank * 4;
+    if (a->n_row <= 16 && a->rank <= LF_RANK && sums <= 96 << 10 &&
+        (long) a->n_row * ceil_div(nslice * (a->rank / 8), LF_WAVES) <= 16 && (long) ceil_div(a->n_out, LF_OUT) * few <= 256) {
+        hx_launch(bf ? "sml_sv_lora_few_bf" : "sml_sv_lora_few", (unsigned) ceil_div(a->n_out, LF_OUT), (unsigned) few,
+                  64 * LF_WAVES, (size_t) parts * 16 * LF_LD * 2 + 64 + sums, st, a);
+        return;
+    }
+    // workgroups share a tile's distinct adapters while there are few tiles (16
+    // rows of 16 adapters, 4096 to 14336, rank 16: 35 us with 1, 19 with 4, 21
+    // with 16; 128 rows: 40, 49 and 106)
+    const int nz = a->n_row <= 32 ? (few < 4 ? few : 4) : a->n_row <= 64 ? 2 : 1;
+    // t: the inputs split for 128 workgroups, as far as the workspace holds
+    // them (509 rows, rank 64, bf16: 8.0 us and 18.0 for y at 4 splits, 6.6 and
+    // 20.8 at 8: every workgroup of y joins them)
+    const int ntile = ceil_div(a->n_row, LD_ROWS), ngroup = ceil_div(a->rank, 64);
     int most = 8192 / a->n_row < 32 ? 8192 / a->n_row : 32;
-    if (most > ceil_div(256, ntile)) most = ceil_div(256, ntile);
+    const int want = ceil_div(128, ntile * ngroup);
+    if (most > want) most = want;
     if (most < 1) most = 1;
     a->chunk = LD_TILE;
     while (ceil_div(a->n_in, a->chunk) > most) a->chunk += LD_TILE;
     a->nsplit = ceil_div(a->n_in, a->chunk);
-    // a tile's distinct adapters side by side for a step's few rows; the rows
-    // of prompts come in runs, a tile mostly of one
-    const int few = a->n_row <= 128, nz = !few ? 1 : a->n_row < 16 ? a->n_row : 16;
-    const int rt = a->rank <= 16 ? 1 : 4, ngroup = ceil_div(a->rank, 16 * rt);
-    snprintf(name, sizeof name, "sml_sv_lora_down_t%d%s", rt, bf ? "_bf" : "");
-    hx_launch3(name, (unsigned) ntile, (unsigned) a->nsplit, (unsigned) (nz * ngroup), 512, 0, st, a);
-    const int rb = few ? 1 : 4, ot = few ? 1 : 2;
-    snprintf(name, sizeof name, "sml_sv_lora_up_b%d%s", rb, bf ? "_bf" : "");
-    const size_t lds = (size_t) (bf ? 3 : 2) * 16 * rb * (size_t) (a->rank + 8) * 2 + (size_t) 16 * rb * 4;
-    hx_launch3(name, (unsigned) ceil_div(a->n_out, 64 * ot), (unsigned) ceil_div(a->n_row, 16 * rb), (unsigned) nz, 256,
-               lds, st, a);
+    hx_launch3(bf ? "sml_sv_lora_down_bf" : "sml_sv_lora_down", (unsigned) a->nsplit, (unsigned) ntile,
+               (unsigned) (nz * ngroup), 64 * LD_WAVES, (size_t) LD_WAVES * LD_WAVE_LDS(parts), st, a);
+    // y: 32 rows a workgroup of a prompt, and about 512 workgroups (the same
+    // case, 256 / 512 / 1024: 22 / 18 / 24 us; 16 rows: 22 / 18 / 23)
+    const int rb = a->n_row <= 128 ? 1 : 2, nrt = ceil_div(a->n_row, 16 * rb);
+    int gx = (512 / nrt + 7) / 8 * 8;
+    if (gx > ceil_div(a->n_out, 4 * LU_OUT)) gx = ceil_div(a->n_out, 4 * LU_OUT);
+    if (gx < 1) gx = 1;
+    const size_t lds = (size_t) 4 * LU_OUT * LD_ROW + (size_t) 16 * rb * (4 + (size_t) parts * ((size_t) ngroup * 64 + 8) * 2);
+    char name[40];
+    snprintf(name, sizeof name, "sml_sv_lora_up%d%s", rb, bf ? "_bf" : "");
+    hx_launch3(name, (unsigned) gx, (unsigned) nrt, (unsigned) nz, 256, lds, st, a);
 }
 
 int sml_hip_lora_add(const sml_hip_adapters * ad, const float * x, size_t x_stride, int n_row, const int32_t * adapter,

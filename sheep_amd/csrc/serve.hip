@@ -133,14 +133,19 @@ __device__ __forceinline__ int scale_of(float mx) {
     return mx > 0.0f && mx < INFINITY ? __builtin_amdgcn_frexp_expf(mx) - 11 : 0;
 }
 
-// element e of the parts of x: each part the rounding of what is left
+// Elements e and e + 1 of the parts of x and y: each part the rounding of what
+// is left, which the subtraction leaves exactly.
 template <int BF>
-__device__ __forceinline__ void parts_of(float x, typename Mx<BF>::v8 (&p)[Mx<BF>::parts], int e) {
+__device__ __forceinline__ void parts_of(float x, float y, typename Mx<BF>::v8 (&p)[Mx<BF>::parts], int e) {
+    typedef typename Mx<BF>::t v2t __attribute__((ext_vector_type(2)));
+    typedef float v2f __attribute__((ext_vector_type(2)));
     #pragma unroll
     for (int k = 0; k < Mx<BF>::parts; k++) {
-        const typename Mx<BF>::t h = (typename Mx<BF>::t) x;
-        p[k][e] = h;
-        x -= (float) h;
+        const v2t h = __builtin_convertvector(v2f{x, y}, v2t);
+        p[k][e] = h[0];
+        p[k][e + 1] = h[1];
+        x = __builtin_fmaf((float) h[0], -1.0f, x);
+        y = __builtin_fmaf((float) h[1], -1.0f, y);
     }
 }
 
@@ -179,7 +184,8 @@ __device__ __forceinline__ void attend_body(const sml_kattend & a) {
         #pragma unroll
         for (int j = 0; j < NJ; j++)
             #pragma unroll
-            for (int e = 0; e < 8; e++) parts_of<BF>(__builtin_amdgcn_ldexpf(x[j][e], -ex), q[j], e);
+            for (int e = 0; e < 8; e += 2)
+                parts_of<BF>(__builtin_amdgcn_ldexpf(x[j][e], -ex), __builtin_amdgcn_ldexpf(x[j][e + 1], -ex), q[j], e);
         back = __builtin_amdgcn_ldexpf(a.scale, ex);
     }
 
@@ -285,10 +291,11 @@ __device__ __forceinline__ void attend_body(const sml_kattend & a) {
         #pragma unroll
         for (int h = 0; h < 2; h++)
             #pragma unroll
-            for (int r = 0; r < 4; r++) {
-                const float w = __builtin_amdgcn_exp2f(s[h][r] - bu);
-                l += w;
-                parts_of<BF>(w, p, 4 * h + r);
+            for (int r = 0; r < 4; r += 2) {
+                const float w0 = __builtin_amdgcn_exp2f(s[h][r] - bu), w1 = __builtin_amdgcn_exp2f(s[h][r + 1] - bu);
+                l += w0;
+                l += w1;
+                parts_of<BF>(w0, w1, p, 4 * h + r);
             }
         #pragma unroll
         for (int u = 0; u < E; u++) {
@@ -388,352 +395,680 @@ ATTEND(64, 1, sml_sv_attend_d64_bf)
 
 // ---------------------------------------------------------------- logits
 //
-// A workgroup takes LG_RANGE tokens of a row. It counts the row's history and
+// A workgroup takes LG_RANGE tokens of a row, K words of four a thread. Its
+// logits and mask bits are on their way while it counts the row's history and
 // finds the biases of its own tokens in LDS (whole numbers, so the order of
-// the atomics does not show), then applies the rules to its logits in the
-// order the header gives, with no contraction, and keeps the greedy pick's
-// candidate.
-#define LG_RANGE 4096
+// the atomics does not show); then the rules are applied in the order the
+// header gives, with no contraction, and the greedy pick's candidate is kept.
+// The logits, read and written once, bound the large calls; every workgroup
+// reads its row's whole history, which stays in L2. A small call is a chain of
+// latencies (the list's bounds, the list, LDS, the biases), and its code's own
+// loading counts: the listed tokens go through one copy of the rules (one
+// division), not sixteen unrolled (1 row of 128256: 10.3 us so, 6.0 with).
+//
+// us a call with the pick, 512 threads of one word / 256 of two (128256 tokens,
+// histories of 2047): 1 row 8.8 / 9.8, 16 rows 11.4 / 11.4, 96 rows 34.6 / 28.3
+// (the last 3.5 TB/s); histories of 65536: 1 row 19.4 / 30.2, 96 rows 58 / 58.
+// 4096 tokens a workgroup: 96 rows 30.5 at best.
 #define LG_SEEN 0x80000000u
 
 __device__ __forceinline__ void amax_take(float v, int i, float & bv, int & bi) {
     if (v > bv || (v == bv && i < bi)) { bv = v; bi = i; }
 }
+// The better of two candidates over all lanes of a wave; first is twice the
+// first permitted index, plus 1 if its value is NaN.
+__device__ __forceinline__ void pick_wave(float & bv, int & bi, unsigned & first) {
+    #pragma unroll
+    for (int o = 32; o; o >>= 1) {
+        const float ov = __shfl_xor(bv, o);
+        const int oi = __shfl_xor(bi, o);
+        amax_take(ov, oi, bv, bi);
+        first = min(first, (unsigned) __shfl_xor((int) first, o));
+    }
+}
+#define LG_NONE 0x7fffffff                            // no index
+#define LG_FIRST 0xffffffffu                          // nothing permitted
 
-extern "C" __global__ __launch_bounds__(256) void sml_sv_logits(const sml_klogits a) {
+__device__ __forceinline__ float pick4(v4f v, int e) { return e & 2 ? (e & 1 ? v[3] : v[2]) : (e & 1 ? v[1] : v[0]); }
+__device__ __forceinline__ unsigned pick4(v4u v, int e) { return e & 2 ? (e & 1 ? v[3] : v[2]) : (e & 1 ? v[1] : v[0]); }
+
+template <int NT, int K>
+__device__ __forceinline__ void logits_body(const sml_klogits & a) {
     #pragma clang fp contract(off)
-    __shared__ unsigned cnt[LG_RANGE];                // generated count, LG_SEEN if listed at all
-    __shared__ int bia[LG_RANGE];                     // the last bias entry's index + 1
-    __shared__ float bv_s[4];
-    __shared__ int bi_s[4], fi_s[4], fn_s[4];
+    static_assert(NT * K * 4 == LG_RANGE, "");
+    __shared__ __align__(16) unsigned cnt[LG_RANGE];     // generated count, LG_SEEN if listed at all
+    __shared__ __align__(16) unsigned bia[LG_RANGE];     // the last bias entry's index + 1
+    __shared__ float rv[NT / 64];
+    __shared__ int ri[NT / 64];
+    __shared__ unsigned rf[NT / 64];
     const int row = blockIdx.y, t0 = blockIdx.x * LG_RANGE, tid = threadIdx.x;
     const int nt = min(LG_RANGE, a.n_vocab - t0);
-    for (int i = tid; i < LG_RANGE; i += 256) { cnt[i] = 0; bia[i] = 0; }
-    __syncthreads();
+    const float * x = a.logits + (size_t) row * a.stride + t0;
+    const int mr = !a.mask ? -1 : a.mask_row ? a.mask_row[row] : row;
+    const bool none = mr < -1 || mr >= a.n_mask;      // a mask that is not there permits nothing
+    v4f l[K];
+    uint32_t ok[K];                                   // bits 0..3: permitted and inside the row
+    #pragma unroll
+    for (int i = 0; i < K; i++) {
+        const int j = 4 * (NT * i + tid);
+        l[i] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+        if (j + 4 <= nt) l[i] = *(const v4fu *) (x + j);
+        else
+            for (int e = 0; e < 3; e++) if (j + e < nt) l[i][e] = x[j + e];
+        ok[i] = j >= nt ? 0u : j + 4 <= nt ? 15u : (1u << (nt - j)) - 1u;
+        if (a.mask && mr != -1) {
+            uint32_t w = 0;
+            if (!none && j < nt) w = a.mask[(size_t) mr * ((a.n_vocab + 31) / 32) + ((t0 + j) >> 5)] >> (j & 31);
+            ok[i] &= w;
+        }
+    }
+    if (a.hist || a.bias) {
+        #pragma unroll
+        for (int i = 0; i < K; i++) {
+            if (a.hist) *(v4u *) (cnt + 4 * (NT * i + tid)) = v4u(0u);
+            if (a.bias) *(v4u *) (bia + 4 * (NT * i + tid)) = v4u(0u);
+        }
+        __syncthreads();
+    }
     if (a.hist) {
         const int h0 = min(max(a.hist_start[row], 0), a.n_hist), h1 = min(max(a.hist_start[row + 1], 0), a.n_hist);
-        const int np = a.n_prompt ? a.n_prompt[row] : 0;
-        for (int i = h0 + tid; i < h1; i += 256) {
-            const int t = a.hist[i];
-            if (t < t0 || t - t0 >= nt) continue;
-            if (i - h0 >= np) atomicAdd(&cnt[t - t0], 1u);
-            atomicOr(&cnt[t - t0], LG_SEEN);
+        const int gen = h0 + (a.n_prompt ? min(max(a.n_prompt[row], 0), max(h1 - h0, 0)) : 0);
+        // four ids a thread in flight
+        for (int i = h0 + tid; i < h1; i += 4 * NT) {
+            int t[4];
+            #pragma unroll
+            for (int k = 0; k < 4; k++) t[k] = a.hist[min(i + k * NT, h1 - 1)] - t0;
+            #pragma unroll
+            for (int k = 0; k < 4; k++)
+                if (i + k * NT < h1 && (unsigned) t[k] < (unsigned) nt) {
+                    if (i + k * NT >= gen) atomicAdd(&cnt[t[k]], 1u);
+                    atomicOr(&cnt[t[k]], LG_SEEN);
+                }
         }
     }
     if (a.bias) {
         const int b0 = min(max(a.bias_start[row], 0), a.n_bias), b1 = min(max(a.bias_start[row + 1], 0), a.n_bias);
-        for (int i = b0 + tid; i < b1; i += 256) {
-            const int t = a.bias_id[i];
-            if (t >= t0 && t - t0 < nt) atomicMax(&bia[t - t0], i + 1);
+        for (int i = b0 + tid; i < b1; i += NT) {
+            const int t = a.bias_id[i] - t0;
+            if ((unsigned) t < (unsigned) nt) atomicMax(&bia[t], (unsigned) i + 1);
         }
     }
-    __syncthreads();
     const float rep = a.rep ? a.rep[row] : 1.0f, fr = a.frequency ? a.frequency[row] : 0.0f,
                 pr = a.presence ? a.presence[row] : 0.0f;
-    const int mr = !a.mask ? -1 : a.mask_row ? a.mask_row[row] : row;
-    const bool none = mr < -1 || mr >= a.n_mask;
-    const uint32_t * mask = mr < 0 || none ? nullptr : a.mask + (size_t) mr * ((a.n_vocab + 31) / 32);
+    if (a.hist || a.bias) __syncthreads();
     float bv = -INFINITY;
-    int bi = 0x7fffffff, fi = 0x7fffffff, fn = 0;
-    for (int j = tid; j < nt; j += 256) {
-        const int t = t0 + j;
-        float l = a.logits[(size_t) row * a.stride + t];
-        const unsigned c = cnt[j];
-        if (c) {
-            if (a.rep) l = l > 0.0f ? l / rep : l * rep;
-            if (c & ~LG_SEEN) {
-                if (a.frequency) l = l - fr * (float) (c & ~LG_SEEN);
-                if (a.presence) l = l - pr;
-            }
+    int bi = LG_NONE;
+    unsigned first = LG_FIRST;
+    #pragma unroll
+    for (int i = 0; i < K; i++) {
+        const int j = 4 * (NT * i + tid);
+        v4u c = v4u(0u), k = v4u(0u);
+        if (a.hist) c = *(const v4u *) (cnt + j);
+        if (a.bias) k = *(const v4u *) (bia + j);
+        // the few listed tokens one by one: one copy of the division
+        unsigned todo = (c[0] | k[0] ? 1u : 0u) | (c[1] | k[1] ? 2u : 0u) | (c[2] | k[2] ? 4u : 0u) | (c[3] | k[3] ? 8u : 0u);
+        while (todo) {
+            const int e = __builtin_ctz(todo);
+            todo &= todo - 1;
+            float v = pick4(l[i], e);
+            const unsigned ce = pick4(c, e), m = ce & ~LG_SEEN, ke = pick4(k, e);
+            if (ce && a.rep) v = v > 0.0f ? v / rep : v * rep;
+            if (m && a.frequency) v = v - fr * (float) m;
+            if (m && a.presence) v = v - pr;
+            if (ke) v = v + a.bias[ke - 1];
+            #pragma unroll
+            for (int f = 0; f < 4; f++) l[i][f] = e == f ? v : l[i][f];
         }
-        if (bia[j]) l = l + a.bias[bia[j] - 1];
-        const bool ok = a.mask == nullptr || mr == -1 || (mask && (mask[t >> 5] >> (t & 31) & 1));
-        if (a.out) a.out[(size_t) row * a.out_stride + t] = ok ? l : -INFINITY;
-        if (ok) {
-            if (fi == 0x7fffffff) { fi = t; fn = l != l; }
-            amax_take(l, t, bv, bi);
+        ok[i] &= 15u;
+        if (ok[i] && first == LG_FIRST) {
+            const int e = __builtin_ctz(ok[i]);
+            const float v = pick4(l[i], e);
+            first = 2u * (unsigned) (t0 + j + e) + (v != v);
+        }
+        #pragma unroll
+        for (int e = 0; e < 4; e++) {
+            l[i][e] = ok[i] >> e & 1 ? l[i][e] : -INFINITY;
+            amax_take(l[i][e], ok[i] >> e & 1 ? t0 + j + e : LG_NONE, bv, bi);
+        }
+        if (a.out) {
+            float * y = a.out + (size_t) row * a.out_stride + t0 + j;
+            if (j + 4 <= nt) *(v4fu *) y = l[i];
+            else
+                for (int e = 0; e < 3; e++) if (j + e < nt) y[e] = l[i][e];
         }
     }
     if (!a.tok) return;
-    #pragma unroll
-    for (int o = 32; o; o >>= 1) {
-        const float ov = __shfl_xor(bv, o);
-        const int oi = __shfl_xor(bi, o), of = __shfl_xor(fi, o), on = __shfl_xor(fn, o);
-        amax_take(ov, oi, bv, bi);
-        if (of < fi) { fi = of; fn = on; }
-    }
-    if ((tid & 63) == 0) { bv_s[tid >> 6] = bv; bi_s[tid >> 6] = bi; fi_s[tid >> 6] = fi; fn_s[tid >> 6] = fn; }
+    pick_wave(bv, bi, first);
+    if ((tid & 63) == 0) { rv[tid >> 6] = bv; ri[tid >> 6] = bi; rf[tid >> 6] = first; }
     __syncthreads();
-    if (tid) return;
-    for (int w = 1; w < 4; w++) {
-        amax_take(bv_s[w], bi_s[w], bv, bi);
-        if (fi_s[w] < fi) { fi = fi_s[w]; fn = fn_s[w]; }
-    }
-    a.part[(size_t) row * a.n_part + blockIdx.x] = make_int4(__float_as_int(bv), bi, fi, fn);
+    if (tid >= 64) return;
+    bv = tid < NT / 64 ? rv[tid] : -INFINITY;
+    bi = tid < NT / 64 ? ri[tid] : LG_NONE;
+    first = tid < NT / 64 ? rf[tid] : LG_FIRST;
+    pick_wave(bv, bi, first);
+    if (!tid) a.part[(size_t) row * a.n_part + blockIdx.x] = make_int4(__float_as_int(bv), bi, (int) first, 0);
 }
+#define LOGITS(NT, K) \
+    extern "C" __global__ __launch_bounds__(NT) void sml_sv_logits_##NT##_##K(const sml_klogits a) { logits_body<NT, K>(a); }
+LOGITS(512, 1)
+LOGITS(256, 2)
 
 // The pick over a row's blocks: the first permitted token if it is NaN (the
 // serial loop never leaves it), else the lowest index of the largest value.
 extern "C" __global__ __launch_bounds__(64) void sml_sv_pick(const sml_klogits a) {
     const int row = blockIdx.x;
     float bv = -INFINITY;
-    int bi = 0x7fffffff, fi = 0x7fffffff, fn = 0;
+    int bi = LG_NONE;
+    unsigned first = LG_FIRST;
     for (int i = threadIdx.x; i < a.n_part; i += 64) {
         const int4 p = a.part[(size_t) row * a.n_part + i];
         amax_take(__int_as_float(p.x), p.y, bv, bi);
-        if (p.z < fi) { fi = p.z; fn = p.w; }
+        first = min(first, (unsigned) p.z);
     }
-    #pragma unroll
-    for (int o = 32; o; o >>= 1) {
-        const float ov = __shfl_xor(bv, o);
-        const int oi = __shfl_xor(bi, o), of = __shfl_xor(fi, o), on = __shfl_xor(fn, o);
-        amax_take(ov, oi, bv, bi);
-        if (of < fi) { fi = of; fn = on; }
-    }
-    if (!threadIdx.x) a.tok[row] = fi == 0x7fffffff ? -1 : fn ? fi : bi;
+    pick_wave(bv, bi, first);
+    if (!threadIdx.x) a.tok[row] = first == LG_FIRST ? -1 : first & 1 ? (int) (first >> 1) : bi;
 }
 
 // ---------------------------------------------------------------- adapters
 //
-// y = base + scale B (A x), two launches: t = A x of every row under its own
-// adapter (split over the inputs, joined by the second launch's prologue), then
-// y. Rows come in tiles of 16, the matrix cores' columns: a workgroup takes the
-// distinct adapters among its tile's rows one by one, computes all columns
-// with each and stores those of its rows. Columns never mix, so a row sees
-// nothing of the others, and no sorting of requests is needed: requests that
-// share an adapter in a tile read it once, those that do not read each their
-// own, which is the least there is to read.
+// y = base + scale B (A x). Rows come in tiles of 16; a tile's distinct adapters
+// are taken one by one, all of its rows computed with each and those of the
+// adapter's own rows kept. Rows never mix in a product, so a row sees nothing
+// of the others, and no sorting of requests is needed: requests of a tile that
+// share an adapter read it once, those that do not read each their own, which
+// is the least there is to read.
 //
 // fp32 x and t meet the 16-bit matrices as parts of their type (fp16: two, and
 // each row scaled by a power of two to below 2^11 first; bf16: three), 22 or 24
 // bits, summed in fp32.
-#define LD_WAVES 8
-#define LD_STEPS 4                                    // inner products of 32 a wave holds at once
-#define LD_TILE (LD_WAVES * LD_STEPS * 32)            // inputs a workgroup takes at once
+//
+// A few rows take one launch (lora_few_body), others two: t = A x, split over
+// the inputs, then y, whose workgroups join the splits. us a call, one launch /
+// two (fp16; rows of so many adapters):
+//   rank 16, 4096 to 4096: 1 row 5.6 / 10.9, 4 of 4 6.0 / 11.7, 16 of 16 8.2 /
+//   13.5, 16 of one 15.6 / 11.5; 4096 to 14336: 4 of 4 6.2 / 11.6, 16 of 16
+//   27 / 19; 14336 to 4096: 1 row 9.0 / 12.6, 4 of one 15.1 / 13.2, 16 of one
+//   39 / 13.6; rank 64, 4096 to 14336: 1 row 10.7 / 12.9, 16 of 16 51 / 24.
+// So one launch pays while each of its workgroups has few rows' products to
+// make in its lanes (rows times rounds of its waves) and the workgroups, each
+// reading its adapter's A again, are at most one a CU.
 
 // The valid adapter id of a row, or -1.
 __device__ __forceinline__ int adapter_of(const sml_klora & a, int row) {
-    const int id = row < a.n_row ? a.adapter[row] : -1;
-    return id >= 0 && id < a.n_adapter ? id : -1;
+    const int id = a.adapter[min(row, a.n_row - 1)];
+    return row < a.n_row && id >= 0 && id < a.n_adapter ? id : -1;
 }
 __device__ __forceinline__ int rank_of(const sml_klora & a, int id) {
     return a.ranks ? min(max(a.ranks[id], 0), a.rank) : a.rank;
 }
 
-template <int BF, int RT>
+// The rows of a tile (bits of valid, id: the lane's) whose adapter is the z-th,
+// z + nz-th, ... distinct one.
+__device__ __forceinline__ unsigned long long my_rows(int id, unsigned long long valid, int z, int nz) {
+    if (nz == 1) return valid;
+    unsigned long long mine = 0;
+    for (int k = 0; valid; k++) {
+        const unsigned long long m = __ballot(id == __builtin_amdgcn_readlane(id, __builtin_ctzll(valid))) & valid;
+        if (k % nz == z) mine |= m;
+        valid &= ~m;
+    }
+    return mine;
+}
+
+// What a wave's lanes wrote to its own part of LDS is there for all of them.
+__device__ __forceinline__ void wave_lds() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// A x: a workgroup takes a tile of 16 rows, 64 ranks and a split of the inputs,
+// a wave every eighth 64 of those. The matrix cores want 16 rows in 16
+// consecutive lanes, and loads in that order cost a cache line a lane (16
+// bytes a cycle and CU measured): rows are loaded whole, 128 or 256 bytes in
+// consecutive lanes, and handed over through the wave's part of LDS, at a
+// stride of LD_ROW bytes that spreads 16 rows over all banks.
+template <int BF>
 __device__ __forceinline__ void lora_down_body(const sml_klora & a) {
     using M = Mx<BF>;
     typedef typename M::v8 v8;
-    __shared__ float red[LD_WAVES][16][16 * RT + 1];
-    const int row0 = blockIdx.x * 16, split = blockIdx.y, tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
+    typedef typename M::t T;
+    typedef T v4t __attribute__((ext_vector_type(4)));
+    constexpr int NP = M::parts, RT = 4, RS = 16 * RT + 1;
+    extern __shared__ __align__(16) uint8_t lds[];
+    const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int ngroup = (a.rank + 16 * RT - 1) / (16 * RT), nz = gridDim.z / ngroup;
-    const int j0 = (blockIdx.z % ngroup) * 16 * RT, z = blockIdx.z / ngroup;
+    uint8_t * const la = lds + wave * LD_WAVE_LDS(NP);              // [rank][LD_ROW]
+    uint8_t * const lx = la + 64 * LD_ROW;                          // [part][row][LD_ROW]
+    int * const le = (int *) (lx + NP * 16 * LD_ROW);               // [row]
+    const int split = blockIdx.x, row0 = blockIdx.y * 16, ngroup = (a.rank + 63) / 64, nz = gridDim.z / ngroup;
+    const int j0 = (blockIdx.z % ngroup) * 64, z = blockIdx.z / ngroup;
     const int k0 = split * a.chunk, k1 = min(a.n_in, k0 + a.chunk);
-    const int id = adapter_of(a, row0 + c);
-    const float * x = a.x + (size_t) min(row0 + c, a.n_row - 1) * a.x_stride;
+    const int id = adapter_of(a, row0 + c), nt = min(RT, (a.rank - j0 + 15) / 16);
+    const unsigned all = (unsigned) my_rows(id, (unsigned) (__ballot(id >= 0) & 0xFFFFu), z, nz);
+    if (!all) return;
+    const int first = __builtin_amdgcn_readlane(id, __builtin_ctz(all));
 
-    unsigned left = (unsigned) (__ballot(id >= 0) & 0xFFFFu);
-    for (int k = 0; left; k++) {
-        const int cur = __builtin_amdgcn_readlane(id, __builtin_ctz(left));
-        const unsigned mine = (unsigned) (__ballot(id == cur) & 0xFFFFu);
-        left &= ~mine;
-        if (k % nz != z) continue;
-        const int rk = rank_of(a, cur);
-        if (j0 >= rk) continue;
-        const int nt = min(RT, (rk - j0 + 15) / 16);
-        const uint16_t * w = a.a + (size_t) cur * a.rank * a.n_in;
-        v4f tot[RT];
+    v4f xr[4];
+    v4u ar[8], an[8];
+    auto load_x = [&](int kb) {
+        const int kk = min(kb + 4 * c, k1 - 4);
         #pragma unroll
-        for (int t = 0; t < RT; t++) tot[t] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-        for (int kb = k0 + wave * 32 * LD_STEPS; kb < k1; kb += LD_TILE) {
-            float xv[LD_STEPS][8], mx = 0.0f;
-            v4u wv[RT][LD_STEPS];
-            #pragma unroll
-            for (int s = 0; s < LD_STEPS; s++) {
-                const int kk = kb + 32 * s + 8 * g;
+        for (int i = 0; i < 4; i++) xr[i] = *(const GLOBAL v4fu *) (a.x + (size_t) min(row0 + 4 * i + g, a.n_row - 1) * a.x_stride + kk);
+    };
+    auto load_a = [&](v4u (&r)[8], int ad, int kb) {
+        const int kk = min(kb + 8 * (lane & 7), k1 - 8);
+        const uint16_t * w = a.a + (size_t) ad * a.rank * a.n_in + kk;
+        #pragma unroll
+        for (int i = 0; i < 8; i++)
+            if (i < 2 * nt) r[i] = *(const GLOBAL v4u *) (w + (size_t) min(j0 + 8 * i + (lane >> 3), a.rank - 1) * a.n_in);
+    };
+    v4f tot[RT];
+    #pragma unroll
+    for (int t = 0; t < RT; t++) tot[t] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+    int kb = k0 + wave * 64;
+    if (kb < k1) { load_x(kb); load_a(ar, first, kb); }
+    for (; kb < k1; kb += 64 * LD_WAVES) {
+        // x's parts, each row scaled for fp16: 16 lanes a row
+        #pragma unroll
+        for (int i = 0; i < 4; i++) {
+            if (kb + 4 * c >= k1) xr[i] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+            int ex = 0;
+            if constexpr (!BF) {
+                ex = scale_of(max16(fmaxf(fmaxf(fabsf(xr[i][0]), fabsf(xr[i][1])), fmaxf(fabsf(xr[i][2]), fabsf(xr[i][3])))));
                 #pragma unroll
-                for (int e = 0; e < 8; e += 4) {
-                    const v4f v = *(const GLOBAL v4fu *) (x + (kk < k1 ? kk + e : 0));
-                    #pragma unroll
-                    for (int i = 0; i < 4; i++) xv[s][e + i] = kk < k1 ? v[i] : 0.0f;
-                }
+                for (int e = 0; e < 4; e++) xr[i][e] = __builtin_amdgcn_ldexpf(xr[i][e], -ex);
+                if (!c) le[4 * i + g] = ex;
             }
+            v8 p[NP];
+            parts_of<BF>(xr[i][0], xr[i][1], p, 0);
+            parts_of<BF>(xr[i][2], xr[i][3], p, 2);
             #pragma unroll
-            for (int t = 0; t < RT; t++)
-                if (t < nt) {
-                    const uint16_t * wr = w + (size_t) min(j0 + 16 * t + c, rk - 1) * a.n_in;
-                    #pragma unroll
-                    for (int s = 0; s < LD_STEPS; s++) {
-                        const int kk = kb + 32 * s + 8 * g;
-                        wv[t][s] = *(const GLOBAL v4u *) (wr + (kk < k1 ? kk : 0));
-                        if (kk >= k1) wv[t][s] = v4u(0u);
-                    }
+            for (int k = 0; k < NP; k++)
+                *(v4t *) (lx + (k * 16 + 4 * i + g) * LD_ROW + 8 * c) = __builtin_shufflevector(p[k], p[k], 0, 1, 2, 3);
+        }
+        const int kn = kb + 64 * LD_WAVES;
+        if (kn < k1) load_x(kn);
+        // the tile's adapters one by one: each one's rows keep its products
+        unsigned left = all;
+        for (int cur = first; left;) {
+            #pragma unroll
+            for (int i = 0; i < 8; i++)
+                if (i < 2 * nt) {
+                    if (kb + 8 * (lane & 7) >= k1) ar[i] = v4u(0u);
+                    *(v4u *) (la + (8 * i + (lane >> 3)) * LD_ROW + 16 * (lane & 7)) = ar[i];
                 }
+            wave_lds();
+            const bool mine = id == cur;
+            left &= ~(unsigned) __ballot(mine);
+            const int then = left ? __builtin_amdgcn_readlane(id, __builtin_ctz(left)) : first;
+            if (left || kn < k1) load_a(an, then, left ? kb : kn);
+            const int ex = BF ? 0 : le[c];
+            v8 xp[2][NP];
             #pragma unroll
-            for (int s = 0; s < LD_STEPS; s++)
+            for (int s = 0; s < 2; s++)
                 #pragma unroll
-                for (int e = 0; e < 8; e++) mx = fmaxf(mx, fabsf(xv[s][e]));
-            mx = fmaxf(mx, __shfl_xor(mx, 16));
-            mx = fmaxf(mx, __shfl_xor(mx, 32));
-            const int ex = BF ? 0 : scale_of(mx);
-            v8 p[LD_STEPS][M::parts];
-            #pragma unroll
-            for (int s = 0; s < LD_STEPS; s++)
-                #pragma unroll
-                for (int e = 0; e < 8; e++) parts_of<BF>(__builtin_amdgcn_ldexpf(xv[s][e], -ex), p[s], e);
+                for (int i = 0; i < NP; i++) xp[s][i] = *(const v8 *) (lx + (i * 16 + c) * LD_ROW + 64 * s + 16 * g);
             #pragma unroll
             for (int t = 0; t < RT; t++)
                 if (t < nt) {
                     v4f acc = v4f{0.0f, 0.0f, 0.0f, 0.0f};
                     #pragma unroll
-                    for (int s = 0; s < LD_STEPS; s++)
+                    for (int s = 0; s < 2; s++) {
+                        const v8 w = *(const v8 *) (la + (16 * t + c) * LD_ROW + 64 * s + 16 * g);
                         #pragma unroll
-                        for (int i = 0; i < M::parts; i++) acc = M::mul(__builtin_bit_cast(v8, wv[t][s]), p[s][i], acc);
+                        for (int i = 0; i < NP; i++) acc = M::mul(w, xp[s][i], acc);
+                    }
                     #pragma unroll
-                    for (int r = 0; r < 4; r++) tot[t][r] += __builtin_amdgcn_ldexpf(acc[r], ex);
+                    for (int r = 0; r < 4; r++) tot[t][r] += mine ? __builtin_amdgcn_ldexpf(acc[r], ex) : 0.0f;
                 }
+            wave_lds();                               // all read before the next is written
+            cur = then;
+            #pragma unroll
+            for (int i = 0; i < 8; i++) ar[i] = an[i];
         }
+    }
+    __syncthreads();                                  // the waves' parts become one
+    float * const red = (float *) lds;                // [wave][row][RS]
+    #pragma unroll
+    for (int t = 0; t < RT; t++)
         #pragma unroll
-        for (int t = 0; t < RT; t++)
-            #pragma unroll
-            for (int r = 0; r < 4; r++) red[wave][c][16 * t + 4 * g + r] = tot[t][r];
-        __syncthreads();
-        for (int i = tid; i < 256 * RT; i += 64 * LD_WAVES) {
-            const int rw = i / (16 * RT), j = i % (16 * RT);
-            float s = 0.0f;
-            #pragma unroll
-            for (int v = 0; v < LD_WAVES; v++) s += red[v][rw][j];
-            if ((mine >> rw & 1) && j0 + j < rk)
-                a.work[((size_t) (row0 + rw) * a.nsplit + split) * a.rank + j0 + j] = s;
-        }
-        __syncthreads();
+        for (int r = 0; r < 4; r++) red[(wave * 16 + c) * RS + 16 * t + 4 * g + r] = tot[t][r];
+    __syncthreads();
+    for (int i = tid; i < 256 * RT; i += 64 * LD_WAVES) {
+        const int rw = i / (16 * RT), j = i % (16 * RT);
+        float s = 0.0f;
+        #pragma unroll
+        for (int v = 0; v < LD_WAVES; v++) s += red[(v * 16 + rw) * RS + j];
+        if ((all >> rw & 1) && j0 + j < a.rank)
+            a.work[((size_t) (row0 + rw) * a.nsplit + split) * a.rank + j0 + j] = s;
     }
 }
 
-// RB tiles of 16 rows and 4 waves of OT tiles of 16 outputs a workgroup.
-template <int BF, int RB, int OT>
-__device__ __forceinline__ void lora_up_body(const sml_klora & a) {
+// Both products of up to 16 rows in one launch: a workgroup of 16 waves computes
+// t of one adapter's rows (all of n_in, the waves sharing it), then 256 outputs
+// of theirs. Each workgroup reads its adapter's whole A again, from L2: less
+// than a second launch costs while A is small. A step holds a row or two of an
+// adapter, too few for the matrix cores' 16 columns (converting all 16 made
+// this 12.6 us for 8.5): the first product is a lane's own fused multiply-adds
+// on 8 inputs of 8 ranks at a time, summed over the wave by halves.
+template <int BF>
+__device__ __forceinline__ void lora_few_body(const sml_klora & a) {
     using M = Mx<BF>;
     typedef typename M::v8 v8;
     typedef typename M::t T;
+    constexpr int NP = M::parts, LD = LF_LD;
     extern __shared__ __align__(16) uint8_t lds[];
-    constexpr int NR = 16 * RB, NP = M::parts;
-    const int ld = a.rank + 8;                        // values of a row of t's parts in LDS
-    T * const tp = (T *) lds;                         // [part][row][ld]
-    int * const ex_s = (int *) (lds + (size_t) NP * NR * ld * 2);
-    const int row0 = blockIdx.y * NR, tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), nz = gridDim.z, z = blockIdx.z;
-    const int o0 = (blockIdx.x * 4 + wave) * 16 * OT;
-
-    // t: the splits' sums, scaled, in parts; lr lanes of 4 values a row
-    {
-        int lr = 2;
-        while (4 * lr < a.rank) lr *= 2;
-        const int q = tid & (lr - 1), step = 256 / lr;
-        for (int r = tid / lr; r < NR; r += step) {
-            const int row = min(row0 + r, a.n_row - 1), id = adapter_of(a, row), rk = id < 0 ? 0 : rank_of(a, id);
-            const float sc = id < 0 ? 0.0f : a.scale ? a.scale[id] : 1.0f;
-            const float * t = a.work + (size_t) row * a.nsplit * a.rank + 4 * q;
-            v4f v = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-            if (4 * q < rk)
-                for (int s = 0; s < a.nsplit; s++) v += *(const v4fu *) (t + (size_t) s * a.rank);
-            float mx = 0.0f;
-            #pragma unroll
-            for (int e = 0; e < 4; e++) { v[e] = 4 * q + e < rk ? v[e] * sc : 0.0f; mx = fmaxf(mx, fabsf(v[e])); }
-            for (int o = 1; o < lr; o *= 2) mx = fmaxf(mx, __shfl_xor(mx, o));
-            const int ex = BF ? 0 : scale_of(mx);
-            if (4 * q < a.rank) {
-                v8 p[NP];
-                #pragma unroll
-                for (int e = 0; e < 4; e++) parts_of<BF>(__builtin_amdgcn_ldexpf(v[e], -ex), p, e);
-                #pragma unroll
-                for (int k = 0; k < NP; k++)
-                    #pragma unroll
-                    for (int e = 0; e < 4; e++) tp[((size_t) k * NR + r) * ld + 4 * q + e] = p[k][e];
-            }
-            if (!q) ex_s[r] = ex;
-        }
-    }
-    __syncthreads();
-    const int id = lane < NR ? adapter_of(a, row0 + lane) : -1;
-    unsigned long long left = __ballot(id >= 0), none = ~left;
-    for (int k = 0; left || none; k++) {
-        // the rows without an adapter are taken like those of one more
+    T * const tp = (T *) lds;                         // [part][row][LD]
+    int * const ex_s = (int *) (tp + NP * 16 * LD);   // [row]
+    float * const red = (float *) (ex_s + 16);        // [slice][row][rank]
+    const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), nz = gridDim.y, z = blockIdx.y;
+    const int o0 = blockIdx.x * LF_OUT + wave * 16, o = o0 + 4 * g, row = c;
+    const int id = adapter_of(a, row), nrg = a.rank / 8, nslice = (a.n_in + LF_SLICE - 1) / LF_SLICE;
+    const bool live = row < a.n_row;
+    v4f base = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+    if (a.base && live && o + 4 <= a.n_out) base = *(const v4fu *) (a.base + (size_t) row * a.y_stride + o);
+    unsigned left = (unsigned) (__ballot(id >= 0) & 0xFFFFu);
+    unsigned none = a.base == a.y ? 0u : (unsigned) (__ballot(id < 0 && live) & 0xFFFFu);
+    for (int k = 0; left | none; k++) {
         int cur = -1;
-        unsigned long long mine = none;
+        unsigned mine = none;
         if (left) {
-            cur = __builtin_amdgcn_readlane(id, __builtin_ctzll(left));
-            mine = __ballot(id == cur);
+            cur = __builtin_amdgcn_readlane(id, __builtin_ctz(left));
+            mine = (unsigned) (__ballot(id == cur) & 0xFFFFu);
             left &= ~mine;
         } else {
             none = 0;
         }
-        if (k % nz != z || (cur < 0 && a.base == a.y)) continue;
-        const int rk = cur < 0 ? 0 : rank_of(a, cur);
-        const uint16_t * w = a.b + (size_t) max(cur, 0) * a.n_out * a.rank;
-        v4f acc[RB][OT];
-        #pragma unroll
-        for (int b = 0; b < RB; b++)
+        if (k % nz != z) continue;
+        v4f acc = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+        int ex = 0;
+        if (cur >= 0) {
+            const int rk = rank_of(a, cur);
+            const uint16_t * wa = a.a + (size_t) cur * a.rank * a.n_in, * wb = a.b + (size_t) cur * a.n_out * a.rank;
+            v4u bw[2];
             #pragma unroll
-            for (int u = 0; u < OT; u++) acc[b][u] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-        for (int k0 = 0; k0 < rk; k0 += 32) {
-            const int kk = k0 + 8 * g, at = kk < a.rank ? kk : 0;
-            v4u wv[OT];
+            for (int s = 0; s < 2; s++) {
+                const int kk = 32 * s + 8 * g;
+                bw[s] = *(const GLOBAL v4u *) (wb + (size_t) min(o0 + c, a.n_out - 1) * a.rank + (kk < a.rank ? kk : 0));
+            }
+            for (int u = wave; u < nrg * nslice; u += LF_WAVES) {
+                const int slice = u / nrg, rg = u - slice * nrg, kk = LF_SLICE * slice + 8 * lane;
+                const bool in = kk < a.n_in;
+                v4u w[8];
+                #pragma unroll
+                for (int i = 0; i < 8; i++) w[i] = *(const GLOBAL v4u *) (wa + (size_t) (8 * rg + i) * a.n_in + (in ? kk : 0));
+                for (unsigned m = mine; m; m &= m - 1) {
+                    const int r = __builtin_ctz(m);
+                    const float * x = a.x + (size_t) r * a.x_stride + (in ? kk : 0);
+                    const v4f x0 = *(const GLOBAL v4fu *) x, x1 = *(const GLOBAL v4fu *) (x + 4);
+                    float t[8];
+                    #pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        const v8 h = __builtin_bit_cast(v8, w[i]);
+                        t[i] = 0.0f;
+                        #pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            t[i] = __builtin_fmaf((float) h[e], x0[e], t[i]);
+                            t[i] = __builtin_fmaf((float) h[e + 4], x1[e], t[i]);
+                        }
+                        if (!in) t[i] = 0.0f;
+                    }
+                    // 8 sums over 64 lanes: lane l ends with that of 4 l5 + 2 l4 + l3
+                    #pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const float s = lane & 32 ? t[i] : t[i + 4];
+                        t[i] = (lane & 32 ? t[i + 4] : t[i]) + __shfl_xor(s, 32);
+                    }
+                    #pragma unroll
+                    for (int i = 0; i < 2; i++) {
+                        const float s = lane & 16 ? t[i] : t[i + 2];
+                        t[i] = (lane & 16 ? t[i + 2] : t[i]) + __shfl_xor(s, 16);
+                    }
+                    const float s = lane & 8 ? t[0] : t[1];
+                    t[0] = (lane & 8 ? t[1] : t[0]) + __shfl_xor(s, 8);
+                    t[0] += dpp_f<0xB1>(t[0]); t[0] += dpp_f<0x4E>(t[0]); t[0] += dpp_f<0x141>(t[0]);
+                    if (!(lane & 7)) red[(slice * 16 + r) * a.rank + 8 * rg + (lane >> 3 & 1) + 2 * (lane >> 4 & 1) + 4 * (lane >> 5)] = t[0];
+                }
+            }
+            __syncthreads();
+            // wave w joins row w: lane j its rank j
+            if (mine >> wave & 1) {
+                float v = 0.0f;
+                if (lane < rk)
+                    for (int s = 0; s < nslice; s++) v += red[(s * 16 + wave) * a.rank + lane];
+                v *= a.scale ? a.scale[cur] : 1.0f;
+                const int et = BF ? 0 : scale_of(wave_max(fabsf(v)));
+                v8 p[NP];
+                parts_of<BF>(__builtin_amdgcn_ldexpf(v, -et), 0.0f, p, 0);
+                #pragma unroll
+                for (int i = 0; i < NP; i++) tp[(i * 16 + wave) * LD + lane] = p[i][0];
+                if (!lane) ex_s[wave] = et;
+            }
+            __syncthreads();
             #pragma unroll
-            for (int u = 0; u < OT; u++) {
-                wv[u] = *(const GLOBAL v4u *) (w + (size_t) min(o0 + 16 * u + c, a.n_out - 1) * a.rank + at);
-                if (k0 + 32 > rk) {
+            for (int s = 0; s < 2; s++)
+                if (32 * s < rk) {
+                    const int kk = 32 * s + 8 * g;
                     #pragma unroll
                     for (int i = 0; i < 4; i++) {
                         const int j = kk + 2 * i;
-                        wv[u][i] = j + 1 < rk ? wv[u][i] : j < rk ? wv[u][i] & 0xFFFFu : 0u;
+                        bw[s][i] = j + 1 < rk ? bw[s][i] : j < rk ? bw[s][i] & 0xFFFFu : 0u;
                     }
-                }
-            }
-            #pragma unroll
-            for (int b = 0; b < RB; b++)
-                #pragma unroll
-                for (int i = 0; i < NP; i++) {
-                    v8 tv = *(const v8 *) (tp + ((size_t) i * NR + 16 * b + c) * ld + at);
-                    if (kk >= a.rank) tv = __builtin_bit_cast(v8, v4u(0u));
                     #pragma unroll
-                    for (int u = 0; u < OT; u++) acc[b][u] = M::mul(__builtin_bit_cast(v8, wv[u]), tv, acc[b][u]);
+                    for (int i = 0; i < NP; i++)
+                        acc = M::mul(__builtin_bit_cast(v8, bw[s]), *(const v8 *) (tp + (i * 16 + c) * LD + kk), acc);
                 }
+            ex = ex_s[c];
+            __syncthreads();                          // red and tp are the next adapter's
         }
+        if (!(mine >> c & 1) || o >= a.n_out) continue;
+        float * y = a.y + (size_t) row * a.y_stride + o;
+        v4f d;
         #pragma unroll
-        for (int b = 0; b < RB; b++) {
-            const int row = row0 + 16 * b + c;
-            if (!(mine >> (16 * b + c) & 1) || row >= a.n_row) continue;
-            const int ex = ex_s[16 * b + c];
-            #pragma unroll
-            for (int u = 0; u < OT; u++) {
-                const int o = o0 + 16 * u + 4 * g;
-                const size_t at = (size_t) row * a.y_stride + o;
-                v4f d;
-                #pragma unroll
-                for (int r = 0; r < 4; r++) d[r] = __builtin_amdgcn_ldexpf(acc[b][u][r], ex);
-                if (o + 4 <= a.n_out) {
-                    if (a.base) d += *(const v4fu *) (a.base + at);
-                    *(v4fu *) (a.y + at) = d;
-                } else {
-                    #pragma unroll
-                    for (int r = 0; r < 4; r++)
-                        if (o + r < a.n_out) a.y[at + r] = (a.base ? a.base[at + r] : 0.0f) + d[r];
-                }
-            }
-        }
+        for (int r = 0; r < 4; r++) d[r] = base[r] + __builtin_amdgcn_ldexpf(acc[r], ex);
+        if (o + 4 <= a.n_out) *(v4fu *) y = d;
+        else
+            for (int r = 0; r < 3; r++)
+                if (o + r < a.n_out) y[r] = d[r] + (a.base ? a.base[(size_t) row * a.y_stride + o + r] : 0.0f);
     }
 }
-#define LORA_DOWN(BF, RT, name) \
-    extern "C" __global__ __launch_bounds__(64 * LD_WAVES) void name(const sml_klora a) { lora_down_body<BF, RT>(a); }
-LORA_DOWN(0, 1, sml_sv_lora_down_t1)
-LORA_DOWN(1, 1, sml_sv_lora_down_t1_bf)
-LORA_DOWN(0, 4, sml_sv_lora_down_t4)
-LORA_DOWN(1, 4, sml_sv_lora_down_t4_bf)
-#define LORA_UP(BF, RB, OT, name) \
-    extern "C" __global__ __launch_bounds__(256) void name(const sml_klora a) { lora_up_body<BF, RB, OT>(a); }
-LORA_UP(0, 1, 1, sml_sv_lora_up_b1)
-LORA_UP(1, 1, 1, sml_sv_lora_up_b1_bf)
-LORA_UP(0, 4, 2, sml_sv_lora_up_b4)
-LORA_UP(1, 4, 2, sml_sv_lora_up_b4_bf)
+
+// A workgroup takes RB tiles of 16 rows and, wave by wave, every so many blocks
+// of 64 outputs: t is joined, scaled and split into parts in LDS once, and the
+// waves then stream B and the base past it with no barrier, the next block's
+// on their way before the present one's products. Rows are the products'
+// rows, and column c of product u is output 4c + u of the block: a lane then
+// holds four outputs side by side and 16 lanes 256 bytes of a row. B's rows
+// come through the wave's part of LDS as A's do above.
+template <int BF, int RB>
+__device__ __forceinline__ void lora_up_body(const sml_klora & a) {
+    using M = Mx<BF>;
+    typedef typename M::v8 v8;
+    typedef typename M::t T;
+    typedef T v4t __attribute__((ext_vector_type(4)));
+    extern __shared__ __align__(16) uint8_t lds[];
+    constexpr int NR = 16 * RB, NP = M::parts;
+    const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), nz = gridDim.z, z = blockIdx.z;
+    uint8_t * const lb = lds + wave * LU_OUT * LD_ROW;              // [16 u + c][LD_ROW], output 4c + u
+    int * const ex_s = (int *) (lds + 4 * LU_OUT * LD_ROW);         // [row]
+    T * const tp = (T *) (ex_s + NR);                               // [part][row][ld]
+    const int ld = (a.rank + 63) / 64 * 64 + 8, row0 = blockIdx.y * NR;
+
+    // the rows of this workgroup: of its adapters and, once, those without
+    const int id = lane < NR ? adapter_of(a, row0 + lane) : -1;
+    const unsigned long long valid = my_rows(id, __ballot(id >= 0), z, nz);
+    const unsigned long long all = valid | (z || a.base == a.y ? 0 : __ballot(id < 0 && lane < NR && row0 + lane < a.n_row));
+    if (!all) return;
+    const int rk_l = id < 0 ? 0 : rank_of(a, id);     // of the lane's row
+    const float sc_l = id < 0 || !a.scale ? 1.0f : a.scale[id];
+    const int first = valid ? __builtin_amdgcn_readlane(id, __builtin_ctzll(valid)) : -1;
+    const unsigned long long mine4 = all >> (4 * g);  // bit 16h + r: row 16h + 4g + r
+
+    const int jump = gridDim.x * 4 * LU_OUT;
+    v4u br[8];
+    v4f base[RB][4], bn[RB][4];
+    // 64 outputs' ranks k0.. (up to 64), 8 lanes a row
+    auto load_b = [&](int ad, int o0, int k0) {
+        const int kk = k0 + 8 * (lane & 7);
+        const uint16_t * b = a.b + (size_t) max(ad, 0) * a.n_out * a.rank + (kk < a.rank ? kk : 0);
+        #pragma unroll
+        for (int i = 0; i < 8; i++) br[i] = *(const GLOBAL v4u *) (b + (size_t) min(o0 + 8 * i + (lane >> 3), a.n_out - 1) * a.rank);
+    };
+    auto load_base = [&](v4f (&v)[RB][4], int o0) {
+        const int o = o0 + 4 * c;
+        #pragma unroll
+        for (int h = 0; h < RB; h++)
+            #pragma unroll
+            for (int r = 0; r < 4; r++) {
+                v[h][r] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+                if (a.base && (mine4 >> (16 * h + r) & 1) && o + 4 <= a.n_out)
+                    v[h][r] = *(const GLOBAL v4fu *) (a.base + (size_t) (row0 + 16 * h + 4 * g + r) * a.y_stride + o);
+            }
+    };
+    int o0 = (blockIdx.x * 4 + wave) * LU_OUT;
+    if (o0 < a.n_out) { load_base(base, o0); load_b(first, o0, 0); }     // neither needs t
+
+    // t's rows: lr lanes of 4 values each, times sg lanes that share the splits
+    // where the tile leaves threads over; up to four rows a thread at once
+    int lr = 2;
+    while (4 * lr < a.rank) lr *= 2;
+    const int sg = max(256 / NR / lr, 1), lanes = lr * sg;
+    const int q = tid & (lr - 1), s0 = tid / lr & (sg - 1), step = 256 / lanes;
+    const bool inq = 4 * q < a.rank;
+    // zeros from the rank to the next multiple of 64
+    for (int i = tid, n8 = (ld - 8 - a.rank) / 8; i < NP * NR * n8; i += 256)
+        *(v4u *) (tp + (size_t) (i / n8) * ld + a.rank + 8 * (i % n8)) = v4u(0u);
+    for (int r0 = tid / lanes; r0 < NR; r0 += 4 * step) {
+        v4f v[4];
+        #pragma unroll
+        for (int i = 0; i < 4; i++) v[i] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+        #pragma unroll 4
+        for (int s = s0; s < a.nsplit; s += sg)
+            #pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int row = row0 + r0 + i * step;
+                if (r0 + i * step < NR && row < a.n_row && inq)
+                    v[i] += *(const v4fu *) (a.work + ((size_t) row * a.nsplit + s) * a.rank + 4 * q);
+            }
+        #pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int r = r0 + i * step;
+            const int rr = __shfl(rk_l, r & 63);
+            const float sc = __shfl(sc_l, r & 63);
+            for (int o = lr; o < lanes; o *= 2)
+                #pragma unroll
+                for (int e = 0; e < 4; e++) v[i][e] += __shfl_xor(v[i][e], o);
+            float mx = 0.0f;
+            #pragma unroll
+            for (int e = 0; e < 4; e++) { v[i][e] = 4 * q + e < rr ? v[i][e] * sc : 0.0f; mx = fmaxf(mx, fabsf(v[i][e])); }
+            int ex = 0;
+            if constexpr (!BF) {
+                for (int o = 1; o < lr; o *= 2) mx = fmaxf(mx, __shfl_xor(mx, o));
+                ex = scale_of(mx);
+            }
+            v8 p[NP];
+            #pragma unroll
+            for (int e = 0; e < 4; e += 2)
+                parts_of<BF>(__builtin_amdgcn_ldexpf(v[i][e], -ex), __builtin_amdgcn_ldexpf(v[i][e + 1], -ex), p, e);
+            if (r < NR && inq && !s0) {
+                #pragma unroll
+                for (int k = 0; k < NP; k++)
+                    *(v4t *) (tp + ((size_t) k * NR + r) * ld + 4 * q) = __builtin_shufflevector(p[k], p[k], 0, 1, 2, 3);
+            }
+            if (r < NR && !(tid & (lanes - 1))) ex_s[r] = ex;
+        }
+    }
+    __syncthreads();
+    int idr[RB][4], ex[RB][4];                        // of row 16h + 4g + r
+    #pragma unroll
+    for (int h = 0; h < RB; h++)
+        #pragma unroll
+        for (int r = 0; r < 4; r++) { idr[h][r] = __shfl(id, 16 * h + 4 * g + r); ex[h][r] = ex_s[16 * h + 4 * g + r]; }
+    for (; o0 < a.n_out; o0 += jump) {
+        const bool more = o0 + jump < a.n_out;
+        if (more) load_base(bn, o0 + jump);
+        // the tile's adapters one by one: each one's rows take its products
+        unsigned long long left = valid;
+        int cur = first;
+        while (left) {
+            const int rk = rank_of(a, cur);
+            const unsigned long long rest = left & ~__ballot(id == cur);
+            const int then = rest ? __builtin_amdgcn_readlane(id, __builtin_ctzll(rest)) : first;
+            v4f acc[RB][4];
+            #pragma unroll
+            for (int h = 0; h < RB; h++)
+                #pragma unroll
+                for (int u = 0; u < 4; u++) acc[h][u] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+            int k0 = 0;
+            do {
+                // zeros past the adapter's rank (t is zero there too), output
+                // 8i + l/8 of the block to its product's row
+                const int keep = rk - k0 - 8 * (lane & 7);
+                #pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    if (keep < 8) {
+                        #pragma unroll
+                        for (int e = 0; e < 4; e++) br[i][e] = 2 * e + 1 < keep ? br[i][e] : 2 * e < keep ? br[i][e] & 0xFFFFu : 0u;
+                    }
+                    const int o = 8 * i + (lane >> 3);
+                    *(v4u *) (lb + (16 * (o & 3) + (o >> 2)) * LD_ROW + 16 * (lane & 7)) = br[i];
+                }
+                wave_lds();
+                const int kc = k0;
+                k0 += 64;
+                if (k0 < rk) load_b(cur, o0, k0);
+                else if (rest || more) load_b(then, rest ? o0 : o0 + jump, 0);
+                #pragma unroll
+                for (int s = 0; s < 2; s++)
+                    if (kc + 32 * s < rk) {
+                        v8 w[4];
+                        #pragma unroll
+                        for (int u = 0; u < 4; u++) w[u] = *(const v8 *) (lb + (16 * u + c) * LD_ROW + 64 * s + 16 * g);
+                        #pragma unroll
+                        for (int h = 0; h < RB; h++)
+                            #pragma unroll
+                            for (int i = 0; i < NP; i++) {
+                                const v8 tv = *(const v8 *) (tp + ((size_t) i * NR + 16 * h + c) * ld + kc + 32 * s + 8 * g);
+                                #pragma unroll
+                                for (int u = 0; u < 4; u++) acc[h][u] = M::mul(tv, w[u], acc[h][u]);
+                            }
+                    }
+                wave_lds();                           // all read before the next is written
+            } while (k0 < rk);
+            #pragma unroll
+            for (int h = 0; h < RB; h++)
+                #pragma unroll
+                for (int r = 0; r < 4; r++)
+                    #pragma unroll
+                    for (int u = 0; u < 4; u++) base[h][r][u] += idr[h][r] == cur ? __builtin_amdgcn_ldexpf(acc[h][u][r], ex[h][r]) : 0.0f;
+            left = rest;
+            cur = then;
+        }
+        const int o = o0 + 4 * c;
+        #pragma unroll
+        for (int h = 0; h < RB; h++)
+            #pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const size_t at = (size_t) (row0 + 16 * h + 4 * g + r) * a.y_stride + o;
+                if (!(mine4 >> (16 * h + r) & 1)) continue;
+                if (o + 4 <= a.n_out) *(GLOBAL v4fu *) (a.y + at) = base[h][r];
+                else
+                    for (int e = 0; e < 3; e++)
+                        if (o + e < a.n_out) a.y[at + e] = base[h][r][e] + (a.base ? a.base[at + e] : 0.0f);
+            }
+        #pragma unroll
+        for (int h = 0; h < RB; h++)
+            #pragma unroll
+            for (int r = 0; r < 4; r++) base[h][r] = bn[h][r];
+    }
+}
+#define LORA(BF, sfx) \
+    extern "C" __global__ __launch_bounds__(64 * LD_WAVES) void sml_sv_lora_down##sfx(const sml_klora a) { lora_down_body<BF>(a); } \
+    extern "C" __global__ __launch_bounds__(256) void sml_sv_lora_up2##sfx(const sml_klora a) { lora_up_body<BF, 2>(a); } \
+    extern "C" __global__ __launch_bounds__(256) void sml_sv_lora_up1##sfx(const sml_klora a) { lora_up_body<BF, 1>(a); } \
+    extern "C" __global__ __launch_bounds__(64 * LF_WAVES) void sml_sv_lora_few##sfx(const sml_klora a) { lora_few_body<BF>(a); }
+LORA(0, )
+LORA(1, _bf)

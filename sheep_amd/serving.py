@@ -13,6 +13,7 @@ it keeps one contiguous cache per sequence (sml/sml-run.c:3414-3434) and picks
 greedily (sml/sml-run.c:3539-3544).
 """
 import ctypes
+import struct
 
 from . import _chk, lib
 
@@ -20,53 +21,39 @@ TYPES = {"f16": 0, "bf16": 1}
 _vp, _int, _size, _float = ctypes.c_void_p, ctypes.c_int, ctypes.c_size_t, ctypes.c_float
 
 
-class _Pages(ctypes.Structure):
-    """sml_hip_pages."""
-    _fields_ = [("k", _vp), ("v", _vp), ("table", _vp), ("page_stride", _size), ("n_pages", _int),
-                ("page_size", _int), ("n_seq", _int), ("seq_pages", _int), ("n_kv", _int), ("hd", _int),
-                ("type", _int)]
+# The header's structures as packed bytes, in the platform's layout: a step
+# makes these calls once a layer, and a ctypes.Structure costs a microsecond more.
+_PAGES = struct.Struct("PPPN7i0N")            # sml_hip_pages
+_RULES = struct.Struct("PPPiPPPPPPiPPi0N")    # sml_hip_rules
+_ADAPTERS = struct.Struct("PPPP5i0N")         # sml_hip_adapters
 
 
-class _Rules(ctypes.Structure):
-    """sml_hip_rules."""
-    _fields_ = [("hist", _vp), ("hist_start", _vp), ("n_prompt", _vp), ("n_hist", _int), ("rep", _vp),
-                ("presence", _vp), ("frequency", _vp), ("bias_id", _vp), ("bias", _vp), ("bias_start", _vp),
-                ("n_bias", _int), ("mask", _vp), ("mask_row", _vp), ("n_mask", _int)]
-
-
-class _Adapters(ctypes.Structure):
-    """sml_hip_adapters."""
-    _fields_ = [("a", _vp), ("b", _vp), ("scale", _vp), ("ranks", _vp), ("n_adapter", _int), ("rank", _int),
-                ("n_in", _int), ("n_out", _int), ("type", _int)]
-
-
-_P = ctypes.POINTER
+_block = ctypes.c_char_p
 _SIGS = [
-    ("sml_hip_paged_append", _int, [_P(_Pages), _vp, _size, _int, _vp, _vp, _vp, _vp, _int, _int, _vp, _vp]),
+    ("sml_hip_paged_append", _int, [_block, _vp, _size, _int, _vp, _vp, _vp, _vp, _int, _int, _vp, _vp]),
     ("sml_hip_paged_part_floats", _size, [_int, _int, _int, _int]),
-    ("sml_hip_paged_attention", _int, [_P(_Pages), _vp, _size, _vp, _int, _int, _float, _vp, _vp, _vp]),
+    ("sml_hip_paged_attention", _int, [_block, _vp, _size, _vp, _int, _int, _float, _vp, _vp, _vp]),
     ("sml_hip_logits_part_bytes", _size, [_int, _int]),
-    ("sml_hip_logits_adjust", _int, [_vp, _size, _int, _int, _P(_Rules), _vp, _size, _vp, _vp, _vp]),
+    ("sml_hip_logits_adjust", _int, [_vp, _size, _int, _int, _block, _vp, _size, _vp, _vp, _vp]),
     ("sml_hip_lora_work_floats", _size, [_int, _int]),
-    ("sml_hip_lora_add", _int, [_P(_Adapters), _vp, _size, _int, _vp, _vp, _vp, _size, _vp, _vp]),
+    ("sml_hip_lora_add", _int, [_block, _vp, _size, _int, _vp, _vp, _vp, _size, _vp, _vp]),
 ]
-_fns = None
+_fns = {}
 
 
 def _fn(name):
-    global _fns
-    if _fns is None:
-        found = {}
+    f = _fns.get(name)
+    if f is None:
         for n, res, args in _SIGS:
-            f = getattr(lib(), n)
-            f.restype, f.argtypes = res, args
-            found[n] = f
-        _fns = found
-    return _fns[name]
+            g = getattr(lib(), n)
+            g.restype, g.argtypes = res, args
+            _fns[n] = g
+        f = _fns[name]
+    return f
 
 
 def _ptr(b):
-    return b.ptr if b is not None else None
+    return b.ptr or 0 if b is not None else 0
 
 
 class Pages:
@@ -77,8 +64,8 @@ class Pages:
     def __init__(self, k, v, table, n_pages, page_size, n_seq, seq_pages, n_kv, hd, dtype="f16", page_stride=0):
         self.buffers = (k, v, table)
         self.n_seq, self.n_kv, self.hd = n_seq, n_kv, hd
-        self.c = _Pages(_ptr(k), _ptr(v), _ptr(table), page_stride, n_pages, page_size, n_seq, seq_pages, n_kv, hd,
-                        TYPES[dtype])
+        self.c = _PAGES.pack(_ptr(k), _ptr(v), _ptr(table), page_stride, n_pages, page_size, n_seq, seq_pages, n_kv, hd,
+                             TYPES[dtype])
 
 
 def append(pages, qkv, n_rows, pos, cos, sin, n_rope, n_head, seq=None, q_out=None, qkv_stride=0, stream=0):
@@ -111,8 +98,8 @@ def adjust_logits(logits, n_row, n_vocab, out=None, tok=None, part=None, hist=No
                   bias_start=None, mask=None, n_mask=0, mask_row=None, stride=0, out_stride=0, stream=0):
     """Penalties, biases and masks on n_row rows of logits into out (which may
     be logits), and each row's greedy pick into tok (sml_hip_logits_adjust)."""
-    r = _Rules(_ptr(hist), _ptr(hist_start), _ptr(n_prompt), n_hist, _ptr(rep), _ptr(presence), _ptr(frequency),
-               _ptr(bias_id), _ptr(bias), _ptr(bias_start), n_bias, _ptr(mask), _ptr(mask_row), n_mask)
+    r = _RULES.pack(_ptr(hist), _ptr(hist_start), _ptr(n_prompt), n_hist, _ptr(rep), _ptr(presence), _ptr(frequency),
+                    _ptr(bias_id), _ptr(bias), _ptr(bias_start), n_bias, _ptr(mask), _ptr(mask_row), n_mask)
     _chk(_fn("sml_hip_logits_adjust")(_ptr(logits), stride, n_row, n_vocab, r, _ptr(out), out_stride, _ptr(tok),
                                       _ptr(part), stream), "logits")
 
@@ -125,7 +112,7 @@ class Adapters:
 
     def __init__(self, a, b, n_adapter, rank, n_in, n_out, dtype="f16", scale=None, ranks=None):
         self.buffers = (a, b, scale, ranks)
-        self.c = _Adapters(_ptr(a), _ptr(b), _ptr(scale), _ptr(ranks), n_adapter, rank, n_in, n_out, TYPES[dtype])
+        self.c = _ADAPTERS.pack(_ptr(a), _ptr(b), _ptr(scale), _ptr(ranks), n_adapter, rank, n_in, n_out, TYPES[dtype])
 
 
 def lora_work_floats(rank, n_row):

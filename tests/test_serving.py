@@ -1,6 +1,6 @@
 """What the operators of a step of many requests refuse, before any device is
 touched, and the sizes of their workspaces (no GPU)."""
-import ctypes
+import struct
 
 import pytest
 
@@ -41,8 +41,11 @@ def test_cache_refusals(change, match):
 
 def test_type_is_checked():
     pg = serving.Pages(**PAGES)
-    pg.c.type = 2
+    pg.c = serving._PAGES.pack(A.ptr, B.ptr, C.ptr, 0, 4, 16, 2, 2, 2, 128, 2)
     refused("type 2", serving.append, pg, A, 1, B, C, C, 8, 4)
+    ad = serving.Adapters(A, B, 2, 16, 64, 100)
+    ad.c = serving._ADAPTERS.pack(A.ptr, B.ptr, 0, 0, 2, 16, 64, 100, -1)
+    refused("type -1", serving.lora, ad, A, 1, B, C, C)
 
 
 @pytest.mark.parametrize("args, kw, match", [
@@ -106,22 +109,28 @@ def test_workspace_sizes():
 
 
 def test_structures_match_the_header(tmp_path):
-    """The ctypes mirrors have the header's sizes and offsets."""
+    """The packed mirrors have the header's sizes and offsets."""
     import os
+    import re
     import subprocess
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
-    mirrors = [("sml_hip_pages", serving._Pages), ("sml_hip_rules", serving._Rules),
-               ("sml_hip_adapters", serving._Adapters)]
+    mirrors = [
+        ("sml_hip_pages", serving._PAGES, "k v table page_stride n_pages page_size n_seq seq_pages n_kv hd type"),
+        ("sml_hip_rules", serving._RULES, "hist hist_start n_prompt n_hist rep presence frequency bias_id bias "
+         "bias_start n_bias mask mask_row n_mask"),
+        ("sml_hip_adapters", serving._ADAPTERS, "a b scale ranks n_adapter rank n_in n_out type")]
     src = '#include <stddef.h>\n#include <stdio.h>\n#include "sml-serve.h"\nint main(void) {\n'
-    for n, c in mirrors:
-        src += f'printf("%zu\\n", sizeof({n}));\n'
-        for f, _ in c._fields_:
-            src += f'printf("%zu\\n", offsetof({n}, {f}));\n'
+    want = []
+    for name, packed, fields in mirrors:
+        codes = re.sub(r"(\d+)([a-zA-Z])", lambda m: m[2] * int(m[1]), packed.format)
+        assert len(codes) == len(fields.split())
+        src += f'printf("%zu\\n", sizeof({name}));\n'
+        want.append(packed.size)
+        for i, f in enumerate(fields.split()):
+            src += f'printf("%zu\\n", offsetof({name}, {f}));\n'
+            want.append(struct.calcsize(codes[:i] + "0" + codes[i]))
     (tmp_path / "t.c").write_text(src + "return 0; }\n")
     subprocess.run(["gcc", "-I", os.path.join(root, "include"), str(tmp_path / "t.c"), "-o", str(tmp_path / "t")],
                    check=True)
     got = [int(x) for x in subprocess.run([str(tmp_path / "t")], check=True, capture_output=True).stdout.split()]
-    want = []
-    for _, c in mirrors:
-        want += [ctypes.sizeof(c)] + [getattr(c, f).offset for f, _ in c._fields_]
     assert got == want
