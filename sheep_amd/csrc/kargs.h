@@ -484,6 +484,7 @@ typedef struct {
     int n_rope, n_head;
 } sml_kappend;
 
+#define AT_SHARED 256             // the most sequences whose lengths every workgroup sums
 typedef struct {
     sml_kpages pg;
     const float * q;
@@ -492,7 +493,8 @@ typedef struct {
     float * part, * out;
     float scale;                  // times log2(e)
     int n_head, max_len;
-    int nsplit, chunk;            // positions [i * chunk, (i + 1) * chunk) of split i
+    int nsplit;                   // the partials' splits a row
+    int chunk, want;              // splits of chunk positions at least, want of them if those are larger (0: of chunk)
 } sml_kattend;
 
 #define LG_RANGE 2048             // tokens of a row a workgroup takes

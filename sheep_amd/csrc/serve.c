@@ -77,20 +77,6 @@ size_t sml_hip_paged_part_floats(int n_seq, int n_head, int hd, int max_len) {
     return (size_t) n_seq * (size_t) n_head * (size_t) (ns < 256 ? ns : 256) * (size_t) (hd + 2);
 }
 
-// Positions of a split: a multiple of the 128 that a workgroup's waves take at
-// once, as few as keep at most 256 splits of the longest sequence (the
-// workspace's count) and about 4096 workgroups, but no more than 512 while
-// 256 splits of those suffice: lengths are ragged, and a workgroup with a long
-// sequence to itself would outlast the rest.
-static void attend_split(sml_kattend * a, int n_seq) {
-    const int n = a->max_len > 0 ? a->max_len : 1;
-    int chunk = 128;
-    while (chunk < 512 && (long) n_seq * a->pg.n_kv * ceil_div(n, chunk) > 4096) chunk += 128;
-    while (ceil_div(n, chunk) > 256) chunk += 128;
-    a->chunk = chunk;
-    a->nsplit = ceil_div(n, chunk);
-}
-
 int sml_hip_paged_attention(const sml_hip_pages * pg, const float * q, size_t q_stride, const int32_t * len,
                             int max_len, int n_head, float scale, float * part, float * out, void * stream) {
     HX_ENTRY(-1);
@@ -109,11 +95,26 @@ int sml_hip_paged_attention(const sml_hip_pages * pg, const float * q, size_t q_
     a.n_head = n_head;
     const long cap = (long) pg->seq_pages * pg->page_size;
     a.max_len = max_len < cap ? max_len : (int) cap;
-    attend_split(&a, pg->n_seq);
+    // splits of 128 positions (a tile a wave) at least, and no more than the
+    // workspace's of the longest sequence
+    a.nsplit = ceil_div(max_len > 1 ? max_len : 1, 64);
+    if (a.nsplit > 256) a.nsplit = 256;
+    // about 512 workgroups, two a CU, where the lengths are shared out (48
+    // sequences up to 8192 / one at 65537, 512: 55 and 37 us, 768: 53 and 38,
+    // 1024: 51 and 39)
+    const int n = a.max_len > 1 ? a.max_len : 1, shared = pg->n_seq <= AT_SHARED, least = shared ? 128 : 512;
+    a.chunk = least * ceil_div(n, least * 256);
+    a.want = shared ? ceil_div(512, pg->n_kv) : 0;
+    // every sequence's first split, and those that the lengths can make beyond
+    long grid = ceil_div(n, a.chunk);
+    if (shared) {
+        grid *= pg->n_seq;
+        if (grid > (long) a.want + pg->n_seq) grid = (long) a.want + pg->n_seq;
+    }
     char name[40];
     sv_name(name, sizeof name, "sml_sv_attend", pg->hd, pg->type);
-    hx_launch3(name, (unsigned) pg->n_kv, (unsigned) a.nsplit, (unsigned) pg->n_seq, 256, 0, (hipStream_t) stream, &a);
-    if (a.nsplit > 1)
+    hx_launch3(name, (unsigned) pg->n_kv, (unsigned) grid, shared ? 1 : (unsigned) pg->n_seq, 256, 0, (hipStream_t) stream, &a);
+    if (n > a.chunk)
         hx_launch(pg->hd == 64 ? "sml_sv_merge_d64" : "sml_sv_merge", (unsigned) n_head, (unsigned) pg->n_seq, 256, 0,
                   (hipStream_t) stream, &a);
     HX_LEAVE();

@@ -18,6 +18,13 @@ template <int BF> __device__ __forceinline__ float of16(uint16_t h) {
     else return h2f(h);
 }
 
+// What a wave's lanes wrote to its own part of LDS is there for all of them.
+__device__ __forceinline__ void wave_lds() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 // The page of entry i of sequence s, or -1.
 __device__ __forceinline__ int page_of(const sml_kpages & pg, int s, int i) {
     const int p = pg.table[(size_t) s * pg.seq_pages + i];
@@ -87,11 +94,13 @@ APPEND(64, 1, sml_sv_append_d64_bf)
 //
 // A workgroup takes a split of a sequence's positions for one KV head, its
 // waves alternate tiles of 32 positions, and a wave keeps all of a tile in
-// registers (no LDS until the waves' sums are joined). The matrix cores take
+// registers while the next is on its way. The matrix cores take
 // S^T = K Q^T and O^T = V^T P^T, heads in the columns (the unused of the 16
 // are zero). With the lane's c = lane % 16, g = lane / 16:
-// - K is the first operand as the cache stores it: lane (c, g) loads 16 bytes
-//   of position c's row, dims 32j + 8g.. for product j.
+// - K is the first operand as the cache stores it: lane (c, g) takes 16 bytes of
+//   position c's row, dims 32j + 8g.. for product j. Loads in that order would
+//   touch 16 rows in 16 consecutive lanes, a cache line a lane: the rows are
+//   loaded whole and handed over through the wave's part of LDS.
 // - S comes back as positions 4g + r of head c, which is just what the second
 //   product takes as its P^T operand if its inner index 8g + i stands for
 //   position 4g + i of the first 16 positions (i < 4) or of the second: P
@@ -112,7 +121,83 @@ APPEND(64, 1, sml_sv_append_d64_bf)
 // from where memory is (the rest of the page, or page 0), their scores
 // replaced by -infinity and their V rows by zeros; tiles of absent pages alone
 // are passed over.
+//
+// Lengths are ragged and the host knows only a bound of them, so the device
+// shares the work out: every wave sums the lengths and finds its workgroup's
+// sequence and split (at_place), splits of one size for all. Past AT_SHARED
+// sequences, whose sum would cost too much, splits have a fixed size and the
+// grid every sequence's most (want 0).
+//
+// Measured with the merge, 32 heads over 8 of 128, fp16: 48 sequences up to
+// 8192 (202 MB) 55 us = 3.7 TB/s (60 with fixed splits of 512 and K in the
+// matrix cores' order from memory), one at 4095 9.7 us, of which 5.8 are this
+// kernel's chain of latencies (length, table, rows, joining) and 3.8 the
+// merge's; bf16, 28 over 4, one at 65537 (134 MB) 36.7 us = 3.7 TB/s. A large
+// copy reaches 4.8 TB/s. Two workgroups (212 registers) a CU: held to three,
+// 58 and 52 us.
 #define AT_WAVES 4
+
+// The positions a sequence attends over.
+__device__ __forceinline__ int at_len(const sml_kattend & a, int b) { return min(max(a.len[b], 0), a.max_len); }
+// The inclusive sums of v over the wave's lanes.
+__device__ __forceinline__ int wave_scan(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);           // row_shr 1, 2, 4, 8
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);           // row_bcast 15 into rows 1 and 3
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);           // row_bcast 31 into rows 2 and 3
+    return v;
+}
+// The positions of a split, by one wave: a multiple of 128, a.chunk at least,
+// else what makes a.want splits in all (counted in units of 128 positions:
+// AT_SHARED lengths of 2^30 stay below 2^31).
+__device__ __forceinline__ int at_size(const sml_kattend & a, int lane) {
+    if (!a.want) return a.chunk;
+    unsigned t = 0;
+    if (a.pg.n_seq == 1) {
+        t = (unsigned) (at_len(a, 0) + 127) >> 7;
+    } else {
+        #pragma unroll 4
+        for (int b = lane; b < a.pg.n_seq; b += 64) t += (unsigned) (at_len(a, b) + 127) >> 7;
+        t = (unsigned) __builtin_amdgcn_readlane(wave_scan((int) t), 63);
+    }
+    return max(a.chunk, (int) min((t + a.want - 1) / a.want, 1u << 23) * 128);
+}
+// A sequence of n positions in splits of about chunk: equal ones, to a tile of
+// 32; per is their size. At least one (an empty sequence's writes its zeros).
+__device__ __forceinline__ int at_splits(int n, int chunk, int & per) {
+    const int p = max((n + chunk - 1) / chunk, 1);
+    per = max(((n + p - 1) / p + 31) & ~31, 32);
+    return max((n + per - 1) / per, 1);
+}
+// Split i of all, in the sequences' order: its sequence, its number there,
+// their size and count; false past the last.
+__device__ __forceinline__ bool at_place(const sml_kattend & a, int i, int lane, int & b, int & split, int & per, int & count) {
+    const int chunk = at_size(a, lane);
+    if (!a.want || a.pg.n_seq == 1) {
+        b = blockIdx.z;
+        split = i;
+        count = at_splits(at_len(a, b), chunk, per);
+        return i < count;
+    }
+    for (int b0 = 0; b0 < a.pg.n_seq; b0 += 64) {
+        int pl = 32, cl = 0;
+        if (b0 + lane < a.pg.n_seq) cl = at_splits(at_len(a, b0 + lane), chunk, pl);
+        const int sum = wave_scan(cl);
+        const unsigned long long at = __ballot(sum > i);
+        if (at) {
+            const int l = __builtin_ctzll(at);
+            b = b0 + l;
+            count = __builtin_amdgcn_readlane(cl, l);
+            per = __builtin_amdgcn_readlane(pl, l);
+            split = i - (__builtin_amdgcn_readlane(sum, l) - count);
+            return true;
+        }
+        i -= __builtin_amdgcn_readlane(sum, 63);
+    }
+    return false;
+}
 
 template <int BF> struct Mx;
 template <> struct Mx<0> {
@@ -155,11 +240,15 @@ __device__ __forceinline__ void attend_body(const sml_kattend & a) {
     typedef typename M::v8 v8;
     constexpr int NJ = D / 32, E = D / 16, NP = M::parts, W = AT_WAVES;
     typedef unsigned vrow __attribute__((ext_vector_type(E / 2)));
-    __shared__ float so[W][16][D + 4], sm[W][16], sl[W][16];
-    const int kh = blockIdx.x, split = blockIdx.y, b = blockIdx.z, tid = threadIdx.x, lane = tid & 63;
+    constexpr int KR = 2 * D + 16;                    // bytes of a K row in LDS: 16 rows fall on different banks
+    __shared__ __align__(16) uint8_t lds[W * 32 * KR];  // a wave's 32 K rows; at the end its sums
+    static_assert(32 * KR >= 16 * (D + 4) * 4, "");
+    __shared__ float sm[W][16], sl[W][16];
+    const int kh = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, g = lane >> 4;
-    const int n = min(a.len[b], a.max_len), t0 = split * a.chunk, t1 = min(n, t0 + a.chunk);
-    if (t0 >= t1 && a.nsplit > 1) return;             // the merge takes the splits below the length only
+    int b, split, per, count;
+    if (!at_place(a, blockIdx.y, lane, b, split, per, count)) return;
+    const int n = at_len(a, b), t0 = split * per, t1 = min(n, t0 + per);
     const int rep = a.n_head / a.pg.n_kv, kvd = a.pg.n_kv * D;
     const int sh = a.pg.page_shift, pmask = (1 << sh) - 1;
     const int32_t * const tab = a.pg.table + (size_t) b * a.pg.seq_pages;
@@ -207,9 +296,13 @@ __device__ __forceinline__ void attend_body(const sml_kattend & a) {
         }
         return t;
     };
-    v4u kr[2][NJ];
+    constexpr int LK = D / 8, RK = 64 / LK;           // lanes of a K row, rows of a load
+    v4u kr[2][16 / RK];
     vrow vr[8];
-    const uint32_t koff = 2u * (uint32_t) (c * kvd + 8 * g);
+    uint8_t * const lk = lds + wave * 32 * KR;
+    uint32_t koff[16 / RK];
+    #pragma unroll
+    for (int i = 0; i < 16 / RK; i++) koff[i] = 2u * (uint32_t) ((RK * i + lane / LK) * kvd + 8 * (lane % LK));
     uint32_t voff[4];
     #pragma unroll
     for (int i = 0; i < 4; i++) voff[i] = 2u * (uint32_t) ((4 * g + i) * kvd + E * c);
@@ -222,7 +315,7 @@ __device__ __forceinline__ void attend_body(const sml_kattend & a) {
         for (int h = 0; h < 2; h++) {
             const GLOBAL char * p = (const GLOBAL char *) (a.pg.k + (h ? xb : xa));
             #pragma unroll
-            for (int j = 0; j < NJ; j++) kr[h][j] = *(const GLOBAL v4u *) (p + koff + 64 * j);
+            for (int i = 0; i < 16 / RK; i++) kr[h][i] = *(const GLOBAL v4u *) (p + koff[i]);
         }
     };
     auto load_v = [&](size_t xa, size_t xb) {
@@ -244,16 +337,24 @@ __device__ __forceinline__ void attend_body(const sml_kattend & a) {
         const bool ha = pa >= 0, hb = pb >= 0, whole = ha && hb && t + 32 <= t1;
         const int tn = seek(t + 32 * W);
         const size_t xa = place(pa, tn), xb = place(pb, tn + 16);
+        #pragma unroll
+        for (int h = 0; h < 2; h++)
+            #pragma unroll
+            for (int i = 0; i < 16 / RK; i++) *(v4u *) (lk + (16 * h + RK * i + lane / LK) * KR + 16 * (lane % LK)) = kr[h][i];
+        wave_lds();
+        if (tn < t1) load_k(xa, xb);
         v4f s[2];
         #pragma unroll
         for (int h = 0; h < 2; h++) {
             s[h] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
             #pragma unroll
-            for (int j = 0; j < NJ; j++)
+            for (int j = 0; j < NJ; j++) {
+                const v8 kj = *(const v8 *) (lk + (16 * h + c) * KR + 64 * j + 16 * g);
                 #pragma unroll
-                for (int k = 0; k < NP; k++) s[h] = M::mul(__builtin_bit_cast(v8, kr[h][j]), q[j][k], s[h]);
+                for (int k = 0; k < NP; k++) s[h] = M::mul(kj, q[j][k], s[h]);
+            }
         }
-        if (tn < t1) load_k(xa, xb);
+        wave_lds();                                   // all read before the next tile is written
         // the lane's scores: positions 4g + r of either half
         float mx = -INFINITY;
         #pragma unroll
@@ -313,6 +414,8 @@ __device__ __forceinline__ void attend_body(const sml_kattend & a) {
     // the waves' sums joined: wave w's head c, dims (D/4)g + Er + u
     l += __shfl_xor(l, 16);
     l += __shfl_xor(l, 32);
+    __syncthreads();                                  // the K rows are done with
+    float (* const so)[16][D + 4] = (float (*)[16][D + 4]) lds;
     if (c < rep) {
         #pragma unroll
         for (int r = 0; r < 4; r++)
@@ -335,7 +438,7 @@ __device__ __forceinline__ void attend_body(const sml_kattend & a) {
             os += f * so[w][h][d];
             ls += f * sl[w][h];
         }
-        if (a.nsplit == 1) {
+        if (count == 1) {
             a.out[(row0 + h) * D + d] = ls == 0.0f ? 0.0f : os / ls;
         } else {
             const size_t at = (row0 + h) * a.nsplit + split;
@@ -353,7 +456,9 @@ __device__ __forceinline__ void attend_merge_body(const sml_kattend & a) {
     constexpr int S = AM_THREADS / D;                 // shares
     __shared__ float f[256], red[S][D], sred[AM_THREADS / 64];
     const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
-    const int n = min(a.len[b], a.max_len), ns = n > 0 ? (n + a.chunk - 1) / a.chunk : 0;
+    int per;
+    const int ns = at_splits(at_len(a, b), at_size(a, tid & 63), per);
+    if (ns == 1) return;                              // written already
     const size_t row = (size_t) b * a.n_head + h;
     const float * po = a.part + row * a.nsplit * D;
     const float2 * pm = (const float2 *) (a.part + (size_t) a.pg.n_seq * a.n_head * a.nsplit * D) + row * a.nsplit;
@@ -613,13 +718,6 @@ __device__ __forceinline__ unsigned long long my_rows(int id, unsigned long long
         valid &= ~m;
     }
     return mine;
-}
-
-// What a wave's lanes wrote to its own part of LDS is there for all of them.
-__device__ __forceinline__ void wave_lds() {
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
 // A x: a workgroup takes a tile of 16 rows, 64 ranks and a split of the inputs,

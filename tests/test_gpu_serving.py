@@ -210,6 +210,34 @@ def test_attention_absent_pages(dtype):
     attend_case([700, 2100], 4, 1, 64, dtype, 128, seed=6, gone={0: [5], 1: range(1, 16)})
 
 
+def test_attention_many_sequences():
+    """Past 256 sequences the splits have a fixed size; at and below, the
+    lengths are shared out, whole waves of them and part of one."""
+    rng = np.random.default_rng(12)
+    for n, kv, longest in ((300, 1, 900), (256, 1, 200), (65, 2, 400), (64, 1, 300)):
+        lens = [int(x) for x in rng.integers(0, longest, n)]
+        lens[n // 2], lens[0] = longest, 0
+        attend_case(lens, 2 * kv, kv, 64, "f16", 16, seed=n)
+
+
+def test_attention_loose_bound():
+    """A bound far above the lengths, and sequences that differ much."""
+    attend_case([1, 3000, 5, 130], 4, 2, 128, "bf16", 32, seed=13)
+    rng = np.random.default_rng(14)
+    k, v, q = rng.standard_normal((2, 16, 1, 64)), rng.standard_normal((2, 16, 1, 64)), rng.standard_normal((1, 64))
+    kb, vb = so.to_bits(k, "f16"), so.to_bits(v, "f16")
+    table = np.full((1, 5000), -1, np.int32)
+    table[0, :2] = [1, 0]
+    pg = serving.Pages(sa.DevBuf.of(kb), sa.DevBuf.of(vb), sa.DevBuf.of(table), 2, 16, 1, 5000, 1, 64)
+    out, part = sa.DevBuf(256), sa.DevBuf(4 * serving.part_floats(1, 1, 64, 1 << 30))
+    for n in (20, 1 << 30):                                  # absent pages behind the second
+        serving.attention(pg, sa.DevBuf.of(q.astype(np.float32)), ints([n]), 1 << 30, 1, part, out)
+        rows = min(n, 32)
+        want, tol = so.attend(q.astype(np.float32), so.from_bits(kb[[1, 0]], "f16").reshape(32, 64)[:rows],
+                              so.from_bits(vb[[1, 0]], "f16").reshape(32, 64)[:rows], 0.125)
+        within(out.read(np.float32).reshape(1, 64), want, tol, str(n))
+
+
 def test_attention_cut_at_max_len():
     attend_case([500, 3, 90], 8, 2, 128, "f16", 32, seed=7, max_len=77)
     attend_case([5, 3], 8, 2, 128, "f16", 32, seed=7, max_len=0)

@@ -63,7 +63,7 @@ def test_append_refusals(args, kw, match):
     ((A, B, 8, 0, C, C), {}, "0 heads"), ((A, B, -1, 4, C, C), {}, "lengths up to -1"),
     ((None, B, 8, 4, C, C), {}, "missing"), ((A, None, 8, 4, C, C), {}, "missing"),
     ((A, B, 8, 4, None, C), {}, "missing"), ((A, B, 8, 4, C, None), {}, "missing"),
-    ((A, B, 8, 4, C, C), dict(q_stride=511), "511 apart"),
+    ((A, B, 8, 4, C, C), dict(q_stride=511), "511 apart"), ((A, B, 8, 4, At(C.ptr + 8), C), {}, "16-byte"),
 ])
 def test_attention_refusals(args, kw, match):
     refused(match, serving.attention, serving.Pages(**PAGES), *args, **kw)
@@ -76,7 +76,8 @@ def test_attention_refusals(args, kw, match):
     (dict(out_stride=99), "99 apart"), (dict(out=A, stride=200), "in place"),
     (dict(hist=C, n_hist=5, rep=C), "hist_start"), (dict(bias=C, n_bias=1, bias_id=C), "bias_start"),
     (dict(bias=C, n_bias=1, bias_start=C), "bias_id"), (dict(mask=C, n_mask=1), "1 masks for 2 rows"),
-    (dict(n_hist=-1), "-1 ids"),
+    (dict(n_hist=-1), "-1 ids"), (dict(n_hist=(1 << 30) + 1), "1073741825 ids"), (dict(n_bias=-2), "-2 biases"),
+    (dict(n_mask=-1), "-1 masks"),
 ])
 def test_logits_refusals(kw, match):
     base = dict(logits=A, n_row=2, n_vocab=100, out=B)
