@@ -521,6 +521,8 @@ typedef struct {
 #define LF_RANK 64                // its highest rank
 #define LF_LD (LF_RANK + 16)      // values of a row of t's parts in LDS
 #define LF_SLICE 512              // inputs of a wave's round (8 ranks)
+#define LS_ROWS 512               // the most rows that are sorted by adapter, and the adapters then
+#define LS_ADAPTERS 255
 #define LU_OUT 64                 // outputs of a wave's block of y
 #define LD_WAVE_LDS(parts) ((64 + 16 * (parts)) * LD_ROW + 64)
 typedef struct {
@@ -531,4 +533,5 @@ typedef struct {
     float * y, * work;            // work [row][split][rank]
     size_t x_stride, y_stride;
     int n_adapter, rank, n_in, n_out, n_row, nsplit, chunk;
+    int sorted;                   // tiles take the rows by adapter
 } sml_klora;

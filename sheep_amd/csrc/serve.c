@@ -193,10 +193,11 @@ static void lora_launch(sml_klora * a, int bf, hipStream_t st) {
                   64 * LF_WAVES, (size_t) parts * 16 * LF_LD * 2 + 64 + sums, st, a);
         return;
     }
-    // workgroups share a tile's distinct adapters while there are few tiles (16
-    // rows of 16 adapters, 4096 to 14336, rank 16: 35 us with 1, 19 with 4, 21
-    // with 16; 128 rows: 40, 49 and 106)
+    // workgroups share a tile's distinct adapters while there are few tiles (32
+    // rows of 16 adapters, 4096 to 14336, rank 16: 36 us with 1, 21 with 4, 33
+    // with 16), and tiles take more rows by adapter
     const int nz = a->n_row <= 32 ? (few < 4 ? few : 4) : a->n_row <= 64 ? 2 : 1;
+    a->sorted = a->n_row > 32 && a->n_row <= LS_ROWS && a->n_adapter > 1 && a->n_adapter <= LS_ADAPTERS;
     // t: the inputs split for 128 workgroups, as far as the workspace holds
     // them (509 rows, rank 64, bf16: 8.0 us and 18.0 for y at 4 splits, 6.6 and
     // 20.8 at 8: every workgroup of y joins them)
@@ -216,6 +217,7 @@ static void lora_launch(sml_klora * a, int bf, hipStream_t st) {
     int gx = (512 / nrt + 7) / 8 * 8;
     if (gx > ceil_div(a->n_out, 4 * LU_OUT)) gx = ceil_div(a->n_out, 4 * LU_OUT);
     if (gx < 1) gx = 1;
+    // (the sort's counts, 8 KB, fit before it)
     const size_t lds = (size_t) 4 * LU_OUT * LD_ROW + (size_t) 16 * rb * (4 + (size_t) parts * ((size_t) ngroup * 64 + 8) * 2);
     char name[40];
     snprintf(name, sizeof name, "sml_sv_lora_up%d%s", rb, bf ? "_bf" : "");

@@ -700,11 +700,83 @@ extern "C" __global__ __launch_bounds__(64) void sml_sv_pick(const sml_klogits a
 
 // The valid adapter id of a row, or -1.
 __device__ __forceinline__ int adapter_of(const sml_klora & a, int row) {
-    const int id = a.adapter[min(row, a.n_row - 1)];
-    return row < a.n_row && id >= 0 && id < a.n_adapter ? id : -1;
+    const int id = a.adapter[min(max(row, 0), a.n_row - 1)];
+    return row >= 0 && row < a.n_row && id >= 0 && id < a.n_adapter ? id : -1;
 }
 __device__ __forceinline__ int rank_of(const sml_klora & a, int id) {
     return a.ranks ? min(max(a.ranks[id], 0), a.rank) : a.rank;
+}
+
+// The rows of tile positions row0 .. row0 + nr - 1 into rows (-1 past the last):
+// the caller's order, or (a.sorted) that of their adapters, rows without one
+// last, so that a mixed batch's tiles hold few adapters each. A counting sort
+// every workgroup makes for itself: 64 rows a wave, each distinct adapter's
+// lanes by ballot; cnt holds (n_adapter + 1) counts of every 64 rows. It takes
+// 1.7 us of a call, two launches; 128 rows of 16 adapters in turn (4096 to
+// 14336, rank 64) go from 50 to 26 us with it, 509 from 100 to 37, 64 from 46
+// (37 shared by four workgroups) to 29, 32 rows lose.
+template <int NW>
+__device__ __forceinline__ void tile_rows(const sml_klora & a, int row0, int nr, int * rows, int * cnt, int * wsum) {
+    constexpr int PER = LS_ROWS / 64 / NW;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    if (!a.sorted) {
+        if (tid < nr) rows[tid] = row0 + tid < a.n_row ? row0 + tid : -1;
+        __syncthreads();
+        return;
+    }
+    const int nch = (a.n_row + 63) / 64, m = (a.n_adapter + 1) * nch;
+    int key[PER], rank[PER], turns = 0;
+    #pragma unroll
+    for (int i = 0; i < PER; i++) {
+        const int row = 64 * (wave + NW * i) + lane;
+        key[i] = -1;
+        if (row < a.n_row) {
+            key[i] = adapter_of(a, row);
+            if (key[i] < 0) key[i] = a.n_adapter;
+        }
+        turns += __builtin_popcountll(__ballot(key[i] != __shfl_down(key[i], 1)));
+    }
+    if (!lane) wsum[wave] = turns;
+    for (int i = tid; i < m; i += 64 * NW) cnt[i] = 0;
+    __syncthreads();
+    turns = 0;
+    #pragma unroll
+    for (int w = 0; w < NW; w++) turns += wsum[w];
+    // runs already, as prompts come: at most about a change a tile
+    const bool runs = 16 * turns <= a.n_row;
+    if (tid < nr) rows[tid] = runs && row0 + tid < a.n_row ? row0 + tid : -1;
+    __syncthreads();                                  // wsum is read by all
+    if (runs) return;
+    #pragma unroll
+    for (int i = 0; i < PER; i++) {
+        rank[i] = 0;
+        for (unsigned long long left = __ballot(key[i] >= 0); left;) {
+            const int cur = __builtin_amdgcn_readlane(key[i], __builtin_ctzll(left));
+            const unsigned long long at = __ballot(key[i] == cur);
+            left &= ~at;
+            if (key[i] == cur) rank[i] = __builtin_amdgcn_mbcnt_hi((unsigned) (at >> 32), __builtin_amdgcn_mbcnt_lo((unsigned) at, 0));
+            if (!lane) cnt[cur * nch + wave + NW * i] = __builtin_popcountll(at);
+        }
+    }
+    __syncthreads();
+    // exclusive sums, adapter by adapter
+    const int each = (m + 64 * NW - 1) / (64 * NW), e0 = min(tid * each, m), e1 = min(e0 + each, m);
+    int sum = 0;
+    for (int i = e0; i < e1; i++) sum += cnt[i];
+    int before = wave_scan(sum);
+    if (lane == 63) wsum[wave] = before;
+    before -= sum;
+    __syncthreads();
+    for (int w = 0; w < wave; w++) before += wsum[w];
+    for (int i = e0; i < e1; i++) { const int v = cnt[i]; cnt[i] = before; before += v; }
+    __syncthreads();
+    #pragma unroll
+    for (int i = 0; i < PER; i++)
+        if (key[i] >= 0) {
+            const int p = cnt[key[i] * nch + wave + NW * i] + rank[i] - row0;
+            if (p >= 0 && p < nr) rows[p] = 64 * (wave + NW * i) + lane;
+        }
+    __syncthreads();
 }
 
 // The rows of a tile (bits of valid, id: the lane's) whose adapter is the z-th,
@@ -742,17 +814,22 @@ __device__ __forceinline__ void lora_down_body(const sml_klora & a) {
     const int split = blockIdx.x, row0 = blockIdx.y * 16, ngroup = (a.rank + 63) / 64, nz = gridDim.z / ngroup;
     const int j0 = (blockIdx.z % ngroup) * 64, z = blockIdx.z / ngroup;
     const int k0 = split * a.chunk, k1 = min(a.n_in, k0 + a.chunk);
-    const int id = adapter_of(a, row0 + c), nt = min(RT, (a.rank - j0 + 15) / 16);
+    __shared__ int rows[16], wsum[LD_WAVES];
+    tile_rows<LD_WAVES>(a, row0, 16, rows, (int *) lds, wsum);
+    const int id = adapter_of(a, rows[c]), nt = min(RT, (a.rank - j0 + 15) / 16);
     const unsigned all = (unsigned) my_rows(id, (unsigned) (__ballot(id >= 0) & 0xFFFFu), z, nz);
     if (!all) return;
     const int first = __builtin_amdgcn_readlane(id, __builtin_ctz(all));
 
+    const float * xrow[4];
+    #pragma unroll
+    for (int i = 0; i < 4; i++) xrow[i] = a.x + (size_t) max(rows[4 * i + g], 0) * a.x_stride;
     v4f xr[4];
     v4u ar[8], an[8];
     auto load_x = [&](int kb) {
         const int kk = min(kb + 4 * c, k1 - 4);
         #pragma unroll
-        for (int i = 0; i < 4; i++) xr[i] = *(const GLOBAL v4fu *) (a.x + (size_t) min(row0 + 4 * i + g, a.n_row - 1) * a.x_stride + kk);
+        for (int i = 0; i < 4; i++) xr[i] = *(const GLOBAL v4fu *) (xrow[i] + kk);
     };
     auto load_a = [&](v4u (&r)[8], int ad, int kb) {
         const int kk = min(kb + 8 * (lane & 7), k1 - 8);
@@ -995,15 +1072,25 @@ __device__ __forceinline__ void lora_up_body(const sml_klora & a) {
     T * const tp = (T *) (ex_s + NR);                               // [part][row][ld]
     const int ld = (a.rank + 63) / 64 * 64 + 8, row0 = blockIdx.y * NR;
 
+    __shared__ int rows[NR], wsum[4];
+    tile_rows<4>(a, row0, NR, rows, (int *) lds, wsum);
+    const int myrow = lane < NR ? rows[lane] : -1;
+
     // the rows of this workgroup: of its adapters and, once, those without
-    const int id = lane < NR ? adapter_of(a, row0 + lane) : -1;
+    const int id = adapter_of(a, myrow);
     const unsigned long long valid = my_rows(id, __ballot(id >= 0), z, nz);
-    const unsigned long long all = valid | (z || a.base == a.y ? 0 : __ballot(id < 0 && lane < NR && row0 + lane < a.n_row));
+    const unsigned long long all = valid | (z || a.base == a.y ? 0 : __ballot(id < 0 && myrow >= 0));
     if (!all) return;
     const int rk_l = id < 0 ? 0 : rank_of(a, id);     // of the lane's row
     const float sc_l = id < 0 || !a.scale ? 1.0f : a.scale[id];
     const int first = valid ? __builtin_amdgcn_readlane(id, __builtin_ctzll(valid)) : -1;
     const unsigned long long mine4 = all >> (4 * g);  // bit 16h + r: row 16h + 4g + r
+
+    int yrow[RB][4];                                  // row of position 16h + 4g + r
+    #pragma unroll
+    for (int h = 0; h < RB; h++)
+        #pragma unroll
+        for (int r = 0; r < 4; r++) yrow[h][r] = rows[16 * h + 4 * g + r];
 
     const int jump = gridDim.x * 4 * LU_OUT;
     v4u br[8];
@@ -1023,7 +1110,7 @@ __device__ __forceinline__ void lora_up_body(const sml_klora & a) {
             for (int r = 0; r < 4; r++) {
                 v[h][r] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
                 if (a.base && (mine4 >> (16 * h + r) & 1) && o + 4 <= a.n_out)
-                    v[h][r] = *(const GLOBAL v4fu *) (a.base + (size_t) (row0 + 16 * h + 4 * g + r) * a.y_stride + o);
+                    v[h][r] = *(const GLOBAL v4fu *) (a.base + (size_t) yrow[h][r] * a.y_stride + o);
             }
     };
     int o0 = (blockIdx.x * 4 + wave) * LU_OUT;
@@ -1150,7 +1237,7 @@ __device__ __forceinline__ void lora_up_body(const sml_klora & a) {
         for (int h = 0; h < RB; h++)
             #pragma unroll
             for (int r = 0; r < 4; r++) {
-                const size_t at = (size_t) (row0 + 16 * h + 4 * g + r) * a.y_stride + o;
+                const size_t at = (size_t) yrow[h][r] * a.y_stride + o;
                 if (!(mine4 >> (16 * h + r) & 1)) continue;
                 if (o + 4 <= a.n_out) *(GLOBAL v4fu *) (a.y + at) = base[h][r];
                 else

@@ -437,6 +437,21 @@ def test_lora(dtype, n, n_in, n_out, rank, A):
     lora_case(n, n_in, n_out, rank, A, dtype, mixed, seed=n + 2, in_place=True, scale=False, y_pad=5, x_pad=8)
 
 
+@pytest.mark.parametrize("n, A, dtype", [(33, 5, "f16"), (64, 16, "bf16"), (200, 16, "f16"), (257, 255, "bf16"),
+                                         (512, 40, "f16"), (513, 40, "f16"), (300, 300, "f16"), (510, 3, "bf16")])
+def test_lora_mixed_batches(n, A, dtype):
+    """Rows of many adapters in no order, in turn, in runs, and mostly without
+    one, around the sizes where tiles take them by adapter."""
+    rng = np.random.default_rng(n + A)
+    mixed = [int(i) for i in rng.integers(-2, A + 2, n)]
+    lora_case(n, 64, 70, 8, A, dtype, mixed, seed=1, y_pad=2)
+    lora_case(n, 72, 33, 16, A, dtype, [r % A for r in range(n)], seed=2, in_place=True)
+    lora_case(n, 64, 40, 24, A, dtype, [r * A // n for r in range(n)], seed=3, base=False)
+    lora_case(n, 64, 40, 8, A, dtype, [0 if r == n - 1 else -1 for r in range(n)], seed=4)
+    lora_case(n, 64, 40, 72, A, dtype, [int(i) for i in rng.zipf(1.5, n) - 1], seed=5,
+              ranks=[int(i) for i in rng.integers(0, 73, A)])
+
+
 def test_lora_no_adapters():
     """Ids outside the pool add nothing, and no rows are no work."""
     lora_case(7, 64, 40, 8, 2, "f16", [-1, 2, -5, 1 << 30, 5, -1, 99])
