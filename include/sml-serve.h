@@ -44,13 +44,13 @@ typedef struct {
     int n_kv, hd, type;           // type: SML_F16 or SML_BF16
 } sml_hip_pages;
 
-// Append n_rows new tokens (0 or more). Row r of qkv (qkv_stride floats apart,
+// Append n_rows new tokens (0..2^22). Row r of qkv (qkv_stride floats apart,
 // 0: (n_head + 2 * n_kv) * hd) holds a token's q, k and v after bias, as the
 // stacked product leaves them; it is position pos[r] of sequence seq[r] (seq
 // NULL: sequence r). q and k are rotated by their position (halved pairs,
 // table rows of hd / 2), k and v rounded to the cache's type (nearest even)
-// and written to their page; the rotated q goes to q_out [n_rows][n_head*hd],
-// or back to its place in qkv when q_out is NULL. In fp16 the cache then holds
+// and written to their page; the rotated q goes to q_out [n_rows][n_head*hd]
+// (apart from qkv), or back to its place in qkv when q_out is NULL. In fp16 the cache then holds
 // what sml_hip_attention would have written, bit for bit.
 // A row is left out, its q_out included, when its position is negative or at
 // or past n_rope or seq_pages * page_size, its sequence is outside 0..n_seq-1
@@ -68,12 +68,16 @@ size_t sml_hip_paged_part_floats(int n_seq, int n_head, int hd, int max_len);
 // n_head * hd; rotated already) over the first len[b] positions of sequence b,
 // scaled by `scale` (0: 1 / sqrt(hd)), into out [n_seq][n_head * hd]. n_head is
 // a multiple of n_kv, at most 16 query heads per KV head. max_len (host) bounds
-// every length and sizes the launch; a longer len[b] is cut to it and to
-// seq_pages * page_size, a negative one is 0. Positions past the length and on
-// absent pages are not read, whatever they hold. A sequence with no position
-// left, or with no score above -infinity, gets zeros. Softmax statistics and
-// sums are fp32; q and the weights meet the cache in the matrix cores as sums
-// of 16-bit parts that together hold them to fp32's accuracy.
+// every length and sizes the launch (a tight bound is faster); a longer len[b]
+// is cut to it and to seq_pages * page_size, a negative one is 0. Positions
+// past the length and on absent pages count for nothing, whatever their memory
+// holds. A sequence with no position left, or with no score above -infinity,
+// gets zeros. Softmax statistics and sums are fp32; q and the weights meet the
+// cache in the matrix cores as sums of 16-bit parts that together hold them to
+// fp32's accuracy (so an infinite key or value that a sequence does attend
+// over makes its KV head's outputs NaN). How the positions are split follows
+// all of the lengths: a sequence's sums depend on the others by their rounding
+// alone, and equal calls give equal bits.
 int sml_hip_paged_attention(const sml_hip_pages * pg, const float * q, size_t q_stride, const int32_t * len,
                             int max_len, int n_head, float scale, float * part, float * out, void * stream);
 
@@ -136,10 +140,12 @@ size_t sml_hip_lora_work_floats(int rank, int n_row);
 // y[r] = base[r] + scale * B (A x[r]) for n_row rows (0..65535) with adapter
 // adapter[r] each; an id outside 0..n_adapter-1 (-1 by custom) adds nothing.
 // x rows lie x_stride floats apart (0: n_in), y's and base's y_stride (0:
-// n_out); base may be y, or NULL for zeros. Products and sums are fp32; the
-// order of a row's sums depends on the call's shape, not on the other rows'
-// values. It follows sml_hip_gemm, whose output is its base, and takes the
-// unquantized input of that product.
+// n_out); base may be y, or NULL for zeros; x and work lie apart from y.
+// Products and sums are fp32, their order set by the call's shape: a row's bits
+// do not depend on the other rows or on which adapters they have, and an
+// infinity or NaN in a row or an adapter reaches only the rows it belongs to.
+// It follows sml_hip_gemm, whose output is its base, and takes the unquantized
+// input of that product.
 int sml_hip_lora_add(const sml_hip_adapters * ad, const float * x, size_t x_stride, int n_row, const int32_t * adapter,
                      const float * base, float * y, size_t y_stride, float * work, void * stream);
 

@@ -54,7 +54,7 @@ int sml_hip_paged_append(const sml_hip_pages * pg, float * qkv, size_t qkv_strid
     sml_kappend a;
     memset(&a, 0, sizeof a);
     check_pages(pg, &a.pg);
-    if (n_rows < 0 || n_rows > 1 << 24 || n_head < 1 || n_head > 65536) hx_failf("append: %d rows of %d heads", n_rows, n_head);
+    if (n_rows < 0 || n_rows > 1 << 22 || n_head < 1 || n_head > 65536) hx_failf("append: %d rows of %d heads", n_rows, n_head);
     const size_t width = ((size_t) n_head + 2 * (size_t) pg->n_kv) * pg->hd;
     if (!qkv || !pos || !cos_t || !sin_t || n_rope < 1) hx_failf("append: missing rows, positions or rotation tables");
     if (qkv_stride && qkv_stride < width) hx_failf("append: rows of %zu floats %zu apart", width, qkv_stride);
@@ -102,7 +102,11 @@ int sml_hip_paged_attention(const sml_hip_pages * pg, const float * q, size_t q_
     // about 512 workgroups, two a CU, where the lengths are shared out (48
     // sequences up to 8192 / one at 65537, 512: 55 and 37 us, 768: 53 and 38,
     // 1024: 51 and 39)
-    const int n = a.max_len > 1 ? a.max_len : 1, shared = pg->n_seq <= AT_SHARED, least = shared ? 128 : 512;
+    // Up to 512 positions a sequence is one split, with no merge (whole / split:
+    // one sequence of 256 5.9 / 8.0 us, of 512 8.0 / 8.5, of 768 9.9 / 8.8; 64 of
+    // 512 23 / 26).
+    const int n = a.max_len > 1 ? a.max_len : 1, shared = pg->n_seq <= AT_SHARED;
+    const int least = shared && n > 512 ? 128 : 512;
     a.chunk = least * ceil_div(n, least * 256);
     a.want = shared ? ceil_div(512, pg->n_kv) : 0;
     // every sequence's first split, and those that the lengths can make beyond

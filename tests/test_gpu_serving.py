@@ -142,7 +142,7 @@ def test_append_equals_the_contiguous_cache(hd):
 # ------------------------------------------------------------ attention
 
 def attend_case(lens, heads, kv, hd, dtype, page, seed=0, gone=None, scale=0.0, q_size=1.0, pad=0, max_len=None,
-                poison=True, spare=3):
+                poison=True, spare=3, kv_size=1.0):
     """One call against the oracle. gone: {sequence: absent page entries};
     poison: NaN and infinities everywhere the call must not look."""
     rng = np.random.default_rng(seed)
@@ -150,7 +150,7 @@ def attend_case(lens, heads, kv, hd, dtype, page, seed=0, gone=None, scale=0.0, 
     seq_pages = max(1, -(-max(lens) // page))
     n_pages = n_seq * seq_pages + spare
     table = make_table(rng, n_seq, seq_pages, n_pages)
-    k, v = (rng.standard_normal((n_pages, page, kv, hd)).astype(np.float32) for _ in range(2))
+    k, v = (kv_size * rng.standard_normal((n_pages, page, kv, hd)).astype(np.float32) for _ in range(2))
     kb, vb = so.to_bits(k, dtype), so.to_bits(v, dtype)
     cut = [max(0, min(n, max_len if max_len is not None else n)) for n in lens]
     keep = np.zeros((n_pages, page), bool)
@@ -248,6 +248,31 @@ def test_attention_cut_at_max_len():
 @pytest.mark.parametrize("q_size, scale", [(40.0, 0.0), (1e-3, 0.0), (1.0, 0.7), (3e5, 1e-6), (1e-7, 1e6), (1.0, -0.2)])
 def test_attention_query_sizes(dtype, q_size, scale):
     attend_case([300, 17], 8, 2, 128, dtype, 16, seed=9, q_size=q_size, scale=scale, pad=4)
+
+
+@pytest.mark.parametrize("kv_size, q_size", [(3e-6, 1.0), (3e-6, 2e5), (9000.0, 1.0), (9000.0, 1e-4)])
+def test_attention_cache_sizes(kv_size, q_size):
+    """fp16's denormals and its largest values in the cache."""
+    attend_case([200, 700], 8, 2, 128, "f16", 16, seed=15, kv_size=kv_size, q_size=q_size)
+
+
+def test_attention_weights_of_all_sizes():
+    """Scores spread over the exponential's range: the weights run from 1 to
+    below fp16's smallest, and the largest come last."""
+    rng = np.random.default_rng(16)
+    for dtype in ("f16", "bf16"):
+        n, hd, page = 900, 64, 32
+        k = np.zeros((n, hd))
+        k[:, 0] = np.sort(rng.uniform(-12, 12, n))
+        kb, vb = so.to_bits(k, dtype), so.to_bits(rng.standard_normal((n, hd)), dtype)
+        pools = [sa.DevBuf.of(np.concatenate([b, np.zeros((29 * page - n, hd), np.uint16)])) for b in (kb, vb)]
+        pg = serving.Pages(*pools, sa.DevBuf.of(np.arange(29, dtype=np.int32)), 29, page, 1, 29, 1, hd, dtype)
+        q = np.zeros((2, hd), np.float32)
+        q[0, 0], q[1, 0] = 8.0, -8.0                         # largest last, largest first
+        out, part = sa.DevBuf(4 * 2 * hd), sa.DevBuf(4 * serving.part_floats(1, 2, hd, n))
+        serving.attention(pg, sa.DevBuf.of(q), ints([n]), n, 2, part, out)
+        want, tol = so.attend(q, so.from_bits(kb, dtype), so.from_bits(vb, dtype), 0.125)
+        within(out.read(np.float32).reshape(2, hd), want, tol, dtype)
 
 
 def test_attention_far_pages():
@@ -426,7 +451,7 @@ def lora_case(n, n_in, n_out, rank, A, dtype, adapter, seed=0, base=True, in_pla
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
 @pytest.mark.parametrize("n, n_in, n_out, rank, A", [
     (1, 8, 1, 8, 1), (1, 1536, 8960, 8, 2), (3, 72, 33, 16, 2), (16, 4096, 1000, 16, 11), (17, 520, 257, 24, 3),
-    (33, 264, 130, 64, 4), (64, 1024, 515, 40, 5), (100, 136, 65, 256, 2), (130, 2048, 64, 8, 1), (5, 14336, 96, 128, 5)])
+    (33, 264, 130, 64, 4), (64, 1024, 515, 40, 5), (1, 12288, 300, 64, 2), (140, 264, 300, 256, 2), (16, 512, 4000, 64, 9), (100, 136, 65, 256, 2), (130, 2048, 64, 8, 1), (5, 14336, 96, 128, 5)])
 def test_lora(dtype, n, n_in, n_out, rank, A):
     rng = np.random.default_rng(n)
     mixed = [int(i) for i in rng.integers(-1, A, n)]
@@ -460,6 +485,27 @@ def test_lora_no_adapters():
     b = sa.DevBuf(1024)
     serving.lora(ad, b, 0, b, b, b)
     sa.sync()
+
+
+def test_lora_rows_do_not_depend_on_others():
+    """A row's bits are the same whatever adapters the other rows have."""
+    rng = np.random.default_rng(3)
+    for n, A in ((12, 5), (30, 5), (150, 9)):
+        n_in, n_out, rank = 520, 90, 16
+        a, b = (sa.DevBuf.of(so.to_bits(rng.standard_normal(sh), "f16")) for sh in ((A, rank, n_in), (A, n_out, rank)))
+        ad = serving.Adapters(a, b, A, rank, n_in, n_out)
+        x = rng.standard_normal((n, n_in)).astype(np.float32)
+        got = []
+        for other in range(3):
+            ids = rng.integers(-1, A, n) if other else np.full(n, 2)
+            ids[[0, n // 2, n - 1]] = [2, 1, 4]
+            xo = x.copy()
+            xo[1] *= 10.0 ** other
+            y, work = sa.DevBuf(4 * n * n_out), sa.DevBuf(4 * serving.lora_work_floats(rank, n))
+            serving.lora(ad, sa.DevBuf.of(xo), n, ints(ids), y, work)
+            got.append(y.read(np.uint32).reshape(n, n_out)[[0, n // 2, n - 1]])
+        np.testing.assert_array_equal(got[0], got[1])
+        np.testing.assert_array_equal(got[0], got[2])
 
 
 def test_lora_zero_and_low_ranks():

@@ -49,7 +49,7 @@ def test_type_is_checked():
 
 
 @pytest.mark.parametrize("args, kw, match", [
-    ((A, -1, B, C, C, 8, 4), {}, "-1 rows"), ((A, 1, B, C, C, 8, 0), {}, "0 heads"),
+    ((A, -1, B, C, C, 8, 4), {}, "-1 rows"), ((A, (1 << 22) + 1, B, C, C, 8, 4), {}, "4194305 rows"), ((A, 1, B, C, C, 8, 0), {}, "0 heads"),
     ((None, 1, B, C, C, 8, 4), {}, "missing"), ((A, 1, None, C, C, 8, 4), {}, "missing"),
     ((A, 1, B, None, C, 8, 4), {}, "missing"), ((A, 1, B, C, C, 0, 4), {}, "missing"),
     ((A, 1, B, C, C, 8, 4), dict(qkv_stride=1023), "1024 floats 1023 apart"),
