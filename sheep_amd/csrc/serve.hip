@@ -512,26 +512,39 @@ ATTEND(64, 1, sml_sv_attend_d64_bf)
 // division), not sixteen unrolled (1 row of 128256: 10.3 us so, 6.0 with).
 //
 // us a call with the pick, 512 threads of one word / 256 of two (128256 tokens,
-// histories of 2047): 1 row 8.8 / 9.8, 16 rows 11.4 / 11.4, 96 rows 34.6 / 28.3
-// (the last 3.5 TB/s); histories of 65536: 1 row 19.4 / 30.2, 96 rows 58 / 58.
-// 4096 tokens a workgroup: 96 rows 30.5 at best.
+// histories of 2047): 1 row 8.1 (5.0 and 1.7 of them the two kernels', the rest
+// between launches) / 9.4, 16 rows 10.7 / 9.9, 96 rows 31 / 26 (3.8 TB/s;
+// 4096 tokens a workgroup: 28.5). The pick looks for the largest value first
+// and for its place in the lanes that have it; with an index carried beside
+// every value the 96 rows took 28 us, 213 instructions a word of four.
 #define LG_SEEN 0x80000000u
 
-__device__ __forceinline__ void amax_take(float v, int i, float & bv, int & bi) {
-    if (v > bv || (v == bv && i < bi)) { bv = v; bi = i; }
+// The largest value and the smallest index over the wave's lanes.
+__device__ __forceinline__ float wave_top(float v) {
+    const int r = __builtin_bit_cast(int, max16(v));
+    const float a = __builtin_bit_cast(float, __builtin_amdgcn_readlane(r, 0)), b = __builtin_bit_cast(float, __builtin_amdgcn_readlane(r, 16));
+    const float c = __builtin_bit_cast(float, __builtin_amdgcn_readlane(r, 32)), d = __builtin_bit_cast(float, __builtin_amdgcn_readlane(r, 48));
+    return fmaxf(fmaxf(a, b), fmaxf(c, d));
 }
-// The better of two candidates over all lanes of a wave; first is twice the
-// first permitted index, plus 1 if its value is NaN.
-__device__ __forceinline__ void pick_wave(float & bv, int & bi, unsigned & first) {
-    #pragma unroll
-    for (int o = 32; o; o >>= 1) {
-        const float ov = __shfl_xor(bv, o);
-        const int oi = __shfl_xor(bi, o);
-        amax_take(ov, oi, bv, bi);
-        first = min(first, (unsigned) __shfl_xor((int) first, o));
-    }
+__device__ __forceinline__ unsigned wave_least(unsigned v) {
+    v = min(v, (unsigned) dpp_i<0xB1>((int) v));
+    v = min(v, (unsigned) dpp_i<0x4E>((int) v));
+    v = min(v, (unsigned) dpp_i<0x141>((int) v));
+    v = min(v, (unsigned) dpp_i<0x140>((int) v));
+    const unsigned a = (unsigned) __builtin_amdgcn_readlane((int) v, 0), b = (unsigned) __builtin_amdgcn_readlane((int) v, 16);
+    const unsigned c = (unsigned) __builtin_amdgcn_readlane((int) v, 32), d = (unsigned) __builtin_amdgcn_readlane((int) v, 48);
+    return min(min(a, b), min(c, d));
 }
-#define LG_NONE 0x7fffffff                            // no index
+// Of the lanes' candidates (value, index; NaN loses, LG_NONE is none) the
+// lowest index of the largest value; of their first permitted tokens (twice the
+// index, plus 1 if the value is NaN) the first.
+__device__ __forceinline__ void pick_wave(float & bv, unsigned & bi, unsigned & first) {
+    const float top = wave_top(bv);
+    bi = wave_least(bv == top ? bi : 0x7fffffffu);
+    bv = top;
+    first = wave_least(first);
+}
+#define LG_NONE 0x7fffffffu                           // no index
 #define LG_FIRST 0xffffffffu                          // nothing permitted
 
 __device__ __forceinline__ float pick4(v4f v, int e) { return e & 2 ? (e & 1 ? v[3] : v[2]) : (e & 1 ? v[1] : v[0]); }
@@ -544,8 +557,7 @@ __device__ __forceinline__ void logits_body(const sml_klogits & a) {
     __shared__ __align__(16) unsigned cnt[LG_RANGE];     // generated count, LG_SEEN if listed at all
     __shared__ __align__(16) unsigned bia[LG_RANGE];     // the last bias entry's index + 1
     __shared__ float rv[NT / 64];
-    __shared__ int ri[NT / 64];
-    __shared__ unsigned rf[NT / 64];
+    __shared__ unsigned ri[NT / 64], rf[NT / 64];
     const int row = blockIdx.y, t0 = blockIdx.x * LG_RANGE, tid = threadIdx.x;
     const int nt = min(LG_RANGE, a.n_vocab - t0);
     const float * x = a.logits + (size_t) row * a.stride + t0;
@@ -578,17 +590,32 @@ __device__ __forceinline__ void logits_body(const sml_klogits & a) {
     if (a.hist) {
         const int h0 = min(max(a.hist_start[row], 0), a.n_hist), h1 = min(max(a.hist_start[row + 1], 0), a.n_hist);
         const int gen = h0 + (a.n_prompt ? min(max(a.n_prompt[row], 0), max(h1 - h0, 0)) : 0);
-        // four ids a thread in flight
-        for (int i = h0 + tid; i < h1; i += 4 * NT) {
-            int t[4];
+        auto take = [&](int i, unsigned t) {
+            if (t < (unsigned) nt) {
+                if (i >= gen) atomicAdd(&cnt[t], 1u);
+                atomicOr(&cnt[t], LG_SEEN);
+            }
+        };
+        // sixteen ids a thread in flight, most of them another workgroup's
+        typedef int v4iu __attribute__((ext_vector_type(4), aligned(4)));
+        int i = h0 + 4 * tid;
+        for (; i + 12 * NT + 4 <= h1; i += 16 * NT) {
+            v4i t[4];
             #pragma unroll
-            for (int k = 0; k < 4; k++) t[k] = a.hist[min(i + k * NT, h1 - 1)] - t0;
+            for (int k = 0; k < 4; k++) t[k] = *(const v4iu *) (a.hist + i + 4 * NT * k) - t0;
             #pragma unroll
             for (int k = 0; k < 4; k++)
-                if (i + k * NT < h1 && (unsigned) t[k] < (unsigned) nt) {
-                    if (i + k * NT >= gen) atomicAdd(&cnt[t[k]], 1u);
-                    atomicOr(&cnt[t[k]], LG_SEEN);
+                if (min(min((unsigned) t[k][0], (unsigned) t[k][1]), min((unsigned) t[k][2], (unsigned) t[k][3])) < (unsigned) nt) {
+                    #pragma unroll
+                    for (int e = 0; e < 4; e++) take(i + 4 * NT * k + e, (unsigned) t[k][e]);
                 }
+        }
+        for (; i < h1; i += 4 * NT) {
+            int t[4];
+            #pragma unroll
+            for (int e = 0; e < 4; e++) t[e] = a.hist[min(i + e, h1 - 1)] - t0;
+            #pragma unroll
+            for (int e = 0; e < 4; e++) if (i + e < h1) take(i + e, (unsigned) t[e]);
         }
     }
     if (a.bias) {
@@ -602,8 +629,6 @@ __device__ __forceinline__ void logits_body(const sml_klogits & a) {
                 pr = a.presence ? a.presence[row] : 0.0f;
     if (a.hist || a.bias) __syncthreads();
     float bv = -INFINITY;
-    int bi = LG_NONE;
-    unsigned first = LG_FIRST;
     #pragma unroll
     for (int i = 0; i < K; i++) {
         const int j = 4 * (NT * i + tid);
@@ -625,16 +650,11 @@ __device__ __forceinline__ void logits_body(const sml_klogits & a) {
             for (int f = 0; f < 4; f++) l[i][f] = e == f ? v : l[i][f];
         }
         ok[i] &= 15u;
-        if (ok[i] && first == LG_FIRST) {
-            const int e = __builtin_ctz(ok[i]);
-            const float v = pick4(l[i], e);
-            first = 2u * (unsigned) (t0 + j + e) + (v != v);
+        if (ok[i] != 15u) {
+            #pragma unroll
+            for (int e = 0; e < 4; e++) l[i][e] = ok[i] >> e & 1 ? l[i][e] : -INFINITY;
         }
-        #pragma unroll
-        for (int e = 0; e < 4; e++) {
-            l[i][e] = ok[i] >> e & 1 ? l[i][e] : -INFINITY;
-            amax_take(l[i][e], ok[i] >> e & 1 ? t0 + j + e : LG_NONE, bv, bi);
-        }
+        bv = fmaxf(bv, fmaxf(fmaxf(l[i][0], l[i][1]), fmaxf(l[i][2], l[i][3])));
         if (a.out) {
             float * y = a.out + (size_t) row * a.out_stride + t0 + j;
             if (j + 4 <= nt) *(v4fu *) y = l[i];
@@ -643,15 +663,32 @@ __device__ __forceinline__ void logits_body(const sml_klogits & a) {
         }
     }
     if (!a.tok) return;
-    pick_wave(bv, bi, first);
-    if ((tid & 63) == 0) { rv[tid >> 6] = bv; ri[tid >> 6] = bi; rf[tid >> 6] = first; }
+    // the wave's largest value, then the lanes that have it look for its place
+    // (indices rise over the words, the waves, the lanes)
+    const float top = wave_top(bv);
+    unsigned bi = LG_NONE, first = LG_FIRST;
+    if (bv == top) {
+        #pragma unroll
+        for (int i = K - 1; i >= 0; i--)
+            #pragma unroll
+            for (int e = 3; e >= 0; e--) bi = (ok[i] >> e & 1) && l[i][e] == top ? (unsigned) (t0 + 4 * (NT * i + tid) + e) : bi;
+    }
+    #pragma unroll
+    for (int i = K - 1; i >= 0; i--) {
+        const int e = __builtin_ctz(ok[i] | 16u);
+        const float v = pick4(l[i], e);
+        first = ok[i] ? 2u * (unsigned) (t0 + 4 * (NT * i + tid) + e) + (v != v) : first;
+    }
+    bi = wave_least(bi);
+    first = wave_least(first);
+    if ((tid & 63) == 0) { rv[tid >> 6] = top; ri[tid >> 6] = bi; rf[tid >> 6] = first; }
     __syncthreads();
     if (tid >= 64) return;
     bv = tid < NT / 64 ? rv[tid] : -INFINITY;
     bi = tid < NT / 64 ? ri[tid] : LG_NONE;
     first = tid < NT / 64 ? rf[tid] : LG_FIRST;
     pick_wave(bv, bi, first);
-    if (!tid) a.part[(size_t) row * a.n_part + blockIdx.x] = make_int4(__float_as_int(bv), bi, (int) first, 0);
+    if (!tid) a.part[(size_t) row * a.n_part + blockIdx.x] = make_int4(__float_as_int(bv), (int) bi, (int) first, 0);
 }
 #define LOGITS(NT, K) \
     extern "C" __global__ __launch_bounds__(NT) void sml_sv_logits_##NT##_##K(const sml_klogits a) { logits_body<NT, K>(a); }
@@ -663,15 +700,17 @@ LOGITS(256, 2)
 extern "C" __global__ __launch_bounds__(64) void sml_sv_pick(const sml_klogits a) {
     const int row = blockIdx.x;
     float bv = -INFINITY;
-    int bi = LG_NONE;
-    unsigned first = LG_FIRST;
+    unsigned bi = LG_NONE, first = LG_FIRST;
     for (int i = threadIdx.x; i < a.n_part; i += 64) {
         const int4 p = a.part[(size_t) row * a.n_part + i];
-        amax_take(__int_as_float(p.x), p.y, bv, bi);
+        const float v = __int_as_float(p.x);
+        // a lane's blocks come in order: only a larger value displaces, or any
+        // index where there was none
+        if (v > bv || bi == LG_NONE) { bv = v; bi = (unsigned) p.y; }
         first = min(first, (unsigned) p.z);
     }
     pick_wave(bv, bi, first);
-    if (!threadIdx.x) a.tok[row] = first == LG_FIRST ? -1 : first & 1 ? (int) (first >> 1) : bi;
+    if (!threadIdx.x) a.tok[row] = first == LG_FIRST ? -1 : first & 1 ? (int) (first >> 1) : (int) bi;
 }
 
 // ---------------------------------------------------------------- adapters
