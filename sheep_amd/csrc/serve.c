@@ -166,9 +166,9 @@ int sml_hip_logits_adjust(const float * logits, size_t stride, int n_row, int n_
     on_device();
     if (n_row) {
         a.n_part = ceil_div(n_vocab, LG_RANGE);
-        // one word a thread while the workgroups are at most 4 a CU (a call of
+        // one word a thread while the workgroups are at most 2 a CU (a call of
         // latencies), else half the threads with two (measured beside the kernel)
-        const int wide = (long) a.n_part * n_row <= 4L * hx.ncu;
+        const int wide = (long) a.n_part * n_row <= 2L * hx.ncu;
         hx_launch(wide ? "sml_sv_logits_512_1" : "sml_sv_logits_256_2", (unsigned) a.n_part, (unsigned) n_row,
                   wide ? 512 : 256, 0, (hipStream_t) stream, &a);
         if (tok) hx_launch("sml_sv_pick", (unsigned) n_row, 1, 64, 0, (hipStream_t) stream, &a);
@@ -186,13 +186,15 @@ size_t sml_hip_lora_work_floats(int rank, int n_row) {
 #define LD_ROWS 16                                    // rows of a tile
 
 // One launch or two, as measured beside the kernels. One: up to 16 rows of rank
-// up to 64, at most 16 row products a wave and 256 workgroups, and sums that
-// fit LDS.
+// up to 64, sums that fit LDS, at most 640 workgroups, and few row products a
+// wave (rounds of its 8 ranks of 512 inputs, each taking the adapter's rows one
+// by one): 8 if the rows share the pool's adapters alike, 16 if all had one.
 static void lora_launch(sml_klora * a, int bf, hipStream_t st) {
     const int parts = bf ? 3 : 2, nslice = ceil_div(a->n_in, LF_SLICE), few = a->n_row < 16 ? a->n_row : 16;
     const size_t sums = (size_t) nslice * 16 * (size_t) a->rank * 4;
-    if (a->n_row <= 16 && a->rank <= LF_RANK && sums <= 96 << 10 &&
-        (long) a->n_row * ceil_div(nslice * (a->rank / 8), LF_WAVES) <= 16 && (long) ceil_div(a->n_out, LF_OUT) * few <= 256) {
+    const long rounds = ceil_div(nslice * (a->rank / 8), LF_WAVES);
+    if (a->n_row <= 16 && a->rank <= LF_RANK && sums <= 96 << 10 && a->n_row * rounds <= 16 &&
+        ceil_div(a->n_row, a->n_adapter) * rounds <= 8 && (long) ceil_div(a->n_out, LF_OUT) * few <= 640) {
         hx_launch(bf ? "sml_sv_lora_few_bf" : "sml_sv_lora_few", (unsigned) ceil_div(a->n_out, LF_OUT), (unsigned) few,
                   64 * LF_WAVES, (size_t) parts * 16 * LF_LD * 2 + 64 + sums, st, a);
         return;

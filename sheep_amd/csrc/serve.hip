@@ -512,11 +512,13 @@ ATTEND(64, 1, sml_sv_attend_d64_bf)
 // division), not sixteen unrolled (1 row of 128256: 10.3 us so, 6.0 with).
 //
 // us a call with the pick, 512 threads of one word / 256 of two (128256 tokens,
-// histories of 2047): 1 row 8.1 (5.0 and 1.7 of them the two kernels', the rest
-// between launches) / 9.4, 16 rows 10.7 / 9.9, 96 rows 31 / 26 (3.8 TB/s;
-// 4096 tokens a workgroup: 28.5). The pick looks for the largest value first
-// and for its place in the lanes that have it; with an index carried beside
-// every value the 96 rows took 28 us, 213 instructions a word of four.
+// masks, histories of 2047): 1 row 8.1 / 8.3 (5.0 and 1.7 of them the kernels',
+// the rest two launches), 16 rows 10.2 / 9.9, 32 rows 13.9 / 13.2, 96 rows 31 /
+// 26 (3.8 TB/s); histories of 65536: 1 row 15 / 23, 96 rows 49 / 45. 4096 tokens
+// a workgroup: 96 rows 28.5 (when this took 27). The pick looks for the
+// largest value first and for its place in the lanes that have it; with an
+// index carried beside every value the 96 rows took 28, 213 instructions a
+// word of four.
 #define LG_SEEN 0x80000000u
 
 // The largest value and the smallest index over the wave's lanes.
@@ -728,14 +730,15 @@ extern "C" __global__ __launch_bounds__(64) void sml_sv_pick(const sml_klogits a
 //
 // A few rows take one launch (lora_few_body), others two: t = A x, split over
 // the inputs, then y, whose workgroups join the splits. us a call, one launch /
-// two (fp16; rows of so many adapters):
-//   rank 16, 4096 to 4096: 1 row 5.6 / 10.9, 4 of 4 6.0 / 11.7, 16 of 16 8.2 /
-//   13.5, 16 of one 15.6 / 11.5; 4096 to 14336: 4 of 4 6.2 / 11.6, 16 of 16
-//   27 / 19; 14336 to 4096: 1 row 9.0 / 12.6, 4 of one 15.1 / 13.2, 16 of one
-//   39 / 13.6; rank 64, 4096 to 14336: 1 row 10.7 / 12.9, 16 of 16 51 / 24.
-// So one launch pays while each of its workgroups has few rows' products to
-// make in its lanes (rows times rounds of its waves) and the workgroups, each
-// reading its adapter's A again, are at most one a CU.
+// two (fp16; "8 of 4" is 8 rows of 4 adapters):
+//   rank 16, 4096 to 4096: 1 of 1 5.4 / 11.0, 4 of 4 5.7 / 11.8, 8 of 1 10.1 /
+//   11.7, 16 of 16 7.8 / 19; 4096 to 14336: 4 of 4 6.0 / 12.1, 8 of 8 (448
+//   workgroups) 11.8 / 14.4, 12 of 12 (672) 18.5 / 16.7; 14336 to 4096: 1 of 1
+//   9.0 / 12.8, 4 of 4 9.5 / 13.8, 4 of 1 15 / 13.3; rank 64, 4096 to 4096: 4 of
+//   4 11.0 / 14.7, 4 of 1 17.5 / 13.7; rank 8, 1536 to 8960: 16 of 16 (560) 16.6
+//   / 18.8.
+// So one launch pays while its waves have few rows' products to make in their
+// lanes and the workgroups, each reading its adapter's A again, are not many.
 
 // The valid adapter id of a row, or -1.
 __device__ __forceinline__ int adapter_of(const sml_klora & a, int row) {
