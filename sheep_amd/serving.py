@@ -38,22 +38,23 @@ _SIGS = [
     ("sml_hip_lora_work_floats", _size, [_int, _int]),
     ("sml_hip_lora_add", _int, [_block, _vp, _size, _int, _vp, _vp, _vp, _size, _vp, _vp]),
 ]
-_fns = {}
+class _Calls:
+    """The library's functions, bound at their first use."""
 
-
-def _fn(name):
-    f = _fns.get(name)
-    if f is None:
+    def __getattr__(self, name):
         for n, res, args in _SIGS:
-            g = getattr(lib(), n)
-            g.restype, g.argtypes = res, args
-            _fns[n] = g
-        f = _fns[name]
-    return f
+            f = getattr(lib(), n)
+            f.restype, f.argtypes = res, args
+            setattr(self, n[8:], f)
+        return self.__dict__[name]
 
 
-def _ptr(b):
-    return b.ptr or 0 if b is not None else 0
+_call = _Calls()
+
+
+def _at(b):
+    """A buffer's device address, 0 for None."""
+    return (b and b.ptr) or 0
 
 
 class Pages:
@@ -64,7 +65,7 @@ class Pages:
     def __init__(self, k, v, table, n_pages, page_size, n_seq, seq_pages, n_kv, hd, dtype="f16", page_stride=0):
         self.buffers = (k, v, table)
         self.n_seq, self.n_kv, self.hd = n_seq, n_kv, hd
-        self.c = _PAGES.pack(_ptr(k), _ptr(v), _ptr(table), page_stride, n_pages, page_size, n_seq, seq_pages, n_kv, hd,
+        self.c = _PAGES.pack(_at(k), _at(v), _at(table), page_stride, n_pages, page_size, n_seq, seq_pages, n_kv, hd,
                              TYPES[dtype])
 
 
@@ -72,25 +73,26 @@ def append(pages, qkv, n_rows, pos, cos, sin, n_rope, n_head, seq=None, q_out=No
     """Rotate n_rows new tokens' q and k by their positions and write their k
     and v to the cache (sml_hip_paged_append); without q_out the rotated q
     goes back to qkv."""
-    _chk(_fn("sml_hip_paged_append")(pages.c, _ptr(qkv), qkv_stride, n_rows, _ptr(seq), _ptr(pos), _ptr(cos),
-                                     _ptr(sin), n_rope, n_head, _ptr(q_out), stream), "paged append")
+    _chk(_call.paged_append(pages.c, qkv and qkv.ptr, qkv_stride, n_rows, seq and seq.ptr, pos and pos.ptr,
+                            cos and cos.ptr, sin and sin.ptr, n_rope, n_head, q_out and q_out.ptr, stream),
+         "paged append")
 
 
 def part_floats(n_seq, n_head, hd, max_len):
     """Floats of attention's workspace."""
-    return _fn("sml_hip_paged_part_floats")(n_seq, n_head, hd, max_len)
+    return _call.paged_part_floats(n_seq, n_head, hd, max_len)
 
 
 def attention(pages, q, lens, max_len, n_head, part, out, scale=0.0, q_stride=0, stream=0):
     """out [n_seq][n_head*hd]: one new token a sequence over its first
     lens[b] positions (sml_hip_paged_attention)."""
-    _chk(_fn("sml_hip_paged_attention")(pages.c, _ptr(q), q_stride, _ptr(lens), max_len, n_head, scale, _ptr(part),
-                                        _ptr(out), stream), "paged attention")
+    _chk(_call.paged_attention(pages.c, q and q.ptr, q_stride, lens and lens.ptr, max_len, n_head, scale,
+                               part and part.ptr, out and out.ptr, stream), "paged attention")
 
 
 def logits_part_bytes(n_row, n_vocab):
     """Bytes of adjust_logits' workspace (with tok)."""
-    return _fn("sml_hip_logits_part_bytes")(n_row, n_vocab)
+    return _call.logits_part_bytes(n_row, n_vocab)
 
 
 def adjust_logits(logits, n_row, n_vocab, out=None, tok=None, part=None, hist=None, n_hist=0, hist_start=None,
@@ -98,10 +100,10 @@ def adjust_logits(logits, n_row, n_vocab, out=None, tok=None, part=None, hist=No
                   bias_start=None, mask=None, n_mask=0, mask_row=None, stride=0, out_stride=0, stream=0):
     """Penalties, biases and masks on n_row rows of logits into out (which may
     be logits), and each row's greedy pick into tok (sml_hip_logits_adjust)."""
-    r = _RULES.pack(_ptr(hist), _ptr(hist_start), _ptr(n_prompt), n_hist, _ptr(rep), _ptr(presence), _ptr(frequency),
-                    _ptr(bias_id), _ptr(bias), _ptr(bias_start), n_bias, _ptr(mask), _ptr(mask_row), n_mask)
-    _chk(_fn("sml_hip_logits_adjust")(_ptr(logits), stride, n_row, n_vocab, r, _ptr(out), out_stride, _ptr(tok),
-                                      _ptr(part), stream), "logits")
+    r = _RULES.pack(_at(hist), _at(hist_start), _at(n_prompt), n_hist, _at(rep), _at(presence), _at(frequency),
+                    _at(bias_id), _at(bias), _at(bias_start), n_bias, _at(mask), _at(mask_row), n_mask)
+    _chk(_call.logits_adjust(logits and logits.ptr, stride, n_row, n_vocab, r, out and out.ptr, out_stride,
+                             tok and tok.ptr, part and part.ptr, stream), "logits")
 
 
 class Adapters:
@@ -112,16 +114,16 @@ class Adapters:
 
     def __init__(self, a, b, n_adapter, rank, n_in, n_out, dtype="f16", scale=None, ranks=None):
         self.buffers = (a, b, scale, ranks)
-        self.c = _ADAPTERS.pack(_ptr(a), _ptr(b), _ptr(scale), _ptr(ranks), n_adapter, rank, n_in, n_out, TYPES[dtype])
+        self.c = _ADAPTERS.pack(_at(a), _at(b), _at(scale), _at(ranks), n_adapter, rank, n_in, n_out, TYPES[dtype])
 
 
 def lora_work_floats(rank, n_row):
     """Floats of lora's workspace."""
-    return _fn("sml_hip_lora_work_floats")(rank, n_row)
+    return _call.lora_work_floats(rank, n_row)
 
 
 def lora(adapters, x, n_row, adapter, y, work, base=None, x_stride=0, y_stride=0, stream=0):
     """y[r] = base[r] + scale * B (A x[r]) with row r's adapter, -1 for none
     (sml_hip_lora_add); base may be y."""
-    _chk(_fn("sml_hip_lora_add")(adapters.c, _ptr(x), x_stride, n_row, _ptr(adapter), _ptr(base), _ptr(y), y_stride,
-                                 _ptr(work), stream), "lora")
+    _chk(_call.lora_add(adapters.c, x and x.ptr, x_stride, n_row, adapter and adapter.ptr, base and base.ptr,
+                        y and y.ptr, y_stride, work and work.ptr, stream), "lora")
