@@ -205,8 +205,8 @@ static void lora_launch(sml_klora * a, int bf, hipStream_t st) {
     const int nz = a->n_row <= 32 ? (few < 4 ? few : 4) : a->n_row <= 64 ? 2 : 1;
     a->sorted = a->n_row > 32 && a->n_row <= LS_ROWS && a->n_adapter > 1 && a->n_adapter <= LS_ADAPTERS;
     // t: the inputs split for 128 workgroups, as far as the workspace holds
-    // them (509 rows, rank 64, bf16: 8.0 us and 18.0 for y at 4 splits, 6.6 and
-    // 20.8 at 8: every workgroup of y joins them)
+    // them (509 rows of 4 adapters, 4096 to 14336, rank 64, a call at 2, 4 and 8
+    // splits: 34.4, 31.2, 31.7 us; every workgroup of y joins them)
     const int ntile = ceil_div(a->n_row, LD_ROWS), ngroup = ceil_div(a->rank, 64);
     int most = 8192 / a->n_row < 32 ? 8192 / a->n_row : 32;
     const int want = ceil_div(128, ntile * ngroup);
@@ -217,10 +217,18 @@ static void lora_launch(sml_klora * a, int bf, hipStream_t st) {
     a->nsplit = ceil_div(a->n_in, a->chunk);
     hx_launch3(bf ? "sml_sv_lora_down_bf" : "sml_sv_lora_down", (unsigned) a->nsplit, (unsigned) ntile,
                (unsigned) (nz * ngroup), 64 * LD_WAVES, (size_t) LD_WAVES * LD_WAVE_LDS(parts), st, a);
-    // y: 32 rows a workgroup of a prompt, and about 512 workgroups (the same
-    // case, 256 / 512 / 1024: 22 / 18 / 24 us; 16 rows: 22 / 18 / 23)
-    const int rb = a->n_row <= 128 ? 1 : 2, nrt = ceil_div(a->n_row, 16 * rb);
-    int gx = (512 / nrt + 7) / 8 * 8;
+    // y: 32 rows a workgroup of a prompt (us a call at 16 / 32, one adapter: 192
+    // rows, 4096 to 14336, rank 64 17.8 / 19.3, 14336 to 4096 19.5 / 23.4; 384
+    // rows 24.5 / 24.3 and 23.8 / 25.9, 1536 to 8960, rank 8 18.7 / 14.9; 509
+    // rows of 4 adapters in runs 33.6 / 31.5, 30.8 / 27.0 at rank 16), and the
+    // 512 workgroups that run at once, never more (the same case with 256 / 512 /
+    // 1024: 37 / 31 / 35; 192 rows, rank 64, with 576: 24.8 for 17.8). A
+    // row tile's workgroups are a multiple of 8, so that the same outputs' B goes
+    // to the same XCD's L2, where that drops few of them (320 rows, rank 64, 48
+    // for 51: 22.7 / 24.8; 700 rows, rank 16, 16 for 23: 29.0 / 27.5).
+    const int rb = a->n_row <= 256 ? 1 : 2, nrt = ceil_div(a->n_row, 16 * rb);
+    int gx = 512 / nrt;
+    if (gx >= 24) gx -= gx % 8;
     if (gx > ceil_div(a->n_out, 4 * LU_OUT)) gx = ceil_div(a->n_out, 4 * LU_OUT);
     if (gx < 1) gx = 1;
     // (the sort's counts, 8 KB, fit before it)

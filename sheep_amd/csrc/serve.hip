@@ -2,8 +2,6 @@
 // cache's append and attention, low-rank adapters, and the rules on logits.
 #include "dev.h"
 
-typedef _Float16 v2h __attribute__((ext_vector_type(2)));
-typedef _Float16 v4h __attribute__((ext_vector_type(4)));
 typedef float v4f __attribute__((ext_vector_type(4)));
 // four floats at a float's alignment: rows start at any stride
 typedef float v4fu __attribute__((ext_vector_type(4), aligned(4)));
@@ -35,7 +33,11 @@ __device__ __forceinline__ int page_of(const sml_kpages & pg, int s, int i) {
 //
 // A thread takes four rotation pairs (d, d + hd/2) of one head of q or k, or
 // four values of v. The pair's products are the decode kernels' (one rounded,
-// the other fused), so a float16 cache equals the contiguous one.
+// the other fused), so a float16 cache equals the contiguous one. It reads and
+// writes each value once; what bounds it is the launch (16 tokens, 32 heads over
+// 8 of 128: 2.9 us of kernel in a call of 5.4) until the rows are thousands (1021
+// tokens, 12 over 2: 16 MB in 4.2 us, 3.9 TB/s). Four pairs a thread make every
+// access 8 or 16 bytes.
 template <int D, int BF>
 __device__ __forceinline__ void append_body(const sml_kappend & a) {
     constexpr int HQ = D / 8;                         // threads of a rotated head
@@ -754,9 +756,9 @@ __device__ __forceinline__ int rank_of(const sml_klora & a, int id) {
 // last, so that a mixed batch's tiles hold few adapters each. A counting sort
 // every workgroup makes for itself: 64 rows a wave, each distinct adapter's
 // lanes by ballot; cnt holds (n_adapter + 1) counts of every 64 rows. It takes
-// 1.7 us of a call, two launches; 128 rows of 16 adapters in turn (4096 to
-// 14336, rank 64) go from 50 to 26 us with it, 509 from 100 to 37, 64 from 46
-// (37 shared by four workgroups) to 29, 32 rows lose.
+// 1.7 us of a call's two launches, 0.6 where the rows lie in runs and stay. Rows
+// of 16 adapters in turn, us a call in the caller's order / by adapter (4096 to
+// 14336, rank 64): 32 rows 25.5 / 25.2, 64 34 / 26, 128 49 / 27, 509 99 / 38.
 template <int NW>
 __device__ __forceinline__ void tile_rows(const sml_klora & a, int row0, int nr, int * rows, int * cnt, int * wsum) {
     constexpr int PER = LS_ROWS / 64 / NW;
@@ -839,7 +841,9 @@ __device__ __forceinline__ unsigned long long my_rows(int id, unsigned long long
 // consecutive lanes, and loads in that order cost a cache line a lane (16
 // bytes a cycle and CU measured): rows are loaded whole, 128 or 256 bytes in
 // consecutive lanes, and handed over through the wave's part of LDS, at a
-// stride of LD_ROW bytes that spreads 16 rows over all banks.
+// stride of LD_ROW bytes that spreads 16 rows over all banks. 509 rows of 4096,
+// rank 64: 10 us, of which a second adapter in a tile's rows takes 2; the reads
+// of x alone (8 MB, each once) would be 2.
 template <int BF>
 __device__ __forceinline__ void lora_down_body(const sml_klora & a) {
     using M = Mx<BF>;
@@ -968,7 +972,9 @@ __device__ __forceinline__ void lora_down_body(const sml_klora & a) {
 // than a second launch costs while A is small. A step holds a row or two of an
 // adapter, too few for the matrix cores' 16 columns (converting all 16 made
 // this 12.6 us for 8.5): the first product is a lane's own fused multiply-adds
-// on 8 inputs of 8 ranks at a time, summed over the wave by halves.
+// on 8 inputs of 8 ranks at a time, summed over the wave by halves. 16 rows of
+// 16 adapters, 4096 to 4096, rank 16: 8.5 us, a chain of latencies (ids, A and x,
+// two exchanges in LDS, B) around 4 MB that would take 1.
 template <int BF>
 __device__ __forceinline__ void lora_few_body(const sml_klora & a) {
     using M = Mx<BF>;
@@ -1098,7 +1104,9 @@ __device__ __forceinline__ void lora_few_body(const sml_klora & a) {
 // on their way before the present one's products. Rows are the products'
 // rows, and column c of product u is output 4c + u of the block: a lane then
 // holds four outputs side by side and 16 lanes 256 bytes of a row. B's rows
-// come through the wave's part of LDS as A's do above.
+// come through the wave's part of LDS as A's do above. 509 rows to 14336, rank
+// 64: 21.6 us, 58 MB of base and y at 2.7 TB/s: about 3 us join t's splits ahead
+// of the first product, and tiles that hold two adapters take 2 more.
 template <int BF, int RB>
 __device__ __forceinline__ void lora_up_body(const sml_klora & a) {
     using M = Mx<BF>;
