@@ -118,9 +118,13 @@ int sml_hip_paged_attention(const sml_hip_pages * pg, const float * q, size_t q_
     char name[40];
     sv_name(name, sizeof name, "sml_sv_attend", pg->hd, pg->type);
     hx_launch3(name, (unsigned) pg->n_kv, (unsigned) grid, shared ? 1 : (unsigned) pg->n_seq, 256, 0, (hipStream_t) stream, &a);
-    if (n > a.chunk)
-        hx_launch(pg->hd == 64 ? "sml_sv_merge_d64" : "sml_sv_merge", (unsigned) n_head, (unsigned) pg->n_seq, 256, 0,
-                  (hipStream_t) stream, &a);
+    if (n > a.chunk) {
+        // more threads a row while the workgroups are at most 2 a CU (measured
+        // beside the kernel)
+        const int nt = (long) n_head * pg->n_seq <= 2L * hx.ncu ? 512 : 256;
+        snprintf(name, sizeof name, "sml_sv_merge%s_%d", pg->hd == 64 ? "_d64" : "", nt);
+        hx_launch(name, (unsigned) n_head, (unsigned) pg->n_seq, (unsigned) nt, 0, (hipStream_t) stream, &a);
+    }
     HX_LEAVE();
     return 0;
 }

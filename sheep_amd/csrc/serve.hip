@@ -451,12 +451,15 @@ __device__ __forceinline__ void attend_body(const sml_kattend & a) {
 }
 
 // The splits of a row joined: a workgroup a (sequence, head), D threads a
-// share of its splits.
-#define AM_THREADS 256
-template <int D>
+// share of its splits. Latency bounds it: the lengths, the splits' bases, then
+// each share's rows, eight in flight. us a call with its attention, 256 / 512 /
+// 1024 threads: 28 heads, one sequence at 65537 (129 splits) 30.6 / 29.2 / 29.7,
+// 32 heads, 4 of 3000 17.0 / 16.3 / 16.4, but 200 of up to 2000 (6400 workgroups)
+// 74 / 80 / 93.
+template <int D, int NT>
 __device__ __forceinline__ void attend_merge_body(const sml_kattend & a) {
-    constexpr int S = AM_THREADS / D;                 // shares
-    __shared__ float f[256], red[S][D], sred[AM_THREADS / 64];
+    constexpr int S = NT / D;                         // shares
+    __shared__ float f[256], red[S][D], sred[NT / 64];
     const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
     int per;
     const int ns = at_splits(at_len(a, b), at_size(a, tid & 63), per);
@@ -470,9 +473,9 @@ __device__ __forceinline__ void attend_merge_body(const sml_kattend & a) {
     __syncthreads();
     m = sred[0];
     #pragma unroll
-    for (int w = 1; w < AM_THREADS / 64; w++) m = fmaxf(m, sred[w]);
+    for (int w = 1; w < NT / 64; w++) m = fmaxf(m, sred[w]);
     const float e = __builtin_amdgcn_exp2f(ml.x - (m == -INFINITY ? 0.0f : m));
-    f[tid] = e;
+    if (NT == 256 || tid < 256) f[tid] = e;
     __syncthreads();                                  // f is whole, and sred read by all
     const float lw = wave_sum(e * ml.y);
     if (!(tid & 63)) sred[tid >> 6] = lw;
@@ -485,13 +488,17 @@ __device__ __forceinline__ void attend_merge_body(const sml_kattend & a) {
     if (tid >= D) return;
     float l = 0.0f;
     #pragma unroll
-    for (int w = 0; w < AM_THREADS / 64; w++) l += sred[w];
+    for (int w = 0; w < NT / 64; w++) l += sred[w];
     #pragma unroll
     for (int s = 1; s < S; s++) o += red[s][d];
     a.out[row * D + d] = l == 0.0f ? 0.0f : o / l;
 }
-extern "C" __global__ __launch_bounds__(AM_THREADS) void sml_sv_merge(const sml_kattend a) { attend_merge_body<128>(a); }
-extern "C" __global__ __launch_bounds__(AM_THREADS) void sml_sv_merge_d64(const sml_kattend a) { attend_merge_body<64>(a); }
+#define MERGE(D, NT, name) \
+    extern "C" __global__ __launch_bounds__(NT) void name##_##NT(const sml_kattend a) { attend_merge_body<D, NT>(a); }
+MERGE(128, 256, sml_sv_merge)
+MERGE(128, 512, sml_sv_merge)
+MERGE(64, 256, sml_sv_merge_d64)
+MERGE(64, 512, sml_sv_merge_d64)
 
 #define ATTEND(D, BF, name) \
     extern "C" __global__ __launch_bounds__(64 * AT_WAVES) void name(const sml_kattend a) { attend_body<D, BF>(a); }
