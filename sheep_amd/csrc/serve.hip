@@ -980,7 +980,7 @@ __device__ __forceinline__ void lora_down_body(const sml_klora & a) {
 // adapter, too few for the matrix cores' 16 columns (converting all 16 made
 // this 12.6 us for 8.5): the first product is a lane's own fused multiply-adds
 // on 8 inputs of 8 ranks at a time, summed over the wave by halves. 16 rows of
-// 16 adapters, 4096 to 4096, rank 16: 8.5 us, a chain of latencies (ids, A and x,
+// 11 adapters, 4096 to 4096, rank 16: 8.5 us, a chain of latencies (ids, A and x,
 // two exchanges in LDS, B) around 4 MB that would take 1.
 template <int BF>
 __device__ __forceinline__ void lora_few_body(const sml_klora & a) {
