@@ -99,9 +99,10 @@ int sml_hip_paged_attention(const sml_hip_pages * pg, const float * q, size_t q_
     // workspace's of the longest sequence
     a.nsplit = ceil_div(max_len > 1 ? max_len : 1, 64);
     if (a.nsplit > 256) a.nsplit = 256;
-    // about 512 workgroups, two a CU, where the lengths are shared out (48
-    // sequences up to 8192 / one at 65537, 512: 55 and 37 us, 768: 53 and 38,
-    // 1024: 51 and 39)
+    // About 512 workgroups, two a CU, where the lengths are shared out (48
+    // sequences up to 8192 / one at 65537 / 16 of 2000 / 32 of 1000 to 9000 with
+    // 12 heads over 2, us: 512 55, 36, 32, 24; 768 54, 37, 37, 27; 1024 52, 37, 35,
+    // 27).
     // Up to 512 positions a sequence is one split, with no merge (whole / split:
     // one sequence of 256 5.9 / 8.0 us, of 512 8.0 / 8.5, of 768 9.9 / 8.8; 64 of
     // 512 23 / 26).

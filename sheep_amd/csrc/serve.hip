@@ -132,9 +132,9 @@ APPEND(64, 1, sml_sv_append_d64_bf)
 //
 // Measured with the merge, 32 heads over 8 of 128, fp16: 48 sequences up to
 // 8192 (202 MB) 55 us = 3.7 TB/s (60 with fixed splits of 512 and K in the
-// matrix cores' order from memory), one at 4095 9.7 us, of which 5.8 are this
+// matrix cores' order from memory), one at 4095 10.2 us, of which 5.8 are this
 // kernel's chain of latencies (length, table, rows, joining) and 3.8 the
-// merge's; bf16, 28 over 4, one at 65537 (134 MB) 36.7 us = 3.7 TB/s. A large
+// merge's; bf16, 28 over 4, one at 65537 (134 MB) 35 us = 3.8 TB/s. A large
 // copy reaches 4.8 TB/s. Two workgroups (212 registers) a CU: held to three,
 // 58 and 52 us.
 #define AT_WAVES 4

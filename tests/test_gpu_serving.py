@@ -668,6 +668,80 @@ def test_two_graphs_with_workspaces_of_their_own():
                 np.testing.assert_array_equal(got[k], w[k], err_msg=k)
 
 
+# ------------------------------------------------------------ sizes
+
+GUARD = 4096
+
+
+class Guarded(sa.DevBuf):
+    """A buffer of exactly the bytes asked for, with a pattern behind them."""
+
+    def __init__(self, nbytes):
+        super().__init__(nbytes + GUARD)
+        self.write(np.full(nbytes + GUARD, 0xA5, np.uint8))
+
+    def intact(self):
+        return (self.read(np.uint8)[-GUARD:] == 0xA5).all()
+
+
+@pytest.mark.parametrize("n_seq, heads, kv, hd, top", [
+    (1, 8, 2, 128, 1), (1, 8, 2, 128, 513), (1, 4, 4, 64, 70001), (7, 16, 1, 64, 1000), (40, 32, 8, 128, 600),
+    (257, 4, 2, 64, 700), (300, 2, 2, 128, 64)])
+def test_attention_stays_in_its_buffers(n_seq, heads, kv, hd, top):
+    rng = np.random.default_rng(top)
+    page = 64
+    pages = -(-top // page)
+    bits = [so.to_bits(rng.standard_normal((pages + 1, page, kv, hd)).astype(np.float32), "f16") for _ in range(2)]
+    table = np.tile(rng.permutation(pages + 1)[:pages], (n_seq, 1)).astype(np.int32)       # a prefix that all share
+    pg = serving.Pages(*map(sa.DevBuf.of, bits), sa.DevBuf.of(table), pages + 1, page, n_seq, pages, kv, hd)
+    part, out = Guarded(4 * serving.part_floats(n_seq, heads, hd, top)), Guarded(4 * n_seq * heads * hd)
+    one = rng.standard_normal(heads * hd).astype(np.float32)
+    q = sa.DevBuf.of(np.tile(one, (n_seq, 1)))
+    for lens in ([top] * n_seq, [top + 99] * n_seq, rng.integers(0, top + 1, n_seq), [0] * (n_seq - 1) + [top], [-1] * n_seq):
+        serving.attention(pg, q, ints(lens), top, heads, part, out)
+        sa.sync()
+        assert part.intact() and out.intact()
+        got = out.read(np.float32, n_seq * heads * hd).reshape(n_seq, -1)
+        assert np.isfinite(got).all()
+        if min(lens) >= top:
+            for h in range(heads):
+                kk, vv = (so.from_bits(w, "f16").reshape(-1, page, kv, hd)[table[0], :, h * kv // heads].reshape(-1, hd)[:top]
+                          for w in bits)
+                want, tol = so.attend(one[None, h * hd:(h + 1) * hd], kk, vv, hd ** -0.5)
+                within(got[:, h * hd:(h + 1) * hd], np.repeat(want, n_seq, 0), np.repeat(tol, n_seq, 0), f"head {h}")
+        assert not got[np.array(lens) <= 0].any()
+
+
+@pytest.mark.parametrize("n, n_in, n_out, rank, A", [
+    (1, 8, 1, 8, 1), (16, 520, 33, 64, 16), (17, 1544, 70, 256, 2), (40, 4096, 65, 8, 5), (200, 264, 257, 24, 16),
+    (600, 72, 130, 64, 3)])
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+def test_lora_stays_in_its_buffers(n, n_in, n_out, rank, A, dtype):
+    rng = np.random.default_rng(n)
+    a, b = (sa.DevBuf.of(so.to_bits(rng.standard_normal(sh).astype(np.float32), dtype)) for sh in ((A, rank, n_in), (A, n_out, rank)))
+    ad = serving.Adapters(a, b, A, rank, n_in, n_out, dtype)
+    x = sa.DevBuf.of(rng.standard_normal((n, n_in)).astype(np.float32))
+    y, work = Guarded(4 * n * n_out), Guarded(4 * serving.lora_work_floats(rank, n))
+    for ids in (rng.integers(-1, A, n), np.arange(n) * A // n, np.full(n, -1)):
+        serving.lora(ad, x, n, ints(ids), y, work)
+        sa.sync()
+        assert y.intact() and work.intact()
+        got = y.read(np.float32, n * n_out).reshape(n, n_out)
+        assert not got[ids < 0].any() and (got[ids >= 0] != 0).any(axis=1).all()
+
+
+@pytest.mark.parametrize("n_row, V", [(1, 1), (3, 2047), (2, 2049), (70, 4098), (600, 2050)])
+def test_logits_stay_in_their_buffers(n_row, V):
+    rng = np.random.default_rng(V)
+    x = rng.standard_normal((n_row, V)).astype(np.float32)
+    out, tok, part = Guarded(4 * n_row * V), Guarded(4 * n_row), Guarded(serving.logits_part_bytes(n_row, V))
+    serving.adjust_logits(sa.DevBuf.of(x), n_row, V, out=out, tok=tok, part=part)
+    sa.sync()
+    assert out.intact() and tok.intact() and part.intact()
+    np.testing.assert_array_equal(out.read(np.float32, n_row * V).reshape(n_row, V), x)
+    np.testing.assert_array_equal(tok.read(np.int32, n_row), x.argmax(1))
+
+
 # ------------------------------------------------------------ a run of them together
 
 def test_requests_decode_together(tmpdir_s):
