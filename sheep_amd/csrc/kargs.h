@@ -524,7 +524,8 @@ typedef struct {
 #define LS_ROWS 512               // the most rows that are sorted by adapter, and the adapters then
 #define LS_ADAPTERS 255
 #define LU_OUT 64                 // outputs of a wave's block of y
-#define LD_WAVE_LDS(parts) ((64 + 16 * (parts)) * LD_ROW + 64)
+// LDS of a wave of A x, rt tiles of 16 ranks
+#define LD_WAVE_LDS(parts, rt) (16 * ((rt) + (parts)) * LD_ROW + 64)
 typedef struct {
     const uint16_t * a, * b;
     const float * scale;

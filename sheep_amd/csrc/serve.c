@@ -205,29 +205,40 @@ static void lora_launch(sml_klora * a, int bf, hipStream_t st) {
         return;
     }
     // workgroups share a tile's distinct adapters while there are few tiles (32
-    // rows of 16 adapters, 4096 to 14336, rank 16: 36 us with 1, 21 with 4, 33
-    // with 16), and tiles take more rows by adapter
+    // rows of 16 adapters, 4096 to 14336, rank 16: 35 us with 1, 20 with 4, 33
+    // with 16); above 32 rows tiles take theirs by adapter
     const int nz = a->n_row <= 32 ? (few < 4 ? few : 4) : a->n_row <= 64 ? 2 : 1;
     a->sorted = a->n_row > 32 && a->n_row <= LS_ROWS && a->n_adapter > 1 && a->n_adapter <= LS_ADAPTERS;
-    // t: the inputs split for 128 workgroups, as far as the workspace holds
-    // them (509 rows of 4 adapters, 4096 to 14336, rank 64, a call at 2, 4 and 8
-    // splits: 34.4, 31.2, 31.7 us; every workgroup of y joins them)
+    // t: the inputs split for 128 workgroups of 64 ranks, twice as many of up to
+    // 16, as far as the workspace holds them (509 rows, us a call at half / so /
+    // twice: rank 64, 4096 to 14336 30.6 / 29.5 / 33.3, rank 16, 14336 to 4096
+    // 21.1 / 20.0 / -): every workgroup of y joins them, so that splits times
+    // ranks stay within 768 too (14336 to 4096, with that and without: 16 rows,
+    // rank 64 16.2 / 20.8, 32 rows, rank 128 19.6 / 31.8, 1 row, rank 256 22.6 /
+    // 21.9).
     const int ntile = ceil_div(a->n_row, LD_ROWS), ngroup = ceil_div(a->rank, 64);
     int most = 8192 / a->n_row < 32 ? 8192 / a->n_row : 32;
-    const int want = ceil_div(128, ntile * ngroup);
+    if (most > 768 / a->rank) most = 768 / a->rank;
+    const int want = ceil_div(a->rank <= 16 ? 256 : 128, ntile * ngroup);
     if (most > want) most = want;
     if (most < 1) most = 1;
     a->chunk = LD_TILE;
     while (ceil_div(a->n_in, a->chunk) > most) a->chunk += LD_TILE;
     a->nsplit = ceil_div(a->n_in, a->chunk);
-    hx_launch3(bf ? "sml_sv_lora_down_bf" : "sml_sv_lora_down", (unsigned) a->nsplit, (unsigned) ntile,
-               (unsigned) (nz * ngroup), 64 * LD_WAVES, (size_t) LD_WAVES * LD_WAVE_LDS(parts), st, a);
+    // 32 ranks a workgroup, of low ranks or few rows 16 (us a call at 16 / 32: 16
+    // rows, rank 64, 14336 to 4096 16.2 / 17.3, 32 rows, rank 16, 4096 to 4096 11.3
+    // / 11.6; 144 rows, rank 64, 14336 to 4096 21.0 / 18.2)
+    const int rt = a->rank <= 16 || a->n_row <= 64 ? 1 : 2;
+    char name[40];
+    snprintf(name, sizeof name, "sml_sv_lora_down%d%s", rt, bf ? "_bf" : "");
+    hx_launch3(name, (unsigned) a->nsplit, (unsigned) ntile, (unsigned) (nz * ceil_div(a->rank, 16 * rt)), 64 * LD_WAVES,
+               (size_t) LD_WAVES * LD_WAVE_LDS(parts, rt), st, a);
     // y: 32 rows a workgroup of a prompt (us a call at 16 / 32, one adapter: 192
     // rows, 4096 to 14336, rank 64 17.8 / 19.3, 14336 to 4096 19.5 / 23.4; 384
     // rows 24.5 / 24.3 and 23.8 / 25.9, 1536 to 8960, rank 8 18.7 / 14.9; 509
     // rows of 4 adapters in runs 33.6 / 31.5, 30.8 / 27.0 at rank 16), and the
     // 512 workgroups that run at once, never more (the same case with 256 / 512 /
-    // 1024: 37 / 31 / 35; 192 rows, rank 64, with 576: 24.8 for 17.8). A
+    // 1024: 35 / 30 / 34; 192 rows, rank 64, with 576: 24.8 for 17.8). A
     // row tile's workgroups are a multiple of 8, so that the same outputs' B goes
     // to the same XCD's L2, where that drops few of them (320 rows, rank 64, 48
     // for 51: 22.7 / 24.8; 700 rows, rank 16, 16 for 23: 29.0 / 27.5).
@@ -238,7 +249,6 @@ static void lora_launch(sml_klora * a, int bf, hipStream_t st) {
     if (gx < 1) gx = 1;
     // (the sort's counts, 8 KB, fit before it)
     const size_t lds = (size_t) 4 * LU_OUT * LD_ROW + (size_t) 16 * rb * (4 + (size_t) parts * ((size_t) ngroup * 64 + 8) * 2);
-    char name[40];
     snprintf(name, sizeof name, "sml_sv_lora_up%d%s", rb, bf ? "_bf" : "");
     hx_launch3(name, (unsigned) gx, (unsigned) nrt, (unsigned) nz, 256, lds, st, a);
 }

@@ -740,12 +740,12 @@ extern "C" __global__ __launch_bounds__(64) void sml_sv_pick(const sml_klogits a
 // A few rows take one launch (lora_few_body), others two: t = A x, split over
 // the inputs, then y, whose workgroups join the splits. us a call, one launch /
 // two (fp16; "8 of 4" is 8 rows of 4 adapters):
-//   rank 16, 4096 to 4096: 1 of 1 5.4 / 11.0, 4 of 4 5.7 / 11.8, 8 of 1 10.1 /
-//   11.7, 16 of 16 7.8 / 19; 4096 to 14336: 4 of 4 6.0 / 12.1, 8 of 8 (448
-//   workgroups) 11.8 / 14.4, 12 of 12 (672) 18.5 / 16.7; 14336 to 4096: 1 of 1
-//   9.0 / 12.8, 4 of 4 9.5 / 13.8, 4 of 1 15 / 13.3; rank 64, 4096 to 4096: 4 of
-//   4 11.0 / 14.7, 4 of 1 17.5 / 13.7; rank 8, 1536 to 8960: 16 of 16 (560) 16.6
-//   / 18.8.
+//   rank 16, 4096 to 4096: 1 of 1 5.3 / 10.6, 4 of 4 5.8 / 11.3, 8 of 1 10.1 /
+//   11.3, 16 of 16 7.9 / 18; 4096 to 14336: 4 of 4 6.0 / 11.6, 8 of 8 (448
+//   workgroups) 11.6 / 13.9, 12 of 12 (672) 18.3 / 15.8; 14336 to 4096: 1 of 1
+//   8.9 / 12.4, 4 of 4 9.6 / 13.3, 4 of 1 14.9 / 12.8; rank 64, 4096 to 4096: 4 of
+//   4 10.9 / 13.4, 4 of 1 17.4 / 12.5; rank 8, 1536 to 8960: 16 of 16 (560) 16.5
+//   / 18.
 // So one launch pays while its waves have few rows' products to make in their
 // lanes and the workgroups, each reading its adapter's A again, are not many.
 
@@ -765,7 +765,7 @@ __device__ __forceinline__ int rank_of(const sml_klora & a, int id) {
 // lanes by ballot; cnt holds (n_adapter + 1) counts of every 64 rows. It takes
 // 1.7 us of a call's two launches, 0.6 where the rows lie in runs and stay. Rows
 // of 16 adapters in turn, us a call in the caller's order / by adapter (4096 to
-// 14336, rank 64): 32 rows 25.5 / 25.2, 64 34 / 26, 128 49 / 27, 509 99 / 38.
+// 14336, rank 64): 32 rows 22.9 / 22.8, 64 29 / 23, 128 46 / 26, 509 92 / 36.
 template <int NW>
 __device__ __forceinline__ void tile_rows(const sml_klora & a, int row0, int nr, int * rows, int * cnt, int * wsum) {
     constexpr int PER = LS_ROWS / 64 / NW;
@@ -843,29 +843,29 @@ __device__ __forceinline__ unsigned long long my_rows(int id, unsigned long long
     return mine;
 }
 
-// A x: a workgroup takes a tile of 16 rows, 64 ranks and a split of the inputs,
-// a wave every eighth 64 of those. The matrix cores want 16 rows in 16
+// A x: a workgroup takes a tile of 16 rows, RT of 16 ranks and a split of the
+// inputs, a wave every eighth 64 of those. The matrix cores want 16 rows in 16
 // consecutive lanes, and loads in that order cost a cache line a lane (16
 // bytes a cycle and CU measured): rows are loaded whole, 128 or 256 bytes in
 // consecutive lanes, and handed over through the wave's part of LDS, at a
 // stride of LD_ROW bytes that spreads 16 rows over all banks. 509 rows of 4096,
-// rank 64: 10 us, of which a second adapter in a tile's rows takes 2; the reads
-// of x alone (8 MB, each once) would be 2.
-template <int BF>
+// rank 64: 8.7 us, of which a second adapter in a tile's rows takes 1.6; the
+// reads of x alone (8 MB, each once) would be 2.
+template <int BF, int RT>
 __device__ __forceinline__ void lora_down_body(const sml_klora & a) {
     using M = Mx<BF>;
     typedef typename M::v8 v8;
     typedef typename M::t T;
     typedef T v4t __attribute__((ext_vector_type(4)));
-    constexpr int NP = M::parts, RT = 4, RS = 16 * RT + 1;
+    constexpr int NP = M::parts, NR = 16 * RT, RS = NR + 1;
     extern __shared__ __align__(16) uint8_t lds[];
     const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    uint8_t * const la = lds + wave * LD_WAVE_LDS(NP);              // [rank][LD_ROW]
-    uint8_t * const lx = la + 64 * LD_ROW;                          // [part][row][LD_ROW]
+    uint8_t * const la = lds + wave * LD_WAVE_LDS(NP, RT);          // [rank][LD_ROW]
+    uint8_t * const lx = la + NR * LD_ROW;                          // [part][row][LD_ROW]
     int * const le = (int *) (lx + NP * 16 * LD_ROW);               // [row]
-    const int split = blockIdx.x, row0 = blockIdx.y * 16, ngroup = (a.rank + 63) / 64, nz = gridDim.z / ngroup;
-    const int j0 = (blockIdx.z % ngroup) * 64, z = blockIdx.z / ngroup;
+    const int split = blockIdx.x, row0 = blockIdx.y * 16, ngroup = (a.rank + NR - 1) / NR, nz = gridDim.z / ngroup;
+    const int j0 = (blockIdx.z % ngroup) * NR, z = blockIdx.z / ngroup;
     const int k0 = split * a.chunk, k1 = min(a.n_in, k0 + a.chunk);
     __shared__ int rows[16], wsum[LD_WAVES];
     tile_rows<LD_WAVES>(a, row0, 16, rows, (int *) lds, wsum);
@@ -878,17 +878,17 @@ __device__ __forceinline__ void lora_down_body(const sml_klora & a) {
     #pragma unroll
     for (int i = 0; i < 4; i++) xrow[i] = a.x + (size_t) max(rows[4 * i + g], 0) * a.x_stride;
     v4f xr[4];
-    v4u ar[8], an[8];
+    v4u ar[2 * RT], an[2 * RT];
     auto load_x = [&](int kb) {
         const int kk = min(kb + 4 * c, k1 - 4);
         #pragma unroll
         for (int i = 0; i < 4; i++) xr[i] = *(const GLOBAL v4fu *) (xrow[i] + kk);
     };
-    auto load_a = [&](v4u (&r)[8], int ad, int kb) {
+    auto load_a = [&](v4u (&r)[2 * RT], int ad, int kb) {
         const int kk = min(kb + 8 * (lane & 7), k1 - 8);
         const uint16_t * w = a.a + (size_t) ad * a.rank * a.n_in + kk;
         #pragma unroll
-        for (int i = 0; i < 8; i++)
+        for (int i = 0; i < 2 * RT; i++)
             if (i < 2 * nt) r[i] = *(const GLOBAL v4u *) (w + (size_t) min(j0 + 8 * i + (lane >> 3), a.rank - 1) * a.n_in);
     };
     v4f tot[RT];
@@ -921,7 +921,7 @@ __device__ __forceinline__ void lora_down_body(const sml_klora & a) {
         unsigned left = all;
         for (int cur = first; left;) {
             #pragma unroll
-            for (int i = 0; i < 8; i++)
+            for (int i = 0; i < 2 * RT; i++)
                 if (i < 2 * nt) {
                     if (kb + 8 * (lane & 7) >= k1) ar[i] = v4u(0u);
                     *(v4u *) (la + (8 * i + (lane >> 3)) * LD_ROW + 16 * (lane & 7)) = ar[i];
@@ -953,7 +953,7 @@ __device__ __forceinline__ void lora_down_body(const sml_klora & a) {
             wave_lds();                               // all read before the next is written
             cur = then;
             #pragma unroll
-            for (int i = 0; i < 8; i++) ar[i] = an[i];
+            for (int i = 0; i < 2 * RT; i++) ar[i] = an[i];
         }
     }
     __syncthreads();                                  // the waves' parts become one
@@ -963,8 +963,8 @@ __device__ __forceinline__ void lora_down_body(const sml_klora & a) {
         #pragma unroll
         for (int r = 0; r < 4; r++) red[(wave * 16 + c) * RS + 16 * t + 4 * g + r] = tot[t][r];
     __syncthreads();
-    for (int i = tid; i < 256 * RT; i += 64 * LD_WAVES) {
-        const int rw = i / (16 * RT), j = i % (16 * RT);
+    for (int i = tid; i < 16 * NR; i += 64 * LD_WAVES) {
+        const int rw = i / NR, j = i % NR;
         float s = 0.0f;
         #pragma unroll
         for (int v = 0; v < LD_WAVES; v++) s += red[(v * 16 + rw) * RS + j];
@@ -1112,8 +1112,8 @@ __device__ __forceinline__ void lora_few_body(const sml_klora & a) {
 // rows, and column c of product u is output 4c + u of the block: a lane then
 // holds four outputs side by side and 16 lanes 256 bytes of a row. B's rows
 // come through the wave's part of LDS as A's do above. 509 rows to 14336, rank
-// 64: 21.6 us, 58 MB of base and y at 2.7 TB/s: about 3 us join t's splits ahead
-// of the first product, and tiles that hold two adapters take 2 more.
+// 64: 22 us, 58 MB of base and y at 2.7 TB/s: about 3 us join t's splits ahead of
+// the first product, and tiles that hold two adapters take 4 more.
 template <int BF, int RB>
 __device__ __forceinline__ void lora_up_body(const sml_klora & a) {
     using M = Mx<BF>;
@@ -1308,7 +1308,8 @@ __device__ __forceinline__ void lora_up_body(const sml_klora & a) {
     }
 }
 #define LORA(BF, sfx) \
-    extern "C" __global__ __launch_bounds__(64 * LD_WAVES) void sml_sv_lora_down##sfx(const sml_klora a) { lora_down_body<BF>(a); } \
+    extern "C" __global__ __launch_bounds__(64 * LD_WAVES) void sml_sv_lora_down2##sfx(const sml_klora a) { lora_down_body<BF, 2>(a); } \
+    extern "C" __global__ __launch_bounds__(64 * LD_WAVES) void sml_sv_lora_down1##sfx(const sml_klora a) { lora_down_body<BF, 1>(a); } \
     extern "C" __global__ __launch_bounds__(256) void sml_sv_lora_up2##sfx(const sml_klora a) { lora_up_body<BF, 2>(a); } \
     extern "C" __global__ __launch_bounds__(256) void sml_sv_lora_up1##sfx(const sml_klora a) { lora_up_body<BF, 1>(a); } \
     extern "C" __global__ __launch_bounds__(64 * LF_WAVES) void sml_sv_lora_few##sfx(const sml_klora a) { lora_few_body<BF>(a); }
