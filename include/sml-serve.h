@@ -34,6 +34,8 @@ enum { SML_F16 = 0, SML_BF16 = 1 };
 // Position p of sequence s lies in page table[s * seq_pages + p / page_size].
 // A table entry outside 0..n_pages-1 (-1 by custom) is no page: nothing is
 // written there, and attention leaves its positions out.
+// Sequences may name the same pages (a common prefix, or several rows of one
+// request).
 typedef struct {
     uint16_t * k, * v;            // the pools, 16-byte aligned
     const int32_t * table;        // [n_seq][seq_pages]
