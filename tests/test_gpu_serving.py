@@ -668,6 +668,30 @@ def test_two_graphs_with_workspaces_of_their_own():
                 np.testing.assert_array_equal(got[k], w[k], err_msg=k)
 
 
+def test_captured_adapters_take_new_ids():
+    """A mixed batch captured once and replayed with other ids, in no order, in
+    runs and without any: every replay equals the eager call bit for bit."""
+    rng = np.random.default_rng(9)
+    n, n_in, n_out, rank, A = 100, 264, 130, 16, 7
+    a, b = (sa.DevBuf.of(so.to_bits(rng.standard_normal(sh).astype(np.float32), "f16")) for sh in ((A, rank, n_in), (A, n_out, rank)))
+    ad = serving.Adapters(a, b, A, rank, n_in, n_out)
+    x, base = (sa.DevBuf.of(rng.standard_normal(sh).astype(np.float32)) for sh in ((n, n_in), (n, n_out)))
+    work, y, ids = sa.DevBuf(4 * serving.lora_work_floats(rank, n)), sa.DevBuf(4 * n * n_out), ints(np.zeros(n))
+    hip = Hip()
+    sa.sync()
+    ex = hip.capture(lambda: serving.lora(ad, x, n, ids, y, work, base=base, stream=hip.stream.value))
+    for which in (rng.integers(-1, A, n), np.arange(n) * A // n, np.full(n, -1), np.arange(n) % A, np.zeros(n)):
+        ids.write(np.array(which, np.int32))
+        serving.lora(ad, x, n, ids, y, work, base=base)
+        sa.sync()
+        want = y.read(np.uint32)
+        for buf in (y, work):
+            buf.write(np.full(buf.nbytes, 0xFF, np.uint8))
+        sa.sync()
+        hip.replay(ex)
+        np.testing.assert_array_equal(y.read(np.uint32), want)
+
+
 # ------------------------------------------------------------ sizes
 
 GUARD = 4096
