@@ -204,10 +204,6 @@ static void lora_launch(sml_klora * a, int bf, hipStream_t st) {
                   64 * LF_WAVES, (size_t) parts * 16 * LF_LD * 2 + 64 + sums, st, a);
         return;
     }
-    // workgroups share a tile's distinct adapters while there are few tiles (32
-    // rows of 16 adapters, 4096 to 14336, rank 16: 35 us with 1, 20 with 4, 33
-    // with 16); above 32 rows tiles take theirs by adapter
-    const int nz = a->n_row <= 32 ? (few < 4 ? few : 4) : a->n_row <= 64 ? 2 : 1;
     a->sorted = a->n_row > 32 && a->n_row <= LS_ROWS && a->n_adapter > 1 && a->n_adapter <= LS_ADAPTERS;
     // t: the inputs split for 128 workgroups of 64 ranks, twice as many of up to
     // 16, as far as the workspace holds them (509 rows, us a call at half / so /
@@ -229,10 +225,6 @@ static void lora_launch(sml_klora * a, int bf, hipStream_t st) {
     // rows, rank 64, 14336 to 4096 16.2 / 17.3, 32 rows, rank 16, 4096 to 4096 11.3
     // / 11.6; 144 rows, rank 64, 14336 to 4096 21.0 / 18.2)
     const int rt = a->rank <= 16 || a->n_row <= 64 ? 1 : 2;
-    char name[40];
-    snprintf(name, sizeof name, "sml_sv_lora_down%d%s", rt, bf ? "_bf" : "");
-    hx_launch3(name, (unsigned) a->nsplit, (unsigned) ntile, (unsigned) (nz * ceil_div(a->rank, 16 * rt)), 64 * LD_WAVES,
-               (size_t) LD_WAVES * LD_WAVE_LDS(parts, rt), st, a);
     // y: 32 rows a workgroup of a prompt (us a call at 16 / 32, one adapter: 192
     // rows, 4096 to 14336, rank 64 17.8 / 19.3, 14336 to 4096 19.5 / 23.4; 384
     // rows 24.5 / 24.3 and 23.8 / 25.9, 1536 to 8960, rank 8 18.7 / 14.9; 509
@@ -247,7 +239,20 @@ static void lora_launch(sml_klora * a, int bf, hipStream_t st) {
     if (gx >= 24) gx -= gx % 8;
     if (gx > ceil_div(a->n_out, 4 * LU_OUT)) gx = ceil_div(a->n_out, 4 * LU_OUT);
     if (gx < 1) gx = 1;
-    // (the sort's counts, 8 KB, fit before it)
+    // a tile's distinct adapters are shared out while both launches then stay
+    // within the workgroups that run at once (us a call with 1 / 2 / 4 / 8 / 16
+    // shares, rank 16: 32 rows of 32 adapters, 4096 to 4096 35 / 25 / 18.5 / 15.3 /
+    // 14.2, 4096 to 14336 35 / 25.5 / 20.3 / 25 / 33; 64 of 64, 4096 to 4096 46 / 35
+    // / 29 / 26 / 38, 14336 to 4096 53 / 39 / 33 / 41 / 68; 128 of 64, 4096 to 14336
+    // 41 / 49 / 67)
+    const int down = a->nsplit * ntile * ceil_div(a->rank, 16 * rt), up = gx * nrt;
+    int nz = 1;
+    while (2 * nz <= few && 2 * nz <= a->n_adapter && 2 * nz * down <= 512 && 2 * nz * up <= 512) nz *= 2;
+    char name[40];
+    snprintf(name, sizeof name, "sml_sv_lora_down%d%s", rt, bf ? "_bf" : "");
+    hx_launch3(name, (unsigned) a->nsplit, (unsigned) ntile, (unsigned) (nz * ceil_div(a->rank, 16 * rt)), 64 * LD_WAVES,
+               (size_t) LD_WAVES * LD_WAVE_LDS(parts, rt), st, a);
+    // (the sort's counts, 8 KB, fit before the rest)
     const size_t lds = (size_t) 4 * LU_OUT * LD_ROW + (size_t) 16 * rb * (4 + (size_t) parts * ((size_t) ngroup * 64 + 8) * 2);
     snprintf(name, sizeof name, "sml_sv_lora_up%d%s", rb, bf ? "_bf" : "");
     hx_launch3(name, (unsigned) gx, (unsigned) nrt, (unsigned) nz, 256, lds, st, a);
