@@ -220,15 +220,20 @@ __device__ __forceinline__ int scale_of(float mx) {
     return mx > 0.0f && mx < INFINITY ? __builtin_amdgcn_frexp_expf(mx) - 11 : 0;
 }
 
-// Elements e and e + 1 of the parts of x and y: each part the rounding of what
-// is left, which the subtraction leaves exactly.
+// Elements e and e + 1 of the parts of x and y: each part what its type holds of
+// what is left, which the subtraction leaves exactly. fp16 rounds (the scaled
+// values stay below its largest); bfloat16 cuts off, so that the largest fp32
+// values do not round up to an infinity, and three cut parts of 8 bits are all
+// of the 24.
 template <int BF>
 __device__ __forceinline__ void parts_of(float x, float y, typename Mx<BF>::v8 (&p)[Mx<BF>::parts], int e) {
     typedef typename Mx<BF>::t v2t __attribute__((ext_vector_type(2)));
     typedef float v2f __attribute__((ext_vector_type(2)));
     #pragma unroll
     for (int k = 0; k < Mx<BF>::parts; k++) {
-        const v2t h = __builtin_convertvector(v2f{x, y}, v2t);
+        v2t h;
+        if constexpr (BF) h = __builtin_bit_cast(v2t, __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, y), __builtin_bit_cast(uint32_t, x), 0x07060302u));
+        else h = __builtin_convertvector(v2f{x, y}, v2t);
         p[k][e] = h[0];
         p[k][e + 1] = h[1];
         x = __builtin_fmaf((float) h[0], -1.0f, x);
