@@ -112,11 +112,15 @@ APPEND(64, 1, sml_sv_append_d64_bf)
 //   is 4 D/16 byte permutes in the lane, and lane (c, g) ends with dims
 //   (D/4)g.. of head c: the base's rescaling is a lane's own too.
 // q and the weights are split into parts of the cache's type (two of fp16,
-// three of bf16: 22 and 24 bits), a matrix instruction each; q's row is scaled
-// by a power of two to below 2^11 first so that fp16 holds it. The base
-// starts 10 below the first maximum and moves when a score passes it by 15:
-// weights then lie up to 2^15, fp16's range, and those that its smallest
-// steps round are 2^-34 of the largest.
+// three of bf16: 22 and 24 bits), a matrix instruction each. fp16 has little
+// range: q's row is scaled by a power of two to below 2^11 first, and the base
+// starts 10 below the first maximum and moves when a score passes it by 15, so
+// that weights lie up to 2^15 and those that fp16's smallest steps round are
+// 2^-34 of the largest. bf16 has fp32's, and so may its keys and values: there
+// q stays as it is, and the base starts 8 above the maximum and moves when a
+// score passes it, so that weights of 1 at most add nothing to what the sums
+// of the definition need. (The base thus moves when the maximum has risen by 5
+// or 8, which few tiles see.)
 //
 // Pages are looked up a tile ahead, once per 16 positions (a page is a
 // multiple of 16). Positions past the length or on absent pages are loaded
@@ -206,12 +210,14 @@ template <> struct Mx<0> {
     typedef _Float16 t;
     typedef t v8 __attribute__((ext_vector_type(8)));
     static constexpr int parts = 2;
+    static constexpr float lift = -10.0f, room = 15.0f;   // of the base over a maximum, of a score over the base
     static __device__ __forceinline__ v4f mul(v8 a, v8 b, v4f c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 };
 template <> struct Mx<1> {
     typedef __bf16 t;
     typedef t v8 __attribute__((ext_vector_type(8)));
     static constexpr int parts = 3;
+    static constexpr float lift = 8.0f, room = 0.0f;
     static __device__ __forceinline__ v4f mul(v8 a, v8 b, v4f c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 };
 
@@ -276,7 +282,7 @@ __device__ __forceinline__ void attend_body(const sml_kattend & a) {
             }
         mx = fmaxf(mx, __shfl_xor(mx, 16));
         mx = fmaxf(mx, __shfl_xor(mx, 32));
-        const int ex = scale_of(mx);
+        const int ex = BF ? 0 : scale_of(mx);
         #pragma unroll
         for (int j = 0; j < NJ; j++)
             #pragma unroll
@@ -382,10 +388,10 @@ __device__ __forceinline__ void attend_body(const sml_kattend & a) {
         for (int h = 0; h < 2; h++)
             #pragma unroll
             for (int r = 0; r < 4; r++) mx = fmaxf(mx, s[h][r]);
-        if (__any(mx > base + 15.0f)) {
+        if (__any(mx > base + M::room)) {
             mx = fmaxf(mx, __shfl_xor(mx, 16));
             mx = fmaxf(mx, __shfl_xor(mx, 32));
-            const float to = mx > base + 15.0f ? mx - 10.0f : base;
+            const float to = mx > base + M::room ? mx + M::lift : base;
             const float al = __builtin_amdgcn_exp2f(base - (to == -INFINITY ? 0.0f : to));
             l *= al;
             #pragma unroll

@@ -24,6 +24,81 @@ def within(got, want, tol, what=""):
     assert off == 0, f"{what}: {off} of {got.size} off"
 
 
+# ------------------------------------------------------------ attention
+
+def attend(q, k, v, dtype, scale=0.0):
+    """One sequence of all rows k, v [n][kv][hd] (16-bit), pages of 16."""
+    (heads, hd), (n, kv, _) = q.shape, k.shape
+    pages = -(-n // 16)
+    pad = np.zeros((16 * pages - n, kv, hd), np.uint16)
+    pg = serving.Pages(*(sa.DevBuf.of(np.concatenate([x, pad])) for x in (k, v)), ints(range(pages)), pages, 16, 1, pages,
+                       kv, hd, dtype)
+    out, part = sa.DevBuf(4 * heads * hd), sa.DevBuf(4 * serving.part_floats(1, heads, hd, n))
+    serving.attention(pg, sa.DevBuf.of(q.astype(np.float32)), ints([n]), n, heads, part, out, scale=scale)
+    return out.read(np.float32).reshape(heads, hd)
+
+
+def check_attend(q, k, v, dtype, scale=0.0):
+    q = q.astype(np.float32)
+    got = attend(q, k, v, dtype, scale)
+    heads, kv, hd = len(q), k.shape[1], q.shape[1]
+    g = heads // kv
+    for h in range(kv):
+        want, tol = so.attend(q[h * g:(h + 1) * g], so.from_bits(k[:, h], dtype), so.from_bits(v[:, h], dtype), scale or hd ** -0.5)
+        within(got[h * g:(h + 1) * g], want, tol, f"kv head {h}")
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("n", [1, 40, 900])
+@pytest.mark.parametrize("k_exp, q_exp, v_exp", [(118, -114, 0), (120, -118, 118), (0, 0, 120), (-100, 101, 119), (-110, 111, -100)])
+def test_bf16_range(hd, n, k_exp, q_exp, v_exp):
+    """bfloat16 keys, values and queries near fp32's largest and smallest."""
+    rng = np.random.default_rng(n + hd)
+    k, v = (so.to_bits(np.clip(rng.standard_normal((n, 2, hd)), -3, 3) * 2.0 ** e, "bf16") for e in (k_exp, v_exp))
+    check_attend(np.clip(rng.standard_normal((8, hd)), -3, 3) * 2.0 ** q_exp, k, v, "bf16")
+
+
+def test_bf16_largest_values():
+    """The largest finite value of the cache comes back; the largest query
+    meets keys that bring it down."""
+    k = np.zeros((1, 1, 64), np.uint16)
+    v = np.full((1, 1, 64), 0x7F7F, np.uint16)
+    v[..., 1::2] = 0xFF7F
+    q = np.zeros((4, 64))
+    check_attend(q, k, v, "bf16")
+    rng = np.random.default_rng(1)
+    n = 300
+    k = np.zeros((n, 1, 64))
+    k[..., 0], k[..., 9] = rng.choice([-1, 1], (2, n, 1)) * rng.uniform(0.5, 1, (2, n, 1)) * 2.0 ** -121
+    q[:, 0] = [3.4028234e38, -3.4028234e38, 3.39e38, 3e38]
+    q[2, 9] = -3.4028234e38
+    check_attend(q, so.to_bits(k, "bf16"), so.to_bits(rng.standard_normal((n, 1, 64)), "bf16"), "bf16", scale=0.02)
+
+
+def test_bf16_rising_scores_of_large_values():
+    """Scores that rise by more than the weights' base leaves room, again and
+    again, over values that leave the sums none."""
+    n, hd = 900, 64
+    k = np.zeros((n, 1, hd))
+    k[:, 0, 0] = np.arange(n)
+    rng = np.random.default_rng(2)
+    q = np.zeros((4, hd))
+    q[:, 0] = [0.5, -0.5, 2.0, 0.01]
+    check_attend(q, so.to_bits(k, "bf16"), so.to_bits(rng.uniform(-1, 1, (n, 1, hd)) * 2.0 ** 118, "bf16"), "bf16", scale=1.0)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+def test_infinite_queries_stay_in_their_heads(dtype):
+    rng = np.random.default_rng(3)
+    k, v = (so.to_bits(rng.standard_normal((700, 2, 64)), dtype) for _ in range(2))
+    q = rng.standard_normal((8, 64)).astype(np.float32)
+    clean = attend(q, k, v, dtype)
+    q[1, 5], q[6, 0], q[3, 63] = np.inf, -np.inf, np.nan
+    got = attend(q, k, v, dtype)
+    np.testing.assert_array_equal(got[[0, 2, 4, 5, 7]], clean[[0, 2, 4, 5, 7]])
+    assert np.isnan(got[[1, 3, 6]]).all()
+
+
 # ------------------------------------------------------------ adapters
 
 def lora(n, n_in, n_out, rank, A, dtype, ids, x, base=None, in_place=False, a=None, b=None, y_pad=0):
