@@ -1008,7 +1008,8 @@ __device__ __forceinline__ void lora_few_body(const sml_klora & a) {
     const int o0 = blockIdx.x * LF_OUT + wave * 16, o = o0 + 4 * g, row = c;
     const int id = adapter_of(a, row), nrg = a.rank / 8, nslice = (a.n_in + LF_SLICE - 1) / LF_SLICE;
     const bool live = row < a.n_row;
-    v4f base = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+    const float zero = a.base ? -0.0f : 0.0f;         // of outputs whose base follows behind: -0 leaves it as it is
+    v4f base = v4f{zero, zero, zero, zero};
     if (a.base && live && o + 4 <= a.n_out) base = *(const v4fu *) (a.base + (size_t) row * a.y_stride + o);
     unsigned left = (unsigned) (__ballot(id >= 0) & 0xFFFFu);
     unsigned none = a.base == a.y ? 0u : (unsigned) (__ballot(id < 0 && live) & 0xFFFFu);
@@ -1108,11 +1109,11 @@ __device__ __forceinline__ void lora_few_body(const sml_klora & a) {
         float * y = a.y + (size_t) row * a.y_stride + o;
         v4f d;
         #pragma unroll
-        for (int r = 0; r < 4; r++) d[r] = base[r] + __builtin_amdgcn_ldexpf(acc[r], ex);
+        for (int r = 0; r < 4; r++) d[r] = base[r] + (cur < 0 ? -0.0f : __builtin_amdgcn_ldexpf(acc[r], ex));
         if (o + 4 <= a.n_out) *(v4fu *) y = d;
         else
             for (int r = 0; r < 3; r++)
-                if (o + r < a.n_out) y[r] = d[r] + (a.base ? a.base[(size_t) row * a.y_stride + o + r] : 0.0f);
+                if (o + r < a.n_out) y[r] = d[r] + (a.base ? a.base[(size_t) row * a.y_stride + o + r] : -0.0f);
     }
 }
 
@@ -1170,13 +1171,16 @@ __device__ __forceinline__ void lora_up_body(const sml_klora & a) {
         #pragma unroll
         for (int i = 0; i < 8; i++) br[i] = *(const GLOBAL v4u *) (b + (size_t) min(o0 + 8 * i + (lane >> 3), a.n_out - 1) * a.rank);
     };
+    // adding -0 leaves any sum as it is: what other rows' adapters add, and
+    // where the last outputs' base follows behind
+    const float zero = a.base ? -0.0f : 0.0f;
     auto load_base = [&](v4f (&v)[RB][4], int o0) {
         const int o = o0 + 4 * c;
         #pragma unroll
         for (int h = 0; h < RB; h++)
             #pragma unroll
             for (int r = 0; r < 4; r++) {
-                v[h][r] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+                v[h][r] = v4f{zero, zero, zero, zero};
                 if (a.base && (mine4 >> (16 * h + r) & 1) && o + 4 <= a.n_out)
                     v[h][r] = *(const GLOBAL v4fu *) (a.base + (size_t) yrow[h][r] * a.y_stride + o);
             }
@@ -1296,7 +1300,7 @@ __device__ __forceinline__ void lora_up_body(const sml_klora & a) {
                 #pragma unroll
                 for (int r = 0; r < 4; r++)
                     #pragma unroll
-                    for (int u = 0; u < 4; u++) base[h][r][u] += idr[h][r] == cur ? __builtin_amdgcn_ldexpf(acc[h][u][r], ex[h][r]) : 0.0f;
+                    for (int u = 0; u < 4; u++) base[h][r][u] += idr[h][r] == cur ? __builtin_amdgcn_ldexpf(acc[h][u][r], ex[h][r]) : -0.0f;
             left = rest;
             cur = then;
         }
@@ -1310,7 +1314,7 @@ __device__ __forceinline__ void lora_up_body(const sml_klora & a) {
                 if (o + 4 <= a.n_out) *(GLOBAL v4fu *) (a.y + at) = base[h][r];
                 else
                     for (int e = 0; e < 3; e++)
-                        if (o + e < a.n_out) a.y[at + e] = base[h][r][e] + (a.base ? a.base[at + e] : 0.0f);
+                        if (o + e < a.n_out) a.y[at + e] = base[h][r][e] + (a.base ? a.base[at + e] : -0.0f);
             }
         #pragma unroll
         for (int h = 0; h < RB; h++)

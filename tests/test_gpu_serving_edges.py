@@ -131,3 +131,37 @@ def test_bf16_adapters_of_the_largest_inputs(n, n_in, n_out, rank, A):
     want, tol = so.lora(x, np.zeros((n, n_out)), so.from_bits(a, "bf16"), so.from_bits(b, "bf16"), np.ones(A, np.float32),
                         [rank] * A, ids)
     within(got, want, tol)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("n, n_in, n_out, rank, A", FORMS)
+@pytest.mark.parametrize("in_place", [False, True])
+def test_rows_without_an_adapter_keep_their_bits(n, n_in, n_out, rank, A, dtype, in_place):
+    """Zeros of either sign, infinities and NaN of the base come back as they
+    are, in the outputs past the last four too."""
+    rng = np.random.default_rng(n)
+    x = rng.standard_normal((n, n_in)).astype(np.float32)
+    base = np.where(rng.random((n, n_out + 3)) < 0.5, -0.0, 1.5).astype(np.float32)
+    base[:, 3], base[:, 5], base[:, 6] = np.nan, np.inf, -np.inf
+    base[:, -4:] = -0.0
+    for ids in (rng.integers(-1, A, n), np.where(np.arange(n) % 5 == 0, 1, -1), np.full(n, A)):
+        got, _, _ = lora(n, n_in, n_out, rank, A, dtype, ids, x, base, in_place, y_pad=3)
+        none = (ids < 0) | (ids >= A)
+        np.testing.assert_array_equal(got[none, :n_out].view(np.uint32), base[none, :n_out].view(np.uint32))
+
+
+@pytest.mark.parametrize("n, n_in, n_out, rank, A", FORMS)
+def test_zeros_do_not_depend_on_other_rows(n, n_in, n_out, rank, A):
+    """A row whose product is zero has the same bits, signs of zeros too,
+    whatever adapters the others have."""
+    rng = np.random.default_rng(n)
+    x = rng.standard_normal((n, n_in)).astype(np.float32)
+    x[::3] = 0.0
+    base = np.full((n, n_out), -0.0, np.float32)
+    seen = []
+    for _ in range(3):
+        ids = rng.integers(-1, A, n)
+        ids[::3] = np.arange(len(ids[::3])) % A
+        seen.append(lora(n, n_in, n_out, rank, A, "f16", ids, x, base)[0][::3].view(np.uint32))
+    np.testing.assert_array_equal(seen[0], seen[1])
+    np.testing.assert_array_equal(seen[0], seen[2])
