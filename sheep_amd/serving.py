@@ -15,7 +15,7 @@ greedily (sml/sml-run.c:3539-3544).
 import ctypes
 import struct
 
-from . import _chk, lib
+from . import HipError, _chk, lib
 
 TYPES = {"f16": 0, "bf16": 1}
 _vp, _int, _size, _float = ctypes.c_void_p, ctypes.c_int, ctypes.c_size_t, ctypes.c_float
@@ -53,8 +53,15 @@ _call = _Calls()
 
 
 def _at(b):
-    """A buffer's device address, 0 for None."""
-    return (b and b.ptr) or 0
+    """The device address of a buffer that may be left out, 0 for None. A freed
+    one is an error: as NULL it would pass for left out. (A buffer's truth value
+    does not count: it may have a length. The buffers that no call can do
+    without the library checks itself.)"""
+    if b is None:
+        return 0
+    if b.ptr is None:
+        raise HipError("a freed buffer")
+    return b.ptr
 
 
 class Pages:
@@ -73,9 +80,9 @@ def append(pages, qkv, n_rows, pos, cos, sin, n_rope, n_head, seq=None, q_out=No
     """Rotate n_rows new tokens' q and k by their positions and write their k
     and v to the cache (sml_hip_paged_append); without q_out the rotated q
     goes back to qkv."""
-    _chk(_call.paged_append(pages.c, qkv and qkv.ptr, qkv_stride, n_rows, seq and seq.ptr, pos and pos.ptr,
-                            cos and cos.ptr, sin and sin.ptr, n_rope, n_head, q_out and q_out.ptr, stream),
-         "paged append")
+    _chk(_call.paged_append(pages.c, qkv is not None and qkv.ptr, qkv_stride, n_rows, _at(seq),
+                            pos is not None and pos.ptr, cos is not None and cos.ptr, sin is not None and sin.ptr,
+                            n_rope, n_head, _at(q_out), stream), "paged append")
 
 
 def part_floats(n_seq, n_head, hd, max_len):
@@ -86,8 +93,9 @@ def part_floats(n_seq, n_head, hd, max_len):
 def attention(pages, q, lens, max_len, n_head, part, out, scale=0.0, q_stride=0, stream=0):
     """out [n_seq][n_head*hd]: one new token a sequence over its first
     lens[b] positions (sml_hip_paged_attention)."""
-    _chk(_call.paged_attention(pages.c, q and q.ptr, q_stride, lens and lens.ptr, max_len, n_head, scale,
-                               part and part.ptr, out and out.ptr, stream), "paged attention")
+    _chk(_call.paged_attention(pages.c, q is not None and q.ptr, q_stride, lens is not None and lens.ptr, max_len,
+                               n_head, scale, part is not None and part.ptr, out is not None and out.ptr, stream),
+         "paged attention")
 
 
 def logits_part_bytes(n_row, n_vocab):
@@ -102,8 +110,8 @@ def adjust_logits(logits, n_row, n_vocab, out=None, tok=None, part=None, hist=No
     be logits), and each row's greedy pick into tok (sml_hip_logits_adjust)."""
     r = _RULES.pack(_at(hist), _at(hist_start), _at(n_prompt), n_hist, _at(rep), _at(presence), _at(frequency),
                     _at(bias_id), _at(bias), _at(bias_start), n_bias, _at(mask), _at(mask_row), n_mask)
-    _chk(_call.logits_adjust(logits and logits.ptr, stride, n_row, n_vocab, r, out and out.ptr, out_stride,
-                             tok and tok.ptr, part and part.ptr, stream), "logits")
+    _chk(_call.logits_adjust(logits is not None and logits.ptr, stride, n_row, n_vocab, r, _at(out), out_stride,
+                             _at(tok), part is not None and part.ptr, stream), "logits")
 
 
 class Adapters:
@@ -125,5 +133,5 @@ def lora_work_floats(rank, n_row):
 def lora(adapters, x, n_row, adapter, y, work, base=None, x_stride=0, y_stride=0, stream=0):
     """y[r] = base[r] + scale * B (A x[r]) with row r's adapter, -1 for none
     (sml_hip_lora_add); base may be y."""
-    _chk(_call.lora_add(adapters.c, x and x.ptr, x_stride, n_row, adapter and adapter.ptr, base and base.ptr,
-                        y and y.ptr, y_stride, work and work.ptr, stream), "lora")
+    _chk(_call.lora_add(adapters.c, x is not None and x.ptr, x_stride, n_row, adapter is not None and adapter.ptr,
+                        _at(base), y is not None and y.ptr, y_stride, work is not None and work.ptr, stream), "lora")
