@@ -57,8 +57,9 @@ typedef struct {
 // A row is left out, its q_out included, when its position is negative or at
 // or past n_rope or seq_pages * page_size, its sequence is outside 0..n_seq-1
 // or its page is none: rows of padding carry position -1. The rows of one
-// call are distinct positions; of two that share one, either may remain, head
-// by head.
+// call are for distinct places; where some share one (a position twice, or a page
+// that two sequences name), each value there is one of theirs, not all of them
+// the same row's.
 int sml_hip_paged_append(const sml_hip_pages * pg, float * qkv, size_t qkv_stride, int n_rows, const int32_t * seq,
                          const int32_t * pos, const float * cos_t, const float * sin_t, int n_rope, int n_head,
                          float * q_out, void * stream);

@@ -99,6 +99,28 @@ def test_infinite_queries_stay_in_their_heads(dtype):
     assert np.isnan(got[[1, 3, 6]]).all()
 
 
+# ------------------------------------------------------------ append
+
+def test_append_twice_to_one_place():
+    """Rows that share a place, by their positions or by a shared page, leave
+    one's value in each of its places, and touch no other."""
+    rng = np.random.default_rng(4)
+    KV, hd, page, rows = 2, 128, 16, 64
+    kb, vb = (sa.DevBuf.of(np.full(2 * page * KV * hd, 0x1234, np.uint16)) for _ in range(2))
+    pg = serving.Pages(kb, vb, ints([[1], [1]]), 2, page, 2, 1, KV, hd)
+    cos, sin = (sa.DevBuf.of(np.full((page, hd // 2), f, np.float32)) for f in (1.0, 0.0))
+    qkv = rng.standard_normal((rows, 1 + 2 * KV, hd)).astype(np.float32)
+    qo = sa.DevBuf(4 * rows * hd)
+    serving.append(pg, sa.DevBuf.of(qkv), rows, ints([7] * rows), cos, sin, page, 1, seq=ints(np.arange(rows) % 2), q_out=qo)
+    np.testing.assert_array_equal(qo.read(np.float32).reshape(rows, hd), qkv[:, 0])
+    for buf, first in ((kb, 1), (vb, 1 + KV)):
+        got = buf.read(np.uint16).reshape(2, page, KV, hd)
+        bits = so.to_bits(qkv[:, first:first + KV], "f16")
+        assert (got[1, 7] == bits).any(axis=0).all()
+        got[1, 7] = 0x1234
+        assert (got == 0x1234).all()
+
+
 # ------------------------------------------------------------ adapters
 
 def lora(n, n_in, n_out, rank, A, dtype, ids, x, base=None, in_place=False, a=None, b=None, y_pad=0):
