@@ -101,6 +101,43 @@ def test_infinite_queries_stay_in_their_heads(dtype):
 
 # ------------------------------------------------------------ append
 
+class At:
+    def __init__(self, p):
+        self.ptr = p
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_append_among_other_layers_turns_q(dtype, hd, in_place):
+    """The rotated q, and the cache, of the middle of three layers in one pool."""
+    rng = np.random.default_rng(hd)
+    H, KV, page, layers, rows = 6, 2, 32, 3, 50
+    size = page * KV * hd
+    cos, sin = so.rope_tables(hd // 2, 128)
+    pools = [sa.DevBuf.of(np.full(4 * layers * size, 0x1234, np.uint16)) for _ in range(2)]
+    table = np.array([[2, 0, 3, 1]], np.int32)
+    pg = serving.Pages(*(At(b.ptr + 2 * size) for b in pools), sa.DevBuf.of(table), 4, page, 1, 4, KV, hd, dtype,
+                       page_stride=layers * size)
+    qkv = rng.standard_normal((rows, H + 2 * KV, hd)).astype(np.float32)
+    pos = rng.permutation(128)[:rows]
+    buf, qo = sa.DevBuf.of(qkv), sa.DevBuf.of(np.full(rows * H * hd, np.nan, np.float32))
+    serving.append(pg, buf, rows, ints(pos), sa.DevBuf.of(cos), sa.DevBuf.of(sin), 128, H, seq=ints([0] * rows),
+                   q_out=None if in_place else qo)
+    after = buf.read(np.float32).reshape(qkv.shape)
+    want, size_of = so.rotate(qkv[:, :H + KV], cos[pos][:, None], sin[pos][:, None])
+    within(after[:, :H] if in_place else qo.read(np.float32).reshape(rows, H, hd), want[:, :H], 2 * so.U * size_of[:, :H], "q")
+    np.testing.assert_array_equal(after[:, H if in_place else 0:], qkv[:, H if in_place else 0:])
+    ks, vs = (b.read(np.uint16).reshape(4, layers, page, KV, hd) for b in pools)
+    place = (table[0, pos // page], 1, pos % page)
+    rot, mag = want[:, H:], size_of[:, H:]
+    within(so.from_bits(ks[place], dtype), rot, so.HALF[dtype] * (np.abs(rot) + 2 * so.U * mag) + 2 * so.U * mag + 2.0 ** -25, "k")
+    np.testing.assert_array_equal(vs[place], so.to_bits(qkv[:, H + KV:], dtype))
+    for x in (ks, vs):
+        x[place] = 0x1234
+        assert (x == 0x1234).all()
+
+
 def test_append_twice_to_one_place():
     """Rows that share a place, by their positions or by a shared page, leave
     one's value in each of its places, and touch no other."""
@@ -153,6 +190,28 @@ def test_bf16_adapters_of_the_largest_inputs(n, n_in, n_out, rank, A):
     want, tol = so.lora(x, np.zeros((n, n_out)), so.from_bits(a, "bf16"), so.from_bits(b, "bf16"), np.ones(A, np.float32),
                         [rank] * A, ids)
     within(got, want, tol)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("n, n_in, n_out, rank, A", FORMS)
+def test_infinite_rows_and_adapters_stay_their_own(n, n_in, n_out, rank, A, dtype):
+    """One launch and two, sorted tiles and not: a row with an infinity or a
+    NaN, and an adapter with them, reach no other row."""
+    rng = np.random.default_rng(n)
+    a, b = (so.to_bits(rng.standard_normal(s), dtype) for s in ((A, rank, n_in), (A, n_out, rank)))
+    a[1, 3, 5], b[1, 6, 2] = (0x7C00, 0x7E00) if dtype == "f16" else (0x7F80, 0x7FC0)
+    x = rng.standard_normal((n, n_in)).astype(np.float32)
+    x[4, 7], x[6, 9] = np.inf, np.nan
+    ids = rng.integers(-1, A, n)
+    ids[4], ids[6] = 0, 2
+    ids[7] = 1
+    got, _, _ = lora(n, n_in, n_out, rank, A, dtype, ids, x, a=a, b=b)
+    clean = [r for r in range(n) if ids[r] != 1 and r not in (4, 6)]
+    want, tol = so.lora(x[clean], np.zeros((len(clean), n_out)), so.from_bits(a, dtype), so.from_bits(b, dtype),
+                        np.ones(A, np.float32), [rank] * A, ids[clean])
+    within(got[clean], want, tol)
+    assert not np.isfinite(got[4]).any() and np.isnan(got[6]).all()
+    assert not np.isfinite(got[ids == 1]).any()
 
 
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
