@@ -52,16 +52,20 @@ class _Calls:
 _call = _Calls()
 
 
+# A buffer's truth value does not count (it may have a length), and a freed one
+# is an error: as NULL it would pass for one that is left out. The buffers that
+# no call can do without the library checks itself.
+
 def _at(b):
-    """The device address of a buffer that may be left out, 0 for None. A freed
-    one is an error: as NULL it would pass for left out. (A buffer's truth value
-    does not count: it may have a length. The buffers that no call can do
-    without the library checks itself.)"""
-    if b is None:
-        return 0
-    if b.ptr is None:
+    """A buffer's device address, 0 for None."""
+    return 0 if b is None else b.ptr
+
+
+def _freed(*buffers):
+    """Refuse freed buffers; 0 (those left, of nothing, lie at no address)."""
+    if any(b is not None and b.ptr is None for b in buffers):
         raise HipError("a freed buffer")
-    return b.ptr
+    return 0
 
 
 class Pages:
@@ -72,17 +76,22 @@ class Pages:
     def __init__(self, k, v, table, n_pages, page_size, n_seq, seq_pages, n_kv, hd, dtype="f16", page_stride=0):
         self.buffers = (k, v, table)
         self.n_seq, self.n_kv, self.hd = n_seq, n_kv, hd
-        self.c = _PAGES.pack(_at(k), _at(v), _at(table), page_stride, n_pages, page_size, n_seq, seq_pages, n_kv, hd,
-                             TYPES[dtype])
+        try:
+            self.c = _PAGES.pack(_at(k), _at(v), _at(table), page_stride, n_pages, page_size, n_seq, seq_pages, n_kv,
+                                 hd, TYPES[dtype])
+        except struct.error:
+            _freed(k, v, table)
+            raise
 
 
 def append(pages, qkv, n_rows, pos, cos, sin, n_rope, n_head, seq=None, q_out=None, qkv_stride=0, stream=0):
     """Rotate n_rows new tokens' q and k by their positions and write their k
     and v to the cache (sml_hip_paged_append); without q_out the rotated q
     goes back to qkv."""
-    _chk(_call.paged_append(pages.c, qkv is not None and qkv.ptr, qkv_stride, n_rows, _at(seq),
-                            pos is not None and pos.ptr, cos is not None and cos.ptr, sin is not None and sin.ptr,
-                            n_rope, n_head, _at(q_out), stream), "paged append")
+    _chk(_call.paged_append(pages.c, qkv is not None and qkv.ptr, qkv_stride, n_rows,
+                            seq is not None and (seq.ptr or _freed(seq)), pos is not None and pos.ptr,
+                            cos is not None and cos.ptr, sin is not None and sin.ptr, n_rope, n_head,
+                            q_out is not None and (q_out.ptr or _freed(q_out)), stream), "paged append")
 
 
 def part_floats(n_seq, n_head, hd, max_len):
@@ -108,10 +117,16 @@ def adjust_logits(logits, n_row, n_vocab, out=None, tok=None, part=None, hist=No
                   bias_start=None, mask=None, n_mask=0, mask_row=None, stride=0, out_stride=0, stream=0):
     """Penalties, biases and masks on n_row rows of logits into out (which may
     be logits), and each row's greedy pick into tok (sml_hip_logits_adjust)."""
-    r = _RULES.pack(_at(hist), _at(hist_start), _at(n_prompt), n_hist, _at(rep), _at(presence), _at(frequency),
-                    _at(bias_id), _at(bias), _at(bias_start), n_bias, _at(mask), _at(mask_row), n_mask)
-    _chk(_call.logits_adjust(logits is not None and logits.ptr, stride, n_row, n_vocab, r, _at(out), out_stride,
-                             _at(tok), part is not None and part.ptr, stream), "logits")
+    try:
+        r = _RULES.pack(_at(hist), _at(hist_start), _at(n_prompt), n_hist, _at(rep), _at(presence), _at(frequency),
+                        _at(bias_id), _at(bias), _at(bias_start), n_bias, _at(mask), _at(mask_row), n_mask)
+    except struct.error:
+        _freed(hist, hist_start, n_prompt, rep, presence, frequency, bias_id, bias, bias_start, mask, mask_row)
+        raise
+    _chk(_call.logits_adjust(logits is not None and logits.ptr, stride, n_row, n_vocab, r,
+                             out is not None and (out.ptr or _freed(out)), out_stride,
+                             tok is not None and (tok.ptr or _freed(tok)), part is not None and part.ptr, stream),
+         "logits")
 
 
 class Adapters:
@@ -122,7 +137,11 @@ class Adapters:
 
     def __init__(self, a, b, n_adapter, rank, n_in, n_out, dtype="f16", scale=None, ranks=None):
         self.buffers = (a, b, scale, ranks)
-        self.c = _ADAPTERS.pack(_at(a), _at(b), _at(scale), _at(ranks), n_adapter, rank, n_in, n_out, TYPES[dtype])
+        try:
+            self.c = _ADAPTERS.pack(_at(a), _at(b), _at(scale), _at(ranks), n_adapter, rank, n_in, n_out, TYPES[dtype])
+        except struct.error:
+            _freed(a, b, scale, ranks)
+            raise
 
 
 def lora_work_floats(rank, n_row):
@@ -134,4 +153,5 @@ def lora(adapters, x, n_row, adapter, y, work, base=None, x_stride=0, y_stride=0
     """y[r] = base[r] + scale * B (A x[r]) with row r's adapter, -1 for none
     (sml_hip_lora_add); base may be y."""
     _chk(_call.lora_add(adapters.c, x is not None and x.ptr, x_stride, n_row, adapter is not None and adapter.ptr,
-                        _at(base), y is not None and y.ptr, y_stride, work is not None and work.ptr, stream), "lora")
+                        base is not None and (base.ptr or _freed(base)), y is not None and y.ptr, y_stride,
+                        work is not None and work.ptr, stream), "lora")
