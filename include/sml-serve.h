@@ -12,9 +12,11 @@
 // stream, where the rest of the kernel-level ABI runs), allocates nothing,
 // never waits and may be captured into a HIP graph once sml_hip_init has run.
 // Buffers used on another stream than the one they were filled on are the
-// caller's to order. Workspaces are the caller's too: calls that may overlap
-// (on two streams, or in two graphs replayed side by side) need one each;
-// nothing in a workspace outlives its call. The calls are made by one host
+// caller's to order, by events: so are the results of sml-hip.h's products,
+// which run on the null stream (and are not captured with these calls), for a
+// stream that does not wait for it. Workspaces are the caller's too: calls that
+// may overlap (on two streams, or in two graphs replayed side by side) need one
+// each; nothing in a workspace outlives its call. The calls are made by one host
 // thread at a time, with the device of sml_hip_init current; with another
 // device current they are refused.
 #pragma once

@@ -1,5 +1,7 @@
 """The operators of a step of many requests at the edges of what their header
 allows, against the 64-bit forms of serving_oracle.py."""
+import ctypes
+
 import numpy as np
 import pytest
 
@@ -246,3 +248,80 @@ def test_zeros_do_not_depend_on_other_rows(n, n_in, n_out, rank, A):
         seen.append(lora(n, n_in, n_out, rank, A, "f16", ids, x, base)[0][::3].view(np.uint32))
     np.testing.assert_array_equal(seen[0], seen[1])
     np.testing.assert_array_equal(seen[0], seen[2])
+
+
+# ------------------------------------------------------------ beside the products
+
+class Hip:
+    """Streams and events of the runtime the library already runs on."""
+
+    def __init__(self):
+        sa.lib()
+        self.l = ctypes.CDLL("libamdhip64.so")
+        self.stream, self.events = ctypes.c_void_p(), [ctypes.c_void_p(), ctypes.c_void_p()]
+        self("hipStreamCreateWithFlags", ctypes.byref(self.stream), 1)      # not ordered with the null stream
+        for e in self.events:
+            self("hipEventCreateWithFlags", ctypes.byref(e), 2)             # no timing
+
+    def __call__(self, name, *args):
+        assert getattr(self.l, name)(*args) == 0, name
+
+    def after_null(self):
+        """What is enqueued on the stream from here on follows the null stream's work so far."""
+        self("hipEventRecord", self.events[0], None)
+        self("hipStreamWaitEvent", self.stream, self.events[0], 0)
+
+    def before_null(self):
+        self("hipEventRecord", self.events[1], self.stream)
+        self("hipStreamWaitEvent", None, self.events[1], 0)
+
+
+def test_products_and_operators_on_two_streams(tmpdir_s):
+    """The documented order of a layer: the shared product on the null stream,
+    its adapters, the append and the attention on a stream that does not wait
+    for it by itself, the next product after them. Several layers in a row,
+    unsynchronized, equal the same calls on the null stream."""
+    rng = np.random.default_rng(8)
+    n, E, H, KV, hd, page, pages, rank, A, layers = 9, 512, 8, 2, 64, 16, 4, 16, 3, 4
+    W = (H + 2 * KV) * hd
+    p = tmpdir_s / "serving_streams.ssf"
+    sa.synth_matrix(p, W, E, nbits=4, seed=3)
+    m = sa.Mat.from_file(p, "w")
+    x = rng.standard_normal((n, E)).astype(np.float32)
+    act = sa.Act(E * n)
+    for r in range(n):
+        one = sa.Act(E)
+        sa.normq(sa.DevBuf.of(x[r]), one)
+        for buf, w, sz in zip((act.q, act.scale, act.sums), one.read(), (E, E // 8, E // 8)):
+            sa._chk(sa.lib().sml_hip_h2d(buf.ptr + r * sz, w.ctypes.data, w.nbytes))
+    a, b = (so.to_bits(rng.standard_normal(s), "f16") for s in ((A, rank, E), (A, W, rank)))
+    ad = serving.Adapters(sa.DevBuf.of(a), sa.DevBuf.of(b), A, rank, E, W)
+    cos, sin = (sa.DevBuf.of(t) for t in so.rope_tables(hd // 2, page * pages))
+    pos, ids = rng.integers(0, page * pages, n), ints(rng.integers(-1, A, n))
+    table, pos_b, len_b = ints(rng.permutation(n * pages).reshape(n, pages)), ints(pos), ints(pos + 1)
+    xb, hip = sa.DevBuf.of(x), Hip()
+    first = [so.to_bits(rng.standard_normal((n * pages, page, KV, hd)), "f16") for _ in range(2)]
+
+    def run(stream):
+        kv = [[sa.DevBuf.of(w) for w in first] for _ in range(layers)]
+        qkv, q, out = sa.DevBuf(4 * n * W), sa.DevBuf(4 * n * H * hd), [sa.DevBuf(4 * n * H * hd) for _ in range(layers)]
+        part = sa.DevBuf(4 * serving.part_floats(n, H, hd, page * pages))
+        work = sa.DevBuf(4 * serving.lora_work_floats(rank, n))
+        sa.sync()
+        for layer in range(layers):
+            sa.gemm(m, act.q, act.scale, act.sums, n, qkv)
+            if stream:
+                hip.after_null()
+            serving.lora(ad, xb, n, ids, qkv, work, base=qkv, stream=stream)
+            pg = serving.Pages(*kv[layer], table, n * pages, page, n, pages, KV, hd)
+            serving.append(pg, qkv, n, pos_b, cos, sin, page * pages, H, q_out=q, stream=stream)
+            serving.attention(pg, q, len_b, page * pages, H, part, out[layer], stream=stream)
+            if stream:
+                hip.before_null()
+        sa.sync()
+        return [o.read(np.uint32) for o in out] + [w.read(np.uint16) for pair in kv for w in pair]
+
+    want = run(0)
+    for _ in range(3):
+        for got, w in zip(run(hip.stream.value), want):
+            np.testing.assert_array_equal(got, w)
