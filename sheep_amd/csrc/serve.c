@@ -99,7 +99,7 @@ int sml_hip_paged_attention(const sml_hip_pages * pg, const float * q, size_t q_
     // workspace's of the longest sequence
     a.nsplit = ceil_div(max_len > 1 ? max_len : 1, 64);
     if (a.nsplit > 256) a.nsplit = 256;
-    // About 512 workgroups, two a CU, where the lengths are shared out (48
+    // Two workgroups a CU, 512, where the lengths are shared out (48
     // sequences up to 8192 / one at 65537 / 16 of 2000 / 32 of 1000 to 9000 with
     // 12 heads over 2, us: 512 55, 36, 32, 24; 768 54, 37, 37, 27; 1024 52, 37, 35,
     // 27).
@@ -109,7 +109,7 @@ int sml_hip_paged_attention(const sml_hip_pages * pg, const float * q, size_t q_
     const int n = a.max_len > 1 ? a.max_len : 1, shared = pg->n_seq <= AT_SHARED;
     const int least = shared && n > 512 ? 128 : 512;
     a.chunk = least * ceil_div(n, least * 256);
-    a.want = shared ? ceil_div(512, pg->n_kv) : 0;
+    a.want = shared ? ceil_div(2 * hx.ncu, pg->n_kv) : 0;
     // every sequence's first split, and those that the lengths can make beyond
     long grid = ceil_div(n, a.chunk);
     if (shared) {
@@ -190,8 +190,17 @@ size_t sml_hip_lora_work_floats(int rank, int n_row) {
 
 #define LD_ROWS 16                                    // rows of a tile
 
+// The workgroups of a product that run at once: two a CU by their registers, if
+// the CU's LDS (a little of it is theirs beside lds) holds them. It does not
+// where bf16's three parts meet 32 ranks of A or, at 32 rows, 256 ranks of B
+// (us a call of bf16 with these taken for two a CU / so: 80 rows of 16 adapters,
+// 14336 to 4096, rank 64 32.1 / 29.0, 256 rows 32.9 / 27.1, 509 rows of 4096 to
+// 4096, rank 256 64 / 45, of 4 adapters in runs 53 / 38; the most that lose, 128
+// rows of 64 adapters 75 / 79).
+static int at_once(size_t lds) { return hx.ncu * (2 * (lds + 256) <= 160 << 10 ? 2 : 1); }
+
 // One launch or two, as measured beside the kernels. One: up to 16 rows of rank
-// up to 64, sums that fit LDS, at most 640 workgroups, and few row products a
+// up to 64, sums that fit LDS, at most 2.5 workgroups a CU, and few row products a
 // wave (rounds of its 8 ranks of 512 inputs, each taking the adapter's rows one
 // by one): 8 if the rows share the pool's adapters alike, 16 if all had one.
 static void lora_launch(sml_klora * a, int bf, hipStream_t st) {
@@ -199,23 +208,23 @@ static void lora_launch(sml_klora * a, int bf, hipStream_t st) {
     const size_t sums = (size_t) nslice * 16 * (size_t) a->rank * 4;
     const long rounds = ceil_div(nslice * (a->rank / 8), LF_WAVES);
     if (a->n_row <= 16 && a->rank <= LF_RANK && sums <= 96 << 10 && a->n_row * rounds <= 16 &&
-        ceil_div(a->n_row, a->n_adapter) * rounds <= 8 && (long) ceil_div(a->n_out, LF_OUT) * few <= 640) {
+        ceil_div(a->n_row, a->n_adapter) * rounds <= 8 && (long) ceil_div(a->n_out, LF_OUT) * few <= 5L * hx.ncu / 2) {
         hx_launch(bf ? "sml_sv_lora_few_bf" : "sml_sv_lora_few", (unsigned) ceil_div(a->n_out, LF_OUT), (unsigned) few,
                   64 * LF_WAVES, (size_t) parts * 16 * LF_LD * 2 + 64 + sums, st, a);
         return;
     }
     a->sorted = a->n_row > 32 && a->n_row <= LS_ROWS && a->n_adapter > 1 && a->n_adapter <= LS_ADAPTERS;
-    // t: the inputs split for 128 workgroups of 64 ranks, twice as many of up to
-    // 16, as far as the workspace holds them (509 rows, us a call at half / so /
-    // twice: rank 64, 4096 to 14336 30.6 / 29.5 / 33.3, rank 16, 14336 to 4096
-    // 21.1 / 20.0 / -): every workgroup of y joins them, so that splits times
+    // t: the inputs split for half a workgroup a CU of 64 ranks, twice as many of
+    // up to 16, as far as the workspace holds them (509 rows, us a call at half /
+    // so / twice: rank 64, 4096 to 14336 30.6 / 29.5 / 33.3, rank 16, 14336 to
+    // 4096 21.1 / 20.0 / -): every workgroup of y joins them, so that splits times
     // ranks stay within 768 too (14336 to 4096, with that and without: 16 rows,
     // rank 64 16.2 / 20.8, 32 rows, rank 128 19.6 / 31.8, 1 row, rank 256 22.6 /
     // 21.9).
     const int ntile = ceil_div(a->n_row, LD_ROWS), ngroup = ceil_div(a->rank, 64);
     int most = 8192 / a->n_row < 32 ? 8192 / a->n_row : 32;
     if (most > 768 / a->rank) most = 768 / a->rank;
-    const int want = ceil_div(a->rank <= 16 ? 256 : 128, ntile * ngroup);
+    const int want = ceil_div(a->rank <= 16 ? hx.ncu : hx.ncu / 2, ntile * ngroup);
     if (most > want) most = want;
     if (most < 1) most = 1;
     a->chunk = LD_TILE;
@@ -229,13 +238,17 @@ static void lora_launch(sml_klora * a, int bf, hipStream_t st) {
     // rows, 4096 to 14336, rank 64 17.8 / 19.3, 14336 to 4096 19.5 / 23.4; 384
     // rows 24.5 / 24.3 and 23.8 / 25.9, 1536 to 8960, rank 8 18.7 / 14.9; 509
     // rows of 4 adapters in runs 33.6 / 31.5, 30.8 / 27.0 at rank 16), and the
-    // 512 workgroups that run at once, never more (the same case with 256 / 512 /
+    // workgroups that run at once, never more (the same case with 256 / 512 /
     // 1024: 35 / 30 / 34; 192 rows, rank 64, with 576: 24.8 for 17.8). A
     // row tile's workgroups are a multiple of 8, so that the same outputs' B goes
     // to the same XCD's L2, where that drops few of them (320 rows, rank 64, 48
     // for 51: 22.7 / 24.8; 700 rows, rank 16, 16 for 23: 29.0 / 27.5).
     const int rb = a->n_row <= 256 ? 1 : 2, nrt = ceil_div(a->n_row, 16 * rb);
-    int gx = 512 / nrt;
+    // (the sort's counts, 8 KB, fit before the rest)
+    const size_t lds_d = (size_t) LD_WAVES * LD_WAVE_LDS(parts, rt),
+                 lds_u = (size_t) 4 * LU_OUT * LD_ROW + (size_t) 16 * rb * (4 + (size_t) parts * ((size_t) ngroup * 64 + 8) * 2);
+    const int once_d = at_once(lds_d), once_u = at_once(lds_u);
+    int gx = once_u / nrt;
     if (gx >= 24) gx -= gx % 8;
     if (gx > ceil_div(a->n_out, 4 * LU_OUT)) gx = ceil_div(a->n_out, 4 * LU_OUT);
     if (gx < 1) gx = 1;
@@ -247,15 +260,13 @@ static void lora_launch(sml_klora * a, int bf, hipStream_t st) {
     // 41 / 49 / 67)
     const int down = a->nsplit * ntile * ceil_div(a->rank, 16 * rt), up = gx * nrt;
     int nz = 1;
-    while (2 * nz <= few && 2 * nz <= a->n_adapter && 2 * nz * down <= 512 && 2 * nz * up <= 512) nz *= 2;
+    while (2 * nz <= few && 2 * nz <= a->n_adapter && 2 * nz * down <= once_d && 2 * nz * up <= once_u) nz *= 2;
     char name[40];
     snprintf(name, sizeof name, "sml_sv_lora_down%d%s", rt, bf ? "_bf" : "");
     hx_launch3(name, (unsigned) a->nsplit, (unsigned) ntile, (unsigned) (nz * ceil_div(a->rank, 16 * rt)), 64 * LD_WAVES,
-               (size_t) LD_WAVES * LD_WAVE_LDS(parts, rt), st, a);
-    // (the sort's counts, 8 KB, fit before the rest)
-    const size_t lds = (size_t) 4 * LU_OUT * LD_ROW + (size_t) 16 * rb * (4 + (size_t) parts * ((size_t) ngroup * 64 + 8) * 2);
+               lds_d, st, a);
     snprintf(name, sizeof name, "sml_sv_lora_up%d%s", rb, bf ? "_bf" : "");
-    hx_launch3(name, (unsigned) gx, (unsigned) nrt, (unsigned) nz, 256, lds, st, a);
+    hx_launch3(name, (unsigned) gx, (unsigned) nrt, (unsigned) nz, 256, lds_u, st, a);
 }
 
 int sml_hip_lora_add(const sml_hip_adapters * ad, const float * x, size_t x_stride, int n_row, const int32_t * adapter,

@@ -178,6 +178,20 @@ FORMS = [(8, 256, 70, 16, 4), (16, 520, 301, 64, 16), (20, 256, 70, 16, 3), (100
          (300, 264, 131, 256, 4), (600, 264, 67, 24, 5)]
 
 
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("n, n_in, n_out, rank, A", [(65, 1544, 300, 64, 16), (80, 520, 1030, 136, 80), (256, 1032, 301, 32, 33),
+                                                     (257, 264, 1500, 256, 16), (500, 520, 517, 200, 9), (513, 72, 600, 256, 40)])
+def test_adapters_shared_out(n, n_in, n_out, rank, A, dtype):
+    """Mixed batches whose tiles' adapters several workgroups share, as many as
+    the LDS of either product's tiles lets run at once."""
+    rng = np.random.default_rng(n)
+    x, base = rng.standard_normal((n, n_in)).astype(np.float32), rng.standard_normal((n, n_out)).astype(np.float32)
+    for ids in (rng.integers(-1, A, n), np.arange(n) % A, np.arange(n) * A // n):
+        got, a, b = lora(n, n_in, n_out, rank, A, dtype, ids, x, base)
+        want, tol = so.lora(x, base, so.from_bits(a, dtype), so.from_bits(b, dtype), np.ones(A, np.float32), [rank] * A, ids)
+        within(got, want, tol)
+
+
 @pytest.mark.parametrize("n, n_in, n_out, rank, A", FORMS)
 def test_bf16_adapters_of_the_largest_inputs(n, n_in, n_out, rank, A):
     """The largest finite inputs, and the same as the first product's results,
