@@ -203,6 +203,12 @@ static int at_once(size_t lds) { return hx.ncu * (2 * (lds + 256) <= 160 << 10 ?
 // up to 64, sums that fit LDS, at most 2.5 workgroups a CU, and few row products a
 // wave (rounds of its 8 ranks of 512 inputs, each taking the adapter's rows one
 // by one): 8 if the rows share the pool's adapters alike, 16 if all had one.
+// Which adapters they have only the device knows: where all rows have the same
+// one of a pool as large as the batch, one launch loses what two would save (us
+// with one launch, a row each of its own adapter / all of one, and two launches,
+// all of one; rank 16, 4096 to 4096: 4 rows 5.8 / 7.4, 11.1, 8 rows 6.5 / 10.1,
+// 11.1, 16 rows 8.0 / 15.6, 11.0; 14336 to 4096: 4 rows 9.7 / 15.1, 13.0; rank 64,
+// 4096 to 4096: 4 rows 11.0 / 17.5, 12.6).
 static void lora_launch(sml_klora * a, int bf, hipStream_t st) {
     const int parts = bf ? 3 : 2, nslice = ceil_div(a->n_in, LF_SLICE), few = a->n_row < 16 ? a->n_row : 16;
     const size_t sums = (size_t) nslice * 16 * (size_t) a->rank * 4;

@@ -136,11 +136,11 @@ APPEND(64, 1, sml_sv_append_d64_bf)
 //
 // Measured with the merge, 32 heads over 8 of 128, fp16: 48 sequences up to
 // 8192 (202 MB) 55 us = 3.7 TB/s (60 with fixed splits of 512 and K in the
-// matrix cores' order from memory), one at 4095 10.2 us, of which 5.8 are this
-// kernel's chain of latencies (length, table, rows, joining) and 3.8 the
-// merge's; bf16, 28 over 4, one at 65537 (134 MB) 35 us = 3.8 TB/s. A large
-// copy reaches 4.8 TB/s. Two workgroups (212 registers) a CU: held to three,
-// 58 and 52 us.
+// matrix cores' order from memory), one at 4095 10.2 us, of which 5.9 are this
+// kernel's chain of latencies (length, table, rows, joining) and 3.6 the
+// merge's; bf16, 28 over 4, one at 65537 (134 MB) 34.7 us = 3.9 TB/s. A large
+// copy reaches 4.8 TB/s. Two workgroups (212 registers, bf16 228) a CU: held to
+// three, 58 and 52 us.
 #define AT_WAVES 4
 
 // The positions a sequence attends over.
@@ -531,14 +531,17 @@ ATTEND(64, 1, sml_sv_attend_d64_bf)
 // loading counts: the listed tokens go through one copy of the rules (one
 // division), not sixteen unrolled (1 row of 128256: 10.3 us so, 6.0 with).
 //
-// us a call with the pick, 512 threads of one word / 256 of two (128256 tokens,
-// masks, histories of 2047): 1 row 8.1 / 8.3 (5.0 and 1.7 of them the kernels',
-// the rest two launches), 16 rows 10.2 / 9.9, 32 rows 13.9 / 13.2, 96 rows 31 /
-// 26 (3.8 TB/s); histories of 65536: 1 row 15 / 23, 96 rows 49 / 45. 4096 tokens
-// a workgroup: 96 rows 28.5 (when this took 27). The pick looks for the
-// largest value first and for its place in the lanes that have it; with an
-// index carried beside every value the 96 rows took 28, 213 instructions a
-// word of four.
+// us a call with the pick, 512 threads of one word / 256 of two / 4096 tokens a
+// workgroup, 512 threads of two / 256 of four (128256 tokens, masks, histories
+// of 2047, from 16 rows four batches in turn): 1 row 7.3 / 8.3 / 8.1 / 10.9 (5.4
+// and 1.4 of the first its kernels'), 12 rows 9.0 / 9.4 / 10.1 / 12.0, 16 rows
+// 10.5 / 10.5 / 11.0 / 13.0, 32 rows 15.5 / 14.6 / 14.7 / 15.6, 96 rows 38.5 /
+// 30.8 / 33.9 / 42; histories of 65536: 1 row 15 / 23 / 17 / 28, 16 rows 18 / 25
+// / 24 / 29, 96 rows 59 / 54 / 55 / 66. So 256 threads of two lose up to 30%
+// where histories are that long. The 96 rows' first kernel streams their 99 MB
+// at 4.1 TB/s. The pick looks for the largest value first and for its place in
+// the lanes that have it; with an index carried beside every value a word of
+// four took 213 instructions, and the 96 rows 2 us more.
 #define LG_SEEN 0x80000000u
 
 // The largest value and the smallest index over the wave's lanes.
@@ -860,7 +863,7 @@ __device__ __forceinline__ unsigned long long my_rows(int id, unsigned long long
 // bytes a cycle and CU measured): rows are loaded whole, 128 or 256 bytes in
 // consecutive lanes, and handed over through the wave's part of LDS, at a
 // stride of LD_ROW bytes that spreads 16 rows over all banks. 509 rows of 4096,
-// rank 64: 8.7 us, of which a second adapter in a tile's rows takes 1.6; the
+// rank 64: 8.4 us, of which a second adapter in a tile's rows takes 2; the
 // reads of x alone (8 MB, each once) would be 2.
 template <int BF, int RT>
 __device__ __forceinline__ void lora_down_body(const sml_klora & a) {
@@ -991,8 +994,10 @@ __device__ __forceinline__ void lora_down_body(const sml_klora & a) {
 // adapter, too few for the matrix cores' 16 columns (converting all 16 made
 // this 12.6 us for 8.5): the first product is a lane's own fused multiply-adds
 // on 8 inputs of 8 ranks at a time, summed over the wave by halves. 16 rows of
-// 11 adapters, 4096 to 4096, rank 16: 8.5 us, a chain of latencies (ids, A and x,
-// two exchanges in LDS, B) around 4 MB that would take 1.
+// 11 adapters, 4096 to 4096, rank 16: 8.4 us, a chain of latencies (ids, A and x,
+// two exchanges in LDS, B) around 4 MB that would take 1; behind the L2s they are
+// 15, since an adapter's output blocks lie on all XCDs, and each fetches its A
+// and x.
 template <int BF>
 __device__ __forceinline__ void lora_few_body(const sml_klora & a) {
     using M = Mx<BF>;
