@@ -146,8 +146,8 @@ typedef struct {
 // Floats of the workspace of sml_hip_lora_add: rank * max(n_row, min(32 * n_row, 8192)).
 size_t sml_hip_lora_work_floats(int rank, int n_row);
 // y[r] = base[r] + scale * B (A x[r]) for n_row rows (0..65535) with adapter
-// adapter[r] each; an id outside 0..n_adapter-1 (-1 by custom) adds nothing, and
-// the row is its base bit for bit.
+// adapter[r] each; an id outside 0..n_adapter-1 (-1 by custom) adds nothing:
+// the row is its base, signs of zeros and NaN included.
 // x rows lie x_stride floats apart (0: n_in), y's and base's y_stride (0:
 // n_out); base may be y, or NULL for zeros; x and work lie apart from y.
 // Products and sums are fp32, their order set by the call's shape: a row's bits

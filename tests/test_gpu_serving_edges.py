@@ -89,6 +89,22 @@ def test_bf16_rising_scores_of_large_values():
     check_attend(q, so.to_bits(k, "bf16"), so.to_bits(rng.uniform(-1, 1, (n, 1, hd)) * 2.0 ** 118, "bf16"), "bf16", scale=1.0)
 
 
+@pytest.mark.parametrize("v_exp", [-116, -122, -125])
+def test_bf16_smallest_values(v_exp):
+    """Values of one sign and near fp32's smallest normal ones, of 40 keys: the
+    weights' and sums' errors (so.attend's), and those of sums that lie in
+    fp32's denormals, 2^-149 in each of at most 3 parts x 2 tiles x 2 halves and
+    4 waves, for weights from 2^-4."""
+    rng = np.random.default_rng(6)
+    k = so.to_bits(rng.standard_normal((40, 1, 64)), "bf16")
+    v = so.to_bits(rng.uniform(1, 2, (40, 1, 64)) * 2.0 ** v_exp, "bf16")
+    q = rng.standard_normal((4, 64)).astype(np.float32)
+    want, _ = so.attend(q, so.from_bits(k[:, 0], "bf16"), so.from_bits(v[:, 0], "bf16"), 0.125)
+    size = np.abs(q.astype(np.float64)) @ np.abs(so.from_bits(k[:, 0], "bf16")).T * 0.125
+    rel = 2 * 88 * so.U * size.max() + (2 * 40 + 32) * so.U
+    within(attend(q, k, v, "bf16"), want, rel * np.abs(want) + 48 * 2.0 ** (4 - 149))
+
+
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
 def test_infinite_queries_stay_in_their_heads(dtype):
     rng = np.random.default_rng(3)
