@@ -1,6 +1,9 @@
 """The operators of a step of many requests at the edges of what their header
 allows, against the 64-bit forms of serving_oracle.py."""
 import ctypes
+import os
+import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -115,6 +118,26 @@ def test_infinite_queries_stay_in_their_heads(dtype):
     got = attend(q, k, v, dtype)
     np.testing.assert_array_equal(got[[0, 2, 4, 5, 7]], clean[[0, 2, 4, 5, 7]])
     assert np.isnan(got[[1, 3, 6]]).all()
+
+
+def test_as_many_sequences_as_there_may_be():
+    """65535 sequences that share their pages: outputs follow from the lengths alone."""
+    rng = np.random.default_rng(7)
+    n, hd, page, pages, top = 65535, 64, 64, 10, 620
+    k, v = (so.to_bits(rng.standard_normal((pages, page, 1, hd)), "f16") for _ in range(2))
+    lens = rng.integers(0, 4, n)
+    lens[[0, 1, 40000, n - 1]] = [600, 513, 620, 128]
+    table = ints(np.tile(rng.permutation(pages), (n, 1)))
+    pg = serving.Pages(sa.DevBuf.of(k), sa.DevBuf.of(v), table, pages, page, n, pages, 1, hd)
+    q = rng.standard_normal(hd).astype(np.float32)
+    out, part = sa.DevBuf.of(np.full((n, hd), np.nan, np.float32)), sa.DevBuf(4 * serving.part_floats(n, 1, hd, top))
+    serving.attention(pg, sa.DevBuf.of(np.tile(q, (n, 1))), ints(lens), top, 1, part, out)
+    got = out.read(np.float32).reshape(n, hd)
+    first = table.read(np.int32, pages)
+    kk, vv = (so.from_bits(w[first], "f16").reshape(-1, hd) for w in (k, v))
+    for m in np.unique(lens):
+        want, tol = so.attend(q[None], kk[:m], vv[:m], hd ** -0.5)
+        within(got[lens == m], np.repeat(want, (lens == m).sum(), 0), np.repeat(tol, (lens == m).sum(), 0), f"length {m}")
 
 
 # ------------------------------------------------------------ append
@@ -280,6 +303,27 @@ def test_zeros_do_not_depend_on_other_rows(n, n_in, n_out, rank, A):
     np.testing.assert_array_equal(seen[0], seen[2])
 
 
+def test_as_many_rows_as_there_may_be():
+    """65535 rows of adapters and of logits."""
+    rng = np.random.default_rng(9)
+    n, n_in, n_out, rank, A = 65535, 16, 9, 8, 3
+    x, base = rng.standard_normal((n, n_in)).astype(np.float32), rng.standard_normal((n, n_out)).astype(np.float32)
+    ids = rng.integers(-1, A, n)
+    got, a, b = lora(n, n_in, n_out, rank, A, "f16", ids, x, base)
+    want, tol = so.lora(x, base, so.from_bits(a, "f16"), so.from_bits(b, "f16"), np.ones(A, np.float32), [rank] * A, ids)
+    within(got, want, tol)
+    logits = rng.integers(-9, 9, (n, n_out)).astype(np.float32)
+    out, tok, part = sa.DevBuf(4 * n * n_out), sa.DevBuf(4 * n), sa.DevBuf(serving.logits_part_bytes(n, n_out))
+    mask = np.array([0b101010101, 0b000110000], np.uint32)
+    which = rng.integers(-1, 3, n)
+    serving.adjust_logits(sa.DevBuf.of(logits), n, n_out, out=out, tok=tok, part=part, mask=sa.DevBuf.of(mask), n_mask=2,
+                          mask_row=ints(which))
+    ok = np.array([mask[0] >> np.arange(n_out) & 1, mask[1] >> np.arange(n_out) & 1, 0 * np.arange(n_out), 0 * np.arange(n_out) + 1]) > 0
+    want = np.where(ok[which], logits, -np.inf)
+    np.testing.assert_array_equal(out.read(np.float32).reshape(n, n_out), want)
+    np.testing.assert_array_equal(tok.read(np.int32), np.where(which == 2, -1, want.argmax(1)))
+
+
 # ------------------------------------------------------------ beside the products
 
 class Hip:
@@ -355,3 +399,33 @@ def test_products_and_operators_on_two_streams(tmpdir_s):
     for _ in range(3):
         for got, w in zip(run(hip.stream.value), want):
             np.testing.assert_array_equal(got, w)
+
+
+FIRST = """
+import sys
+sys.path[:0] = sys.argv[1:]
+import numpy as np
+import sheep_amd as sa
+import test_gpu_serving as t
+sa.init(0)
+s = t.step_state(1)
+d, hip = t.step_buffers(s), t.Hip()
+sa.sync()
+ex = hip.capture(lambda: t.step_run(s, d, hip.stream.value))
+for _ in range(2):
+    hip.replay(ex)
+got = t.step_outputs(d)
+d = t.step_buffers(s)
+t.step_run(s, d, 0)
+sa.sync()
+for k, w in t.step_outputs(d).items():
+    np.testing.assert_array_equal(got[k], w, err_msg=k)
+print("equal")
+"""
+
+
+def test_first_calls_of_a_process_inside_a_capture():
+    """Nothing but sml_hip_init has to run before a capture."""
+    here = os.path.dirname(os.path.abspath(__file__))
+    r = subprocess.run([sys.executable, "-c", FIRST, os.path.dirname(here), here], capture_output=True, text=True, timeout=100)
+    assert r.returncode == 0 and r.stdout.strip().endswith("equal"), r.stdout + r.stderr
