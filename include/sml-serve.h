@@ -1,7 +1,9 @@
 // Operators of a step that serves many requests at once, on device buffers:
-// a paged key/value cache and the attention of one new token a sequence over
-// it, low-rank adapters beside a shared projection, and penalties, biases and
-// grammar masks on logits with the greedy pick. They stand beside the
+// a paged key/value cache and the attention of one new token a sequence, or of
+// several (a draft's tree, a prompt's chunk), over it, what such a cache's
+// upkeep takes (accepted drafts, forks, compaction), low-rank adapters beside a
+// shared projection, and penalties, biases and grammar masks on logits with the
+// greedy pick. They stand beside the
 // contiguous cache, the products and the pick of sml-hip.h, whose conventions
 // hold here: device pointers unless a comment says host, 0 on success and -1
 // on failure with the reason in sml_hip_last_error(). The reference has no
@@ -88,6 +90,111 @@ size_t sml_hip_paged_part_floats(int n_seq, int n_head, int hd, int max_len);
 // calls give equal bits.
 int sml_hip_paged_attention(const sml_hip_pages * pg, const float * q, size_t q_stride, const int32_t * len,
                             int max_len, int n_head, float scale, float * part, float * out, void * stream);
+
+// ------------------------------------------------------------ several rows a sequence
+// Append with the place and the rotation of a row apart: row r goes to position
+// slot[r] of its sequence's pages, and pair d of its q and k (halved pairs, d <
+// hd / 2) is turned by row pos[axis[d] * n_rows + r] of the tables. One axis: the
+// drafts of a tree, whose siblings share a position and not a slot. Several (at
+// most 4): time, height and width of an image's or a video's rows, axis giving
+// each pair its own in sections, in turn or as the model has it. axis lies in
+// host memory ([hd / 2], read before the call returns); a pair whose axis is
+// n_axis or more is not turned.
+// Everything else is sml_hip_paged_append's: a row is left out when its slot is
+// outside the sequence's pages, any of its n_axis positions outside
+// 0..n_rope - 1, its sequence outside 0..n_seq - 1 or its page none.
+int sml_hip_paged_append_axes(const sml_hip_pages * pg, float * qkv, size_t qkv_stride, int n_rows, const int32_t * seq,
+                              const int32_t * slot, const int32_t * pos, int n_axis, const uint8_t * axis,
+                              const float * cos_t, const float * sin_t, int n_rope, int n_head, float * q_out,
+                              void * stream);
+
+// New rows of ragged sequences and what each of them attends to. Rows
+// start[b] .. start[b+1] - 1 are sequence b's m newest positions: they lie in its
+// slots h .. len[b] - 1, h = len[b] - m, in order (appended already).
+typedef struct {
+    const int32_t * start;        // [n_seq + 1], not falling; clamped to 0..n_row
+    const int32_t * len;          // [n_seq] the sequence's positions, its new rows among them
+    // Row r attends to slots first[r] .. last[r] - 1. first NULL: 0; last NULL:
+    // up to its own slot, that included, or with a tree up to h. A window, packed
+    // documents, a prefix that all of its rows see, or an empty row of padding
+    // are these two.
+    const int32_t * first, * last;   // [n_row]
+    // and to slot h + j for each bit j set (bit j % 32 of word j / 32), j < m: a
+    // drafted row's ancestors and itself
+    const uint32_t * tree;        // [n_row][tree_words], NULL: none
+    // The bias of distance: slope[head] * |the row's position - the slot's| is
+    // subtracted from a score. A new row's position, and its slot's, is pos[r]
+    // (NULL: its slot); an earlier slot's is its number.
+    const int32_t * pos;          // [n_row], at most 2^30 in size
+    const float * slope;          // [n_head], NULL: no bias
+    float cap;                    // a score s becomes cap * tanh(s / cap) before the bias; 0: it stays
+    int tree_words;
+    int n_row;                    // 0..65535
+    int max_len;                  // (host) bounds every length, as above
+} sml_hip_rows;
+
+// Floats of the workspace of sml_hip_paged_attention_rows: n_kv * (2 *
+// ceil(512 / n_kv) + min(n_seq, n_row)) * min(128, n_row * n_head / n_kv) * (hd + 2).
+size_t sml_hip_paged_rows_floats(int n_seq, int n_row, int n_kv, int n_head, int hd, int max_len);
+// Attention of every new row over its sequence's pages, each page read once for
+// the rows and heads that share it: q row r (q_stride floats apart, 0: n_head *
+// hd; rotated already), scaled by `scale` (0: 1 / sqrt(hd)), into row r of out
+// [n_row][n_head * hd]. n_head is a multiple of n_kv, at most 16 query heads per
+// KV head. A longer len[b] is cut to max_len and to seq_pages * page_size, a
+// negative one is 0. Slots past the length and on absent pages are nobody's.
+// What a row does not attend to does not count, whatever its memory holds, and
+// also where other rows of the call do attend to it; a row with no slot left, or
+// with no score above -infinity, gets zeros. Rows outside every sequence's are
+// left as they were. Precision, ranges and infinities are
+// sml_hip_paged_attention's; the cap and the bias are fp32. How the positions are
+// split follows all of the lengths: a row's sums depend on the other rows by
+// their rounding alone, and equal calls give equal bits.
+int sml_hip_paged_attention_rows(const sml_hip_pages * pg, const sml_hip_rows * rows, const float * q, size_t q_stride,
+                                 int n_head, float scale, float * part, float * out, void * stream);
+
+// ------------------------------------------------------------ the cache's upkeep
+// These act on n_layer layers of one cache at once, which share pg's table: layer
+// l's pools lie l * layer_stride values behind pg's (a multiple of 8, at least a
+// page; unused with one layer). Both ways of laying layers out are meant: whole
+// pools one after another, or each page's layers side by side (page_stride).
+
+// What the picks of a drafted step accept. Row start[b] of sequence b is the last
+// token that was sure, the others are its drafted tree: tok[r] is the token
+// drafted at row r, parent[r] the number in the sequence (0: the root) of the row
+// it follows, which comes before it, pick[r] the model's pick behind row r
+// (sml_hip_logits_adjust's tok). From the root on, the path goes on to the first
+// child whose token is its row's pick, until there is none or max_kept (1..1024)
+// rows are kept. Out: n_kept[b]; kept[b][j], the path's rows by number; next[b][j],
+// the tokens that follow them (row j's pick; the last is the next step's root);
+// both [n_seq][max_kept], -1 behind; len_out[b] = len[b] - m + n_kept[b] (apart
+// from len). Keys and values of the path's rows move to slots h, h + 1 and on, in all
+// layers; n_layer 0 moves nothing. Any of the outputs may be NULL. A sequence of
+// no rows keeps none. The slots of new rows belong to one sequence alone.
+int sml_hip_draft_accept(const sml_hip_pages * pg, int n_layer, size_t layer_stride, int n_row, const int32_t * start,
+                         const int32_t * len, const int32_t * tok, const int32_t * parent, const int32_t * pick,
+                         int max_kept, int32_t * n_kept, int32_t * kept, int32_t * next, int32_t * len_out,
+                         void * stream);
+
+// n_fork (0..65535) sequences that go on from others: row i of table_out
+// [n_fork][seq_pages] (apart from pg's table) gets the full pages of sequence
+// parent[i]'s first len[parent[i]] positions; the page after them, if it is
+// begun, is fresh[i], into which the positions it has are copied in all layers;
+// -1 behind. len_out[i] = len[parent[i]] (apart from len), cut to 0..seq_pages *
+// page_size. fresh[i] outside 0..n_pages - 1 copies nothing and names the
+// parent's page itself: for the one child that goes on in it. A parent outside
+// 0..n_seq - 1 gives an empty sequence. Fresh pages are distinct and nobody's
+// before the call; of an absent page nothing is copied.
+int sml_hip_paged_fork(const sml_hip_pages * pg, int n_layer, size_t layer_stride, const int32_t * len, int n_fork,
+                       const int32_t * parent, const int32_t * fresh, int32_t * table_out, int32_t * len_out,
+                       void * stream);
+
+// n_move (0..65534) pages moved: page src[i] is copied to page dst[i] in all
+// layers, and every entry of table ([n_seq][seq_pages], as a rule pg's; NULL:
+// none) that names src[i] names dst[i] then, whichever sequences share it. src is
+// ascending; dst are distinct pages that nobody names and that are none of src.
+// Pages outside 0..n_pages - 1 move nothing.
+int sml_hip_paged_compact(const sml_hip_pages * pg, int n_layer, size_t layer_stride, int n_move, const int32_t * src,
+                          const int32_t * dst, int32_t * table, void * stream);
 
 // ------------------------------------------------------------ logits
 // What changes a row of logits before the pick; any of the parts may be NULL.

@@ -1,5 +1,5 @@
-// The gfx950 code objects built from kernels.hip, ingest.hip, prompt.hip and
-// serve.hip, linked into the library as read-only data and loaded with hipModuleLoadData at init.
+// The gfx950 code objects built from kernels.hip, ingest.hip, prompt.hip,
+// serve.hip and rows.hip, linked into the library as read-only data and loaded with hipModuleLoadData at init.
     .section .rodata
     .balign 4096
     .global sml_code_object
@@ -32,5 +32,13 @@ sml_serve_object:
     .incbin "serve.hsaco"
     .global sml_serve_object_end
 sml_serve_object_end:
+    .byte 0
+    .balign 4096
+    .global sml_rows_object
+    .type sml_rows_object, @object
+sml_rows_object:
+    .incbin "rows.hsaco"
+    .global sml_rows_object_end
+sml_rows_object_end:
     .byte 0
     .section .note.GNU-stack,"",@progbits

@@ -11,11 +11,12 @@ static struct { char name[64]; hipFunction_t f; } fn_cache[FN_CACHE];
 static int fn_n;
 
 // the gfx950 code objects, linked in from kernels.hsaco, ingest.hsaco,
-// prompt.hsaco and serve.hsaco (code_object.S)
+// prompt.hsaco, serve.hsaco and rows.hsaco (code_object.S)
 extern const unsigned char sml_code_object[];
 extern const unsigned char sml_ingest_object[];
 extern const unsigned char sml_prompt_object[];
 extern const unsigned char sml_serve_object[];
+extern const unsigned char sml_rows_object[];
 
 void hx_fail(const char * what, hipError_t e) {
     snprintf(hx.err, sizeof hx.err, "%s: %s", what, hipGetErrorString(e));
@@ -49,11 +50,13 @@ void hx_init(int device) {
         HX(hipModuleUnload(hx.mod_ingest));
         HX(hipModuleUnload(hx.mod_prompt));
         HX(hipModuleUnload(hx.mod_serve));
+        HX(hipModuleUnload(hx.mod_rows));
     }
     HX(hipModuleLoadData(&hx.mod, sml_code_object));
     HX(hipModuleLoadData(&hx.mod_ingest, sml_ingest_object));
     HX(hipModuleLoadData(&hx.mod_prompt, sml_prompt_object));
     HX(hipModuleLoadData(&hx.mod_serve, sml_serve_object));
+    HX(hipModuleLoadData(&hx.mod_rows, sml_rows_object));
     fn_n = 0;
     hx.ncu = p.multiProcessorCount > 0 ? p.multiProcessorCount : 256;
     if (hx.kpart) {
@@ -78,6 +81,7 @@ hipFunction_t hx_fn(const char * name) {
     HX(hipModuleGetFunction(&f, strncmp(name, "sml_ing_", 8) == 0  ? hx.mod_ingest
                                 : strncmp(name, "sml_pp_", 7) == 0 ? hx.mod_prompt
                                 : strncmp(name, "sml_sv_", 7) == 0 ? hx.mod_serve
+                                : strncmp(name, "sml_rw_", 7) == 0 ? hx.mod_rows
                                                                    : hx.mod, name));
     if (fn_n < FN_CACHE) {
         snprintf(fn_cache[fn_n].name, sizeof fn_cache[fn_n].name, "%s", name);

@@ -22,6 +22,7 @@ typedef struct {
     hipModule_t mod_ingest;       // the ingest kernels (built without contraction)
     hipModule_t mod_prompt;       // the prompt-reading kernels (sml_pp_*)
     hipModule_t mod_serve;        // the kernels of a step of many requests (sml_sv_*)
+    hipModule_t mod_rows;         // those of several rows a request and of a cache's upkeep (sml_rw_*)
     int       ncu;                // compute units of the device
     long      fail_after;         // test hook: fail the Nth HIP call from now (< 0: off)
     long      calls;              // HIP calls made through HX() so far

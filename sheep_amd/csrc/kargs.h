@@ -536,3 +536,55 @@ typedef struct {
     int n_adapter, rank, n_in, n_out, n_row, nsplit, chunk;
     int sorted;                   // tiles take the rows by adapter
 } sml_klora;
+
+// ------------------------------------------------------------ rows.hip
+#define AX_MOST 4                 // the most axes of a rotation
+typedef struct {
+    sml_kpages pg;
+    float * qkv;
+    size_t stride;
+    const int32_t * seq, * slot;  // seq NULL: sequence r
+    const int32_t * pos;          // [n_axis][n_rows]
+    const float * cos_t, * sin_t;
+    float * q_out;                // NULL: in place
+    int n_rows, n_rope, n_head, n_axis;
+    uint8_t axis[64];             // of each pair; n_axis and above: not rotated
+} sml_kaxes;
+
+typedef struct {
+    sml_kpages pg;
+    const float * q;
+    size_t q_stride;
+    const int32_t * start, * len, * first, * last, * pos;
+    const uint32_t * tree;
+    const float * slope;
+    float * part, * out;
+    float scale, cap;
+    int n_head, n_row, max_len, words;
+} sml_krows;
+
+// Layers of a cache: layer l's pools lie l * layer_stride values behind pg's.
+#define AC_MOST 1024              // the most rows of a kept path
+typedef struct {
+    sml_kpages pg;
+    size_t layer_stride;
+    const int32_t * start, * len, * tok, * parent, * pick;
+    int32_t * n_kept, * kept, * next, * len_out;
+    int n_layer, n_row, most;
+} sml_kaccept;
+
+typedef struct {
+    sml_kpages pg;
+    size_t layer_stride;
+    const int32_t * len, * parent, * fresh;
+    int32_t * table_out, * len_out;
+    int n_layer, n_fork;
+} sml_kfork;
+
+typedef struct {
+    sml_kpages pg;
+    size_t layer_stride;
+    const int32_t * src, * dst;
+    int32_t * table;              // NULL: left as it is
+    int n_layer, n_move;
+} sml_kcompact;

@@ -1,26 +1,22 @@
 // The operators of a step that serves many requests at once (sml-serve.h):
 // argument checks and launches. The checks come before the device is touched,
 // so they refuse alike on a machine without one.
-#include "ops.h"
-#include "sml-serve.h"
+#include "serve.h"
 
 #include <math.h>
 #include <stdio.h>
 #include <string.h>
 
-static int al16(const void * p) { return ((uintptr_t) p & 15u) == 0; }
-static int ceil_div(int a, int b) { return (int) (((long) a + b - 1) / b); }
-
 // The device of sml_hip_init has to be the calling thread's: the stream and
 // the buffers of another one would meet kernels loaded for this one.
-static void on_device(void) {
+void sv_on_device(void) {
     if (!hx.inited) hx_init(0);
     int d = -1;
     HX(hipGetDevice(&d));
     if (d != hx.device) hx_failf("device %d is current, the library runs on device %d", d, hx.device);
 }
 
-static void check_pages(const sml_hip_pages * p, sml_kpages * k) {
+void sv_check_pages(const sml_hip_pages * p, sml_kpages * k) {
     if (!p || !p->k || !p->v || !p->table) hx_failf("paged cache: missing pools or table");
     if (p->type != SML_F16 && p->type != SML_BF16) hx_failf("paged cache: type %d", p->type);
     if (p->hd != 64 && p->hd != 128) hx_failf("paged cache: head_dim %d (64 or 128)", p->hd);
@@ -43,7 +39,7 @@ static void check_pages(const sml_hip_pages * p, sml_kpages * k) {
     k->n_seq = p->n_seq; k->seq_pages = p->seq_pages; k->n_kv = p->n_kv; k->hd = p->hd;
 }
 
-static void sv_name(char * s, size_t n, const char * base, int hd, int type) {
+void sv_name(char * s, size_t n, const char * base, int hd, int type) {
     snprintf(s, n, "%s%s%s", base, hd == 64 ? "_d64" : "", type == SML_BF16 ? "_bf" : "");
 }
 
@@ -53,12 +49,12 @@ int sml_hip_paged_append(const sml_hip_pages * pg, float * qkv, size_t qkv_strid
     HX_ENTRY(-1);
     sml_kappend a;
     memset(&a, 0, sizeof a);
-    check_pages(pg, &a.pg);
+    sv_check_pages(pg, &a.pg);
     if (n_rows < 0 || n_rows > 1 << 22 || n_head < 1 || n_head > 65536) hx_failf("append: %d rows of %d heads", n_rows, n_head);
     const size_t width = ((size_t) n_head + 2 * (size_t) pg->n_kv) * pg->hd;
     if (!qkv || !pos || !cos_t || !sin_t || n_rope < 1) hx_failf("append: missing rows, positions or rotation tables");
     if (qkv_stride && qkv_stride < width) hx_failf("append: rows of %zu floats %zu apart", width, qkv_stride);
-    on_device();
+    sv_on_device();
     if (n_rows) {
         a.qkv = qkv; a.stride = qkv_stride ? qkv_stride : width; a.seq = seq; a.pos = pos;
         a.cos_t = cos_t; a.sin_t = sin_t; a.q_out = q_out; a.n_rope = n_rope; a.n_head = n_head;
@@ -82,14 +78,14 @@ int sml_hip_paged_attention(const sml_hip_pages * pg, const float * q, size_t q_
     HX_ENTRY(-1);
     sml_kattend a;
     memset(&a, 0, sizeof a);
-    check_pages(pg, &a.pg);
+    sv_check_pages(pg, &a.pg);
     if (n_head < 1 || n_head % pg->n_kv || n_head / pg->n_kv > 16)
         hx_failf("paged attention: %d heads over %d kv heads (1 to 16 each)", n_head, pg->n_kv);
     if (!q || !len || !part || !out || max_len < 0) hx_failf("paged attention: missing buffers, or lengths up to %d", max_len);
     if (!al16(part)) hx_failf("paged attention: workspace off a 16-byte boundary");
     const size_t width = (size_t) n_head * pg->hd;
     if (q_stride && q_stride < width) hx_failf("paged attention: rows of %zu floats %zu apart", width, q_stride);
-    on_device();
+    sv_on_device();
     a.q = q; a.q_stride = q_stride ? q_stride : width; a.len = len; a.part = part; a.out = out;
     a.scale = (scale != 0.0f ? scale : 1.0f / sqrtf((float) pg->hd)) * 1.44269504088896341f;
     a.n_head = n_head;
@@ -168,7 +164,7 @@ int sml_hip_logits_adjust(const float * logits, size_t stride, int n_row, int n_
             a.mask = r->mask; a.mask_row = r->mask_row; a.n_mask = r->n_mask;
         }
     }
-    on_device();
+    sv_on_device();
     if (n_row) {
         a.n_part = ceil_div(n_vocab, LG_RANGE);
         // one word a thread while the workgroups are at most 2 a CU (a call of
@@ -289,7 +285,7 @@ int sml_hip_lora_add(const sml_hip_adapters * ad, const float * x, size_t x_stri
     if (!x || !adapter || !y || !work) hx_failf("adapters: missing rows, ids, output or workspace");
     if ((x_stride && x_stride < (size_t) ad->n_in) || (y_stride && y_stride < (size_t) ad->n_out))
         hx_failf("adapters: rows of %d and %d floats %zu and %zu apart", ad->n_in, ad->n_out, x_stride, y_stride);
-    on_device();
+    sv_on_device();
     if (n_row) {
         sml_klora a;
         memset(&a, 0, sizeof a);

@@ -5,9 +5,12 @@ Keys and values live in a paged cache (`Pages`): `append` rotates the new
 tokens' keys and writes them with their values, `attention` lets one new token
 a sequence attend over its pages, `lora` adds each request's adapter beside a
 shared projection (`sheep_amd.gemm`), and `adjust_logits` applies penalties,
-biases and grammar masks and picks greedily. Buffers are DevBuf or anything
-with a device pointer in `.ptr`; workspaces are the caller's, sized by
-`part_floats`, `logits_part_bytes` and `lora_work_floats`. `stream` is a
+biases and grammar masks and picks greedily. Several rows a sequence (a draft's
+tree, a prompt's chunk; `Rows`) go through `append_axes` and `attention_rows`,
+`accept` keeps what the picks accept of a draft, and `fork` and `compact` look
+after the pages. Buffers are DevBuf or anything with a device pointer in
+`.ptr`; workspaces are the caller's, sized by `part_floats`, `rows_floats`,
+`logits_part_bytes` and `lora_work_floats`. `stream` is a
 hipStream_t as an int (0: the null stream). The reference has no counterpart:
 it keeps one contiguous cache per sequence (sml/sml-run.c:3414-3434) and picks
 greedily (sml/sml-run.c:3539-3544).
@@ -26,6 +29,7 @@ _vp, _int, _size, _float = ctypes.c_void_p, ctypes.c_int, ctypes.c_size_t, ctype
 _PAGES = struct.Struct("PPPN7i0N")            # sml_hip_pages
 _RULES = struct.Struct("PPPiPPPPPPiPPi0N")    # sml_hip_rules
 _ADAPTERS = struct.Struct("PPPP5i0N")         # sml_hip_adapters
+_ROWS = struct.Struct("7Pf3i0N")              # sml_hip_rows
 
 
 _block = ctypes.c_char_p
@@ -33,6 +37,13 @@ _SIGS = [
     ("sml_hip_paged_append", _int, [_block, _vp, _size, _int, _vp, _vp, _vp, _vp, _int, _int, _vp, _vp]),
     ("sml_hip_paged_part_floats", _size, [_int, _int, _int, _int]),
     ("sml_hip_paged_attention", _int, [_block, _vp, _size, _vp, _int, _int, _float, _vp, _vp, _vp]),
+    ("sml_hip_paged_append_axes", _int, [_block, _vp, _size, _int, _vp, _vp, _vp, _int, _block, _vp, _vp, _int, _int, _vp,
+                                         _vp]),
+    ("sml_hip_paged_rows_floats", _size, [_int] * 6),
+    ("sml_hip_paged_attention_rows", _int, [_block, _block, _vp, _size, _int, _float, _vp, _vp, _vp]),
+    ("sml_hip_draft_accept", _int, [_block, _int, _size, _int, _vp, _vp, _vp, _vp, _vp, _int, _vp, _vp, _vp, _vp, _vp]),
+    ("sml_hip_paged_fork", _int, [_block, _int, _size, _vp, _int, _vp, _vp, _vp, _vp, _vp]),
+    ("sml_hip_paged_compact", _int, [_block, _int, _size, _int, _vp, _vp, _vp, _vp]),
     ("sml_hip_logits_part_bytes", _size, [_int, _int]),
     ("sml_hip_logits_adjust", _int, [_vp, _size, _int, _int, _block, _vp, _size, _vp, _vp, _vp]),
     ("sml_hip_lora_work_floats", _size, [_int, _int]),
@@ -105,6 +116,81 @@ def attention(pages, q, lens, max_len, n_head, part, out, scale=0.0, q_stride=0,
     _chk(_call.paged_attention(pages.c, q is not None and q.ptr, q_stride, lens is not None and lens.ptr, max_len,
                                n_head, scale, part is not None and part.ptr, out is not None and out.ptr, stream),
          "paged attention")
+
+
+def sections(*pairs):
+    """append_axes' axis of each rotated pair, in sections: the first pairs[0] turn by axis 0, the next by 1 and so on."""
+    return b"".join(bytes([i]) * n for i, n in enumerate(pairs))
+
+
+def append_axes(pages, qkv, n_rows, slot, pos, axis, cos, sin, n_rope, n_head, n_axis=1, seq=None, q_out=None,
+                qkv_stride=0, stream=0):
+    """append with each row's place in its sequence in slot, and the rotation of
+    pair d by pos[axis[d]] of pos [n_axis][n_rows] (sml_hip_paged_append_axes);
+    axis: bytes, one for each of the hd / 2 pairs."""
+    if axis is not None and len(axis) != pages.hd // 2:
+        raise HipError(f"axes of {len(axis)} pairs for heads of {pages.hd}")
+    _chk(_call.paged_append_axes(pages.c, qkv is not None and qkv.ptr, qkv_stride, n_rows,
+                                 seq is not None and (seq.ptr or _freed(seq)), slot is not None and slot.ptr,
+                                 pos is not None and pos.ptr, n_axis, axis, cos is not None and cos.ptr,
+                                 sin is not None and sin.ptr, n_rope, n_head,
+                                 q_out is not None and (q_out.ptr or _freed(q_out)), stream), "paged append")
+
+
+class Rows:
+    """New rows of ragged sequences and what each attends to (sml_hip_rows):
+    start [n_seq+1], lens [n_seq], first and last [n_row] int32, tree [n_row]
+    [tree_words] bits, pos [n_row] int32, slope [n_head] floats. The buffers
+    stay alive with the object."""
+
+    def __init__(self, start, lens, n_row, max_len, first=None, last=None, tree=None, tree_words=0, pos=None, slope=None,
+                 cap=0.0):
+        self.buffers = (start, lens, first, last, tree, pos, slope)
+        try:
+            self.c = _ROWS.pack(_at(start), _at(lens), _at(first), _at(last), _at(tree), _at(pos), _at(slope), cap,
+                                tree_words, n_row, max_len)
+        except struct.error:
+            _freed(*self.buffers)
+            raise
+
+
+def rows_floats(n_seq, n_row, n_kv, n_head, hd, max_len):
+    """Floats of attention_rows' workspace."""
+    return _call.paged_rows_floats(n_seq, n_row, n_kv, n_head, hd, max_len)
+
+
+def attention_rows(pages, rows, q, n_head, part, out, scale=0.0, q_stride=0, stream=0):
+    """out [n_row][n_head*hd]: every new row over what it attends to of its
+    sequence's pages (sml_hip_paged_attention_rows)."""
+    _chk(_call.paged_attention_rows(pages.c, rows.c, q is not None and q.ptr, q_stride, n_head, scale,
+                                    part is not None and part.ptr, out is not None and out.ptr, stream),
+         "rows' attention")
+
+
+def accept(pages, n_row, start, lens, tok, parent, pick, max_kept, n_kept=None, kept=None, next=None, len_out=None,
+           n_layer=1, layer_stride=0, stream=0):
+    """Which drafted rows the picks accept, and their keys and values moved
+    together in all layers (sml_hip_draft_accept)."""
+    if (n_kept is not None and not n_kept.ptr) or (kept is not None and not kept.ptr) or \
+            (next is not None and not next.ptr) or (len_out is not None and not len_out.ptr):
+        _freed(n_kept, kept, next, len_out)
+    _chk(_call.draft_accept(pages.c, n_layer, layer_stride, n_row, _at(start), _at(lens), _at(tok), _at(parent), _at(pick),
+                            max_kept, _at(n_kept), _at(kept), _at(next), _at(len_out), stream), "accept")
+
+
+def fork(pages, lens, n_fork, parent, fresh, table_out, len_out, n_layer=1, layer_stride=0, stream=0):
+    """table_out [n_fork][seq_pages] and len_out of sequences that go on from
+    others, each one's begun page copied to its fresh page in all layers
+    (sml_hip_paged_fork)."""
+    _chk(_call.paged_fork(pages.c, n_layer, layer_stride, _at(lens), n_fork, _at(parent), _at(fresh), _at(table_out),
+                          _at(len_out), stream), "fork")
+
+
+def compact(pages, n_move, src, dst, table=None, n_layer=1, layer_stride=0, stream=0):
+    """Pages src (ascending) copied to pages dst in all layers, and the table's
+    entries renamed (sml_hip_paged_compact)."""
+    _chk(_call.paged_compact(pages.c, n_layer, layer_stride, n_move, _at(src), _at(dst),
+                             table is not None and (table.ptr or _freed(table)), stream), "compact")
 
 
 def logits_part_bytes(n_row, n_vocab):
