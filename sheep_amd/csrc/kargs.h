@@ -559,9 +559,17 @@ typedef struct {
     const uint32_t * tree;
     const float * slope;
     float * part, * out;
-    float scale, cap;
+    float scale, sign;            // |scale| times log2(e), or over the cap; the scale's sign
+    float cap;                    // times log2(e)
     int n_head, n_row, max_len, words;
+    int cols;                     // columns of a tile
+    int want, least;              // splits wanted in all (0: none), blocks of one at least
+    int items, part_cols;         // the partials' items a KV head, and the columns of one
 } sml_krows;
+#define RW_BLOCK 64               // positions of a block
+#define RW_STAGE(d) (2 * RW_BLOCK * 2 * (d))   // LDS of a block: its K rows, then its V rows
+#define RW_EXTRA (2 * RW_BLOCK * 4 + 64 * 4)   // and beside two of them
+#define RW_SPLITS 512             // the most splits of a tile
 
 // Layers of a cache: layer l's pools lie l * layer_stride values behind pg's.
 #define AC_MOST 1024              // the most rows of a kept path

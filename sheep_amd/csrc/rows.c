@@ -4,6 +4,7 @@
 #include "serve.h"
 
 #include <math.h>
+#include <stdio.h>
 #include <string.h>
 
 int sml_hip_paged_append_axes(const sml_hip_pages * pg, float * qkv, size_t qkv_stride, int n_rows, const int32_t * seq,
@@ -42,6 +43,35 @@ size_t sml_hip_paged_rows_floats(int n_seq, int n_row, int n_kv, int n_head, int
     return (size_t) n_kv * blocks * (cols < 128 ? cols : 128) * (size_t) (hd + 2);
 }
 
+#define LOG2E 1.44269504088896341f
+// A grid of items (y, z) for each KV head (x): the heads of neighbouring items
+// run on the same XCDs, whose L2s each hold a head's pages once.
+static void items_launch(const char * name, int n_kv, long items, unsigned threads, size_t lds, hipStream_t st, void * a) {
+    const long y = items < 32768 ? items : 32768;
+    hx_launch3(name, (unsigned) n_kv, (unsigned) y, (unsigned) ((items + y - 1) / y), threads, lds, st, a);
+}
+
+static void rows_launch(sml_krows * a, int hd, int type, hipStream_t st) {
+    const int n_kv = a->pg.n_kv, rep = a->n_head / n_kv, n_seq = a->pg.n_seq;
+    const int ncol = a->n_row * rep, some = n_seq < a->n_row ? n_seq : a->n_row;
+    const int waves = ncol > 64L * some ? 8 : 4;
+    a->cols = 16 * waves;
+    // two workgroups a CU; not split where the tiles are as many
+    const int want = ceil_div(2 * hx.ncu < 512 ? 2 * hx.ncu : 512, n_kv);
+    a->least = 2;
+    const int split = n_seq <= AT_SHARED && ceil_div(ncol, a->cols) < want && a->max_len > RW_BLOCK * a->least;
+    a->want = split ? want : 0;
+    long tiles = (long) ncol / a->cols + (split ? some : n_seq);
+    long items = split ? tiles + want : tiles;
+    a->items = (int) items;
+    a->part_cols = ncol < a->cols ? ncol : a->cols;
+    char base[24], name[40];
+    snprintf(base, sizeof base, "sml_rw_rows%d", waves);
+    sv_name(name, sizeof name, base, hd, type);
+    items_launch(name, n_kv, items, 64 * (unsigned) waves, (size_t) 2 * RW_STAGE(hd) + RW_EXTRA, st, a);
+    if (split) items_launch(hd == 64 ? "sml_rw_merge_d64" : "sml_rw_merge", n_kv, tiles * (a->cols / 16), 256, 0, st, a);
+}
+
 int sml_hip_paged_attention_rows(const sml_hip_pages * pg, const sml_hip_rows * rows, const float * q, size_t q_stride,
                                  int n_head, float scale, float * part, float * out, void * stream) {
     HX_ENTRY(-1);
@@ -65,13 +95,14 @@ int sml_hip_paged_attention_rows(const sml_hip_pages * pg, const sml_hip_rows * 
         a.q = q; a.q_stride = q_stride ? q_stride : width; a.part = part; a.out = out;
         a.start = rows->start; a.len = rows->len; a.first = rows->first; a.last = rows->last; a.pos = rows->pos;
         a.tree = rows->tree; a.words = rows->tree_words; a.slope = rows->slope; a.cap = rows->cap;
-        a.scale = scale != 0.0f ? scale : 1.0f / sqrtf((float) pg->hd);
+        if (scale == 0.0f) scale = 1.0f / sqrtf((float) pg->hd);
+        a.sign = scale < 0.0f ? -1.0f : 1.0f;
+        a.scale = rows->cap > 0.0f ? fabsf(scale) / rows->cap : fabsf(scale) * LOG2E;
+        a.cap = rows->cap * LOG2E;
         a.n_head = n_head; a.n_row = rows->n_row;
         const long cap = (long) pg->seq_pages * pg->page_size;
         a.max_len = rows->max_len < cap ? rows->max_len : (int) cap;
-        char name[40];
-        sv_name(name, sizeof name, "sml_rw_rows", pg->hd, pg->type);
-        hx_launch(name, (unsigned) n_head, (unsigned) a.n_row, 256, 0, (hipStream_t) stream, &a);
+        rows_launch(&a, pg->hd, pg->type, (hipStream_t) stream);
     }
     HX_LEAVE();
     return 0;

@@ -72,107 +72,574 @@ AXES(64, 0, sml_rw_append_d64)
 AXES(64, 1, sml_rw_append_d64_bf)
 
 // ---------------------------------------------------------------- attention
+//
+// out = sum_t 2^(s_t - m) v_t / sum_t 2^(s_t - m) over the slots a row attends
+// to, s_t = log2(e) (cap tanh(scale q.k_t / cap) - slope |distance|), in one pass
+// over the cache with a running base m.
+//
+// The (row, query head) pairs of a sequence and KV head are columns, a row's
+// heads side by side. A workgroup takes a tile of 16 W of them, 16 a wave, and a
+// split of the positions, in blocks of 64 whose keys and values all its waves
+// share in LDS. The matrix cores take S^T = K Q^T and O^T = V^T P^T, columns in
+// the columns. With the lane's c = lane % 16, g = lane / 16:
+// - K is read from LDS as the first operand: lane (c, g) takes position 16j + c's
+//   dims 32i + 8g..; S comes back as positions 16j + 4g + r of column c.
+// - That is just what the second product takes as P^T if its inner index 8g + i
+//   stands for position 4g + i of an even 16 positions (i < 4) or of the next odd
+//   ones: P never crosses lanes.
+// - V^T comes by transposing LDS reads (ds_read_b64_tr_b16: 16 lanes read 4 rows
+//   of 16 dims and take a dim's 4 rows each) in the same order, and lane (c, g)
+//   ends with dims 16u + 4g.. of column c: the base's rescaling is a lane's own.
+// q and the weights are split into 16-bit parts, as in sml_sv_attend, whose base
+// and room these are. K and V go from memory to LDS without registers, a block
+// ahead, 16-byte words swizzled by row so that both kinds of read touch each bank
+// as often as any other.
+//
+// Masks cost a block only where it is not whole for all of a wave's columns: each
+// lane then makes its column's 64 bits of the block, of the range, the tree and
+// the pages that are there. What a column does not attend to has no weight, but
+// 0 times a NaN or an infinity is none either: rows that no column of the tile
+// may see are loaded as zeros, and where columns differ, waves look their share of
+// the values through on its arrival and take a block with any that is not finite
+// value by value.
+//
+// Lengths and counts are ragged and on the device: every wave sums them up and
+// finds its workgroup's tile and split (rows_place), splits of one size for all
+// but cut to what a tile's rows see. Calls with tiles enough are not split, and
+// sequences past AT_SHARED neither; those tiles are found by halving.
+typedef short v4s __attribute__((ext_vector_type(4)));
 
-// The sequence of row r: the last whose rows begin at or before it. -1 where
-// the row is nobody's.
-__device__ __forceinline__ int row_seq(const sml_krows & a, int r) {
-    int lo = 0, hi = a.pg.n_seq;                      // start[lo] <= r < start[hi], if they do not fall
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (a.start[mid] <= r) lo = mid;
-        else hi = mid;
-    }
-    return a.start[lo] <= r && r < a.start[lo + 1] ? lo : -1;
+// What no column may see is read from here.
+__device__ const uint8_t rw_zeros[16] = { 0 };
+
+// 16 bytes a lane straight into LDS, the wave's 64 lanes side by side from dst (a
+// wave-uniform address) on; the caller waits (vmcnt) and then meets the other
+// waves before any of the bytes is read. Written out because the compiler, which
+// cannot tell the buffers apart, otherwise waits for every copy in flight before
+// the next LDS read.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"             // m0 among the clobbers: it is what the statement sets
+__device__ __forceinline__ void copy_lds16(const void * src, const void * dst) {
+    const uint32_t at = (uint32_t) (uintptr_t) (const __attribute__((address_space(3))) void *) dst;
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
+                 :: "s"(__builtin_amdgcn_readfirstlane(at)), "v"(src) : "m0", "memory");
+}
+#pragma clang diagnostic pop
+
+struct rows_of { int s0, m, n; };                     // a sequence's first row, its rows and its positions
+__device__ __forceinline__ rows_of rows_seq(const sml_krows & a, int b) {
+    rows_of x;
+    x.s0 = min(max(a.start[b], 0), a.n_row);
+    x.m = min(max(a.start[b + 1], x.s0), a.n_row) - x.s0;
+    x.n = min(max(a.len[b], 0), a.max_len);
+    return x;
 }
 
-// A workgroup a row and head, its waves alternating chunks of 64 positions, a
-// position a lane for the scores and dims a lane for the sum of values: fp32
-// throughout.
-template <int D, int BF>
+struct rows_at { int b, tile, count, split, item; };  // a tile, its splits, this one's number, and the first's among all items
+// Item i's (or, of TILES, tile i's) place; false past the last. Without splits
+// (want 0) sequence b's tiles are numbered from start[b] * rep / cols + b on, which
+// leaves each as many numbers as it has tiles, and the number says whose it is.
+template <bool TILES>
+__device__ __forceinline__ bool rows_place(const sml_krows & a, int i, int lane, rows_at & p) {
+    const int rep = a.n_head / a.pg.n_kv, cols = a.cols;
+    if (!a.want) {
+        int lo = 0, hi = a.pg.n_seq;
+        while (hi - lo > 1) {
+            const int step = (hi - lo + 63) / 64, at = lo + lane * step;
+            const bool in = at < hi && min(max(a.start[at], 0), a.n_row) * rep / cols + at <= i;
+            const unsigned long long hit = __ballot(in);
+            const int k = hit ? 63 - __builtin_clzll(hit) : 0;
+            lo += k * step;
+            hi = min(hi, lo + step);
+        }
+        const rows_of x = rows_seq(a, lo);
+        p.b = lo;
+        p.tile = i - (x.s0 * rep / cols + lo);
+        p.count = 1;
+        p.split = 0;
+        p.item = i;
+        return p.tile >= 0 && p.tile * cols < x.m * rep;
+    }
+    // the blocks of a split: what makes want of them in all, and some more
+    float sum = 0.0f;
+    for (int b = lane; b < a.pg.n_seq; b += 64) {
+        const rows_of x = rows_seq(a, b);
+        sum += (float) ((x.m * rep + cols - 1) / cols) * (float) ((x.n + RW_BLOCK - 1) / RW_BLOCK);
+    }
+    const int chunk = max(a.least, (int) (wave_sum(sum) * 1.0001f / (float) a.want) + 1);
+    p.item = 0;
+    for (int b0 = 0; b0 < a.pg.n_seq; b0 += 64) {
+        int nt = 0, count = 1;
+        if (b0 + lane < a.pg.n_seq) {
+            const rows_of x = rows_seq(a, b0 + lane);
+            nt = (x.m * rep + cols - 1) / cols;
+            count = max(((x.n + RW_BLOCK - 1) / RW_BLOCK + chunk - 1) / chunk, 1);
+        }
+        const int items = wave_scan(nt * count), mine = TILES ? wave_scan(nt) : items;
+        const unsigned long long hit = __ballot(mine > i);
+        if (hit) {
+            const int l = __builtin_ctzll(hit);
+            p.b = b0 + l;
+            p.count = __builtin_amdgcn_readlane(count, l);
+            const int n = __builtin_amdgcn_readlane(nt, l);
+            const int k = i - (__builtin_amdgcn_readlane(mine, l) - (TILES ? n : n * p.count));
+            p.tile = TILES ? k : k / p.count;
+            p.split = TILES ? 0 : k % p.count;
+            p.item += __builtin_amdgcn_readlane(items, l) - n * p.count + p.tile * p.count;
+            return true;
+        }
+        i -= __builtin_amdgcn_readlane(mine, 63);
+        p.item += __builtin_amdgcn_readlane(items, 63);
+    }
+    return false;
+}
+__device__ __forceinline__ int rows_item() { return (int) (blockIdx.z * gridDim.y + blockIdx.y); }
+// The sums of an item's columns, and their bases and weights' sums.
+__device__ __forceinline__ float * part_o(const sml_krows & a, int kh, int item, int d) {
+    return a.part + ((size_t) kh * a.items + item) * a.part_cols * d;
+}
+__device__ __forceinline__ float2 * part_ml(const sml_krows & a, int kh, int item, int d) {
+    return (float2 *) (a.part + (size_t) a.pg.n_kv * a.items * a.part_cols * d) + ((size_t) kh * a.items + item) * a.part_cols;
+}
+
+// tanh(y) for |y| up to 0.625: y times a polynomial of y^2 (least relative error
+// on that range, 4e-9; 1.1e-7 as evaluated). Past it 1 - 2 / (e^2y + 1), whose
+// cancellation costs less than a bit there.
+__device__ __forceinline__ float tanh_small(float y) {
+    const float z = y * y;
+    float p = __builtin_fmaf(-0.0056599886f, z, 0.020590989f);
+    p = __builtin_fmaf(p, z, -0.053721067f);
+    p = __builtin_fmaf(p, z, 0.13331127f);
+    p = __builtin_fmaf(p, z, -0.33333260f);
+    return y * __builtin_fmaf(p, z, 1.0f);
+}
+__device__ __forceinline__ float tanh_any(float y) {
+    const float e = __builtin_amdgcn_exp2f(y * 2.88539008177792681f);
+    const float t = __builtin_fmaf(-2.0f, __builtin_amdgcn_rcpf(e + 1.0f), 1.0f);
+    return fabsf(y) > 0.625f ? t : tanh_small(y);
+}
+
+// Bits lo..hi-1 of 64.
+__device__ __forceinline__ uint64_t bits_range(int lo, int hi) {
+    lo = min(max(lo, 0), 64);
+    hi = min(max(hi, 0), 64);
+    if (lo >= hi) return 0;
+    return (~0ull >> (64 - (hi - lo))) << lo;
+}
+
+template <int D, int BF, int W>
 __device__ __forceinline__ void rows_body(const sml_krows & a) {
-    __shared__ float q[D], pw[4][64], so[4][D], sm[4], sl[4];
-    const int h = blockIdx.x, r = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int b = row_seq(a, r);
-    if (b < 0) return;
-    const int s0 = min(max(a.start[b], 0), a.n_row), s1 = min(max(a.start[b + 1], s0), a.n_row);
-    const int n = min(max(a.len[b], 0), a.max_len), m = s1 - s0, past = n - m, own = past + r - s0;
+    using M = Mx<BF>;
+    typedef typename M::v8 v8;
+    constexpr int NJ = D / 32, E = D / 16, NP = M::parts, RB = 2 * D, POOL = RW_BLOCK * RB, STAGE = 2 * POOL;
+    constexpr int RC = 1024 / RB, NC = RW_BLOCK / RC / W;   // rows of a copy, a wave's copies of a block
+    static_assert(NC >= 1, "");
+    extern __shared__ __align__(16) uint8_t lds[];    // two stages, their new rows' positions, what waves found in V
+    int * const kpos = (int *) (lds + 2 * STAGE);
+    int * const found = kpos + 2 * RW_BLOCK;
+    const int kh = blockIdx.x, tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    rows_at p;
+    if (!rows_place<false>(a, rows_item(), lane, p)) return;
+    const rows_of sq = rows_seq(a, p.b);
+    const int rep = a.n_head / a.pg.n_kv, ncol = sq.m * rep, past = sq.n - sq.m, kvd = a.pg.n_kv * D;
+    const int sh = a.pg.page_shift, pmask = (1 << sh) - 1;
+    const int32_t * const tab = a.pg.table + (size_t) p.b * a.pg.seq_pages;
+
+    // the lane's column: its row's range, its tree's bits and its position
+    const int col = p.tile * a.cols + wave * 16 + c;
+    const bool mine = col < ncol;
+    const int i = min(col, ncol - 1) / rep, r = sq.s0 + i, h = kh * rep + (min(col, ncol - 1) - i * rep);
     const int lo = a.first ? max(a.first[r], 0) : 0;
-    const int hi = min(a.last ? a.last[r] : a.tree ? past : own + 1, n);
-    const int kh = h / (a.n_head / a.pg.n_kv), kvd = a.pg.n_kv * D, sh = a.pg.page_shift, pmask = (1 << sh) - 1;
-    const uint32_t * bits = a.tree ? a.tree + (size_t) r * a.words : nullptr;
-    const int qpos = a.pos ? a.pos[r] : own;
-    if (tid < D) q[tid] = a.q[(size_t) r * a.q_stride + (size_t) h * D + tid];
-    __syncthreads();
-    const float slope = a.slope ? a.slope[h] : 0.0f;
-    float m_run = -INFINITY, l = 0.0f, o[D / 64];
-    #pragma unroll
-    for (int u = 0; u < D / 64; u++) o[u] = 0.0f;
-    for (int t0 = 64 * wave; t0 < n; t0 += 256) {
-        const int t = t0 + lane, j = t - past;
-        bool see = t < n && t >= lo && t < hi;
-        if (bits && t < n && j >= 0 && j < m && j < 32 * a.words) see |= (bits[j >> 5] >> (j & 31)) & 1;
-        int page = see ? page_of(a.pg, b, t >> sh) : -1;
-        see &= page >= 0;
-        size_t at = see ? (size_t) page * a.pg.page_stride + (size_t) (t & pmask) * kvd + (size_t) kh * D : 0;
-        float s = -INFINITY;
-        if (see) {
-            s = 0.0f;
-            for (int d = 0; d < D; d += 8) {
-                const v4u w = *(const v4u *) (a.pg.k + at + d);
-                #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    s = __builtin_fmaf(of16<BF>((uint16_t) (w[e] & 0xFFFF)), q[d + 2 * e], s);
-                    s = __builtin_fmaf(of16<BF>((uint16_t) (w[e] >> 16)), q[d + 2 * e + 1], s);
-                }
-            }
-            s *= a.scale;
-            if (a.cap > 0.0f) s = a.cap * tanhf(s / a.cap);
-            if (a.slope) {
-                const int kpos = j >= 0 && a.pos ? a.pos[s0 + j] : t;
-                s -= slope * fabsf((float) (qpos - kpos));
-            }
-        }
-        const float top = fmaxf(m_run, wave_max(s)), tu = top == -INFINITY ? 0.0f : top;
-        const float al = expf(m_run - tu), p = see ? expf(s - tu) : 0.0f;
-        m_run = top;
-        l = l * al + p;
-        pw[wave][lane] = p;
-        wave_lds();
+    const int hi = min(a.last ? a.last[r] : a.tree ? past : past + i + 1, sq.n);
+    const int nbit = a.tree ? min(sq.m, 32 * a.words) : 0;
+    const uint32_t * const bits = a.tree + (size_t) r * a.words;
+    const int qpos = a.pos ? a.pos[r] : past + i;
+    bool some = lo < hi;                              // does it attend to anything
+    if (nbit) {
+        if (a.words > 8) some = true;
+        else
+            for (int w = 0; w < a.words; w++) some |= bits[w] != 0;
+    }
+    some &= mine;
+    // what any column of the wave, of the tile attends to lies in w_lo..w_hi, t_lo..t_hi;
+    // every one that attends to anything has all of f_lo..f_hi (f4_: of the tile)
+    int w_lo, w_hi, f_lo, f_hi, t_lo, t_hi, t_flo, t_fhi;
+    {
+        const bool range = some && lo < hi, tree = some && nbit > 0 && past + nbit > 0;
+        int x0 = range ? lo : 0x7fffffff, x1 = range ? hi : 0;
+        if (tree) { x0 = min(x0, max(past, 0)); x1 = max(x1, min(past + nbit, sq.n)); }
+        int x2 = some ? (lo < hi ? lo : 0x7fffffff) : 0, x3 = some ? (lo < hi ? hi : 0) : 0x7fffffff;
         #pragma unroll
-        for (int u = 0; u < D / 64; u++) o[u] *= al;
-        const unsigned long long any = __ballot(see);
-        for (int i = 0; i < 64; i++) {
-            if (!((any >> i) & 1)) continue;
-            const float w = pw[wave][i];
-            const size_t v = ((size_t) (unsigned) __shfl((int) (at >> 32), i) << 32) | (unsigned) __shfl((int) at, i);
-            #pragma unroll
-            for (int u = 0; u < D / 64; u++) o[u] = __builtin_fmaf(w, of16<BF>(a.pg.v[v + 64 * u + lane]), o[u]);
+        for (int o = 1; o < 16; o <<= 1) {
+            x0 = min(x0, __shfl_xor(x0, o));
+            x1 = max(x1, __shfl_xor(x1, o));
+            x2 = max(x2, __shfl_xor(x2, o));
+            x3 = min(x3, __shfl_xor(x3, o));
         }
-        wave_lds();
+        w_lo = __builtin_amdgcn_readfirstlane(x0);
+        w_hi = __builtin_amdgcn_readfirstlane(x1);
+        f_lo = __builtin_amdgcn_readfirstlane(x2);
+        f_hi = __builtin_amdgcn_readfirstlane(x3);
+        int * const red = kpos;
+        if (!lane) { red[4 * wave] = w_lo; red[4 * wave + 1] = w_hi; red[4 * wave + 2] = f_lo; red[4 * wave + 3] = f_hi; }
+        __syncthreads();
+        t_lo = red[0]; t_hi = red[1]; t_flo = red[2]; t_fhi = red[3];
+        #pragma unroll
+        for (int w = 1; w < W; w++) {
+            t_lo = min(t_lo, red[4 * w]);
+            t_hi = max(t_hi, red[4 * w + 1]);
+            t_flo = max(t_flo, red[4 * w + 2]);
+            t_fhi = min(t_fhi, red[4 * w + 3]);
+        }
+        __syncthreads();                              // the positions may be written
+        t_lo = __builtin_amdgcn_readfirstlane(t_lo);
+        t_hi = __builtin_amdgcn_readfirstlane(t_hi);
+        t_flo = __builtin_amdgcn_readfirstlane(t_flo);
+        t_fhi = __builtin_amdgcn_readfirstlane(t_fhi);
     }
-    l = wave_sum(l);
-    if (!lane) { sm[wave] = m_run; sl[wave] = l; }
+    // this split's blocks
+    int t_at = 0, t_end = 0;
+    if (t_lo < t_hi) {
+        const int b0 = t_lo / RW_BLOCK, nb = (t_hi + RW_BLOCK - 1) / RW_BLOCK - b0, per = (nb + p.count - 1) / p.count;
+        t_at = (b0 + p.split * per) * RW_BLOCK;
+        t_end = min((b0 + min(nb, (p.split + 1) * per)) * RW_BLOCK, t_hi);
+    }
+
+    // the query: lane (c, g) holds dims 32j + 8g.. of column c, in parts
+    v8 q[NJ][NP];
+    float back;                                       // what a product of the scaled q is multiplied by
+    {
+        float x[NJ][8], mx = 0.0f;
+        const float * qp = a.q + (size_t) r * a.q_stride + (size_t) h * D + 8 * g;
+        #pragma unroll
+        for (int j = 0; j < NJ; j++)
+            #pragma unroll
+            for (int e = 0; e < 8; e += 4) {
+                const v4f v = *(const v4fu *) (qp + 32 * j + e);
+                #pragma unroll
+                for (int k = 0; k < 4; k++) { x[j][e + k] = mine ? v[k] * a.sign : 0.0f; mx = fmaxf(mx, fabsf(x[j][e + k])); }
+            }
+        mx = fmaxf(mx, __shfl_xor(mx, 16));
+        mx = fmaxf(mx, __shfl_xor(mx, 32));
+        const int ex = BF ? 0 : scale_of(mx);
+        #pragma unroll
+        for (int j = 0; j < NJ; j++)
+            #pragma unroll
+            for (int e = 0; e < 8; e += 2)
+                parts_of<BF>(__builtin_amdgcn_ldexpf(x[j][e], -ex), __builtin_amdgcn_ldexpf(x[j][e + 1], -ex), q[j], e);
+        back = __builtin_amdgcn_ldexpf(a.scale, ex);
+    }
+    const float slope = a.slope ? -1.44269504088896341f * a.slope[h] : 0.0f;
+    const bool plain = a.cap == 0.0f && !a.slope;
+
+    v4f o[E];
     #pragma unroll
-    for (int u = 0; u < D / 64; u++) so[wave][64 * u + lane] = o[u];
-    __syncthreads();
-    if (tid >= D) return;
-    float top = sm[0];
-    for (int w = 1; w < 4; w++) top = fmaxf(top, sm[w]);
-    const float tu = top == -INFINITY ? 0.0f : top;
-    float os = 0.0f, ls = 0.0f;
-    for (int w = 0; w < 4; w++) {
-        const float f = expf(sm[w] - tu);
-        os += f * so[w][tid];
-        ls += f * sl[w];
+    for (int u = 0; u < E; u++) o[u] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+    float base = -INFINITY, l = 0.0f;
+
+    // the next block at or after t with a page, and its pages by 16 positions
+    int page[4];
+    auto seek = [&](int t) {
+        for (; t < t_end; t += RW_BLOCK) {
+            int any = -1;
+            #pragma unroll
+            for (int e = 0; e < 4; e++) {
+                int x = t + 16 * e < t_hi ? tab[(t + 16 * e) >> sh] : -1;
+                x = x >= 0 && x < a.pg.n_pages ? x : -1;
+                page[e] = x;
+                any = max(any, x);
+            }
+            if (any >= 0) break;
+        }
+        return t;
+    };
+    // a lane of a copy: its row and its word there; word w of row x lies at w ^ swz(x)
+    const int crow = lane / (RB / 16), cword = (lane % (RB / 16)) ^ (D == 128 ? 2 * ((RC * wave + crow) & 7) : ((RC * wave + crow) >> 1) & 7);
+    static_assert(RC * W % 16 == 0, "a wave's copies have one swizzle");
+    auto fetch = [&](int buf, int t) {
+        uint8_t * const st = lds + buf * STAGE;
+        #pragma unroll
+        for (int e = 0; e < NC; e++) {
+            const int row0 = RC * (W * e + wave), at = t + row0 + crow;
+            const int pg = row0 < 32 ? (row0 < 16 ? page[0] : page[1]) : (row0 < 48 ? page[2] : page[3]);
+            const size_t off = (size_t) max(pg, 0) * a.pg.page_stride + (size_t) (at & pmask) * kvd + (size_t) kh * D + 8 * cword;
+            const bool in = pg >= 0 && at >= t_lo && at < t_hi;
+            copy_lds16(in ? (const void *) (a.pg.k + off) : (const void *) rw_zeros, st + row0 * RB);
+            copy_lds16(in ? (const void *) (a.pg.v + off) : (const void *) rw_zeros, st + POOL + row0 * RB);
+        }
+        if (a.slope && a.pos && t + RW_BLOCK > past && wave == 0)
+            kpos[buf * RW_BLOCK + lane] = a.pos[sq.s0 + min(max(t + lane - past, 0), max(sq.m - 1, 0))];
+    };
+    const int krow = c * RB, kx = D == 128 ? 2 * (c & 7) : (c >> 1) & 7;
+    const int vrow = 4 * g + (c >> 2), vx = D == 128 ? vrow & 7 : (vrow >> 2) & 3;    // the V row this lane reads for its 16
+    const int vat = POOL + vrow * RB + (D == 128 ? 8 * (c & 3) : 16 * (((c >> 1) & 1) ^ ((vrow >> 1) & 1)) + 8 * (c & 1));
+
+    auto compute = [&](int buf, int t, const int (&pg)[4]) {
+        const uint8_t * st = lds + buf * STAGE;
+        v4f s[4];
+        #pragma unroll
+        for (int j = 0; j < 4; j++) {
+            s[j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+            #pragma unroll
+            for (int e = 0; e < NJ; e++) {
+                const v8 ka = *(const v8 *) (st + 16 * j * RB + krow + 16 * ((4 * e + g) ^ kx));
+                #pragma unroll
+                for (int k = 0; k < NP; k++) s[j] = M::mul(ka, q[e][k], s[j]);
+            }
+        }
+        float f = back;                               // log2 weights are f times the scores
+        if (!plain) {
+            f = 1.0f;
+            if (a.cap > 0.0f) {
+                float top = 0.0f;
+                #pragma unroll
+                for (int j = 0; j < 4; j++)
+                    #pragma unroll
+                    for (int e = 0; e < 4; e++) { s[j][e] *= back; top = fmaxf(top, fabsf(s[j][e])); }
+                if (__any(!(top <= 0.625f))) {
+                    #pragma unroll
+                    for (int j = 0; j < 4; j++)
+                        #pragma unroll
+                        for (int e = 0; e < 4; e++) s[j][e] = a.cap * tanh_any(s[j][e]);
+                } else {
+                    #pragma unroll
+                    for (int j = 0; j < 4; j++)
+                        #pragma unroll
+                        for (int e = 0; e < 4; e++) s[j][e] = a.cap * tanh_small(s[j][e]);
+                }
+            } else {
+                #pragma unroll
+                for (int j = 0; j < 4; j++)
+                    #pragma unroll
+                    for (int e = 0; e < 4; e++) s[j][e] *= back;
+            }
+            if (a.slope) {
+                const bool given = a.pos && t + RW_BLOCK > past;
+                const float d0 = (float) (t + 4 * g - qpos);
+                #pragma unroll
+                for (int j = 0; j < 4; j++)
+                    #pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        float d = d0 + (float) (16 * j + e);
+                        const int x = 16 * j + 4 * g + e;
+                        if (given && t + x >= past) d = (float) (kpos[buf * RW_BLOCK + x] - qpos);
+                        s[j][e] = __builtin_fmaf(slope, fabsf(d), s[j][e]);
+                    }
+            }
+        }
+        const bool all = pg[0] >= 0 && pg[1] >= 0 && pg[2] >= 0 && pg[3] >= 0;
+        const bool whole = all && t >= f_lo && t + RW_BLOCK <= f_hi;
+        uint64_t vm = ~0ull;
+        if (!whole) {
+            vm = bits_range(lo - t, hi - t);
+            const int j0 = t - past;
+            if (nbit && j0 + RW_BLOCK > 0 && j0 < nbit) {
+                const int w0 = j0 >> 5;               // bits 32 w0.. of the row, 96 of them
+                uint32_t x[3];
+                #pragma unroll
+                for (int e = 0; e < 3; e++) x[e] = w0 + e >= 0 && w0 + e < a.words ? bits[w0 + e] : 0u;
+                const int s5 = j0 & 31;
+                uint64_t tr = ((uint64_t) x[1] << 32 | x[0]) >> s5;
+                if (s5) tr |= (uint64_t) x[2] << (64 - s5);
+                vm |= tr & bits_range(-j0, min(nbit, sq.m) - j0);
+            }
+            vm &= bits_range(0, sq.n - t);
+            #pragma unroll
+            for (int e = 0; e < 4; e++)
+                if (pg[e] < 0) vm &= ~(0xFFFFull << (16 * e));
+            if (!some) vm = 0;
+            vm >>= 4 * g;
+            #pragma unroll
+            for (int j = 0; j < 4; j++)
+                #pragma unroll
+                for (int e = 0; e < 4; e++) s[j][e] = (vm >> (16 * j + e)) & 1 ? s[j][e] : -INFINITY;
+        }
+        float mx = -INFINITY;
+        #pragma unroll
+        for (int j = 0; j < 4; j++)
+            #pragma unroll
+            for (int e = 0; e < 4; e++) mx = fmaxf(mx, s[j][e]);
+        mx *= f;
+        if (__any(mx > base + M::room)) {
+            mx = fmaxf(mx, __shfl_xor(mx, 16));
+            mx = fmaxf(mx, __shfl_xor(mx, 32));
+            const float to = mx > base + M::room ? mx + M::lift : base;
+            const float al = __builtin_amdgcn_exp2f(base - (to == -INFINITY ? 0.0f : to));
+            l *= al;
+            #pragma unroll
+            for (int u = 0; u < E; u++)
+                #pragma unroll
+                for (int e = 0; e < 4; e++) o[u][e] *= al;
+            base = to;
+        }
+        const float bu = base == -INFINITY ? 0.0f : base;
+        v8 w[2][NP];
+        #pragma unroll
+        for (int j = 0; j < 4; j++)
+            #pragma unroll
+            for (int e = 0; e < 4; e += 2) {
+                const float w0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j][e], f, -bu)), w1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j][e + 1], f, -bu));
+                l += w0;
+                l += w1;
+                s[j][e] = w0;
+                s[j][e + 1] = w1;
+                parts_of<BF>(w0, w1, w[j >> 1], 4 * (j & 1) + e);
+            }
+        if (t < t_flo || t + RW_BLOCK > t_fhi) {
+            // columns differ here: values that are not finite are added one by one
+            int bad = 0;
+            #pragma unroll
+            for (int x = 0; x < W; x++) bad |= found[buf * W + x];
+            if (bad) {
+                #pragma unroll
+                for (int j = 0; j < 4; j++)
+                    #pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const int see = whole || ((vm >> (16 * j + e)) & 1);
+                        for (int y = 0; y < 4; y++) {
+                            const float pw = __shfl(s[j][e], c + 16 * y);
+                            if (!__shfl(see, c + 16 * y)) continue;
+                            const int row = 16 * j + 4 * y + e, x = D == 128 ? 2 * (row & 7) : (row >> 1) & 7;
+                            #pragma unroll
+                            for (int u = 0; u < E; u++) {
+                                const int word = 2 * u + (g >> 1);
+                                const uint16_t * v = (const uint16_t *) (st + POOL + row * RB + 16 * (word ^ x) + 8 * (g & 1));
+                                #pragma unroll
+                                for (int z = 0; z < 4; z++) o[u][z] = __builtin_fmaf(pw, of16<BF>(v[z]), o[u][z]);
+                            }
+                        }
+                    }
+                return;
+            }
+        }
+        #pragma unroll
+        for (int u = 0; u < E; u++) {
+            const uint8_t * vr = st + vat + ((u ^ vx) << 5);
+            #pragma unroll
+            for (int k = 0; k < 2; k++) {
+                typedef __attribute__((address_space(3))) v4s lv4s;
+                const v4s x0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lv4s *) (vr + 32 * k * RB));
+                const v4s x1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lv4s *) (vr + (32 * k + 16) * RB));
+                const v8 vv = __builtin_bit_cast(v8, __builtin_shufflevector(x0, x1, 0, 1, 2, 3, 4, 5, 6, 7));
+                #pragma unroll
+                for (int y = 0; y < NP; y++) o[u] = M::mul(vv, w[k][y], o[u]);
+            }
+        }
+    };
+
+    int t = seek(t_at), buf = 0;
+    if (t < t_end) fetch(0, t);
+    while (t < t_end) {
+        const int pg[4] = { page[0], page[1], page[2], page[3] };
+        const int tn = seek(t + RW_BLOCK);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");     // this wave's rows of the block are in LDS
+        if (t < t_flo || t + RW_BLOCK > t_fhi) {
+            unsigned bad = 0;
+            #pragma unroll
+            for (int e = 0; e < NC; e++) {
+                const v4u x = *(const v4u *) (lds + buf * STAGE + POOL + RC * (W * e + wave) * RB + 16 * lane);
+                #pragma unroll
+                for (int k = 0; k < 4; k++)                   // an exponent of all ones carries into the top bit
+                    bad |= BF ? (((x[k] & 0x7F807F80u) + 0x00800080u) & 0x80008000u) : (((x[k] & 0x7C007C00u) + 0x04000400u) & 0x80008000u);
+            }
+            const int any = __any(bad != 0);
+            if (!lane) found[buf * W + wave] = any;
+        }
+        __syncthreads();
+        if (tn < t_end) fetch(buf ^ 1, tn);                   // past the barrier: nobody reads the last block
+        if (t < w_hi && t + RW_BLOCK > w_lo) compute(buf, t, pg);
+        t = tn;
+        buf ^= 1;
     }
-    a.out[((size_t) r * a.n_head + h) * D + tid] = ls == 0.0f ? 0.0f : os / ls;
+
+    l += __shfl_xor(l, 16);
+    l += __shfl_xor(l, 32);
+    if (!mine) return;
+    if (p.count == 1) {
+        float * const to = a.out + ((size_t) r * a.n_head + h) * D + 4 * g;
+        #pragma unroll
+        for (int u = 0; u < E; u++) {
+            v4f x;
+            #pragma unroll
+            for (int e = 0; e < 4; e++) x[e] = some && l != 0.0f ? o[u][e] / l : 0.0f;
+            *(v4fu *) (to + 16 * u) = x;
+        }
+    } else {
+        const int pc = wave * 16 + c;
+        if (!g) part_ml(a, kh, p.item + p.split, D)[pc] = some ? make_float2(base, l) : make_float2(-INFINITY, 0.0f);
+        float * const to = part_o(a, kh, p.item + p.split, D) + (size_t) pc * D + 4 * g;
+        #pragma unroll
+        for (int u = 0; u < E; u++) *(v4f *) (to + 16 * u) = o[u];
+    }
 }
-#define ROWS(D, BF, name) \
-    extern "C" __global__ __launch_bounds__(256) void name(const sml_krows a) { rows_body<D, BF>(a); }
-ROWS(128, 0, sml_rw_rows)
-ROWS(128, 1, sml_rw_rows_bf)
-ROWS(64, 0, sml_rw_rows_d64)
-ROWS(64, 1, sml_rw_rows_d64_bf)
+#define ROWS(D, BF, W, EU, name) \
+    extern "C" __global__ __launch_bounds__(64 * W, EU) void name(const sml_krows a) { rows_body<D, BF, W>(a); }
+ROWS(128, 0, 4, 2, sml_rw_rows4)
+ROWS(128, 1, 4, 2, sml_rw_rows4_bf)
+ROWS(64, 0, 4, 4, sml_rw_rows4_d64)
+ROWS(64, 1, 4, 4, sml_rw_rows4_d64_bf)
+ROWS(128, 0, 8, 4, sml_rw_rows8)
+ROWS(128, 1, 8, 2, sml_rw_rows8_bf)
+ROWS(64, 0, 8, 4, sml_rw_rows8_d64)
+ROWS(64, 1, 8, 4, sml_rw_rows8_d64_bf)
+
+// The splits of a tile joined, 16 columns a workgroup, 16 lanes a column: the
+// bases of its splits shared out over the lanes, then each lane's dims of every
+// split in turn.
+template <int D>
+__device__ __forceinline__ void rows_merge_body(const sml_krows & a) {
+    __shared__ float f[16][RW_SPLITS + 1];
+    const int kh = blockIdx.x, tid = threadIdx.x, c = tid >> 4, l = tid & 15;
+    const int groups = (a.cols + 15) / 16, unit = rows_item();
+    rows_at p;
+    if (!rows_place<true>(a, unit / groups, tid & 63, p) || p.count == 1) return;
+    const rows_of sq = rows_seq(a, p.b);
+    const int rep = a.n_head / a.pg.n_kv, pc = 16 * (unit % groups) + c, col = p.tile * a.cols + pc;
+    if (16 * (unit % groups) + p.tile * a.cols >= sq.m * rep || p.item + p.count > a.items || p.count > RW_SPLITS) return;
+    const bool mine = col < sq.m * rep;
+    const float2 * ml = part_ml(a, kh, p.item, D) + (mine ? pc : 0);
+    const float * po = part_o(a, kh, p.item, D) + (size_t) (mine ? pc : 0) * D + 4 * l;
+    const size_t step = (size_t) a.part_cols;
+    float m = -INFINITY;
+    for (int s = l; s < p.count; s += 16) m = fmaxf(m, ml[s * step].x);
+    m = max16(m);
+    const float mu = m == -INFINITY ? 0.0f : m;
+    float sum = 0.0f;
+    for (int s = l; s < p.count; s += 16) {
+        const float2 x = ml[s * step];
+        const float e = __builtin_amdgcn_exp2f(x.x - mu);
+        f[c][s] = x.x == -INFINITY ? -1.0f : e;       // no sums: what lies there counts for nothing
+        if (x.x != -INFINITY) sum += e * x.y;
+    }
+    sum = sum16(sum);
+    wave_lds();
+    if (!mine) return;
+    v4f o[D / 64];
+    #pragma unroll
+    for (int u = 0; u < D / 64; u++) o[u] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+    #pragma unroll 4
+    for (int s = 0; s < p.count; s++) {
+        const float e = f[c][s];
+        #pragma unroll
+        for (int u = 0; u < D / 64; u++) {
+            const v4f x = *(const v4f *) (po + s * step * D + 64 * u);
+            #pragma unroll
+            for (int k = 0; k < 4; k++) o[u][k] = e >= 0.0f || e != e ? __builtin_fmaf(e, x[k], o[u][k]) : o[u][k];
+        }
+    }
+    const int i = col / rep;
+    float * const to = a.out + ((size_t) (sq.s0 + i) * a.n_head + kh * rep + (col - i * rep)) * D + 4 * l;
+    #pragma unroll
+    for (int u = 0; u < D / 64; u++) {
+        v4f x;
+        #pragma unroll
+        for (int k = 0; k < 4; k++) x[k] = sum == 0.0f ? 0.0f : o[u][k] / sum;
+        *(v4fu *) (to + 64 * u) = x;
+    }
+}
+extern "C" __global__ __launch_bounds__(256) void sml_rw_merge(const sml_krows a) { rows_merge_body<128>(a); }
+extern "C" __global__ __launch_bounds__(256) void sml_rw_merge_d64(const sml_krows a) { rows_merge_body<64>(a); }
 
 // ---------------------------------------------------------------- layers of a cache
 
