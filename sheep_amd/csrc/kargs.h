@@ -568,7 +568,7 @@ typedef struct {
 } sml_krows;
 #define RW_BLOCK 64               // positions of a block
 #define RW_STAGE(d) (2 * RW_BLOCK * 2 * (d))   // LDS of a block: its K rows, then its V rows
-#define RW_EXTRA (2 * RW_BLOCK * 4 + 64 * 4)   // and beside two of them
+#define RW_EXTRA (2 * RW_BLOCK * 4 + 2 * 8 * 8)  // and beside two of them
 #define RW_SPLITS 512             // the most splits of a tile
 
 // Layers of a cache: layer l's pools lie l * layer_stride values behind pg's.

@@ -5,6 +5,7 @@
 
 #include <math.h>
 #include <stdio.h>
+#include <stdlib.h>
 #include <string.h>
 
 int sml_hip_paged_append_axes(const sml_hip_pages * pg, float * qkv, size_t qkv_stride, int n_rows, const int32_t * seq,
@@ -54,8 +55,8 @@ static void items_launch(const char * name, int n_kv, long items, unsigned threa
 static void rows_launch(sml_krows * a, int hd, int type, hipStream_t st) {
     const int n_kv = a->pg.n_kv, rep = a->n_head / n_kv, n_seq = a->pg.n_seq;
     const int ncol = a->n_row * rep, some = n_seq < a->n_row ? n_seq : a->n_row;
-    const int waves = ncol > 64L * some ? 8 : 4;
-    a->cols = 16 * waves;
+    const int form = ncol <= 64L * some ? 41 : getenv("RW81") ? 81 : 42, waves = form / 10;
+    a->cols = 16 * waves * (form % 10);
     // two workgroups a CU; not split where the tiles are as many
     const int want = ceil_div(2 * hx.ncu < 512 ? 2 * hx.ncu : 512, n_kv);
     a->least = 2;
@@ -66,7 +67,7 @@ static void rows_launch(sml_krows * a, int hd, int type, hipStream_t st) {
     a->items = (int) items;
     a->part_cols = ncol < a->cols ? ncol : a->cols;
     char base[24], name[40];
-    snprintf(base, sizeof base, "sml_rw_rows%d", waves);
+    snprintf(base, sizeof base, "sml_rw_rows%d%s", form, a->cap > 0.0f || a->slope ? "r" : "");
     sv_name(name, sizeof name, base, hd, type);
     items_launch(name, n_kv, items, 64 * (unsigned) waves, (size_t) 2 * RW_STAGE(hd) + RW_EXTRA, st, a);
     if (split) items_launch(hd == 64 ? "sml_rw_merge_d64" : "sml_rw_merge", n_kv, tiles * (a->cols / 16), 256, 0, st, a);

@@ -99,9 +99,9 @@ AXES(64, 1, sml_rw_append_d64_bf)
 // lane then makes its column's 64 bits of the block, of the range, the tree and
 // the pages that are there. What a column does not attend to has no weight, but
 // 0 times a NaN or an infinity is none either: rows that no column of the tile
-// may see are loaded as zeros, and where columns differ, waves look their share of
-// the values through on its arrival and take a block with any that is not finite
-// value by value.
+// may see are loaded as zeros, and where columns differ, each wave looks its share
+// of the values through on its arrival, puts zeros for those that are not finite
+// and notes their positions: a column that attends to one gets NaN.
 //
 // Lengths and counts are ragged and on the device: every wave sums them up and
 // finds its workgroup's tile and split (rows_place), splits of one size for all
@@ -219,24 +219,23 @@ __device__ __forceinline__ float tanh_any(float y) {
     return fabsf(y) > 0.625f ? t : tanh_small(y);
 }
 
-// Bits lo..hi-1 of 64.
-__device__ __forceinline__ uint64_t bits_range(int lo, int hi) {
-    lo = min(max(lo, 0), 64);
-    hi = min(max(hi, 0), 64);
-    if (lo >= hi) return 0;
-    return (~0ull >> (64 - (hi - lo))) << lo;
+// Bits lo..hi-1 of 32.
+__device__ __forceinline__ uint32_t bits_range(int lo, int hi) {
+    lo = min(max(lo, 0), 32);
+    hi = min(max(hi, 0), 32);
+    return lo < hi ? (~0u >> (32 - (hi - lo))) << lo : 0;
 }
 
-template <int D, int BF, int W>
+template <int D, int BF, int W, int CB, bool RULES>
 __device__ __forceinline__ void rows_body(const sml_krows & a) {
     using M = Mx<BF>;
     typedef typename M::v8 v8;
     constexpr int NJ = D / 32, E = D / 16, NP = M::parts, RB = 2 * D, POOL = RW_BLOCK * RB, STAGE = 2 * POOL;
     constexpr int RC = 1024 / RB, NC = RW_BLOCK / RC / W;   // rows of a copy, a wave's copies of a block
     static_assert(NC >= 1, "");
-    extern __shared__ __align__(16) uint8_t lds[];    // two stages, their new rows' positions, what waves found in V
+    extern __shared__ __align__(16) uint8_t lds[];    // two stages, their new rows' positions, positions whose V is not finite
     int * const kpos = (int *) (lds + 2 * STAGE);
-    int * const found = kpos + 2 * RW_BLOCK;
+    uint64_t * const found = (uint64_t *) (kpos + 2 * RW_BLOCK);
     const int kh = blockIdx.x, tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     rows_at p;
@@ -246,41 +245,46 @@ __device__ __forceinline__ void rows_body(const sml_krows & a) {
     const int sh = a.pg.page_shift, pmask = (1 << sh) - 1;
     const int32_t * const tab = a.pg.table + (size_t) p.b * a.pg.seq_pages;
 
-    // the lane's column: its row's range, its tree's bits and its position
-    const int col = p.tile * a.cols + wave * 16 + c;
-    const bool mine = col < ncol;
-    const int i = min(col, ncol - 1) / rep, r = sq.s0 + i, h = kh * rep + (min(col, ncol - 1) - i * rep);
-    const int lo = a.first ? max(a.first[r], 0) : 0;
-    const int hi = min(a.last ? a.last[r] : a.tree ? past : past + i + 1, sq.n);
+    // the lane's columns: their rows' ranges, trees' bits and positions
+    int r[CB], h[CB], lo[CB], hi[CB], qpos[CB];
+    bool mine[CB], some[CB];                          // is there one, does it attend to anything
     const int nbit = a.tree ? min(sq.m, 32 * a.words) : 0;
-    const uint32_t * const bits = a.tree + (size_t) r * a.words;
-    const int qpos = a.pos ? a.pos[r] : past + i;
-    bool some = lo < hi;                              // does it attend to anything
-    if (nbit) {
-        if (a.words > 8) some = true;
-        else
-            for (int w = 0; w < a.words; w++) some |= bits[w] != 0;
-    }
-    some &= mine;
     // what any column of the wave, of the tile attends to lies in w_lo..w_hi, t_lo..t_hi;
-    // every one that attends to anything has all of f_lo..f_hi (f4_: of the tile)
-    int w_lo, w_hi, f_lo, f_hi, t_lo, t_hi, t_flo, t_fhi;
+    // every one that attends to anything has all of f_lo..f_hi (t_flo.. of the tile)
+    int w_lo = 0x7fffffff, w_hi = 0, f_lo = 0, f_hi = 0x7fffffff, t_lo, t_hi, t_flo, t_fhi;
     {
-        const bool range = some && lo < hi, tree = some && nbit > 0 && past + nbit > 0;
-        int x0 = range ? lo : 0x7fffffff, x1 = range ? hi : 0;
-        if (tree) { x0 = min(x0, max(past, 0)); x1 = max(x1, min(past + nbit, sq.n)); }
-        int x2 = some ? (lo < hi ? lo : 0x7fffffff) : 0, x3 = some ? (lo < hi ? hi : 0) : 0x7fffffff;
         #pragma unroll
-        for (int o = 1; o < 16; o <<= 1) {
-            x0 = min(x0, __shfl_xor(x0, o));
-            x1 = max(x1, __shfl_xor(x1, o));
-            x2 = max(x2, __shfl_xor(x2, o));
-            x3 = min(x3, __shfl_xor(x3, o));
+        for (int x = 0; x < CB; x++) {
+            const int col = p.tile * a.cols + 16 * (CB * wave + x) + c, i = min(col, ncol - 1) / rep;
+            mine[x] = col < ncol;
+            r[x] = sq.s0 + i;
+            h[x] = kh * rep + (min(col, ncol - 1) - i * rep);
+            lo[x] = a.first ? max(a.first[r[x]], 0) : 0;
+            hi[x] = min(a.last ? a.last[r[x]] : a.tree ? past : past + i + 1, sq.n);
+            qpos[x] = a.pos ? a.pos[r[x]] : past + i;
+            const bool range = lo[x] < hi[x];
+            bool tree = false;
+            if (nbit) {
+                if (a.words > 8) tree = true;
+                else
+                    for (int w = 0; w < a.words; w++) tree |= a.tree[(size_t) r[x] * a.words + w] != 0;
+            }
+            some[x] = mine[x] && (range || tree);
+            if (mine[x] && range) { w_lo = min(w_lo, lo[x]); w_hi = max(w_hi, hi[x]); }
+            if (mine[x] && tree && past + nbit > 0) { w_lo = min(w_lo, max(past, 0)); w_hi = max(w_hi, min(past + nbit, sq.n)); }
+            if (some[x]) { f_lo = max(f_lo, range ? lo[x] : 0x7fffffff); f_hi = min(f_hi, range ? hi[x] : 0); }
         }
-        w_lo = __builtin_amdgcn_readfirstlane(x0);
-        w_hi = __builtin_amdgcn_readfirstlane(x1);
-        f_lo = __builtin_amdgcn_readfirstlane(x2);
-        f_hi = __builtin_amdgcn_readfirstlane(x3);
+        #pragma unroll
+        for (int e = 1; e < 16; e <<= 1) {
+            w_lo = min(w_lo, __shfl_xor(w_lo, e));
+            w_hi = max(w_hi, __shfl_xor(w_hi, e));
+            f_lo = max(f_lo, __shfl_xor(f_lo, e));
+            f_hi = min(f_hi, __shfl_xor(f_hi, e));
+        }
+        w_lo = __builtin_amdgcn_readfirstlane(w_lo);
+        w_hi = __builtin_amdgcn_readfirstlane(w_hi);
+        f_lo = __builtin_amdgcn_readfirstlane(f_lo);
+        f_hi = __builtin_amdgcn_readfirstlane(f_hi);
         int * const red = kpos;
         if (!lane) { red[4 * wave] = w_lo; red[4 * wave + 1] = w_hi; red[4 * wave + 2] = f_lo; red[4 * wave + 3] = f_hi; }
         __syncthreads();
@@ -306,19 +310,20 @@ __device__ __forceinline__ void rows_body(const sml_krows & a) {
         t_end = min((b0 + min(nb, (p.split + 1) * per)) * RW_BLOCK, t_hi);
     }
 
-    // the query: lane (c, g) holds dims 32j + 8g.. of column c, in parts
-    v8 q[NJ][NP];
-    float back;                                       // what a product of the scaled q is multiplied by
-    {
+    // the queries: lane (c, g) holds dims 32j + 8g.. of its columns, in parts
+    v8 q[CB][NJ][NP];
+    float back[CB], slope[CB];                        // what a product of the scaled q is multiplied by
+    #pragma unroll
+    for (int y = 0; y < CB; y++) {
         float x[NJ][8], mx = 0.0f;
-        const float * qp = a.q + (size_t) r * a.q_stride + (size_t) h * D + 8 * g;
+        const float * qp = a.q + (size_t) r[y] * a.q_stride + (size_t) h[y] * D + 8 * g;
         #pragma unroll
         for (int j = 0; j < NJ; j++)
             #pragma unroll
             for (int e = 0; e < 8; e += 4) {
                 const v4f v = *(const v4fu *) (qp + 32 * j + e);
                 #pragma unroll
-                for (int k = 0; k < 4; k++) { x[j][e + k] = mine ? v[k] * a.sign : 0.0f; mx = fmaxf(mx, fabsf(x[j][e + k])); }
+                for (int k = 0; k < 4; k++) { x[j][e + k] = mine[y] ? v[k] * a.sign : 0.0f; mx = fmaxf(mx, fabsf(x[j][e + k])); }
             }
         mx = fmaxf(mx, __shfl_xor(mx, 16));
         mx = fmaxf(mx, __shfl_xor(mx, 32));
@@ -327,16 +332,20 @@ __device__ __forceinline__ void rows_body(const sml_krows & a) {
         for (int j = 0; j < NJ; j++)
             #pragma unroll
             for (int e = 0; e < 8; e += 2)
-                parts_of<BF>(__builtin_amdgcn_ldexpf(x[j][e], -ex), __builtin_amdgcn_ldexpf(x[j][e + 1], -ex), q[j], e);
-        back = __builtin_amdgcn_ldexpf(a.scale, ex);
+                parts_of<BF>(__builtin_amdgcn_ldexpf(x[j][e], -ex), __builtin_amdgcn_ldexpf(x[j][e + 1], -ex), q[y][j], e);
+        back[y] = __builtin_amdgcn_ldexpf(a.scale, ex);
+        slope[y] = RULES && a.slope ? -1.44269504088896341f * a.slope[h[y]] : 0.0f;
     }
-    const float slope = a.slope ? -1.44269504088896341f * a.slope[h] : 0.0f;
-    const bool plain = a.cap == 0.0f && !a.slope;
 
-    v4f o[E];
+    v4f o[CB][E];
+    float base[CB], l[CB];
     #pragma unroll
-    for (int u = 0; u < E; u++) o[u] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-    float base = -INFINITY, l = 0.0f;
+    for (int y = 0; y < CB; y++) {
+        base[y] = -INFINITY;
+        l[y] = 0.0f;
+        #pragma unroll
+        for (int u = 0; u < E; u++) o[y][u] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+    }
 
     // the next block at or after t with a page, and its pages by 16 positions
     int page[4];
@@ -368,163 +377,134 @@ __device__ __forceinline__ void rows_body(const sml_krows & a) {
             copy_lds16(in ? (const void *) (a.pg.k + off) : (const void *) rw_zeros, st + row0 * RB);
             copy_lds16(in ? (const void *) (a.pg.v + off) : (const void *) rw_zeros, st + POOL + row0 * RB);
         }
-        if (a.slope && a.pos && t + RW_BLOCK > past && wave == 0)
+        if (RULES && a.slope && a.pos && t + RW_BLOCK > past && wave == 0)
             kpos[buf * RW_BLOCK + lane] = a.pos[sq.s0 + min(max(t + lane - past, 0), max(sq.m - 1, 0))];
     };
     const int krow = c * RB, kx = D == 128 ? 2 * (c & 7) : (c >> 1) & 7;
     const int vrow = 4 * g + (c >> 2), vx = D == 128 ? vrow & 7 : (vrow >> 2) & 3;    // the V row this lane reads for its 16
     const int vat = POOL + vrow * RB + (D == 128 ? 8 * (c & 3) : 16 * (((c >> 1) & 1) ^ ((vrow >> 1) & 1)) + 8 * (c & 1));
 
-    auto compute = [&](int buf, int t, const int (&pg)[4]) {
-        const uint8_t * st = lds + buf * STAGE;
-        v4f s[4];
+    // positions t.. of a stage's 32 rows from row0, with their pages pa and pb
+    auto compute = [&](const uint8_t * st, int buf, int row0, int t, int pa, int pb) {
+        v4f s[CB][2];
         #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            s[j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int j = 0; j < 2; j++) {
+            #pragma unroll
+            for (int y = 0; y < CB; y++) s[y][j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
             #pragma unroll
             for (int e = 0; e < NJ; e++) {
-                const v8 ka = *(const v8 *) (st + 16 * j * RB + krow + 16 * ((4 * e + g) ^ kx));
+                const v8 ka = *(const v8 *) (st + (row0 + 16 * j) * RB + krow + 16 * ((4 * e + g) ^ kx));
                 #pragma unroll
-                for (int k = 0; k < NP; k++) s[j] = M::mul(ka, q[e][k], s[j]);
+                for (int k = 0; k < NP; k++)
+                    #pragma unroll
+                    for (int y = 0; y < CB; y++) s[y][j] = M::mul(ka, q[y][e][k], s[y][j]);
             }
         }
-        float f = back;                               // log2 weights are f times the scores
-        if (!plain) {
-            f = 1.0f;
-            if (a.cap > 0.0f) {
+        const bool whole = pa >= 0 && pb >= 0 && t >= f_lo && t + 32 <= f_hi;
+        v8 w[CB][NP];
+        #pragma unroll
+        for (int y = 0; y < CB; y++) {
+            float f = back[y];                        // log2 weights are f times the scores
+            if constexpr (RULES) {
+                f = 1.0f;
                 float top = 0.0f;
                 #pragma unroll
-                for (int j = 0; j < 4; j++)
+                for (int j = 0; j < 2; j++)
                     #pragma unroll
-                    for (int e = 0; e < 4; e++) { s[j][e] *= back; top = fmaxf(top, fabsf(s[j][e])); }
-                if (__any(!(top <= 0.625f))) {
-                    #pragma unroll
-                    for (int j = 0; j < 4; j++)
+                    for (int e = 0; e < 4; e++) { s[y][j][e] *= back[y]; top = fmaxf(top, fabsf(s[y][j][e])); }
+                if (a.cap > 0.0f) {
+                    if (__any(!(top <= 0.625f))) {
                         #pragma unroll
-                        for (int e = 0; e < 4; e++) s[j][e] = a.cap * tanh_any(s[j][e]);
-                } else {
-                    #pragma unroll
-                    for (int j = 0; j < 4; j++)
-                        #pragma unroll
-                        for (int e = 0; e < 4; e++) s[j][e] = a.cap * tanh_small(s[j][e]);
-                }
-            } else {
-                #pragma unroll
-                for (int j = 0; j < 4; j++)
-                    #pragma unroll
-                    for (int e = 0; e < 4; e++) s[j][e] *= back;
-            }
-            if (a.slope) {
-                const bool given = a.pos && t + RW_BLOCK > past;
-                const float d0 = (float) (t + 4 * g - qpos);
-                #pragma unroll
-                for (int j = 0; j < 4; j++)
-                    #pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        float d = d0 + (float) (16 * j + e);
-                        const int x = 16 * j + 4 * g + e;
-                        if (given && t + x >= past) d = (float) (kpos[buf * RW_BLOCK + x] - qpos);
-                        s[j][e] = __builtin_fmaf(slope, fabsf(d), s[j][e]);
-                    }
-            }
-        }
-        const bool all = pg[0] >= 0 && pg[1] >= 0 && pg[2] >= 0 && pg[3] >= 0;
-        const bool whole = all && t >= f_lo && t + RW_BLOCK <= f_hi;
-        uint64_t vm = ~0ull;
-        if (!whole) {
-            vm = bits_range(lo - t, hi - t);
-            const int j0 = t - past;
-            if (nbit && j0 + RW_BLOCK > 0 && j0 < nbit) {
-                const int w0 = j0 >> 5;               // bits 32 w0.. of the row, 96 of them
-                uint32_t x[3];
-                #pragma unroll
-                for (int e = 0; e < 3; e++) x[e] = w0 + e >= 0 && w0 + e < a.words ? bits[w0 + e] : 0u;
-                const int s5 = j0 & 31;
-                uint64_t tr = ((uint64_t) x[1] << 32 | x[0]) >> s5;
-                if (s5) tr |= (uint64_t) x[2] << (64 - s5);
-                vm |= tr & bits_range(-j0, min(nbit, sq.m) - j0);
-            }
-            vm &= bits_range(0, sq.n - t);
-            #pragma unroll
-            for (int e = 0; e < 4; e++)
-                if (pg[e] < 0) vm &= ~(0xFFFFull << (16 * e));
-            if (!some) vm = 0;
-            vm >>= 4 * g;
-            #pragma unroll
-            for (int j = 0; j < 4; j++)
-                #pragma unroll
-                for (int e = 0; e < 4; e++) s[j][e] = (vm >> (16 * j + e)) & 1 ? s[j][e] : -INFINITY;
-        }
-        float mx = -INFINITY;
-        #pragma unroll
-        for (int j = 0; j < 4; j++)
-            #pragma unroll
-            for (int e = 0; e < 4; e++) mx = fmaxf(mx, s[j][e]);
-        mx *= f;
-        if (__any(mx > base + M::room)) {
-            mx = fmaxf(mx, __shfl_xor(mx, 16));
-            mx = fmaxf(mx, __shfl_xor(mx, 32));
-            const float to = mx > base + M::room ? mx + M::lift : base;
-            const float al = __builtin_amdgcn_exp2f(base - (to == -INFINITY ? 0.0f : to));
-            l *= al;
-            #pragma unroll
-            for (int u = 0; u < E; u++)
-                #pragma unroll
-                for (int e = 0; e < 4; e++) o[u][e] *= al;
-            base = to;
-        }
-        const float bu = base == -INFINITY ? 0.0f : base;
-        v8 w[2][NP];
-        #pragma unroll
-        for (int j = 0; j < 4; j++)
-            #pragma unroll
-            for (int e = 0; e < 4; e += 2) {
-                const float w0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j][e], f, -bu)), w1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j][e + 1], f, -bu));
-                l += w0;
-                l += w1;
-                s[j][e] = w0;
-                s[j][e + 1] = w1;
-                parts_of<BF>(w0, w1, w[j >> 1], 4 * (j & 1) + e);
-            }
-        if (t < t_flo || t + RW_BLOCK > t_fhi) {
-            // columns differ here: values that are not finite are added one by one
-            int bad = 0;
-            #pragma unroll
-            for (int x = 0; x < W; x++) bad |= found[buf * W + x];
-            if (bad) {
-                #pragma unroll
-                for (int j = 0; j < 4; j++)
-                    #pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        const int see = whole || ((vm >> (16 * j + e)) & 1);
-                        for (int y = 0; y < 4; y++) {
-                            const float pw = __shfl(s[j][e], c + 16 * y);
-                            if (!__shfl(see, c + 16 * y)) continue;
-                            const int row = 16 * j + 4 * y + e, x = D == 128 ? 2 * (row & 7) : (row >> 1) & 7;
+                        for (int j = 0; j < 2; j++)
                             #pragma unroll
-                            for (int u = 0; u < E; u++) {
-                                const int word = 2 * u + (g >> 1);
-                                const uint16_t * v = (const uint16_t *) (st + POOL + row * RB + 16 * (word ^ x) + 8 * (g & 1));
-                                #pragma unroll
-                                for (int z = 0; z < 4; z++) o[u][z] = __builtin_fmaf(pw, of16<BF>(v[z]), o[u][z]);
-                            }
-                        }
+                            for (int e = 0; e < 4; e++) s[y][j][e] = a.cap * tanh_any(s[y][j][e]);
+                    } else {
+                        #pragma unroll
+                        for (int j = 0; j < 2; j++)
+                            #pragma unroll
+                            for (int e = 0; e < 4; e++) s[y][j][e] = a.cap * tanh_small(s[y][j][e]);
                     }
-                return;
+                }
+                if (a.slope) {
+                    const bool given = a.pos && t + 32 > past;
+                    const float d0 = (float) (t + 4 * g - qpos[y]);
+                    #pragma unroll
+                    for (int j = 0; j < 2; j++)
+                        #pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            float d = d0 + (float) (16 * j + e);
+                            const int x = 16 * j + 4 * g + e;
+                            if (given && t + x >= past) d = (float) (kpos[buf * RW_BLOCK + row0 + x] - qpos[y]);
+                            s[y][j][e] = __builtin_fmaf(slope[y], fabsf(d), s[y][j][e]);
+                        }
+                }
             }
+            if (!whole) {
+                uint32_t vm = bits_range(lo[y] - t, hi[y] - t);
+                const int j0 = t - past;
+                if (nbit && j0 + 32 > 0 && j0 < nbit) {
+                    const uint32_t * const bits = a.tree + (size_t) r[y] * a.words;
+                    const int w0 = j0 >> 5;           // bits 32 w0.. of the row, 64 of them
+                    const uint32_t x0 = w0 >= 0 && w0 < a.words ? bits[w0] : 0u, x1 = w0 + 1 >= 0 && w0 + 1 < a.words ? bits[w0 + 1] : 0u;
+                    vm |= (uint32_t) (((uint64_t) x1 << 32 | x0) >> (j0 & 31)) & bits_range(-j0, nbit - j0);
+                }
+                vm &= bits_range(0, sq.n - t);
+                if (pa < 0) vm &= 0xFFFF0000u;
+                if (pb < 0) vm &= 0x0000FFFFu;
+                if (!some[y]) vm = 0;
+                if (t < t_flo || t + 32 > t_fhi) {
+                    uint64_t bad = 0;
+                    #pragma unroll
+                    for (int x = 0; x < W; x++) bad |= found[buf * W + x];
+                    if (vm & (uint32_t) (bad >> row0)) l[y] = NAN;
+                }
+                vm >>= 4 * g;
+                #pragma unroll
+                for (int j = 0; j < 2; j++)
+                    #pragma unroll
+                    for (int e = 0; e < 4; e++) s[y][j][e] = (vm >> (16 * j + e)) & 1 ? s[y][j][e] : -INFINITY;
+            }
+            float mx = -INFINITY;
+            #pragma unroll
+            for (int j = 0; j < 2; j++)
+                #pragma unroll
+                for (int e = 0; e < 4; e++) mx = fmaxf(mx, s[y][j][e]);
+            mx *= f;
+            if (__any(mx > base[y] + M::room)) {
+                mx = fmaxf(mx, __shfl_xor(mx, 16));
+                mx = fmaxf(mx, __shfl_xor(mx, 32));
+                const float to = mx > base[y] + M::room ? mx + M::lift : base[y];
+                const float al = __builtin_amdgcn_exp2f(base[y] - (to == -INFINITY ? 0.0f : to));
+                l[y] *= al;
+                #pragma unroll
+                for (int u = 0; u < E; u++)
+                    #pragma unroll
+                    for (int e = 0; e < 4; e++) o[y][u][e] *= al;
+                base[y] = to;
+            }
+            const float bu = base[y] == -INFINITY ? 0.0f : base[y];
+            #pragma unroll
+            for (int j = 0; j < 2; j++)
+                #pragma unroll
+                for (int e = 0; e < 4; e += 2) {
+                    const float w0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[y][j][e], f, -bu));
+                    const float w1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[y][j][e + 1], f, -bu));
+                    l[y] += w0;
+                    l[y] += w1;
+                    parts_of<BF>(w0, w1, w[y], 4 * j + e);
+                }
         }
         #pragma unroll
         for (int u = 0; u < E; u++) {
-            const uint8_t * vr = st + vat + ((u ^ vx) << 5);
+            const uint8_t * vr = st + vat + row0 * RB + ((u ^ vx) << 5);
+            typedef __attribute__((address_space(3))) v4s lv4s;
+            const v4s x0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lv4s *) vr);
+            const v4s x1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lv4s *) (vr + 16 * RB));
+            const v8 vv = __builtin_bit_cast(v8, __builtin_shufflevector(x0, x1, 0, 1, 2, 3, 4, 5, 6, 7));
             #pragma unroll
-            for (int k = 0; k < 2; k++) {
-                typedef __attribute__((address_space(3))) v4s lv4s;
-                const v4s x0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lv4s *) (vr + 32 * k * RB));
-                const v4s x1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lv4s *) (vr + (32 * k + 16) * RB));
-                const v8 vv = __builtin_bit_cast(v8, __builtin_shufflevector(x0, x1, 0, 1, 2, 3, 4, 5, 6, 7));
+            for (int k = 0; k < NP; k++)
                 #pragma unroll
-                for (int y = 0; y < NP; y++) o[u] = M::mul(vv, w[k][y], o[u]);
-            }
+                for (int y = 0; y < CB; y++) o[y][u] = M::mul(vv, w[y][k], o[y][u]);
         }
     };
 
@@ -535,54 +515,74 @@ __device__ __forceinline__ void rows_body(const sml_krows & a) {
         const int tn = seek(t + RW_BLOCK);
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");     // this wave's rows of the block are in LDS
         if (t < t_flo || t + RW_BLOCK > t_fhi) {
-            unsigned bad = 0;
+            uint64_t bad = 0;
             #pragma unroll
             for (int e = 0; e < NC; e++) {
-                const v4u x = *(const v4u *) (lds + buf * STAGE + POOL + RC * (W * e + wave) * RB + 16 * lane);
+                const int row0 = RC * (W * e + wave);
+                v4u * const at = (v4u *) (lds + buf * STAGE + POOL + row0 * RB + 16 * lane);
+                v4u x = *at;
+                uint32_t any = 0;
                 #pragma unroll
-                for (int k = 0; k < 4; k++)                   // an exponent of all ones carries into the top bit
-                    bad |= BF ? (((x[k] & 0x7F807F80u) + 0x00800080u) & 0x80008000u) : (((x[k] & 0x7C007C00u) + 0x04000400u) & 0x80008000u);
+                for (int k = 0; k < 4; k++) {                 // an exponent of all ones carries into the top bit
+                    const uint32_t up = BF ? ((x[k] & 0x7F807F80u) + 0x00800080u) & 0x80008000u : ((x[k] & 0x7C007C00u) + 0x04000400u) & 0x80008000u;
+                    x[k] &= ~((up >> 15) * 0xFFFFu);
+                    any |= up;
+                }
+                const uint64_t hit = __ballot(any != 0);
+                if (hit) {
+                    *at = x;
+                    #pragma unroll
+                    for (int k = 0; k < RC; k++)
+                        if (hit >> (64 / RC * k) & ((1ull << (64 / RC)) - 1)) bad |= 1ull << (row0 + k);
+                }
             }
-            const int any = __any(bad != 0);
-            if (!lane) found[buf * W + wave] = any;
+            if (!lane) found[buf * W + wave] = bad;
         }
         __syncthreads();
         if (tn < t_end) fetch(buf ^ 1, tn);                   // past the barrier: nobody reads the last block
-        if (t < w_hi && t + RW_BLOCK > w_lo) compute(buf, t, pg);
+        #pragma unroll 1
+        for (int e = 0; e < 2; e++) {
+            const int te = t + 32 * e;
+            if (te < w_hi && te + 32 > w_lo) compute(lds + buf * STAGE, buf, 32 * e, te, e ? pg[2] : pg[0], e ? pg[3] : pg[1]);
+        }
         t = tn;
         buf ^= 1;
     }
 
-    l += __shfl_xor(l, 16);
-    l += __shfl_xor(l, 32);
-    if (!mine) return;
-    if (p.count == 1) {
-        float * const to = a.out + ((size_t) r * a.n_head + h) * D + 4 * g;
-        #pragma unroll
-        for (int u = 0; u < E; u++) {
-            v4f x;
+    #pragma unroll
+    for (int y = 0; y < CB; y++) {
+        l[y] += __shfl_xor(l[y], 16);
+        l[y] += __shfl_xor(l[y], 32);
+        if (!mine[y]) continue;
+        if (p.count == 1) {
+            float * const to = a.out + ((size_t) r[y] * a.n_head + h[y]) * D + 4 * g;
             #pragma unroll
-            for (int e = 0; e < 4; e++) x[e] = some && l != 0.0f ? o[u][e] / l : 0.0f;
-            *(v4fu *) (to + 16 * u) = x;
+            for (int u = 0; u < E; u++) {
+                v4f x;
+                #pragma unroll
+                for (int e = 0; e < 4; e++) x[e] = some[y] && l[y] != 0.0f ? o[y][u][e] / l[y] : 0.0f;
+                *(v4fu *) (to + 16 * u) = x;
+            }
+        } else {
+            const int pc = 16 * (CB * wave + y) + c;
+            if (!g) part_ml(a, kh, p.item + p.split, D)[pc] = some[y] ? make_float2(base[y], l[y]) : make_float2(-INFINITY, 0.0f);
+            float * const to = part_o(a, kh, p.item + p.split, D) + (size_t) pc * D + 4 * g;
+            #pragma unroll
+            for (int u = 0; u < E; u++) *(v4f *) (to + 16 * u) = o[y][u];
         }
-    } else {
-        const int pc = wave * 16 + c;
-        if (!g) part_ml(a, kh, p.item + p.split, D)[pc] = some ? make_float2(base, l) : make_float2(-INFINITY, 0.0f);
-        float * const to = part_o(a, kh, p.item + p.split, D) + (size_t) pc * D + 4 * g;
-        #pragma unroll
-        for (int u = 0; u < E; u++) *(v4f *) (to + 16 * u) = o[u];
     }
 }
-#define ROWS(D, BF, W, EU, name) \
-    extern "C" __global__ __launch_bounds__(64 * W, EU) void name(const sml_krows a) { rows_body<D, BF, W>(a); }
-ROWS(128, 0, 4, 2, sml_rw_rows4)
-ROWS(128, 1, 4, 2, sml_rw_rows4_bf)
-ROWS(64, 0, 4, 4, sml_rw_rows4_d64)
-ROWS(64, 1, 4, 4, sml_rw_rows4_d64_bf)
-ROWS(128, 0, 8, 4, sml_rw_rows8)
-ROWS(128, 1, 8, 2, sml_rw_rows8_bf)
-ROWS(64, 0, 8, 4, sml_rw_rows8_d64)
-ROWS(64, 1, 8, 4, sml_rw_rows8_d64_bf)
+#define ROWS(D, BF, W, CB, EU, name, sfx) \
+    extern "C" __global__ __launch_bounds__(64 * W, EU) void name##sfx(const sml_krows a) { rows_body<D, BF, W, CB, false>(a); } \
+    extern "C" __global__ __launch_bounds__(64 * W, EU) void name##r##sfx(const sml_krows a) { rows_body<D, BF, W, CB, true>(a); }
+#define ROWS4(W, CB, E1, E2, E3, E4, name) \
+    ROWS(128, 0, W, CB, E1, name, ) \
+    ROWS(128, 1, W, CB, E2, name, _bf) \
+    ROWS(64, 0, W, CB, E3, name, _d64) \
+    ROWS(64, 1, W, CB, E4, name, _d64_bf)
+ROWS4(4, 1, 2, 2, 4, 4, sml_rw_rows41)
+ROWS4(4, 2, 2, 2, 3, 3, sml_rw_rows42)
+ROWS4(8, 1, 4, 4, 4, 4, sml_rw_rows81)
 
 // The splits of a tile joined, 16 columns a workgroup, 16 lanes a column: the
 // bases of its splits shared out over the lanes, then each lane's dims of every
