@@ -566,9 +566,7 @@ typedef struct {
     int want, least;              // splits wanted in all (0: none), blocks of one at least
     int items, part_cols;         // the partials' items a KV head, and the columns of one
 } sml_krows;
-#define RW_BLOCK 64               // positions of a block
-#define RW_STAGE(d) (2 * RW_BLOCK * 2 * (d))   // LDS of a block: its K rows, then its V rows
-#define RW_EXTRA (2 * RW_BLOCK * 4 + 2 * 8 * 8)  // and beside two of them
+#define RW_BLOCK 64               // positions that splits are made of
 #define RW_SPLITS 512             // the most splits of a tile
 
 // Layers of a cache: layer l's pools lie l * layer_stride values behind pg's.

@@ -52,24 +52,34 @@ static void items_launch(const char * name, int n_kv, long items, unsigned threa
     hx_launch3(name, (unsigned) n_kv, (unsigned) y, (unsigned) ((items + y - 1) / y), threads, lds, st, a);
 }
 
+static const struct form { const char * name; int cols, cw, pg, per_cu; } forms[] = {
+    { "rows16", 16, 1, 8, 1 }, { "rows32", 32, 1, 8, 1 }, { "rows64", 64, 2, 4, 1 }, { "rows128", 128, 4, 2, 1 },
+    { "rows128l", 128, 4, 1, 2 },
+};
 static void rows_launch(sml_krows * a, int hd, int type, hipStream_t st) {
     const int n_kv = a->pg.n_kv, rep = a->n_head / n_kv, n_seq = a->pg.n_seq;
     const int ncol = a->n_row * rep, some = n_seq < a->n_row ? n_seq : a->n_row;
-    const int form = ncol <= 64L * some ? 41 : getenv("RW81") ? 81 : 42, waves = form / 10;
-    a->cols = 16 * waves * (form % 10);
-    // two workgroups a CU; not split where the tiles are as many
-    const int want = ceil_div(2 * hx.ncu < 512 ? 2 * hx.ncu : 512, n_kv);
-    a->least = 2;
-    const int split = n_seq <= AT_SHARED && ceil_div(ncol, a->cols) < want && a->max_len > RW_BLOCK * a->least;
+    int f = 0;
+    while (f < 3 && ncol > (long) forms[f].cols * some) f++;
+    if (getenv("RWF")) f = atoi(getenv("RWF"));
+    const struct form * const fm = forms + f;
+    a->cols = fm->cols;
+    // workgroups that run at once; not split where the tiles are as many
+    const int want = ceil_div((hx.ncu < 256 ? hx.ncu : 256) * fm->per_cu, n_kv);
+    a->least = getenv("RWL") ? atoi(getenv("RWL")) : 2;
+    const int split = n_seq <= AT_SHARED && 2 * ceil_div(ncol, a->cols) <= want && a->max_len > RW_BLOCK * a->least;
     a->want = split ? want : 0;
     long tiles = (long) ncol / a->cols + (split ? some : n_seq);
     long items = split ? tiles + want : tiles;
     a->items = (int) items;
     a->part_cols = ncol < a->cols ? ncol : a->cols;
+    const int block = fm->cw >= 4 ? 64 : 32, bufs = fm->cw > 1 ? 2 : 1;
+    const size_t stages = (size_t) fm->pg * bufs * 4 * block * hd + 4 * fm->pg * bufs * block + 8 * fm->pg * bufs * fm->cw + 16 * fm->cw;
+    const size_t joined = fm->pg > 1 ? (size_t) fm->pg * fm->cols * ((hd + 4) * 4 + 8) : 0;
     char base[24], name[40];
-    snprintf(base, sizeof base, "sml_rw_rows%d%s", form, a->cap > 0.0f || a->slope ? "r" : "");
+    snprintf(base, sizeof base, "sml_rw_%s%s", fm->name, a->cap > 0.0f || a->slope ? "r" : "");
     sv_name(name, sizeof name, base, hd, type);
-    items_launch(name, n_kv, items, 64 * (unsigned) waves, (size_t) 2 * RW_STAGE(hd) + RW_EXTRA, st, a);
+    items_launch(name, n_kv, items, 64 * (unsigned) (fm->cw * fm->pg), stages > joined ? stages : joined, st, a);
     if (split) items_launch(hd == 64 ? "sml_rw_merge_d64" : "sml_rw_merge", n_kv, tiles * (a->cols / 16), 256, 0, st, a);
 }
 

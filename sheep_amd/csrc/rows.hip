@@ -112,8 +112,8 @@ typedef short v4s __attribute__((ext_vector_type(4)));
 // What no column may see is read from here.
 __device__ const uint8_t rw_zeros[16] = { 0 };
 
-// 16 bytes a lane straight into LDS, the wave's 64 lanes side by side from dst (a
-// wave-uniform address) on; the caller waits (vmcnt) and then meets the other
+// 16 bytes a lane straight into LDS, from an address of its own or from base + off,
+// the wave's 64 lanes side by side from dst (a wave-uniform address) on; the caller waits (vmcnt) and then meets the other
 // waves before any of the bytes is read. Written out because the compiler, which
 // cannot tell the buffers apart, otherwise waits for every copy in flight before
 // the next LDS read.
@@ -123,6 +123,11 @@ __device__ __forceinline__ void copy_lds16(const void * src, const void * dst) {
     const uint32_t at = (uint32_t) (uintptr_t) (const __attribute__((address_space(3))) void *) dst;
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
                  :: "s"(__builtin_amdgcn_readfirstlane(at)), "v"(src) : "m0", "memory");
+}
+__device__ __forceinline__ void copy_lds16(const void * base, uint32_t off, const void * dst) {
+    const uint32_t at = (uint32_t) (uintptr_t) (const __attribute__((address_space(3))) void *) dst;
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+                 :: "s"(__builtin_amdgcn_readfirstlane(at)), "v"(off), "s"(base) : "m0", "memory");
 }
 #pragma clang diagnostic pop
 
@@ -134,8 +139,25 @@ __device__ __forceinline__ rows_of rows_seq(const sml_krows & a, int b) {
     x.n = min(max(a.len[b], 0), a.max_len);
     return x;
 }
+// The sum of v over the wave's lanes.
+__device__ __forceinline__ float wave_total(float v) {
+    v += dpp_f<0x111>(v);                             // row_shr 1, 2, 4, 8: lane 15 of a row has its sum
+    v += dpp_f<0x112>(v);
+    v += dpp_f<0x114>(v);
+    v += dpp_f<0x118>(v);
+    const int x = __builtin_bit_cast(int, v);
+    return (__builtin_bit_cast(float, __builtin_amdgcn_readlane(x, 15)) + __builtin_bit_cast(float, __builtin_amdgcn_readlane(x, 31))) +
+           (__builtin_bit_cast(float, __builtin_amdgcn_readlane(x, 47)) + __builtin_bit_cast(float, __builtin_amdgcn_readlane(x, 63)));
+}
+// The least and the largest of 16 lanes, in each of them.
+__device__ __forceinline__ int least16(int v) {
+    v = min(v, dpp_i<0xB1>(v)); v = min(v, dpp_i<0x4E>(v)); v = min(v, dpp_i<0x141>(v)); return min(v, dpp_i<0x140>(v));
+}
+__device__ __forceinline__ int most16(int v) {
+    v = max(v, dpp_i<0xB1>(v)); v = max(v, dpp_i<0x4E>(v)); v = max(v, dpp_i<0x141>(v)); return max(v, dpp_i<0x140>(v));
+}
 
-struct rows_at { int b, tile, count, split, item; };  // a tile, its splits, this one's number, and the first's among all items
+struct rows_at { int b, tile, count, split, item; rows_of sq; };  // a tile, its splits, this one's number, the first's among all items
 // Item i's (or, of TILES, tile i's) place; false past the last. Without splits
 // (want 0) sequence b's tiles are numbered from start[b] * rep / cols + b on, which
 // leaves each as many numbers as it has tiles, and the number says whose it is.
@@ -152,45 +174,49 @@ __device__ __forceinline__ bool rows_place(const sml_krows & a, int i, int lane,
             lo += k * step;
             hi = min(hi, lo + step);
         }
-        const rows_of x = rows_seq(a, lo);
+        p.sq = rows_seq(a, lo);
         p.b = lo;
-        p.tile = i - (x.s0 * rep / cols + lo);
+        p.tile = i - (p.sq.s0 * rep / cols + lo);
         p.count = 1;
         p.split = 0;
         p.item = i;
-        return p.tile >= 0 && p.tile * cols < x.m * rep;
+        return p.tile >= 0 && p.tile * cols < p.sq.m * rep;
     }
     // the blocks of a split: what makes want of them in all, and some more
+    rows_of x[AT_SHARED / 64];
     float sum = 0.0f;
-    for (int b = lane; b < a.pg.n_seq; b += 64) {
-        const rows_of x = rows_seq(a, b);
-        sum += (float) ((x.m * rep + cols - 1) / cols) * (float) ((x.n + RW_BLOCK - 1) / RW_BLOCK);
-    }
-    const int chunk = max(a.least, (int) (wave_sum(sum) * 1.0001f / (float) a.want) + 1);
+    #pragma unroll
+    for (int k = 0; k < AT_SHARED / 64; k++)
+        if (k == 0 || 64 * k < a.pg.n_seq) {
+            x[k] = rows_of{0, 0, 0};
+            if (64 * k + lane < a.pg.n_seq) x[k] = rows_seq(a, 64 * k + lane);
+            sum += (float) ((x[k].m * rep + cols - 1) / cols) * (float) ((x[k].n + RW_BLOCK - 1) / RW_BLOCK);
+        }
+    const int chunk = max(a.least, (int) (wave_total(sum) * 1.0001f / (float) a.want) + 1);
     p.item = 0;
-    for (int b0 = 0; b0 < a.pg.n_seq; b0 += 64) {
-        int nt = 0, count = 1;
-        if (b0 + lane < a.pg.n_seq) {
-            const rows_of x = rows_seq(a, b0 + lane);
-            nt = (x.m * rep + cols - 1) / cols;
-            count = max(((x.n + RW_BLOCK - 1) / RW_BLOCK + chunk - 1) / chunk, 1);
+    #pragma unroll
+    for (int k = 0; k < AT_SHARED / 64; k++)
+        if (k == 0 || 64 * k < a.pg.n_seq) {
+            const int nt = (x[k].m * rep + cols - 1) / cols;
+            const int count = max(((x[k].n + RW_BLOCK - 1) / RW_BLOCK + chunk - 1) / chunk, 1);
+            const int items = wave_scan(nt * count), mine = TILES ? wave_scan(nt) : items;
+            const unsigned long long hit = __ballot(mine > i);
+            if (hit) {
+                const int l = __builtin_ctzll(hit), n = __builtin_amdgcn_readlane(nt, l);
+                p.b = 64 * k + l;
+                p.count = __builtin_amdgcn_readlane(count, l);
+                p.sq.s0 = __builtin_amdgcn_readlane(x[k].s0, l);
+                p.sq.m = __builtin_amdgcn_readlane(x[k].m, l);
+                p.sq.n = __builtin_amdgcn_readlane(x[k].n, l);
+                const int e = i - (__builtin_amdgcn_readlane(mine, l) - (TILES ? n : n * p.count));
+                p.tile = TILES || p.count == 1 ? e : e / p.count;
+                p.split = TILES ? 0 : e - p.tile * p.count;
+                p.item += __builtin_amdgcn_readlane(items, l) - n * p.count + p.tile * p.count;
+                return true;
+            }
+            i -= __builtin_amdgcn_readlane(mine, 63);
+            p.item += __builtin_amdgcn_readlane(items, 63);
         }
-        const int items = wave_scan(nt * count), mine = TILES ? wave_scan(nt) : items;
-        const unsigned long long hit = __ballot(mine > i);
-        if (hit) {
-            const int l = __builtin_ctzll(hit);
-            p.b = b0 + l;
-            p.count = __builtin_amdgcn_readlane(count, l);
-            const int n = __builtin_amdgcn_readlane(nt, l);
-            const int k = i - (__builtin_amdgcn_readlane(mine, l) - (TILES ? n : n * p.count));
-            p.tile = TILES ? k : k / p.count;
-            p.split = TILES ? 0 : k % p.count;
-            p.item += __builtin_amdgcn_readlane(items, l) - n * p.count + p.tile * p.count;
-            return true;
-        }
-        i -= __builtin_amdgcn_readlane(mine, 63);
-        p.item += __builtin_amdgcn_readlane(items, 63);
-    }
     return false;
 }
 __device__ __forceinline__ int rows_item() { return (int) (blockIdx.z * gridDim.y + blockIdx.y); }
@@ -219,6 +245,26 @@ __device__ __forceinline__ float tanh_any(float y) {
     return fabsf(y) > 0.625f ? t : tanh_small(y);
 }
 
+// The parts of two weights, as parts_of makes them; fp16's remainder is one mixed
+// instruction each.
+template <int BF>
+__device__ __forceinline__ void weights_of(float x, float y, typename Mx<BF>::v8 (&p)[Mx<BF>::parts], int e) {
+    if constexpr (BF) parts_of<BF>(x, y, p, e);
+    else {
+        typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+        typedef float v2f __attribute__((ext_vector_type(2)));
+        const v2h h = __builtin_convertvector(v2f{x, y}, v2h);
+        float r0, r1;
+        asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(r0) : "v"(h), "v"(x));
+        asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r1) : "v"(h), "v"(y));
+        const v2h l = __builtin_convertvector(v2f{r0, r1}, v2h);
+        p[0][e] = h[0];
+        p[0][e + 1] = h[1];
+        p[1][e] = l[0];
+        p[1][e + 1] = l[1];
+    }
+}
+
 // Bits lo..hi-1 of 32.
 __device__ __forceinline__ uint32_t bits_range(int lo, int hi) {
     lo = min(max(lo, 0), 32);
@@ -226,21 +272,35 @@ __device__ __forceinline__ uint32_t bits_range(int lo, int hi) {
     return lo < hi ? (~0u >> (32 - (hi - lo))) << lo : 0;
 }
 
-template <int D, int BF, int W, int CB, bool RULES>
+// A form of the rows' attention: CW waves beside each other, PG groups of them,
+// CB tiles of 16 columns a wave; the positions of a group's block and how many
+// stages of them it has, all stages' LDS, and where the groups' joined sums end.
+template <int D, int CW, int PG, int CB> struct RowsForm {
+    static constexpr int block = CW >= 4 ? 64 : 32, bufs = CW > 1 ? 2 : 1;
+    static constexpr int stages = PG * bufs * 4 * block * D;
+    static constexpr int joined = PG * 16 * CB * CW * (D + 4) * 4;
+};
+
+// CW waves side by side take 16 CB CW columns; PG such groups take the blocks of a
+// split in turn and are joined in LDS at the end.
+template <int D, int BF, int CW, int PG, int CB, bool RULES>
 __device__ __forceinline__ void rows_body(const sml_krows & a) {
     using M = Mx<BF>;
     typedef typename M::v8 v8;
-    constexpr int NJ = D / 32, E = D / 16, NP = M::parts, RB = 2 * D, POOL = RW_BLOCK * RB, STAGE = 2 * POOL;
-    constexpr int RC = 1024 / RB, NC = RW_BLOCK / RC / W;   // rows of a copy, a wave's copies of a block
-    static_assert(NC >= 1, "");
-    extern __shared__ __align__(16) uint8_t lds[];    // two stages, their new rows' positions, positions whose V is not finite
-    int * const kpos = (int *) (lds + 2 * STAGE);
-    uint64_t * const found = (uint64_t *) (kpos + 2 * RW_BLOCK);
+    using F = RowsForm<D, CW, PG, CB>;
+    constexpr int NJ = D / 32, E = D / 16, NP = M::parts, RB = 2 * D, W = CW * PG, KB = F::block, POOL = KB * RB, STAGE = 2 * POOL;
+    constexpr int RC = 1024 / RB, NC = KB / RC / CW;  // rows of a copy, a wave's copies of a block's keys
+    static_assert(NC >= 1 && RC <= 16, "");
+    extern __shared__ __align__(16) uint8_t lds[];    // the groups' stages; their new rows' positions, positions whose V is not finite, ranges
     const int kh = blockIdx.x, tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), cw = wave % CW, pgi = wave / CW;
+    uint8_t * const stages = lds + pgi * F::bufs * STAGE;
+    int * const kpos = (int *) (lds + F::stages) + pgi * F::bufs * KB;
+    uint64_t * const found = (uint64_t *) (lds + F::stages + 4 * PG * F::bufs * KB) + pgi * F::bufs * CW;
+    int * const red = (int *) (lds + F::stages + 4 * PG * F::bufs * KB + 8 * PG * F::bufs * CW);
     rows_at p;
     if (!rows_place<false>(a, rows_item(), lane, p)) return;
-    const rows_of sq = rows_seq(a, p.b);
+    const rows_of sq = p.sq;
     const int rep = a.n_head / a.pg.n_kv, ncol = sq.m * rep, past = sq.n - sq.m, kvd = a.pg.n_kv * D;
     const int sh = a.pg.page_shift, pmask = (1 << sh) - 1;
     const int32_t * const tab = a.pg.table + (size_t) p.b * a.pg.seq_pages;
@@ -255,7 +315,7 @@ __device__ __forceinline__ void rows_body(const sml_krows & a) {
     {
         #pragma unroll
         for (int x = 0; x < CB; x++) {
-            const int col = p.tile * a.cols + 16 * (CB * wave + x) + c, i = min(col, ncol - 1) / rep;
+            const int col = p.tile * a.cols + 16 * (CB * cw + x) + c, i = min(col, ncol - 1) / rep;
             mine[x] = col < ncol;
             r[x] = sq.s0 + i;
             h[x] = kh * rep + (min(col, ncol - 1) - i * rep);
@@ -274,33 +334,33 @@ __device__ __forceinline__ void rows_body(const sml_krows & a) {
             if (mine[x] && tree && past + nbit > 0) { w_lo = min(w_lo, max(past, 0)); w_hi = max(w_hi, min(past + nbit, sq.n)); }
             if (some[x]) { f_lo = max(f_lo, range ? lo[x] : 0x7fffffff); f_hi = min(f_hi, range ? hi[x] : 0); }
         }
-        #pragma unroll
-        for (int e = 1; e < 16; e <<= 1) {
-            w_lo = min(w_lo, __shfl_xor(w_lo, e));
-            w_hi = max(w_hi, __shfl_xor(w_hi, e));
-            f_lo = max(f_lo, __shfl_xor(f_lo, e));
-            f_hi = min(f_hi, __shfl_xor(f_hi, e));
+        t_lo = w_lo = __builtin_amdgcn_readfirstlane(least16(w_lo));
+        t_hi = w_hi = __builtin_amdgcn_readfirstlane(most16(w_hi));
+        t_flo = f_lo = __builtin_amdgcn_readfirstlane(most16(f_lo));
+        t_fhi = f_hi = __builtin_amdgcn_readfirstlane(least16(f_hi));
+        if constexpr (CW > 1) {
+            if (!lane && !pgi) { red[4 * cw] = w_lo; red[4 * cw + 1] = w_hi; red[4 * cw + 2] = f_lo; red[4 * cw + 3] = f_hi; }
+            __syncthreads();
+            #pragma unroll
+            for (int w = 0; w < CW; w++) {
+                t_lo = min(t_lo, red[4 * w]);
+                t_hi = max(t_hi, red[4 * w + 1]);
+                t_flo = max(t_flo, red[4 * w + 2]);
+                t_fhi = min(t_fhi, red[4 * w + 3]);
+            }
+            t_lo = __builtin_amdgcn_readfirstlane(t_lo);
+            t_hi = __builtin_amdgcn_readfirstlane(t_hi);
+            t_flo = __builtin_amdgcn_readfirstlane(t_flo);
+            t_fhi = __builtin_amdgcn_readfirstlane(t_fhi);
         }
-        w_lo = __builtin_amdgcn_readfirstlane(w_lo);
-        w_hi = __builtin_amdgcn_readfirstlane(w_hi);
-        f_lo = __builtin_amdgcn_readfirstlane(f_lo);
-        f_hi = __builtin_amdgcn_readfirstlane(f_hi);
-        int * const red = kpos;
-        if (!lane) { red[4 * wave] = w_lo; red[4 * wave + 1] = w_hi; red[4 * wave + 2] = f_lo; red[4 * wave + 3] = f_hi; }
-        __syncthreads();
-        t_lo = red[0]; t_hi = red[1]; t_flo = red[2]; t_fhi = red[3];
+    }
+    // the queries: lane (c, g) holds dims 32j + 8g.. of its columns
+    v4f x[CB][2 * NJ];
+    #pragma unroll
+    for (int y = 0; y < CB; y++) {
+        const float * qp = a.q + (size_t) r[y] * a.q_stride + (size_t) h[y] * D + 8 * g;
         #pragma unroll
-        for (int w = 1; w < W; w++) {
-            t_lo = min(t_lo, red[4 * w]);
-            t_hi = max(t_hi, red[4 * w + 1]);
-            t_flo = max(t_flo, red[4 * w + 2]);
-            t_fhi = min(t_fhi, red[4 * w + 3]);
-        }
-        __syncthreads();                              // the positions may be written
-        t_lo = __builtin_amdgcn_readfirstlane(t_lo);
-        t_hi = __builtin_amdgcn_readfirstlane(t_hi);
-        t_flo = __builtin_amdgcn_readfirstlane(t_flo);
-        t_fhi = __builtin_amdgcn_readfirstlane(t_fhi);
+        for (int j = 0; j < 2 * NJ; j++) x[y][j] = *(const v4fu *) (qp + 32 * (j / 2) + 4 * (j % 2));
     }
     // this split's blocks
     int t_at = 0, t_end = 0;
@@ -310,21 +370,87 @@ __device__ __forceinline__ void rows_body(const sml_krows & a) {
         t_end = min((b0 + min(nb, (p.split + 1) * per)) * RW_BLOCK, t_hi);
     }
 
-    // the queries: lane (c, g) holds dims 32j + 8g.. of its columns, in parts
+    // Pages of 64 times 16 positions from t_tab on, one a lane (negative: none), and
+    // of as many behind; where in a pool the first of the 16 lies, in bytes.
+    auto look = [&](int t) {
+        t += 16 * lane;
+        const int e = t < t_end ? tab[t >> sh] : -1;
+        return e < a.pg.n_pages ? e : -1;
+    };
+    int t_tab = t_at, ent = look(t_at), next = look(t_at + 1024);
+    uint64_t at_ent;
+    auto place = [&]() { at_ent = 2 * ((uint64_t) max(ent, 0) * a.pg.page_stride + (uint64_t) (uint32_t) (((t_tab + 16 * lane) & pmask) * kvd + kh * D)); };
+    place();
+    // the next step (a block of each group) at or after t with a page
+    constexpr int STEP = PG * KB;
+    auto seek = [&](int t) {
+        while (t < t_end) {
+            if (t - t_tab >= 1024) {
+                t_tab += 1024;
+                ent = next;
+                next = look(t_tab + 1024);
+                place();
+                continue;
+            }
+            if (__ballot(ent >= 0) >> ((t - t_tab) >> 4) & ((1ull << (STEP / 16)) - 1)) break;
+            t += STEP;
+        }
+        return t;
+    };
+    auto page = [&](int t, int e) { return __builtin_amdgcn_readlane(ent, ((t - t_tab) >> 4) + pgi * (KB / 16) + e); };
+    // A lane of a copy: its row and its word there; word w of row x lies at w ^ swz(x).
+    auto swz = [](int x) { return D == 128 ? 2 * (x & 7) : (x >> 1) & 7; };
+    const int crow = RC * cw + lane / (RB / 16), cword = lane % (RB / 16);
+    uint32_t coff[CW == 1 ? 2 : 1];                   // by the copy's oddness, where that changes the swizzle
+    #pragma unroll
+    for (int e = 0; e < (CW == 1 ? 2 : 1); e++) coff[e] = 2u * (uint32_t) ((crow & 15) * kvd + 8 * (cword ^ swz(RC * e + crow)));
+    auto fetch = [&](uint8_t * st, const uint16_t * pool, int t) {
+        const int i0 = ((t - t_tab) >> 4) + pgi * (KB / 16), from = t + pgi * KB;
+        constexpr uint64_t MASK = (1ull << (KB / 16)) - 1;
+        if ((~__ballot(ent >= 0) >> i0 & MASK) == 0 && from >= t_lo && from + KB <= t_hi) {
+            #pragma unroll
+            for (int e = 0; e < NC; e++) {
+                const int row0 = RC * (CW * e + cw), i = i0 + (row0 >> 4);
+                const uint64_t at = (uint64_t) (uint32_t) __builtin_amdgcn_readlane((int) (at_ent >> 32), i) << 32 | (uint32_t) __builtin_amdgcn_readlane((int) at_ent, i);
+                copy_lds16((const uint8_t *) pool + at + (uint32_t) (2 * ((RC * CW * e) & 15) * kvd), coff[CW == 1 ? e & 1 : 0], st + row0 * RB);
+            }
+        } else {
+            #pragma unroll 1
+            for (int e = 0; e < NC; e++) {
+                const int row0 = RC * (CW * e + cw), row = RC * CW * e + crow, i = i0 + (row0 >> 4), pos = from + row;
+                const uint64_t at = (uint64_t) (uint32_t) __builtin_amdgcn_readlane((int) (at_ent >> 32), i) << 32 | (uint32_t) __builtin_amdgcn_readlane((int) at_ent, i);
+                const bool in = __builtin_amdgcn_readlane(ent, i) >= 0 && pos >= t_lo && pos < t_hi;
+                const uint8_t * p8 = (const uint8_t *) pool + at + 2u * (uint32_t) ((row & 15) * kvd + 8 * (cword ^ swz(row)));
+                copy_lds16(in ? (const void *) p8 : (const void *) rw_zeros, st + row0 * RB);
+            }
+        }
+    };
+    // The positions of a block's new rows, on their way; they are in LDS with the block.
+    int at_pos = 0;
+    auto fetch_pos = [&](int t) {
+        if (RULES && a.slope && a.pos && t + pgi * KB + KB > past && cw == 0)
+            at_pos = a.pos[sq.s0 + min(max(t + pgi * KB + lane - past, 0), max(sq.m - 1, 0))];
+    };
+    auto keep_pos = [&](int * kp) {
+        if (RULES && a.slope && a.pos && cw == 0 && lane < KB) kp[lane] = at_pos;
+    };
+    int t = seek(t_at), buf = 0;
+    if (t < t_end) {
+        fetch(stages, a.pg.k, t);
+        fetch(stages + POOL, a.pg.v, t);
+        fetch_pos(t);
+    }
+
+    // the queries in parts
     v8 q[CB][NJ][NP];
     float back[CB], slope[CB];                        // what a product of the scaled q is multiplied by
     #pragma unroll
     for (int y = 0; y < CB; y++) {
-        float x[NJ][8], mx = 0.0f;
-        const float * qp = a.q + (size_t) r[y] * a.q_stride + (size_t) h[y] * D + 8 * g;
+        float mx = 0.0f;
         #pragma unroll
-        for (int j = 0; j < NJ; j++)
+        for (int j = 0; j < 2 * NJ; j++)
             #pragma unroll
-            for (int e = 0; e < 8; e += 4) {
-                const v4f v = *(const v4fu *) (qp + 32 * j + e);
-                #pragma unroll
-                for (int k = 0; k < 4; k++) { x[j][e + k] = mine[y] ? v[k] * a.sign : 0.0f; mx = fmaxf(mx, fabsf(x[j][e + k])); }
-            }
+            for (int k = 0; k < 4; k++) { x[y][j][k] = mine[y] ? x[y][j][k] * a.sign : 0.0f; mx = fmaxf(mx, fabsf(x[y][j][k])); }
         mx = fmaxf(mx, __shfl_xor(mx, 16));
         mx = fmaxf(mx, __shfl_xor(mx, 32));
         const int ex = BF ? 0 : scale_of(mx);
@@ -332,7 +458,7 @@ __device__ __forceinline__ void rows_body(const sml_krows & a) {
         for (int j = 0; j < NJ; j++)
             #pragma unroll
             for (int e = 0; e < 8; e += 2)
-                parts_of<BF>(__builtin_amdgcn_ldexpf(x[j][e], -ex), __builtin_amdgcn_ldexpf(x[j][e + 1], -ex), q[y][j], e);
+                parts_of<BF>(__builtin_amdgcn_ldexpf(x[y][2 * j + e / 4][e % 4], -ex), __builtin_amdgcn_ldexpf(x[y][2 * j + e / 4][e % 4 + 1], -ex), q[y][j], e);
         back[y] = __builtin_amdgcn_ldexpf(a.scale, ex);
         slope[y] = RULES && a.slope ? -1.44269504088896341f * a.slope[h[y]] : 0.0f;
     }
@@ -347,61 +473,67 @@ __device__ __forceinline__ void rows_body(const sml_krows & a) {
         for (int u = 0; u < E; u++) o[y][u] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
     }
 
-    // the next block at or after t with a page, and its pages by 16 positions
-    int page[4];
-    auto seek = [&](int t) {
-        for (; t < t_end; t += RW_BLOCK) {
-            int any = -1;
-            #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                int x = t + 16 * e < t_hi ? tab[(t + 16 * e) >> sh] : -1;
-                x = x >= 0 && x < a.pg.n_pages ? x : -1;
-                page[e] = x;
-                any = max(any, x);
-            }
-            if (any >= 0) break;
-        }
-        return t;
-    };
-    // a lane of a copy: its row and its word there; word w of row x lies at w ^ swz(x)
-    const int crow = lane / (RB / 16), cword = (lane % (RB / 16)) ^ (D == 128 ? 2 * ((RC * wave + crow) & 7) : ((RC * wave + crow) >> 1) & 7);
-    static_assert(RC * W % 16 == 0, "a wave's copies have one swizzle");
-    auto fetch = [&](int buf, int t) {
-        uint8_t * const st = lds + buf * STAGE;
-        #pragma unroll
-        for (int e = 0; e < NC; e++) {
-            const int row0 = RC * (W * e + wave), at = t + row0 + crow;
-            const int pg = row0 < 32 ? (row0 < 16 ? page[0] : page[1]) : (row0 < 48 ? page[2] : page[3]);
-            const size_t off = (size_t) max(pg, 0) * a.pg.page_stride + (size_t) (at & pmask) * kvd + (size_t) kh * D + 8 * cword;
-            const bool in = pg >= 0 && at >= t_lo && at < t_hi;
-            copy_lds16(in ? (const void *) (a.pg.k + off) : (const void *) rw_zeros, st + row0 * RB);
-            copy_lds16(in ? (const void *) (a.pg.v + off) : (const void *) rw_zeros, st + POOL + row0 * RB);
-        }
-        if (RULES && a.slope && a.pos && t + RW_BLOCK > past && wave == 0)
-            kpos[buf * RW_BLOCK + lane] = a.pos[sq.s0 + min(max(t + lane - past, 0), max(sq.m - 1, 0))];
-    };
-    const int krow = c * RB, kx = D == 128 ? 2 * (c & 7) : (c >> 1) & 7;
+    const int krow = c * RB, kx = swz(c);
     const int vrow = 4 * g + (c >> 2), vx = D == 128 ? vrow & 7 : (vrow >> 2) & 3;    // the V row this lane reads for its 16
     const int vat = POOL + vrow * RB + (D == 128 ? 8 * (c & 3) : 16 * (((c >> 1) & 1) ^ ((vrow >> 1) & 1)) + 8 * (c & 1));
+    // Values that are not finite among those that this wave has fetched, where columns
+    // differ: zeros in their place; their positions in the block.
+    auto screen = [&](uint8_t * st) {
+        uint64_t bad = 0;
+        #pragma unroll 1
+        for (int e = 0; e < NC; e++) {
+            const int row0 = RC * (CW * e + cw);
+            v4u * const at = (v4u *) (st + POOL + row0 * RB + 16 * lane);
+            v4u x = *at;
+            uint32_t any = 0;
+            #pragma unroll
+            for (int k = 0; k < 4; k++) {             // an exponent of all ones carries into the top bit
+                const uint32_t up = BF ? ((x[k] & 0x7F807F80u) + 0x00800080u) & 0x80008000u : ((x[k] & 0x7C007C00u) + 0x04000400u) & 0x80008000u;
+                x[k] &= ~((up >> 15) * 0xFFFFu);
+                any |= up;
+            }
+            const uint64_t hit = __ballot(any != 0);
+            if (hit) {
+                *at = x;
+                #pragma unroll 1
+                for (int k = 0; k < RC; k++)
+                    if (hit >> (64 / RC * k) & ((1ull << (64 / RC)) - 1)) bad |= 1ull << (row0 + k);
+            }
+        }
+        return bad;
+    };
 
-    // positions t.. of a stage's 32 rows from row0, with their pages pa and pb
-    auto compute = [&](const uint8_t * st, int buf, int row0, int t, int pa, int pb) {
-        v4f s[CB][2];
+    // 32 positions from t on, rows row0.. of stage st, whose pages are pa and pb: the scores, then the weights and the sums.
+    auto products = [&](const uint8_t * st, int row0, v4f (&s)[CB][2], auto && loaded) {
+        v8 ka[2][NJ];
+        #pragma unroll
+        for (int j = 0; j < 2; j++)
+            #pragma unroll
+            for (int e = 0; e < NJ; e++) ka[j][e] = *(const v8 *) (st + (row0 + 16 * j) * RB + krow + 16 * ((4 * e + g) ^ kx));
+        __builtin_amdgcn_sched_barrier(0);
+        loaded();
         #pragma unroll
         for (int j = 0; j < 2; j++) {
             #pragma unroll
             for (int y = 0; y < CB; y++) s[y][j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
             #pragma unroll
-            for (int e = 0; e < NJ; e++) {
-                const v8 ka = *(const v8 *) (st + (row0 + 16 * j) * RB + krow + 16 * ((4 * e + g) ^ kx));
+            for (int e = 0; e < NJ; e++)
                 #pragma unroll
                 for (int k = 0; k < NP; k++)
                     #pragma unroll
-                    for (int y = 0; y < CB; y++) s[y][j] = M::mul(ka, q[y][e][k], s[y][j]);
-            }
+                    for (int y = 0; y < CB; y++) s[y][j] = M::mul(ka[j][e], q[y][e][k], s[y][j]);
         }
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    auto value = [&](const uint8_t * st, int row0, int u) {
+        typedef __attribute__((address_space(3))) v4s lv4s;
+        const uint8_t * vr = st + vat + row0 * RB + ((u ^ vx) << 5);
+        const v4s x0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lv4s *) vr);
+        const v4s x1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lv4s *) (vr + 16 * RB));
+        return __builtin_bit_cast(v8, __builtin_shufflevector(x0, x1, 0, 1, 2, 3, 4, 5, 6, 7));
+    };
+    auto weigh = [&](v4f (&s)[CB][2], v8 (&w)[CB][NP], const int * kp, int t, int pa, int pb, uint32_t bad) {
         const bool whole = pa >= 0 && pb >= 0 && t >= f_lo && t + 32 <= f_hi;
-        v8 w[CB][NP];
         #pragma unroll
         for (int y = 0; y < CB; y++) {
             float f = back[y];                        // log2 weights are f times the scores
@@ -426,17 +558,22 @@ __device__ __forceinline__ void rows_body(const sml_krows & a) {
                     }
                 }
                 if (a.slope) {
-                    const bool given = a.pos && t + 32 > past;
                     const float d0 = (float) (t + 4 * g - qpos[y]);
-                    #pragma unroll
-                    for (int j = 0; j < 2; j++)
+                    if (a.pos && t + 32 > past) {
                         #pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            float d = d0 + (float) (16 * j + e);
-                            const int x = 16 * j + 4 * g + e;
-                            if (given && t + x >= past) d = (float) (kpos[buf * RW_BLOCK + row0 + x] - qpos[y]);
-                            s[y][j][e] = __builtin_fmaf(slope[y], fabsf(d), s[y][j][e]);
-                        }
+                        for (int j = 0; j < 2; j++)
+                            #pragma unroll
+                            for (int e = 0; e < 4; e++) {
+                                const int x = 16 * j + 4 * g + e;
+                                const float d = t + x >= past ? (float) (kp[x] - qpos[y]) : d0 + (float) (16 * j + e);
+                                s[y][j][e] = __builtin_fmaf(slope[y], fabsf(d), s[y][j][e]);
+                            }
+                    } else {
+                        #pragma unroll
+                        for (int j = 0; j < 2; j++)
+                            #pragma unroll
+                            for (int e = 0; e < 4; e++) s[y][j][e] = __builtin_fmaf(slope[y], fabsf(d0 + (float) (16 * j + e)), s[y][j][e]);
+                    }
                 }
             }
             if (!whole) {
@@ -452,17 +589,14 @@ __device__ __forceinline__ void rows_body(const sml_krows & a) {
                 if (pa < 0) vm &= 0xFFFF0000u;
                 if (pb < 0) vm &= 0x0000FFFFu;
                 if (!some[y]) vm = 0;
-                if (t < t_flo || t + 32 > t_fhi) {
-                    uint64_t bad = 0;
-                    #pragma unroll
-                    for (int x = 0; x < W; x++) bad |= found[buf * W + x];
-                    if (vm & (uint32_t) (bad >> row0)) l[y] = NAN;
-                }
+                if (vm & bad) l[y] = NAN;
                 vm >>= 4 * g;
                 #pragma unroll
                 for (int j = 0; j < 2; j++)
                     #pragma unroll
                     for (int e = 0; e < 4; e++) s[y][j][e] = (vm >> (16 * j + e)) & 1 ? s[y][j][e] : -INFINITY;
+            } else if (bad) {
+                l[y] = NAN;
             }
             float mx = -INFINITY;
             #pragma unroll
@@ -491,59 +625,99 @@ __device__ __forceinline__ void rows_body(const sml_krows & a) {
                     const float w1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[y][j][e + 1], f, -bu));
                     l[y] += w0;
                     l[y] += w1;
-                    parts_of<BF>(w0, w1, w[y], 4 * j + e);
+                    weights_of<BF>(w0, w1, w[y], 4 * j + e);
                 }
-        }
-        #pragma unroll
-        for (int u = 0; u < E; u++) {
-            const uint8_t * vr = st + vat + row0 * RB + ((u ^ vx) << 5);
-            typedef __attribute__((address_space(3))) v4s lv4s;
-            const v4s x0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lv4s *) vr);
-            const v4s x1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lv4s *) (vr + 16 * RB));
-            const v8 vv = __builtin_bit_cast(v8, __builtin_shufflevector(x0, x1, 0, 1, 2, 3, 4, 5, 6, 7));
-            #pragma unroll
-            for (int k = 0; k < NP; k++)
-                #pragma unroll
-                for (int y = 0; y < CB; y++) o[y][u] = M::mul(vv, w[y][k], o[y][u]);
         }
     };
-
-    int t = seek(t_at), buf = 0;
-    if (t < t_end) fetch(0, t);
-    while (t < t_end) {
-        const int pg[4] = { page[0], page[1], page[2], page[3] };
-        const int tn = seek(t + RW_BLOCK);
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");     // this wave's rows of the block are in LDS
-        if (t < t_flo || t + RW_BLOCK > t_fhi) {
-            uint64_t bad = 0;
+    auto sums = [&](const v8 & vv, int u, const v8 (&w)[CB][NP]) {
+        #pragma unroll
+        for (int k = 0; k < NP; k++)
             #pragma unroll
-            for (int e = 0; e < NC; e++) {
-                const int row0 = RC * (W * e + wave);
-                v4u * const at = (v4u *) (lds + buf * STAGE + POOL + row0 * RB + 16 * lane);
-                v4u x = *at;
-                uint32_t any = 0;
+            for (int y = 0; y < CB; y++) o[y][u] = M::mul(vv, w[y][k], o[y][u]);
+    };
+
+    // Values are on their way to registers while the weights are made, if those hold
+    // them all (bfloat16's parts leave room for half).
+    constexpr int EARLY = BF && CB == 2 ? E / 2 : E;
+    while (t < t_end) {
+        const int cur = t + pgi * KB;
+        int pg[KB / 16];
+        #pragma unroll
+        for (int e = 0; e < KB / 16; e++) pg[e] = page(t, e);
+        const int tn = seek(t + STEP);
+        const bool differ = cur < t_flo || cur + KB > t_fhi;
+        if constexpr (CW == 1) {
+            // One stage, the wave's own: a block's keys are fetched over the last one's
+            // when those are in registers, its values likewise.
+            const bool on = cur < t_end && cur < w_hi && cur + KB > w_lo;
+            v4f s[CB][2];
+            v8 w[CB][NP], vv[EARLY];
+            asm volatile("s_waitcnt vmcnt(%0)" :: "n"(NC) : "memory");
+            products(stages, 0, s, [&]() {
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                if (tn < t_end) fetch(stages, a.pg.k, tn);
+            });
+            if (tn < t_end) asm volatile("s_waitcnt vmcnt(%0)" :: "n"(NC) : "memory");
+            else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            keep_pos(kpos);
+            uint64_t bad = 0;
+            if (differ) bad = screen(stages);
+            #pragma unroll
+            for (int u = 0; u < EARLY; u++) vv[u] = value(stages, 0, u);
+            __builtin_amdgcn_sched_barrier(0);
+            if (on) {
+                weigh(s, w, kpos, cur, pg[0], pg[1], (uint32_t) bad);
                 #pragma unroll
-                for (int k = 0; k < 4; k++) {                 // an exponent of all ones carries into the top bit
-                    const uint32_t up = BF ? ((x[k] & 0x7F807F80u) + 0x00800080u) & 0x80008000u : ((x[k] & 0x7C007C00u) + 0x04000400u) & 0x80008000u;
-                    x[k] &= ~((up >> 15) * 0xFFFFu);
-                    any |= up;
-                }
-                const uint64_t hit = __ballot(any != 0);
-                if (hit) {
-                    *at = x;
-                    #pragma unroll
-                    for (int k = 0; k < RC; k++)
-                        if (hit >> (64 / RC * k) & ((1ull << (64 / RC)) - 1)) bad |= 1ull << (row0 + k);
+                for (int u = 0; u < E - EARLY; u++) {
+                    sums(vv[u], u, w);
+                    vv[u] = value(stages, 0, u + EARLY);
                 }
             }
-            if (!lane) found[buf * W + wave] = bad;
-        }
-        __syncthreads();
-        if (tn < t_end) fetch(buf ^ 1, tn);                   // past the barrier: nobody reads the last block
-        #pragma unroll 1
-        for (int e = 0; e < 2; e++) {
-            const int te = t + 32 * e;
-            if (te < w_hi && te + 32 > w_lo) compute(lds + buf * STAGE, buf, 32 * e, te, e ? pg[2] : pg[0], e ? pg[3] : pg[1]);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            if (tn < t_end) {
+                fetch(stages + POOL, a.pg.v, tn);
+                fetch_pos(tn);
+            }
+            if (on) {
+                #pragma unroll
+                for (int u = E - EARLY; u < E; u++) sums(vv[u % EARLY], u, w);
+            }
+        } else {
+            uint8_t * const st = stages + buf * STAGE;
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");     // this wave's rows of the block are in LDS
+            keep_pos(kpos + buf * KB);
+            if (differ) {
+                const uint64_t bad = screen(st);
+                if (!lane) found[buf * CW + cw] = bad;
+            }
+            __syncthreads();
+            if (tn < t_end) {                                    // past the barrier: nobody reads the last block
+                fetch(stages + (buf ^ 1) * STAGE, a.pg.k, tn);
+                fetch(stages + (buf ^ 1) * STAGE + POOL, a.pg.v, tn);
+                fetch_pos(tn);
+            }
+            #pragma unroll 1
+            for (int e = 0; e < KB / 32; e++) {
+                const int te = cur + 32 * e;
+                if (te >= t_end || te >= w_hi || te + 32 <= w_lo) continue;
+                v4f s[CB][2];
+                v8 w[CB][NP], vv[EARLY];
+                uint64_t bad = 0;
+                products(st, 32 * e, s, []() {});
+                #pragma unroll
+                for (int u = 0; u < EARLY; u++) vv[u] = value(st, 32 * e, u);
+                __builtin_amdgcn_sched_barrier(0);
+                if (differ) {
+                    #pragma unroll
+                    for (int x = 0; x < CW; x++) bad |= found[buf * CW + x];
+                }
+                weigh(s, w, kpos + buf * KB + 32 * e, te, e ? pg[KB / 16 - 2] : pg[0], e ? pg[KB / 16 - 1] : pg[1], (uint32_t) (bad >> (32 * e)));
+                #pragma unroll
+                for (int u = 0; u < E; u++) {
+                    sums(vv[u % EARLY], u, w);
+                    if (u + EARLY < E) vv[u % EARLY] = value(st, 32 * e, u + EARLY);
+                }
+            }
         }
         t = tn;
         buf ^= 1;
@@ -553,36 +727,90 @@ __device__ __forceinline__ void rows_body(const sml_krows & a) {
     for (int y = 0; y < CB; y++) {
         l[y] += __shfl_xor(l[y], 16);
         l[y] += __shfl_xor(l[y], 32);
-        if (!mine[y]) continue;
-        if (p.count == 1) {
-            float * const to = a.out + ((size_t) r[y] * a.n_head + h[y]) * D + 4 * g;
-            #pragma unroll
-            for (int u = 0; u < E; u++) {
-                v4f x;
+        if (!some[y]) { base[y] = -INFINITY; l[y] = 0.0f; }
+    }
+    if constexpr (PG == 1) {
+        #pragma unroll
+        for (int y = 0; y < CB; y++) {
+            if (!mine[y]) continue;
+            if (p.count == 1) {
+                float * const to = a.out + ((size_t) r[y] * a.n_head + h[y]) * D + 4 * g;
                 #pragma unroll
-                for (int e = 0; e < 4; e++) x[e] = some[y] && l[y] != 0.0f ? o[y][u][e] / l[y] : 0.0f;
-                *(v4fu *) (to + 16 * u) = x;
+                for (int u = 0; u < E; u++) {
+                    v4f x;
+                    #pragma unroll
+                    for (int e = 0; e < 4; e++) x[e] = l[y] != 0.0f ? o[y][u][e] / l[y] : 0.0f;
+                    *(v4fu *) (to + 16 * u) = x;
+                }
+            } else {
+                const int pc = 16 * (CB * cw + y) + c;
+                if (!g) part_ml(a, kh, p.item + p.split, D)[pc] = make_float2(base[y], l[y]);
+                float * const to = part_o(a, kh, p.item + p.split, D) + (size_t) pc * D + 4 * g;
+                #pragma unroll
+                for (int u = 0; u < E; u++) *(v4f *) (to + 16 * u) = o[y][u];
             }
-        } else {
-            const int pc = 16 * (CB * wave + y) + c;
-            if (!g) part_ml(a, kh, p.item + p.split, D)[pc] = some[y] ? make_float2(base[y], l[y]) : make_float2(-INFINITY, 0.0f);
-            float * const to = part_o(a, kh, p.item + p.split, D) + (size_t) pc * D + 4 * g;
+        }
+    } else {
+        // The groups joined: their sums over the stages, rows of D + 4 floats on
+        // different banks, their bases and weights' sums behind.
+        constexpr int QT = 16 * CB * CW, LD = D + 4;
+        float * const so = (float *) lds;
+        float2 * const sml = (float2 *) (lds + F::joined);
+        __syncthreads();                              // all are done with the stages
+        #pragma unroll
+        for (int y = 0; y < CB; y++) {
+            const int pc = 16 * (CB * cw + y) + c;
+            float * const to = so + (size_t) (pgi * QT + pc) * LD + 4 * g;
             #pragma unroll
             for (int u = 0; u < E; u++) *(v4f *) (to + 16 * u) = o[y][u];
+            if (!g) sml[pgi * QT + pc] = make_float2(base[y], l[y]);
+        }
+        __syncthreads();
+        for (int x = tid; x < QT * (D / 4); x += 64 * W) {
+            const int pc = x / (D / 4), d = 4 * (x % (D / 4)), col = p.tile * a.cols + pc;
+            if (col >= ncol) break;
+            float m = -INFINITY;
+            #pragma unroll
+            for (int k = 0; k < PG; k++) m = fmaxf(m, sml[k * QT + pc].x);
+            const float mu = m == -INFINITY ? 0.0f : m;
+            float ls = 0.0f;
+            v4f os = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+            #pragma unroll
+            for (int k = 0; k < PG; k++) {
+                const float2 ml = sml[k * QT + pc];
+                const float f = __builtin_amdgcn_exp2f(ml.x - mu);
+                const v4f v = *(const v4f *) (so + (size_t) (k * QT + pc) * LD + d);
+                if (ml.x != -INFINITY || ml.y != 0.0f) {
+                    ls += f * ml.y;
+                    #pragma unroll
+                    for (int e = 0; e < 4; e++) os[e] = __builtin_fmaf(f, v[e], os[e]);
+                }
+            }
+            if (p.count == 1) {
+                const int i = col / rep;
+                #pragma unroll
+                for (int e = 0; e < 4; e++) os[e] = ls != 0.0f ? os[e] / ls : 0.0f;
+                *(v4fu *) (a.out + ((size_t) (sq.s0 + i) * a.n_head + kh * rep + (col - i * rep)) * D + d) = os;
+            } else {
+                if (!d) part_ml(a, kh, p.item + p.split, D)[pc] = make_float2(m, ls);
+                *(v4f *) (part_o(a, kh, p.item + p.split, D) + (size_t) pc * D + d) = os;
+            }
         }
     }
 }
-#define ROWS(D, BF, W, CB, EU, name, sfx) \
-    extern "C" __global__ __launch_bounds__(64 * W, EU) void name##sfx(const sml_krows a) { rows_body<D, BF, W, CB, false>(a); } \
-    extern "C" __global__ __launch_bounds__(64 * W, EU) void name##r##sfx(const sml_krows a) { rows_body<D, BF, W, CB, true>(a); }
-#define ROWS4(W, CB, E1, E2, E3, E4, name) \
-    ROWS(128, 0, W, CB, E1, name, ) \
-    ROWS(128, 1, W, CB, E2, name, _bf) \
-    ROWS(64, 0, W, CB, E3, name, _d64) \
-    ROWS(64, 1, W, CB, E4, name, _d64_bf)
-ROWS4(4, 1, 2, 2, 4, 4, sml_rw_rows41)
-ROWS4(4, 2, 2, 2, 3, 3, sml_rw_rows42)
-ROWS4(8, 1, 4, 4, 4, 4, sml_rw_rows81)
+#define ROWS(D, BF, CW, PG, CB, EU, name, sfx) \
+    extern "C" __global__ __launch_bounds__(64 * CW * PG, EU) void name##sfx(const sml_krows a) { rows_body<D, BF, CW, PG, CB, false>(a); } \
+    extern "C" __global__ __launch_bounds__(64 * CW * PG, EU) void name##r##sfx(const sml_krows a) { rows_body<D, BF, CW, PG, CB, true>(a); }
+#define ROWS4(CW, PG, CB, E, name) \
+    ROWS(128, 0, CW, PG, CB, 2, name, ) \
+    ROWS(128, 1, CW, PG, CB, 2, name, _bf) \
+    ROWS(64, 0, CW, PG, CB, E, name, _d64) \
+    ROWS(64, 1, CW, PG, CB, E, name, _d64_bf)
+ROWS4(1, 8, 1, 4, sml_rw_rows16)
+ROWS4(1, 8, 2, 2, sml_rw_rows32)
+ROWS4(2, 4, 2, 2, sml_rw_rows64)
+ROWS4(4, 2, 2, 2, sml_rw_rows128)
+ROWS4(4, 1, 2, 3, sml_rw_rows128l)
 
 // The splits of a tile joined, 16 columns a workgroup, 16 lanes a column: the
 // bases of its splits shared out over the lanes, then each lane's dims of every
@@ -609,8 +837,9 @@ __device__ __forceinline__ void rows_merge_body(const sml_krows & a) {
     for (int s = l; s < p.count; s += 16) {
         const float2 x = ml[s * step];
         const float e = __builtin_amdgcn_exp2f(x.x - mu);
-        f[c][s] = x.x == -INFINITY ? -1.0f : e;       // no sums: what lies there counts for nothing
-        if (x.x != -INFINITY) sum += e * x.y;
+        const bool none = x.x == -INFINITY && x.y == 0.0f;    // what lies there counts for nothing
+        f[c][s] = none ? -1.0f : e;
+        if (!none) sum += e * x.y;
     }
     sum = sum16(sum);
     wave_lds();
