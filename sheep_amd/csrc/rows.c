@@ -53,8 +53,7 @@ static void items_launch(const char * name, int n_kv, long items, unsigned threa
 }
 
 static const struct form { const char * name; int cols, cw, pg, per_cu; } forms[] = {
-    { "rows16", 16, 1, 8, 1 }, { "rows32", 32, 1, 8, 1 }, { "rows64", 64, 2, 4, 1 }, { "rows128", 128, 4, 2, 1 },
-    { "rows128l", 128, 4, 1, 2 },
+    { "rows32", 32, 1, 8, 1 }, { "rows64", 64, 2, 4, 1 }, { "rows128", 128, 4, 2, 1 }, { "rows128l", 128, 4, 1, 2 },
 };
 static void rows_launch(sml_krows * a, int hd, int type, hipStream_t st) {
     const int n_kv = a->pg.n_kv, rep = a->n_head / n_kv, n_seq = a->pg.n_seq;
@@ -73,8 +72,8 @@ static void rows_launch(sml_krows * a, int hd, int type, hipStream_t st) {
     long items = split ? tiles + want : tiles;
     a->items = (int) items;
     a->part_cols = ncol < a->cols ? ncol : a->cols;
-    const int block = fm->cw >= 4 ? 64 : 32, bufs = fm->cw > 1 ? 2 : 1;
-    const size_t stages = (size_t) fm->pg * bufs * 4 * block * hd + 4 * fm->pg * bufs * block + 8 * fm->pg * bufs * fm->cw + 16 * fm->cw;
+    const int bufs = fm->cw == 1 ? 1 : fm->cw == 2 ? 2 : 3;
+    const size_t stages = (size_t) fm->pg * bufs * (4 * 32 * hd + 4 * 32 + 4 * fm->cw) + 16 * fm->cw;
     const size_t joined = fm->pg > 1 ? (size_t) fm->pg * fm->cols * ((hd + 4) * 4 + 8) : 0;
     char base[24], name[40];
     snprintf(base, sizeof base, "sml_rw_%s%s", fm->name, a->cap > 0.0f || a->slope ? "r" : "");

@@ -108,6 +108,7 @@ AXES(64, 1, sml_rw_append_d64_bf)
 // but cut to what a tile's rows see. Calls with tiles enough are not split, and
 // sequences past AT_SHARED neither; those tiles are found by halving.
 typedef short v4s __attribute__((ext_vector_type(4)));
+typedef float v16f __attribute__((ext_vector_type(16)));
 
 // What no column may see is read from here.
 __device__ const uint8_t rw_zeros[16] = { 0 };
@@ -131,6 +132,7 @@ __device__ __forceinline__ void copy_lds16(const void * base, uint32_t off, cons
 }
 #pragma clang diagnostic pop
 
+#define RW_WEAVE 6               // vector instructions beside a matrix instruction
 struct rows_of { int s0, m, n; };                     // a sequence's first row, its rows and its positions
 __device__ __forceinline__ rows_of rows_seq(const sml_krows & a, int b) {
     rows_of x;
@@ -149,14 +151,17 @@ __device__ __forceinline__ float wave_total(float v) {
     return (__builtin_bit_cast(float, __builtin_amdgcn_readlane(x, 15)) + __builtin_bit_cast(float, __builtin_amdgcn_readlane(x, 31))) +
            (__builtin_bit_cast(float, __builtin_amdgcn_readlane(x, 47)) + __builtin_bit_cast(float, __builtin_amdgcn_readlane(x, 63)));
 }
-// The least and the largest of 16 lanes, in each of them.
-__device__ __forceinline__ int least16(int v) {
-    v = min(v, dpp_i<0xB1>(v)); v = min(v, dpp_i<0x4E>(v)); v = min(v, dpp_i<0x141>(v)); return min(v, dpp_i<0x140>(v));
+// The least and the largest of the first 32 lanes.
+__device__ __forceinline__ int least32(int v) {
+    v = min(v, dpp_i<0xB1>(v)); v = min(v, dpp_i<0x4E>(v)); v = min(v, dpp_i<0x141>(v)); v = min(v, dpp_i<0x140>(v));
+    return min(__builtin_amdgcn_readlane(v, 0), __builtin_amdgcn_readlane(v, 16));
 }
-__device__ __forceinline__ int most16(int v) {
-    v = max(v, dpp_i<0xB1>(v)); v = max(v, dpp_i<0x4E>(v)); v = max(v, dpp_i<0x141>(v)); return max(v, dpp_i<0x140>(v));
+__device__ __forceinline__ int most32(int v) {
+    v = max(v, dpp_i<0xB1>(v)); v = max(v, dpp_i<0x4E>(v)); v = max(v, dpp_i<0x141>(v)); v = max(v, dpp_i<0x140>(v));
+    return max(__builtin_amdgcn_readlane(v, 0), __builtin_amdgcn_readlane(v, 16));
 }
 
+struct rows_block { int t, pa, pb; uint64_t aa, ab; };  // a step's start, a group's block's two pages and their places in a pool
 struct rows_at { int b, tile, count, split, item; rows_of sq; };  // a tile, its splits, this one's number, the first's among all items
 // Item i's (or, of TILES, tile i's) place; false past the last. Without splits
 // (want 0) sequence b's tiles are numbered from start[b] * rep / cols + b on, which
@@ -245,19 +250,16 @@ __device__ __forceinline__ float tanh_any(float y) {
     return fabsf(y) > 0.625f ? t : tanh_small(y);
 }
 
-// The parts of two weights, as parts_of makes them; fp16's remainder is one mixed
-// instruction each.
+// The parts of two weights, as parts_of makes them; fp16's remainders are a mixed
+// instruction each if the compiler does not know that m1 is -1.
 template <int BF>
-__device__ __forceinline__ void weights_of(float x, float y, typename Mx<BF>::v8 (&p)[Mx<BF>::parts], int e) {
+__device__ __forceinline__ void weights_of(float x, float y, float m1, typename Mx<BF>::v8 (&p)[Mx<BF>::parts], int e) {
     if constexpr (BF) parts_of<BF>(x, y, p, e);
     else {
         typedef _Float16 v2h __attribute__((ext_vector_type(2)));
         typedef float v2f __attribute__((ext_vector_type(2)));
         const v2h h = __builtin_convertvector(v2f{x, y}, v2h);
-        float r0, r1;
-        asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(r0) : "v"(h), "v"(x));
-        asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r1) : "v"(h), "v"(y));
-        const v2h l = __builtin_convertvector(v2f{r0, r1}, v2h);
+        const v2h l = __builtin_convertvector(v2f{__builtin_fmaf((float) h[0], m1, x), __builtin_fmaf((float) h[1], m1, y)}, v2h);
         p[0][e] = h[0];
         p[0][e + 1] = h[1];
         p[1][e] = l[0];
@@ -272,32 +274,41 @@ __device__ __forceinline__ uint32_t bits_range(int lo, int hi) {
     return lo < hi ? (~0u >> (32 - (hi - lo))) << lo : 0;
 }
 
-// A form of the rows' attention: CW waves beside each other, PG groups of them,
-// CB tiles of 16 columns a wave; the positions of a group's block and how many
-// stages of them it has, all stages' LDS, and where the groups' joined sums end.
-template <int D, int CW, int PG, int CB> struct RowsForm {
-    static constexpr int block = CW >= 4 ? 64 : 32, bufs = CW > 1 ? 2 : 1;
-    static constexpr int stages = PG * bufs * 4 * block * D;
-    static constexpr int joined = PG * 16 * CB * CW * (D + 4) * 4;
+// A form of the rows' attention: CW waves of 32 columns beside each other, PG groups of them; the stages of 32 positions that a group has (one
+// wave alone needs no more than one), all stages' LDS, and where the groups'
+// joined sums end.
+template <int D, int CW, int PG> struct RowsForm {
+    static constexpr int bufs = CW == 1 ? 1 : CW == 2 ? 2 : 3;
+    static constexpr int stages = PG * bufs * 4 * 32 * D;
+    static constexpr int joined = PG * 32 * CW * (D + 4) * 4;
 };
 
-// CW waves side by side take 16 CB CW columns; PG such groups take the blocks of a
+template <int BF> struct Mx32;
+template <> struct Mx32<0> {
+    static __device__ __forceinline__ v16f mul(Mx<0>::v8 a, Mx<0>::v8 b, v16f c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+};
+template <> struct Mx32<1> {
+    static __device__ __forceinline__ v16f mul(Mx<1>::v8 a, Mx<1>::v8 b, v16f c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+};
+
+// CW waves side by side take 32 CW columns; PG such groups take the blocks of a
 // split in turn and are joined in LDS at the end.
-template <int D, int BF, int CW, int PG, int CB, bool RULES>
+template <int D, int BF, int CW, int PG, bool RULES>
 __device__ __forceinline__ void rows_body(const sml_krows & a) {
     using M = Mx<BF>;
+    using MM = Mx32<BF>;
     typedef typename M::v8 v8;
-    using F = RowsForm<D, CW, PG, CB>;
-    constexpr int NJ = D / 32, E = D / 16, NP = M::parts, RB = 2 * D, W = CW * PG, KB = F::block, POOL = KB * RB, STAGE = 2 * POOL;
+    using F = RowsForm<D, CW, PG>;
+    constexpr int NJ = D / 16, E = D / 32, NP = M::parts, RB = 2 * D, W = CW * PG, KB = 32, POOL = KB * RB, STAGE = 2 * POOL;
     constexpr int RC = 1024 / RB, NC = KB / RC / CW;  // rows of a copy, a wave's copies of a block's keys
     static_assert(NC >= 1 && RC <= 16, "");
     extern __shared__ __align__(16) uint8_t lds[];    // the groups' stages; their new rows' positions, positions whose V is not finite, ranges
-    const int kh = blockIdx.x, tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
+    const int kh = blockIdx.x, tid = threadIdx.x, lane = tid & 63, c = lane & 31, g = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), cw = wave % CW, pgi = wave / CW;
     uint8_t * const stages = lds + pgi * F::bufs * STAGE;
     int * const kpos = (int *) (lds + F::stages) + pgi * F::bufs * KB;
-    uint64_t * const found = (uint64_t *) (lds + F::stages + 4 * PG * F::bufs * KB) + pgi * F::bufs * CW;
-    int * const red = (int *) (lds + F::stages + 4 * PG * F::bufs * KB + 8 * PG * F::bufs * CW);
+    uint32_t * const found = (uint32_t *) (lds + F::stages + 4 * PG * F::bufs * KB) + pgi * F::bufs * CW;
+    int * const red = (int *) (lds + F::stages + 4 * PG * F::bufs * (KB + CW));
     rows_at p;
     if (!rows_place<false>(a, rows_item(), lane, p)) return;
     const rows_of sq = p.sq;
@@ -305,39 +316,40 @@ __device__ __forceinline__ void rows_body(const sml_krows & a) {
     const int sh = a.pg.page_shift, pmask = (1 << sh) - 1;
     const int32_t * const tab = a.pg.table + (size_t) p.b * a.pg.seq_pages;
 
-    // the lane's columns: their rows' ranges, trees' bits and positions
-    int r[CB], h[CB], lo[CB], hi[CB], qpos[CB];
-    bool mine[CB], some[CB];                          // is there one, does it attend to anything
+    // the lane's column: its row's range, its tree's bits (if they are no more than 64) and its position
+    const int col = p.tile * a.cols + 32 * cw + c, in_seq = min(col, ncol - 1) / rep;
+    const bool mine = col < ncol;
+    const int r = sq.s0 + in_seq, h = kh * rep + (min(col, ncol - 1) - in_seq * rep);
+    const int lo = a.first ? max(a.first[r], 0) : 0;
+    const int hi = min(a.last ? a.last[r] : a.tree ? past : past + in_seq + 1, sq.n);
+    const int qpos = a.pos ? a.pos[r] : past + in_seq;
     const int nbit = a.tree ? min(sq.m, 32 * a.words) : 0;
+    uint64_t tw = 0;
+    if (nbit) {
+        const uint32_t * const bits = a.tree + (size_t) r * a.words;
+        tw = bits[0];
+        if (a.words > 1) tw |= (uint64_t) bits[1] << 32;
+    }
+    // the query: lane (c, g) holds dims 16j + 8g.. of column c
+    v4f x[2 * NJ];
+    {
+        const float * qp = a.q + (size_t) r * a.q_stride + (size_t) h * D + 8 * g;
+        #pragma unroll
+        for (int j = 0; j < 2 * NJ; j++) x[j] = *(const v4fu *) (qp + 16 * (j / 2) + 4 * (j % 2));
+    }
+    const bool range = lo < hi, tree = nbit && (tw || a.words > 2);
+    const bool some = mine && (range || tree);        // does it attend to anything
     // what any column of the wave, of the tile attends to lies in w_lo..w_hi, t_lo..t_hi;
     // every one that attends to anything has all of f_lo..f_hi (t_flo.. of the tile)
     int w_lo = 0x7fffffff, w_hi = 0, f_lo = 0, f_hi = 0x7fffffff, t_lo, t_hi, t_flo, t_fhi;
     {
-        #pragma unroll
-        for (int x = 0; x < CB; x++) {
-            const int col = p.tile * a.cols + 16 * (CB * cw + x) + c, i = min(col, ncol - 1) / rep;
-            mine[x] = col < ncol;
-            r[x] = sq.s0 + i;
-            h[x] = kh * rep + (min(col, ncol - 1) - i * rep);
-            lo[x] = a.first ? max(a.first[r[x]], 0) : 0;
-            hi[x] = min(a.last ? a.last[r[x]] : a.tree ? past : past + i + 1, sq.n);
-            qpos[x] = a.pos ? a.pos[r[x]] : past + i;
-            const bool range = lo[x] < hi[x];
-            bool tree = false;
-            if (nbit) {
-                if (a.words > 8) tree = true;
-                else
-                    for (int w = 0; w < a.words; w++) tree |= a.tree[(size_t) r[x] * a.words + w] != 0;
-            }
-            some[x] = mine[x] && (range || tree);
-            if (mine[x] && range) { w_lo = min(w_lo, lo[x]); w_hi = max(w_hi, hi[x]); }
-            if (mine[x] && tree && past + nbit > 0) { w_lo = min(w_lo, max(past, 0)); w_hi = max(w_hi, min(past + nbit, sq.n)); }
-            if (some[x]) { f_lo = max(f_lo, range ? lo[x] : 0x7fffffff); f_hi = min(f_hi, range ? hi[x] : 0); }
-        }
-        t_lo = w_lo = __builtin_amdgcn_readfirstlane(least16(w_lo));
-        t_hi = w_hi = __builtin_amdgcn_readfirstlane(most16(w_hi));
-        t_flo = f_lo = __builtin_amdgcn_readfirstlane(most16(f_lo));
-        t_fhi = f_hi = __builtin_amdgcn_readfirstlane(least16(f_hi));
+        if (mine && range) { w_lo = lo; w_hi = hi; }
+        if (mine && tree && past + nbit > 0) { w_lo = min(w_lo, max(past, 0)); w_hi = max(w_hi, min(past + nbit, sq.n)); }
+        if (some) { f_lo = range ? lo : 0x7fffffff; f_hi = range ? hi : 0; }
+        t_lo = w_lo = least32(w_lo);
+        t_hi = w_hi = most32(w_hi);
+        t_flo = f_lo = most32(f_lo);
+        t_fhi = f_hi = least32(f_hi);
         if constexpr (CW > 1) {
             if (!lane && !pgi) { red[4 * cw] = w_lo; red[4 * cw + 1] = w_hi; red[4 * cw + 2] = f_lo; red[4 * cw + 3] = f_hi; }
             __syncthreads();
@@ -353,14 +365,6 @@ __device__ __forceinline__ void rows_body(const sml_krows & a) {
             t_flo = __builtin_amdgcn_readfirstlane(t_flo);
             t_fhi = __builtin_amdgcn_readfirstlane(t_fhi);
         }
-    }
-    // the queries: lane (c, g) holds dims 32j + 8g.. of its columns
-    v4f x[CB][2 * NJ];
-    #pragma unroll
-    for (int y = 0; y < CB; y++) {
-        const float * qp = a.q + (size_t) r[y] * a.q_stride + (size_t) h[y] * D + 8 * g;
-        #pragma unroll
-        for (int j = 0; j < 2 * NJ; j++) x[y][j] = *(const v4fu *) (qp + 32 * (j / 2) + 4 * (j % 2));
     }
     // this split's blocks
     int t_at = 0, t_end = 0;
@@ -397,31 +401,42 @@ __device__ __forceinline__ void rows_body(const sml_krows & a) {
         }
         return t;
     };
-    auto page = [&](int t, int e) { return __builtin_amdgcn_readlane(ent, ((t - t_tab) >> 4) + pgi * (KB / 16) + e); };
+    // a group's block of the step at t: the pages of its two halves, and where these lie
+    auto locate = [&](int t) {
+        rows_block x = { t, -1, -1, 0, 0 };
+        if (t < t_end) {
+            const int i = ((t - t_tab) >> 4) + 2 * pgi;
+            x.pa = __builtin_amdgcn_readlane(ent, i);
+            x.pb = __builtin_amdgcn_readlane(ent, i + 1);
+            x.aa = (uint64_t) (uint32_t) __builtin_amdgcn_readlane((int) (at_ent >> 32), i) << 32 | (uint32_t) __builtin_amdgcn_readlane((int) at_ent, i);
+            x.ab = (uint64_t) (uint32_t) __builtin_amdgcn_readlane((int) (at_ent >> 32), i + 1) << 32 | (uint32_t) __builtin_amdgcn_readlane((int) at_ent, i + 1);
+        }
+        return x;
+    };
     // A lane of a copy: its row and its word there; word w of row x lies at w ^ swz(x).
-    auto swz = [](int x) { return D == 128 ? 2 * (x & 7) : (x >> 1) & 7; };
+    // (A row's words fill its bytes to the power of two, so that another copy's
+    // swizzle is an exclusive or of the offset.)
+    auto swz_k = [](int x) { return D == 128 ? x & 15 : (x >> 1) & 7; };
+    auto swz_v = [](int x) { return D == 128 ? 2 * (x & 7) : (x >> 1) & 7; };
     const int crow = RC * cw + lane / (RB / 16), cword = lane % (RB / 16);
-    uint32_t coff[CW == 1 ? 2 : 1];                   // by the copy's oddness, where that changes the swizzle
-    #pragma unroll
-    for (int e = 0; e < (CW == 1 ? 2 : 1); e++) coff[e] = 2u * (uint32_t) ((crow & 15) * kvd + 8 * (cword ^ swz(RC * e + crow)));
-    auto fetch = [&](uint8_t * st, const uint16_t * pool, int t) {
-        const int i0 = ((t - t_tab) >> 4) + pgi * (KB / 16), from = t + pgi * KB;
-        constexpr uint64_t MASK = (1ull << (KB / 16)) - 1;
-        if ((~__ballot(ent >= 0) >> i0 & MASK) == 0 && from >= t_lo && from + KB <= t_hi) {
+    const uint32_t koff = 2u * (uint32_t) ((crow & 15) * kvd + 8 * (cword ^ swz_k(crow)));
+    const uint32_t voff = 2u * (uint32_t) ((crow & 15) * kvd + 8 * (cword ^ swz_v(crow)));
+    auto fetch = [&](uint8_t * st, bool values, const rows_block & x) {
+        const int from = x.t + pgi * KB;
+        const uint8_t * const pool = (const uint8_t *) (values ? a.pg.v : a.pg.k);
+        if (x.pa >= 0 && x.pb >= 0 && from >= t_lo && from + KB <= t_hi) {
             #pragma unroll
             for (int e = 0; e < NC; e++) {
-                const int row0 = RC * (CW * e + cw), i = i0 + (row0 >> 4);
-                const uint64_t at = (uint64_t) (uint32_t) __builtin_amdgcn_readlane((int) (at_ent >> 32), i) << 32 | (uint32_t) __builtin_amdgcn_readlane((int) at_ent, i);
-                copy_lds16((const uint8_t *) pool + at + (uint32_t) (2 * ((RC * CW * e) & 15) * kvd), coff[CW == 1 ? e & 1 : 0], st + row0 * RB);
+                const int row0 = RC * (CW * e + cw), turn = 16 * (values ? swz_v(RC * CW * e) : swz_k(RC * CW * e));
+                copy_lds16(pool + (row0 < 16 ? x.aa : x.ab) + (uint32_t) (2 * ((RC * CW * e) & 15) * kvd), (values ? voff : koff) ^ turn, st + row0 * RB);
             }
         } else {
             #pragma unroll 1
             for (int e = 0; e < NC; e++) {
-                const int row0 = RC * (CW * e + cw), row = RC * CW * e + crow, i = i0 + (row0 >> 4), pos = from + row;
-                const uint64_t at = (uint64_t) (uint32_t) __builtin_amdgcn_readlane((int) (at_ent >> 32), i) << 32 | (uint32_t) __builtin_amdgcn_readlane((int) at_ent, i);
-                const bool in = __builtin_amdgcn_readlane(ent, i) >= 0 && pos >= t_lo && pos < t_hi;
-                const uint8_t * p8 = (const uint8_t *) pool + at + 2u * (uint32_t) ((row & 15) * kvd + 8 * (cword ^ swz(row)));
-                copy_lds16(in ? (const void *) p8 : (const void *) rw_zeros, st + row0 * RB);
+                const int row0 = RC * (CW * e + cw), row = RC * CW * e + crow, pos = from + row;
+                const bool in = (row0 < 16 ? x.pa : x.pb) >= 0 && pos >= t_lo && pos < t_hi;
+                const uint8_t * at = pool + (row0 < 16 ? x.aa : x.ab) + 2u * (uint32_t) ((row & 15) * kvd + 8 * (cword ^ (values ? swz_v(row) : swz_k(row))));
+                copy_lds16(in ? (const void *) at : (const void *) rw_zeros, st + row0 * RB);
             }
         }
     };
@@ -434,52 +449,49 @@ __device__ __forceinline__ void rows_body(const sml_krows & a) {
     auto keep_pos = [&](int * kp) {
         if (RULES && a.slope && a.pos && cw == 0 && lane < KB) kp[lane] = at_pos;
     };
-    int t = seek(t_at), buf = 0;
-    if (t < t_end) {
-        fetch(stages, a.pg.k, t);
-        fetch(stages + POOL, a.pg.v, t);
-        fetch_pos(t);
+    rows_block b0 = locate(seek(t_at));
+    if (b0.t < t_end) {
+        fetch(stages, false, b0);
+        fetch(stages + POOL, true, b0);
+        fetch_pos(b0.t);
     }
 
-    // the queries in parts
-    v8 q[CB][NJ][NP];
-    float back[CB], slope[CB];                        // what a product of the scaled q is multiplied by
-    #pragma unroll
-    for (int y = 0; y < CB; y++) {
+    // the query in parts
+    v8 q[NJ][NP];
+    float back;                                       // what a product of the scaled q is multiplied by
+    {
         float mx = 0.0f;
         #pragma unroll
         for (int j = 0; j < 2 * NJ; j++)
             #pragma unroll
-            for (int k = 0; k < 4; k++) { x[y][j][k] = mine[y] ? x[y][j][k] * a.sign : 0.0f; mx = fmaxf(mx, fabsf(x[y][j][k])); }
-        mx = fmaxf(mx, __shfl_xor(mx, 16));
+            for (int k = 0; k < 4; k++) { x[j][k] = mine ? x[j][k] * a.sign : 0.0f; mx = fmaxf(mx, fabsf(x[j][k])); }
         mx = fmaxf(mx, __shfl_xor(mx, 32));
         const int ex = BF ? 0 : scale_of(mx);
         #pragma unroll
         for (int j = 0; j < NJ; j++)
             #pragma unroll
             for (int e = 0; e < 8; e += 2)
-                parts_of<BF>(__builtin_amdgcn_ldexpf(x[y][2 * j + e / 4][e % 4], -ex), __builtin_amdgcn_ldexpf(x[y][2 * j + e / 4][e % 4 + 1], -ex), q[y][j], e);
-        back[y] = __builtin_amdgcn_ldexpf(a.scale, ex);
-        slope[y] = RULES && a.slope ? -1.44269504088896341f * a.slope[h[y]] : 0.0f;
+                parts_of<BF>(__builtin_amdgcn_ldexpf(x[2 * j + e / 4][e % 4], -ex), __builtin_amdgcn_ldexpf(x[2 * j + e / 4][e % 4 + 1], -ex), q[j], e);
+        back = __builtin_amdgcn_ldexpf(a.scale, ex);
     }
+    const float slope = RULES && a.slope ? -1.44269504088896341f * a.slope[h] : 0.0f;
+    const float f = RULES ? 1.0f : back;              // log2 weights are f times the settled scores
 
-    v4f o[CB][E];
-    float base[CB], l[CB];
+    v16f o[E];
     #pragma unroll
-    for (int y = 0; y < CB; y++) {
-        base[y] = -INFINITY;
-        l[y] = 0.0f;
+    for (int u = 0; u < E; u++)
         #pragma unroll
-        for (int u = 0; u < E; u++) o[y][u] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-    }
+        for (int e = 0; e < 16; e++) o[u][e] = 0.0f;
+    float base = -INFINITY, l = 0.0f;
 
-    const int krow = c * RB, kx = swz(c);
-    const int vrow = 4 * g + (c >> 2), vx = D == 128 ? vrow & 7 : (vrow >> 2) & 3;    // the V row this lane reads for its 16
-    const int vat = POOL + vrow * RB + (D == 128 ? 8 * (c & 3) : 16 * (((c >> 1) & 1) ^ ((vrow >> 1) & 1)) + 8 * (c & 1));
+    const int krow = c * RB, kx = swz_k(c);
+    // the V row that this lane reads for its 16, and its eight bytes there
+    const int vrow = 4 * g + ((lane & 15) >> 2), q16 = (lane >> 4) & 1;
+    const int vx = D == 128 ? vrow : g, vat = POOL + vrow * RB + (D == 128 ? 8 * (lane & 3) : 16 * (((lane >> 1) & 1) ^ ((lane >> 3) & 1)) + 8 * (lane & 1));
     // Values that are not finite among those that this wave has fetched, where columns
     // differ: zeros in their place; their positions in the block.
     auto screen = [&](uint8_t * st) {
-        uint64_t bad = 0;
+        uint32_t bad = 0;
         #pragma unroll 1
         for (int e = 0; e < NC; e++) {
             const int row0 = RC * (CW * e + cw);
@@ -497,273 +509,344 @@ __device__ __forceinline__ void rows_body(const sml_krows & a) {
                 *at = x;
                 #pragma unroll 1
                 for (int k = 0; k < RC; k++)
-                    if (hit >> (64 / RC * k) & ((1ull << (64 / RC)) - 1)) bad |= 1ull << (row0 + k);
+                    if (hit >> (64 / RC * k) & ((1ull << (64 / RC)) - 1)) bad |= 1u << (row0 + k);
             }
         }
         return bad;
     };
 
-    // 32 positions from t on, rows row0.. of stage st, whose pages are pa and pb: the scores, then the weights and the sums.
-    auto products = [&](const uint8_t * st, int row0, v4f (&s)[CB][2], auto && loaded) {
-        v8 ka[2][NJ];
+    float m1;
+    asm("v_mov_b32 %0, -1.0" : "=v"(m1));
+    // A block's keys in registers; the scores; a tile's dims of 16 positions' values; the sums.
+    auto keys = [&](const uint8_t * st, v8 (&ka)[NJ]) {
         #pragma unroll
-        for (int j = 0; j < 2; j++)
-            #pragma unroll
-            for (int e = 0; e < NJ; e++) ka[j][e] = *(const v8 *) (st + (row0 + 16 * j) * RB + krow + 16 * ((4 * e + g) ^ kx));
-        __builtin_amdgcn_sched_barrier(0);
-        loaded();
-        #pragma unroll
-        for (int j = 0; j < 2; j++) {
-            #pragma unroll
-            for (int y = 0; y < CB; y++) s[y][j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-            #pragma unroll
-            for (int e = 0; e < NJ; e++)
-                #pragma unroll
-                for (int k = 0; k < NP; k++)
-                    #pragma unroll
-                    for (int y = 0; y < CB; y++) s[y][j] = M::mul(ka[j][e], q[y][e][k], s[y][j]);
-        }
-        __builtin_amdgcn_sched_barrier(0);
+        for (int e = 0; e < NJ; e++) ka[e] = *(const v8 *) (st + krow + 16 * ((2 * e + g) ^ kx));
     };
-    auto value = [&](const uint8_t * st, int row0, int u) {
+    auto products = [&](const v8 (&ka)[NJ]) {
+        v16f s;
+        #pragma unroll
+        for (int e = 0; e < 16; e++) s[e] = 0.0f;
+        #pragma unroll
+        for (int e = 0; e < NJ; e++)
+            #pragma unroll
+            for (int k = 0; k < NP; k++) s = MM::mul(ka[e], q[e][k], s);
+        return s;
+    };
+    auto value = [&](const uint8_t * st, int u, int k) {
         typedef __attribute__((address_space(3))) v4s lv4s;
-        const uint8_t * vr = st + vat + row0 * RB + ((u ^ vx) << 5);
-        const v4s x0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lv4s *) vr);
-        const v4s x1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lv4s *) (vr + 16 * RB));
+        const uint8_t * const vr = st + vat + 16 * k * RB;
+        const v4s x0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lv4s *) (vr + (((2 * u + q16) ^ vx) << 5)));
+        const v4s x1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lv4s *) (vr + 8 * RB + (((2 * u + q16) ^ (D == 128 ? vx : vx | 2)) << 5)));
         return __builtin_bit_cast(v8, __builtin_shufflevector(x0, x1, 0, 1, 2, 3, 4, 5, 6, 7));
     };
-    auto weigh = [&](v4f (&s)[CB][2], v8 (&w)[CB][NP], const int * kp, int t, int pa, int pb, uint32_t bad) {
-        const bool whole = pa >= 0 && pb >= 0 && t >= f_lo && t + 32 <= f_hi;
+    auto sums = [&](const v8 & vv, int u, const v8 (&w)[NP]) {
         #pragma unroll
-        for (int y = 0; y < CB; y++) {
-            float f = back[y];                        // log2 weights are f times the scores
-            if constexpr (RULES) {
-                f = 1.0f;
-                float top = 0.0f;
-                #pragma unroll
-                for (int j = 0; j < 2; j++)
-                    #pragma unroll
-                    for (int e = 0; e < 4; e++) { s[y][j][e] *= back[y]; top = fmaxf(top, fabsf(s[y][j][e])); }
-                if (a.cap > 0.0f) {
-                    if (__any(!(top <= 0.625f))) {
-                        #pragma unroll
-                        for (int j = 0; j < 2; j++)
-                            #pragma unroll
-                            for (int e = 0; e < 4; e++) s[y][j][e] = a.cap * tanh_any(s[y][j][e]);
-                    } else {
-                        #pragma unroll
-                        for (int j = 0; j < 2; j++)
-                            #pragma unroll
-                            for (int e = 0; e < 4; e++) s[y][j][e] = a.cap * tanh_small(s[y][j][e]);
-                    }
-                }
-                if (a.slope) {
-                    const float d0 = (float) (t + 4 * g - qpos[y]);
-                    if (a.pos && t + 32 > past) {
-                        #pragma unroll
-                        for (int j = 0; j < 2; j++)
-                            #pragma unroll
-                            for (int e = 0; e < 4; e++) {
-                                const int x = 16 * j + 4 * g + e;
-                                const float d = t + x >= past ? (float) (kp[x] - qpos[y]) : d0 + (float) (16 * j + e);
-                                s[y][j][e] = __builtin_fmaf(slope[y], fabsf(d), s[y][j][e]);
-                            }
-                    } else {
-                        #pragma unroll
-                        for (int j = 0; j < 2; j++)
-                            #pragma unroll
-                            for (int e = 0; e < 4; e++) s[y][j][e] = __builtin_fmaf(slope[y], fabsf(d0 + (float) (16 * j + e)), s[y][j][e]);
-                    }
-                }
-            }
-            if (!whole) {
-                uint32_t vm = bits_range(lo[y] - t, hi[y] - t);
-                const int j0 = t - past;
-                if (nbit && j0 + 32 > 0 && j0 < nbit) {
-                    const uint32_t * const bits = a.tree + (size_t) r[y] * a.words;
-                    const int w0 = j0 >> 5;           // bits 32 w0.. of the row, 64 of them
-                    const uint32_t x0 = w0 >= 0 && w0 < a.words ? bits[w0] : 0u, x1 = w0 + 1 >= 0 && w0 + 1 < a.words ? bits[w0 + 1] : 0u;
-                    vm |= (uint32_t) (((uint64_t) x1 << 32 | x0) >> (j0 & 31)) & bits_range(-j0, nbit - j0);
-                }
-                vm &= bits_range(0, sq.n - t);
-                if (pa < 0) vm &= 0xFFFF0000u;
-                if (pb < 0) vm &= 0x0000FFFFu;
-                if (!some[y]) vm = 0;
-                if (vm & bad) l[y] = NAN;
-                vm >>= 4 * g;
-                #pragma unroll
-                for (int j = 0; j < 2; j++)
-                    #pragma unroll
-                    for (int e = 0; e < 4; e++) s[y][j][e] = (vm >> (16 * j + e)) & 1 ? s[y][j][e] : -INFINITY;
-            } else if (bad) {
-                l[y] = NAN;
-            }
-            float mx = -INFINITY;
+        for (int y = 0; y < NP; y++) o[u] = MM::mul(vv, w[y], o[u]);
+    };
+    // Scores of positions t.., whose pages are pa and pb, under the rules and the
+    // masks; the base that their weights have. Score e is position at(e) + 4g.
+    auto at = [](int e) { return 8 * (e >> 2) + (e & 3); };
+    auto settle = [&](v16f & s, const int * kp, int t, int pa, int pb, uint32_t bad) {
+        if constexpr (RULES) {
+            float top = 0.0f;
             #pragma unroll
-            for (int j = 0; j < 2; j++)
-                #pragma unroll
-                for (int e = 0; e < 4; e++) mx = fmaxf(mx, s[y][j][e]);
-            mx *= f;
-            if (__any(mx > base[y] + M::room)) {
-                mx = fmaxf(mx, __shfl_xor(mx, 16));
-                mx = fmaxf(mx, __shfl_xor(mx, 32));
-                const float to = mx > base[y] + M::room ? mx + M::lift : base[y];
-                const float al = __builtin_amdgcn_exp2f(base[y] - (to == -INFINITY ? 0.0f : to));
-                l[y] *= al;
-                #pragma unroll
-                for (int u = 0; u < E; u++)
+            for (int e = 0; e < 16; e++) { s[e] *= back; top = fmaxf(top, fabsf(s[e])); }
+            if (a.cap > 0.0f) {
+                if (__any(!(top <= 0.625f))) {
                     #pragma unroll
-                    for (int e = 0; e < 4; e++) o[y][u][e] *= al;
-                base[y] = to;
-            }
-            const float bu = base[y] == -INFINITY ? 0.0f : base[y];
-            #pragma unroll
-            for (int j = 0; j < 2; j++)
-                #pragma unroll
-                for (int e = 0; e < 4; e += 2) {
-                    const float w0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[y][j][e], f, -bu));
-                    const float w1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[y][j][e + 1], f, -bu));
-                    l[y] += w0;
-                    l[y] += w1;
-                    weights_of<BF>(w0, w1, w[y], 4 * j + e);
+                    for (int e = 0; e < 16; e++) s[e] = a.cap * tanh_any(s[e]);
+                } else {
+                    #pragma unroll
+                    for (int e = 0; e < 16; e++) s[e] = a.cap * tanh_small(s[e]);
                 }
+            }
+            if (a.slope) {
+                const float d0 = (float) (t + 4 * g - qpos);
+                if (a.pos && t + 32 > past) {
+                    #pragma unroll
+                    for (int e = 0; e < 16; e++) {
+                        const int y = at(e) + 4 * g;
+                        const float d = t + y >= past ? (float) (kp[y] - qpos) : d0 + (float) at(e);
+                        s[e] = __builtin_fmaf(slope, fabsf(d), s[e]);
+                    }
+                } else {
+                    #pragma unroll
+                    for (int e = 0; e < 16; e++) s[e] = __builtin_fmaf(slope, fabsf(d0 + (float) at(e)), s[e]);
+                }
+            }
+        }
+        if (pa < 0 || pb < 0 || t < f_lo || t + 32 > f_hi) {
+            uint32_t vm = bits_range(lo - t, hi - t);
+            const int j0 = t - past;
+            if (nbit && j0 + 32 > 0 && j0 < nbit) {
+                uint64_t y = tw;
+                const int w0 = j0 >> 5;               // bits 32 w0.. of the row, 64 of them
+                if (a.words > 2) {
+                    const uint32_t * const bits = a.tree + (size_t) r * a.words;
+                    y = (uint64_t) (w0 + 1 >= 0 && w0 + 1 < a.words ? bits[w0 + 1] : 0u) << 32 | (w0 >= 0 && w0 < a.words ? bits[w0] : 0u);
+                } else if (w0) {
+                    y = w0 == -1 ? y << 32 : w0 == 1 ? y >> 32 : 0;
+                }
+                vm |= (uint32_t) (y >> (j0 & 31)) & bits_range(-j0, nbit - j0);
+            }
+            vm &= bits_range(0, sq.n - t);
+            if (pa < 0) vm &= 0xFFFF0000u;
+            if (pb < 0) vm &= 0x0000FFFFu;
+            if (!some) vm = 0;
+            if (vm & bad) l = NAN;
+            vm >>= 4 * g;
+            #pragma unroll
+            for (int e = 0; e < 16; e++) s[e] = (vm >> at(e)) & 1 ? s[e] : -INFINITY;
+        } else if (bad) {
+            l = NAN;
+        }
+        float mx = -INFINITY;
+        #pragma unroll
+        for (int e = 0; e < 16; e++) mx = fmaxf(mx, s[e]);
+        mx *= f;
+        if (__any(mx > base + M::room)) {
+            mx = fmaxf(mx, __shfl_xor(mx, 32));
+            const float to = mx > base + M::room ? mx + M::lift : base;
+            const float al = __builtin_amdgcn_exp2f(base - (to == -INFINITY ? 0.0f : to));
+            l *= al;
+            #pragma unroll
+            for (int u = 0; u < E; u++)
+                #pragma unroll
+                for (int e = 0; e < 16; e++) o[u][e] *= al;
+            base = to;
         }
     };
-    auto sums = [&](const v8 & vv, int u, const v8 (&w)[CB][NP]) {
+    auto weights = [&](const v16f & s, v8 (&w)[2][NP]) {
+        const float bu = base == -INFINITY ? 0.0f : base;
         #pragma unroll
-        for (int k = 0; k < NP; k++)
-            #pragma unroll
-            for (int y = 0; y < CB; y++) o[y][u] = M::mul(vv, w[y][k], o[y][u]);
+        for (int e = 0; e < 16; e += 2) {
+            const float w0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], f, -bu)), w1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e + 1], f, -bu));
+            l += w0;
+            l += w1;
+            weights_of<BF>(w0, w1, m1, w[e >> 3], e & 7);
+        }
+    };
+    // One matrix instruction, then what the vector unit does meanwhile.
+    auto woven = [&]() {
+        #pragma unroll
+        for (int k = 0; k < NJ * NP; k++) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x402, RW_WEAVE, 0);
+        }
     };
 
-    // Values are on their way to registers while the weights are made, if those hold
-    // them all (bfloat16's parts leave room for half).
-    constexpr int EARLY = BF && CB == 2 ? E / 2 : E;
-    while (t < t_end) {
-        const int cur = t + pgi * KB;
-        int pg[KB / 16];
-        #pragma unroll
-        for (int e = 0; e < KB / 16; e++) pg[e] = page(t, e);
-        const int tn = seek(t + STEP);
-        const bool differ = cur < t_flo || cur + KB > t_fhi;
-        if constexpr (CW == 1) {
-            // One stage, the wave's own: a block's keys are fetched over the last one's
-            // when those are in registers, its values likewise.
-            const bool on = cur < t_end && cur < w_hi && cur + KB > w_lo;
-            v4f s[CB][2];
-            v8 w[CB][NP], vv[EARLY];
+    // A step makes the next block's scores (sn) while it turns this one's (s) into weights.
+    v16f s, sn;
+    v8 ka[NJ], w[2][NP];
+    rows_block b1 = locate(seek(b0.t + STEP));        // the next block; b2: the one behind it
+    if constexpr (CW == 1) {
+        // One stage, the wave's own: keys are fetched over the last block's when those
+        // are in registers, values likewise.
+        if (b0.t < t_end) {
             asm volatile("s_waitcnt vmcnt(%0)" :: "n"(NC) : "memory");
-            products(stages, 0, s, [&]() {
-                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-                if (tn < t_end) fetch(stages, a.pg.k, tn);
-            });
-            if (tn < t_end) asm volatile("s_waitcnt vmcnt(%0)" :: "n"(NC) : "memory");
-            else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            keep_pos(kpos);
-            uint64_t bad = 0;
-            if (differ) bad = screen(stages);
-            #pragma unroll
-            for (int u = 0; u < EARLY; u++) vv[u] = value(stages, 0, u);
-            __builtin_amdgcn_sched_barrier(0);
-            if (on) {
-                weigh(s, w, kpos, cur, pg[0], pg[1], (uint32_t) bad);
-                #pragma unroll
-                for (int u = 0; u < E - EARLY; u++) {
-                    sums(vv[u], u, w);
-                    vv[u] = value(stages, 0, u + EARLY);
-                }
-            }
+            keys(stages, ka);
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-            if (tn < t_end) {
-                fetch(stages + POOL, a.pg.v, tn);
-                fetch_pos(tn);
+            if (b1.t < t_end) fetch(stages, false, b1);
+            s = products(ka);
+        }
+        bool first = true;
+        while (b0.t < t_end) {
+            const int cur = b0.t + pgi * KB;
+            const bool more = b1.t < t_end;
+            uint32_t bad = 0;
+            if (cur < t_flo || cur + KB > t_fhi) {
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                keep_pos(kpos);
+                bad = screen(stages);
+            } else {
+                keep_pos(kpos);
             }
-            if (on) {
-                #pragma unroll
-                for (int u = E - EARLY; u < E; u++) sums(vv[u % EARLY], u, w);
+            settle(s, kpos, cur, b0.pa, b0.pb, bad);
+            const rows_block b2 = more ? locate(seek(b1.t + STEP)) : b1;
+            if (more) {
+                // the next keys: behind this block's values in the first step, before them then
+                if (first) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                else asm volatile("s_waitcnt vmcnt(%0)" :: "n"(NC) : "memory");
+                keys(stages, ka);
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                if (b2.t < t_end) fetch(stages, false, b2);
+                sn = products(ka);
+                weights(s, w);
+                woven();
+            } else {
+                weights(s, w);
             }
-        } else {
-            uint8_t * const st = stages + buf * STAGE;
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");     // this wave's rows of the block are in LDS
-            keep_pos(kpos + buf * KB);
+            if (b2.t < t_end) asm volatile("s_waitcnt vmcnt(%0)" :: "n"(NC) : "memory");
+            else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            v8 vv[2 * E];
+            #pragma unroll
+            for (int u = 0; u < 2 * E; u++) vv[u] = value(stages, u % E, u / E);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            if (more) {
+                fetch(stages + POOL, true, b1);
+                fetch_pos(b1.t);
+            }
+            #pragma unroll
+            for (int u = 0; u < 2 * E; u++) sums(vv[u], u % E, w[u / E]);
+            s = sn;
+            b0 = b1;
+            b1 = b2;
+            first = false;
+        }
+    } else if constexpr (CW == 2) {
+        // Two stages, one in use and one that is filled.
+        int i0 = 0;
+        while (b0.t < t_end) {
+            const int cur = b0.t + pgi * KB;
+            uint8_t * const st = stages + i0 * STAGE;
+            const bool differ = cur < t_flo || cur + KB > t_fhi;
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            keep_pos(kpos + i0 * KB);
             if (differ) {
-                const uint64_t bad = screen(st);
-                if (!lane) found[buf * CW + cw] = bad;
+                const uint32_t bad = screen(st);
+                if (!lane) found[i0 * CW + cw] = bad;
+            }
+            __syncthreads();                          // the block is whole, and nobody reads the last one
+            if (b1.t < t_end) {
+                fetch(stages + (i0 ^ 1) * STAGE, false, b1);
+                fetch(stages + (i0 ^ 1) * STAGE + POOL, true, b1);
+                fetch_pos(b1.t);
+            }
+            const rows_block b2 = b1.t < t_end ? locate(seek(b1.t + STEP)) : b1;
+            keys(st, ka);
+            __builtin_amdgcn_sched_barrier(0);
+            s = products(ka);
+            __builtin_amdgcn_sched_barrier(0);
+            v8 vv[E];
+            #pragma unroll
+            for (int u = 0; u < E; u++) vv[u] = value(st, u, 0);
+            __builtin_amdgcn_sched_barrier(0);
+            uint32_t bad = 0;
+            if (differ) {
+                #pragma unroll
+                for (int y = 0; y < CW; y++) bad |= found[i0 * CW + y];
+            }
+            settle(s, kpos + i0 * KB, cur, b0.pa, b0.pb, bad);
+            weights(s, w);
+            #pragma unroll
+            for (int u = 0; u < 2 * E; u++) {
+                sums(vv[u % E], u % E, w[u / E]);
+                if (u < E) vv[u] = value(st, u, 1);
+            }
+            b0 = b1;
+            b1 = b2;
+            i0 ^= 1;
+        }
+    } else {
+        // Three stages: one whose values are in use, the next block's, and one that is filled.
+        int i0 = 0;
+        auto noted = [&](int i, int cur) {            // what the wave has fetched of stage i is there
+            keep_pos(kpos + i * KB);
+            uint32_t bad = 0;
+            if (cur < t_flo || cur + KB > t_fhi) bad = screen(stages + i * STAGE);
+            if (!lane) found[i * CW + cw] = bad;
+        };
+        if (b0.t < t_end) {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            noted(0, b0.t + pgi * KB);
+            if (b1.t < t_end) {
+                fetch(stages + STAGE, false, b1);
+                fetch(stages + STAGE + POOL, true, b1);
+                fetch_pos(b1.t);
             }
             __syncthreads();
-            if (tn < t_end) {                                    // past the barrier: nobody reads the last block
-                fetch(stages + (buf ^ 1) * STAGE, a.pg.k, tn);
-                fetch(stages + (buf ^ 1) * STAGE + POOL, a.pg.v, tn);
-                fetch_pos(tn);
-            }
-            #pragma unroll 1
-            for (int e = 0; e < KB / 32; e++) {
-                const int te = cur + 32 * e;
-                if (te >= t_end || te >= w_hi || te + 32 <= w_lo) continue;
-                v4f s[CB][2];
-                v8 w[CB][NP], vv[EARLY];
-                uint64_t bad = 0;
-                products(st, 32 * e, s, []() {});
-                #pragma unroll
-                for (int u = 0; u < EARLY; u++) vv[u] = value(st, 32 * e, u);
-                __builtin_amdgcn_sched_barrier(0);
-                if (differ) {
-                    #pragma unroll
-                    for (int x = 0; x < CW; x++) bad |= found[buf * CW + x];
-                }
-                weigh(s, w, kpos + buf * KB + 32 * e, te, e ? pg[KB / 16 - 2] : pg[0], e ? pg[KB / 16 - 1] : pg[1], (uint32_t) (bad >> (32 * e)));
-                #pragma unroll
-                for (int u = 0; u < E; u++) {
-                    sums(vv[u % EARLY], u, w);
-                    if (u + EARLY < E) vv[u % EARLY] = value(st, 32 * e, u + EARLY);
-                }
-            }
+            keys(stages, ka);
+            s = products(ka);
         }
-        t = tn;
-        buf ^= 1;
+        while (b0.t < t_end) {
+            const int cur = b0.t + pgi * KB, i1 = i0 == 2 ? 0 : i0 + 1, i2 = i1 == 2 ? 0 : i1 + 1;
+            const bool more = b1.t < t_end;
+            const uint8_t * const st = stages + i0 * STAGE;
+            uint32_t bad = 0;
+            if (cur < t_flo || cur + KB > t_fhi) {
+                #pragma unroll
+                for (int y = 0; y < CW; y++) bad |= found[i0 * CW + y];
+            }
+            settle(s, kpos + i0 * KB, cur, b0.pa, b0.pb, bad);
+            const rows_block b2 = more ? locate(seek(b1.t + STEP)) : b1;
+            if (more) {
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                noted(i1, b1.t + pgi * KB);
+                __syncthreads();                      // the next block is whole, and nobody reads the last one
+                if (b2.t < t_end) {
+                    fetch(stages + i2 * STAGE, false, b2);
+                    fetch(stages + i2 * STAGE + POOL, true, b2);
+                    fetch_pos(b2.t);
+                }
+                keys(stages + i1 * STAGE, ka);
+                sn = products(ka);
+                weights(s, w);
+                woven();
+            } else {
+                weights(s, w);
+            }
+            v8 vv[4];
+            vv[0] = value(st, 0, 0);
+            vv[1] = value(st, 1, 0);
+            #pragma unroll
+            for (int u = 0; u < 2 * E; u += 2) {
+                if (u + 2 < 2 * E) {
+                    vv[(u + 2) & 3] = value(st, (u + 2) % E, (u + 2) / E);
+                    vv[(u + 3) & 3] = value(st, (u + 3) % E, (u + 3) / E);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+                #pragma unroll
+                for (int y = 0; y < NP; y++) {
+                    o[u % E] = MM::mul(vv[u & 3], w[u / E][y], o[u % E]);
+                    o[(u + 1) % E] = MM::mul(vv[(u + 1) & 3], w[u / E][y], o[(u + 1) % E]);
+                }
+            }
+            s = sn;
+            b0 = b1;
+            b1 = b2;
+            i0 = i1;
+        }
     }
 
-    #pragma unroll
-    for (int y = 0; y < CB; y++) {
-        l[y] += __shfl_xor(l[y], 16);
-        l[y] += __shfl_xor(l[y], 32);
-        if (!some[y]) { base[y] = -INFINITY; l[y] = 0.0f; }
-    }
+    l += __shfl_xor(l, 32);
+    if (!some) { base = -INFINITY; l = 0.0f; }
     if constexpr (PG == 1) {
-        #pragma unroll
-        for (int y = 0; y < CB; y++) {
-            if (!mine[y]) continue;
-            if (p.count == 1) {
-                float * const to = a.out + ((size_t) r[y] * a.n_head + h[y]) * D + 4 * g;
+        if (!mine) return;
+        if (p.count == 1) {
+            float * const to = a.out + ((size_t) r * a.n_head + h) * D + 4 * g;
+            #pragma unroll
+            for (int u = 0; u < E; u++)
                 #pragma unroll
-                for (int u = 0; u < E; u++) {
-                    v4f x;
+                for (int k = 0; k < 4; k++) {
+                    v4f y;
                     #pragma unroll
-                    for (int e = 0; e < 4; e++) x[e] = l[y] != 0.0f ? o[y][u][e] / l[y] : 0.0f;
-                    *(v4fu *) (to + 16 * u) = x;
+                    for (int e = 0; e < 4; e++) y[e] = l != 0.0f ? o[u][4 * k + e] / l : 0.0f;
+                    *(v4fu *) (to + 32 * u + 8 * k) = y;
                 }
-            } else {
-                const int pc = 16 * (CB * cw + y) + c;
-                if (!g) part_ml(a, kh, p.item + p.split, D)[pc] = make_float2(base[y], l[y]);
-                float * const to = part_o(a, kh, p.item + p.split, D) + (size_t) pc * D + 4 * g;
+        } else {
+            const int pc = 32 * cw + c;
+            if (!g) part_ml(a, kh, p.item + p.split, D)[pc] = make_float2(base, l);
+            float * const to = part_o(a, kh, p.item + p.split, D) + (size_t) pc * D + 4 * g;
+            #pragma unroll
+            for (int u = 0; u < E; u++)
                 #pragma unroll
-                for (int u = 0; u < E; u++) *(v4f *) (to + 16 * u) = o[y][u];
-            }
+                for (int k = 0; k < 4; k++) *(v4f *) (to + 32 * u + 8 * k) = v4f{o[u][4 * k], o[u][4 * k + 1], o[u][4 * k + 2], o[u][4 * k + 3]};
         }
     } else {
         // The groups joined: their sums over the stages, rows of D + 4 floats on
         // different banks, their bases and weights' sums behind.
-        constexpr int QT = 16 * CB * CW, LD = D + 4;
+        constexpr int QT = 32 * CW, LD = D + 4;
         float * const so = (float *) lds;
         float2 * const sml = (float2 *) (lds + F::joined);
         __syncthreads();                              // all are done with the stages
-        #pragma unroll
-        for (int y = 0; y < CB; y++) {
-            const int pc = 16 * (CB * cw + y) + c;
+        {
+            const int pc = 32 * cw + c;
             float * const to = so + (size_t) (pgi * QT + pc) * LD + 4 * g;
             #pragma unroll
-            for (int u = 0; u < E; u++) *(v4f *) (to + 16 * u) = o[y][u];
-            if (!g) sml[pgi * QT + pc] = make_float2(base[y], l[y]);
+            for (int u = 0; u < E; u++)
+                #pragma unroll
+                for (int k = 0; k < 4; k++) *(v4f *) (to + 32 * u + 8 * k) = v4f{o[u][4 * k], o[u][4 * k + 1], o[u][4 * k + 2], o[u][4 * k + 3]};
+            if (!g) sml[pgi * QT + pc] = make_float2(base, l);
         }
         __syncthreads();
         for (int x = tid; x < QT * (D / 4); x += 64 * W) {
@@ -798,19 +881,18 @@ __device__ __forceinline__ void rows_body(const sml_krows & a) {
         }
     }
 }
-#define ROWS(D, BF, CW, PG, CB, EU, name, sfx) \
-    extern "C" __global__ __launch_bounds__(64 * CW * PG, EU) void name##sfx(const sml_krows a) { rows_body<D, BF, CW, PG, CB, false>(a); } \
-    extern "C" __global__ __launch_bounds__(64 * CW * PG, EU) void name##r##sfx(const sml_krows a) { rows_body<D, BF, CW, PG, CB, true>(a); }
-#define ROWS4(CW, PG, CB, E, name) \
-    ROWS(128, 0, CW, PG, CB, 2, name, ) \
-    ROWS(128, 1, CW, PG, CB, 2, name, _bf) \
-    ROWS(64, 0, CW, PG, CB, E, name, _d64) \
-    ROWS(64, 1, CW, PG, CB, E, name, _d64_bf)
-ROWS4(1, 8, 1, 4, sml_rw_rows16)
-ROWS4(1, 8, 2, 2, sml_rw_rows32)
-ROWS4(2, 4, 2, 2, sml_rw_rows64)
-ROWS4(4, 2, 2, 2, sml_rw_rows128)
-ROWS4(4, 1, 2, 3, sml_rw_rows128l)
+#define ROWS(D, BF, CW, PG, EU, name, sfx) \
+    extern "C" __global__ __launch_bounds__(64 * CW * PG, EU) void name##sfx(const sml_krows a) { rows_body<D, BF, CW, PG, false>(a); } \
+    extern "C" __global__ __launch_bounds__(64 * CW * PG, EU) void name##r##sfx(const sml_krows a) { rows_body<D, BF, CW, PG, true>(a); }
+#define ROWS4(CW, PG, E, name) \
+    ROWS(128, 0, CW, PG, 2, name, ) \
+    ROWS(128, 1, CW, PG, 2, name, _bf) \
+    ROWS(64, 0, CW, PG, E, name, _d64) \
+    ROWS(64, 1, CW, PG, E, name, _d64_bf)
+ROWS4(1, 8, 2, sml_rw_rows32)
+ROWS4(2, 4, 2, sml_rw_rows64)
+ROWS4(4, 2, 2, sml_rw_rows128)
+ROWS4(4, 1, 2, sml_rw_rows128l)
 
 // The splits of a tile joined, 16 columns a workgroup, 16 lanes a column: the
 // bases of its splits shared out over the lanes, then each lane's dims of every
