@@ -53,13 +53,12 @@ static void items_launch(const char * name, int n_kv, long items, unsigned threa
 }
 
 static const struct form { const char * name; int cols, cw, pg, per_cu; } forms[] = {
-    { "rows32", 32, 1, 8, 1 }, { "rows64", 64, 2, 4, 1 }, { "rows128", 128, 4, 2, 1 }, { "rows128l", 128, 4, 1, 2 },
+    { "rows64", 64, 2, 4, 1 }, { "rows128", 128, 4, 2, 1 },
 };
 static void rows_launch(sml_krows * a, int hd, int type, hipStream_t st) {
     const int n_kv = a->pg.n_kv, rep = a->n_head / n_kv, n_seq = a->pg.n_seq;
     const int ncol = a->n_row * rep, some = n_seq < a->n_row ? n_seq : a->n_row;
-    int f = 0;
-    while (f < 3 && ncol > (long) forms[f].cols * some) f++;
+    int f = ncol > 64L * some && ((long) ceil_div(ncol, 128) * n_kv >= hx.ncu || (long) ceil_div(ncol, 64) * n_kv < hx.ncu);
     if (getenv("RWF")) f = atoi(getenv("RWF"));
     const struct form * const fm = forms + f;
     a->cols = fm->cols;
@@ -72,14 +71,18 @@ static void rows_launch(sml_krows * a, int hd, int type, hipStream_t st) {
     long items = split ? tiles + want : tiles;
     a->items = (int) items;
     a->part_cols = ncol < a->cols ? ncol : a->cols;
-    const int bufs = fm->cw == 1 ? 1 : fm->cw == 2 ? 2 : 3;
-    const size_t stages = (size_t) fm->pg * bufs * (4 * 32 * hd + 4 * 32 + 4 * fm->cw) + 16 * fm->cw;
+    const size_t stages = (size_t) fm->pg * 2 * (4 * 32 * hd + 4 * 32 + 4 * fm->cw) + 16 * fm->cw;
     const size_t joined = fm->pg > 1 ? (size_t) fm->pg * fm->cols * ((hd + 4) * 4 + 8) : 0;
     char base[24], name[40];
     snprintf(base, sizeof base, "sml_rw_%s%s", fm->name, a->cap > 0.0f || a->slope ? "r" : "");
     sv_name(name, sizeof name, base, hd, type);
     items_launch(name, n_kv, items, 64 * (unsigned) (fm->cw * fm->pg), stages > joined ? stages : joined, st, a);
-    if (split) items_launch(hd == 64 ? "sml_rw_merge_d64" : "sml_rw_merge", n_kv, tiles * (a->cols / 16), 256, 0, st, a);
+    if (split) {
+        // a wave a column while that makes at most two workgroups a CU
+        const int per = tiles * (a->cols / 4) * n_kv <= 2L * hx.ncu ? 4 : 16;
+        snprintf(name, sizeof name, "sml_rw_merge%d%s", per, hd == 64 ? "_d64" : "");
+        items_launch(name, n_kv, tiles * (a->cols / per), 256, 0, st, a);
+    }
 }
 
 int sml_hip_paged_attention_rows(const sml_hip_pages * pg, const sml_hip_rows * rows, const float * q, size_t q_stride,

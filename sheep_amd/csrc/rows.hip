@@ -132,7 +132,6 @@ __device__ __forceinline__ void copy_lds16(const void * base, uint32_t off, cons
 }
 #pragma clang diagnostic pop
 
-#define RW_WEAVE 6               // vector instructions beside a matrix instruction
 struct rows_of { int s0, m, n; };                     // a sequence's first row, its rows and its positions
 __device__ __forceinline__ rows_of rows_seq(const sml_krows & a, int b) {
     rows_of x;
@@ -187,27 +186,51 @@ __device__ __forceinline__ bool rows_place(const sml_krows & a, int i, int lane,
         p.item = i;
         return p.tile >= 0 && p.tile * cols < p.sq.m * rep;
     }
-    // the blocks of a split: what makes want of them in all, and some more
+    if (a.pg.n_seq == 1) {
+        p.sq = rows_seq(a, 0);
+        const int nb = (p.sq.n + RW_BLOCK - 1) / RW_BLOCK, nt = (p.sq.m * rep + cols - 1) / cols, most = max(a.want / max(nt, 1), 1);
+        const int chunk = max(a.least, (nb + most - 1) / most);
+        p.b = 0;
+        p.count = max((nb + chunk - 1) / chunk, 1);
+        p.tile = TILES || p.count == 1 ? i : i / p.count;
+        p.split = TILES ? 0 : i - p.tile * p.count;
+        p.item = p.tile * p.count;
+        return p.tile < nt;
+    }
+    // The blocks of a split: what makes want of them in all if each tile's came out
+    // even, and more until they are no more than that, or a tile's each.
     rows_of x[AT_SHARED / 64];
+    int nb[AT_SHARED / 64], nt[AT_SHARED / 64];
     float sum = 0.0f;
     #pragma unroll
     for (int k = 0; k < AT_SHARED / 64; k++)
         if (k == 0 || 64 * k < a.pg.n_seq) {
             x[k] = rows_of{0, 0, 0};
             if (64 * k + lane < a.pg.n_seq) x[k] = rows_seq(a, 64 * k + lane);
-            sum += (float) ((x[k].m * rep + cols - 1) / cols) * (float) ((x[k].n + RW_BLOCK - 1) / RW_BLOCK);
+            nt[k] = (x[k].m * rep + cols - 1) / cols;
+            nb[k] = (x[k].n + RW_BLOCK - 1) / RW_BLOCK;
+            sum += (float) nt[k] * (float) nb[k];
         }
-    const int chunk = max(a.least, (int) (wave_total(sum) * 1.0001f / (float) a.want) + 1);
+    sum = wave_total(sum);
+    int chunk = max(a.least, (int) (sum * 1.0001f / (float) a.want) + 1);
+    for (int tries = 0; tries < 3; tries++) {
+        float made = 0.0f;
+        #pragma unroll
+        for (int k = 0; k < AT_SHARED / 64; k++)
+            if (k == 0 || 64 * k < a.pg.n_seq) made += (float) (nt[k] * max((nb[k] + chunk - 1) / chunk, 1));
+        made = wave_total(made);
+        if (made <= (float) a.want) break;
+        chunk += (int) ((float) chunk * (made / (float) a.want - 1.0f)) + 1;
+    }
     p.item = 0;
     #pragma unroll
     for (int k = 0; k < AT_SHARED / 64; k++)
         if (k == 0 || 64 * k < a.pg.n_seq) {
-            const int nt = (x[k].m * rep + cols - 1) / cols;
-            const int count = max(((x[k].n + RW_BLOCK - 1) / RW_BLOCK + chunk - 1) / chunk, 1);
-            const int items = wave_scan(nt * count), mine = TILES ? wave_scan(nt) : items;
+            const int count = max((nb[k] + chunk - 1) / chunk, 1);
+            const int items = wave_scan(nt[k] * count), mine = TILES ? wave_scan(nt[k]) : items;
             const unsigned long long hit = __ballot(mine > i);
             if (hit) {
-                const int l = __builtin_ctzll(hit), n = __builtin_amdgcn_readlane(nt, l);
+                const int l = __builtin_ctzll(hit), n = __builtin_amdgcn_readlane(nt[k], l);
                 p.b = 64 * k + l;
                 p.count = __builtin_amdgcn_readlane(count, l);
                 p.sq.s0 = __builtin_amdgcn_readlane(x[k].s0, l);
@@ -274,12 +297,11 @@ __device__ __forceinline__ uint32_t bits_range(int lo, int hi) {
     return lo < hi ? (~0u >> (32 - (hi - lo))) << lo : 0;
 }
 
-// A form of the rows' attention: CW waves of 32 columns beside each other, PG groups of them; the stages of 32 positions that a group has (one
-// wave alone needs no more than one), all stages' LDS, and where the groups'
+// A form of the rows' attention: CW waves of 32 columns beside each other, PG
+// groups of them; two stages of 32 positions a group, and where the groups'
 // joined sums end.
 template <int D, int CW, int PG> struct RowsForm {
-    static constexpr int bufs = CW == 1 ? 1 : CW == 2 ? 2 : 3;
-    static constexpr int stages = PG * bufs * 4 * 32 * D;
+    static constexpr int stages = PG * 2 * 4 * 32 * D;
     static constexpr int joined = PG * 32 * CW * (D + 4) * 4;
 };
 
@@ -304,11 +326,11 @@ __device__ __forceinline__ void rows_body(const sml_krows & a) {
     static_assert(NC >= 1 && RC <= 16, "");
     extern __shared__ __align__(16) uint8_t lds[];    // the groups' stages; their new rows' positions, positions whose V is not finite, ranges
     const int kh = blockIdx.x, tid = threadIdx.x, lane = tid & 63, c = lane & 31, g = lane >> 5;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), cw = wave % CW, pgi = wave / CW;
-    uint8_t * const stages = lds + pgi * F::bufs * STAGE;
-    int * const kpos = (int *) (lds + F::stages) + pgi * F::bufs * KB;
-    uint32_t * const found = (uint32_t *) (lds + F::stages + 4 * PG * F::bufs * KB) + pgi * F::bufs * CW;
-    int * const red = (int *) (lds + F::stages + 4 * PG * F::bufs * (KB + CW));
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), pgi = wave % PG, cw = wave / PG;
+    uint8_t * const stages = lds + pgi * 2 * STAGE;
+    int * const kpos = (int *) (lds + F::stages) + pgi * 2 * KB;
+    uint32_t * const found = (uint32_t *) (lds + F::stages + 4 * PG * 2 * KB) + pgi * 2 * CW;
+    int * const red = (int *) (lds + F::stages + 4 * PG * 2 * (KB + CW));
     rows_at p;
     if (!rows_place<false>(a, rows_item(), lane, p)) return;
     const rows_of sq = p.sq;
@@ -626,93 +648,29 @@ __device__ __forceinline__ void rows_body(const sml_krows & a) {
             weights_of<BF>(w0, w1, m1, w[e >> 3], e & 7);
         }
     };
-    // One matrix instruction, then what the vector unit does meanwhile.
-    auto woven = [&]() {
-        #pragma unroll
-        for (int k = 0; k < NJ * NP; k++) {
-            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-            __builtin_amdgcn_sched_group_barrier(0x402, RW_WEAVE, 0);
-        }
-    };
-
-    // A step makes the next block's scores (sn) while it turns this one's (s) into weights.
-    v16f s, sn;
+    v16f s;
     v8 ka[NJ], w[2][NP];
     rows_block b1 = locate(seek(b0.t + STEP));        // the next block; b2: the one behind it
-    if constexpr (CW == 1) {
-        // One stage, the wave's own: keys are fetched over the last block's when those
-        // are in registers, values likewise.
-        if (b0.t < t_end) {
-            asm volatile("s_waitcnt vmcnt(%0)" :: "n"(NC) : "memory");
-            keys(stages, ka);
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-            if (b1.t < t_end) fetch(stages, false, b1);
-            s = products(ka);
+    // Two stages, one in use and one that is filled.
+    int i0 = 0;
+    while (b0.t < t_end) {
+        const int cur = b0.t + pgi * KB;
+        uint8_t * const st = stages + i0 * STAGE;
+        const bool differ = cur < t_flo || cur + KB > t_fhi;
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        keep_pos(kpos + i0 * KB);
+        if (differ) {
+            const uint32_t bad = screen(st);
+            if (!lane) found[i0 * CW + cw] = bad;
         }
-        bool first = true;
-        while (b0.t < t_end) {
-            const int cur = b0.t + pgi * KB;
-            const bool more = b1.t < t_end;
-            uint32_t bad = 0;
-            if (cur < t_flo || cur + KB > t_fhi) {
-                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-                keep_pos(kpos);
-                bad = screen(stages);
-            } else {
-                keep_pos(kpos);
-            }
-            settle(s, kpos, cur, b0.pa, b0.pb, bad);
-            const rows_block b2 = more ? locate(seek(b1.t + STEP)) : b1;
-            if (more) {
-                // the next keys: behind this block's values in the first step, before them then
-                if (first) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-                else asm volatile("s_waitcnt vmcnt(%0)" :: "n"(NC) : "memory");
-                keys(stages, ka);
-                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-                if (b2.t < t_end) fetch(stages, false, b2);
-                sn = products(ka);
-                weights(s, w);
-                woven();
-            } else {
-                weights(s, w);
-            }
-            if (b2.t < t_end) asm volatile("s_waitcnt vmcnt(%0)" :: "n"(NC) : "memory");
-            else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            v8 vv[2 * E];
-            #pragma unroll
-            for (int u = 0; u < 2 * E; u++) vv[u] = value(stages, u % E, u / E);
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-            if (more) {
-                fetch(stages + POOL, true, b1);
-                fetch_pos(b1.t);
-            }
-            #pragma unroll
-            for (int u = 0; u < 2 * E; u++) sums(vv[u], u % E, w[u / E]);
-            s = sn;
-            b0 = b1;
-            b1 = b2;
-            first = false;
+        __syncthreads();                          // the block is whole, and nobody reads the last one
+        if (b1.t < t_end) {
+            fetch(stages + (i0 ^ 1) * STAGE, false, b1);
+            fetch(stages + (i0 ^ 1) * STAGE + POOL, true, b1);
+            fetch_pos(b1.t);
         }
-    } else if constexpr (CW == 2) {
-        // Two stages, one in use and one that is filled.
-        int i0 = 0;
-        while (b0.t < t_end) {
-            const int cur = b0.t + pgi * KB;
-            uint8_t * const st = stages + i0 * STAGE;
-            const bool differ = cur < t_flo || cur + KB > t_fhi;
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            keep_pos(kpos + i0 * KB);
-            if (differ) {
-                const uint32_t bad = screen(st);
-                if (!lane) found[i0 * CW + cw] = bad;
-            }
-            __syncthreads();                          // the block is whole, and nobody reads the last one
-            if (b1.t < t_end) {
-                fetch(stages + (i0 ^ 1) * STAGE, false, b1);
-                fetch(stages + (i0 ^ 1) * STAGE + POOL, true, b1);
-                fetch_pos(b1.t);
-            }
-            const rows_block b2 = b1.t < t_end ? locate(seek(b1.t + STEP)) : b1;
+        const rows_block b2 = b1.t < t_end ? locate(seek(b1.t + STEP)) : b1;
+        if (cur < t_end && cur < w_hi && cur + KB > w_lo) {
             keys(st, ka);
             __builtin_amdgcn_sched_barrier(0);
             s = products(ka);
@@ -733,79 +691,10 @@ __device__ __forceinline__ void rows_body(const sml_krows & a) {
                 sums(vv[u % E], u % E, w[u / E]);
                 if (u < E) vv[u] = value(st, u, 1);
             }
-            b0 = b1;
-            b1 = b2;
-            i0 ^= 1;
         }
-    } else {
-        // Three stages: one whose values are in use, the next block's, and one that is filled.
-        int i0 = 0;
-        auto noted = [&](int i, int cur) {            // what the wave has fetched of stage i is there
-            keep_pos(kpos + i * KB);
-            uint32_t bad = 0;
-            if (cur < t_flo || cur + KB > t_fhi) bad = screen(stages + i * STAGE);
-            if (!lane) found[i * CW + cw] = bad;
-        };
-        if (b0.t < t_end) {
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            noted(0, b0.t + pgi * KB);
-            if (b1.t < t_end) {
-                fetch(stages + STAGE, false, b1);
-                fetch(stages + STAGE + POOL, true, b1);
-                fetch_pos(b1.t);
-            }
-            __syncthreads();
-            keys(stages, ka);
-            s = products(ka);
-        }
-        while (b0.t < t_end) {
-            const int cur = b0.t + pgi * KB, i1 = i0 == 2 ? 0 : i0 + 1, i2 = i1 == 2 ? 0 : i1 + 1;
-            const bool more = b1.t < t_end;
-            const uint8_t * const st = stages + i0 * STAGE;
-            uint32_t bad = 0;
-            if (cur < t_flo || cur + KB > t_fhi) {
-                #pragma unroll
-                for (int y = 0; y < CW; y++) bad |= found[i0 * CW + y];
-            }
-            settle(s, kpos + i0 * KB, cur, b0.pa, b0.pb, bad);
-            const rows_block b2 = more ? locate(seek(b1.t + STEP)) : b1;
-            if (more) {
-                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-                noted(i1, b1.t + pgi * KB);
-                __syncthreads();                      // the next block is whole, and nobody reads the last one
-                if (b2.t < t_end) {
-                    fetch(stages + i2 * STAGE, false, b2);
-                    fetch(stages + i2 * STAGE + POOL, true, b2);
-                    fetch_pos(b2.t);
-                }
-                keys(stages + i1 * STAGE, ka);
-                sn = products(ka);
-                weights(s, w);
-                woven();
-            } else {
-                weights(s, w);
-            }
-            v8 vv[4];
-            vv[0] = value(st, 0, 0);
-            vv[1] = value(st, 1, 0);
-            #pragma unroll
-            for (int u = 0; u < 2 * E; u += 2) {
-                if (u + 2 < 2 * E) {
-                    vv[(u + 2) & 3] = value(st, (u + 2) % E, (u + 2) / E);
-                    vv[(u + 3) & 3] = value(st, (u + 3) % E, (u + 3) / E);
-                }
-                __builtin_amdgcn_sched_barrier(0);
-                #pragma unroll
-                for (int y = 0; y < NP; y++) {
-                    o[u % E] = MM::mul(vv[u & 3], w[u / E][y], o[u % E]);
-                    o[(u + 1) % E] = MM::mul(vv[(u + 1) & 3], w[u / E][y], o[(u + 1) % E]);
-                }
-            }
-            s = sn;
-            b0 = b1;
-            b1 = b2;
-            i0 = i1;
-        }
+        b0 = b1;
+        b1 = b2;
+        i0 ^= 1;
     }
 
     l += __shfl_xor(l, 32);
@@ -889,68 +778,80 @@ __device__ __forceinline__ void rows_body(const sml_krows & a) {
     ROWS(128, 1, CW, PG, 2, name, _bf) \
     ROWS(64, 0, CW, PG, E, name, _d64) \
     ROWS(64, 1, CW, PG, E, name, _d64_bf)
-ROWS4(1, 8, 2, sml_rw_rows32)
 ROWS4(2, 4, 2, sml_rw_rows64)
 ROWS4(4, 2, 2, sml_rw_rows128)
-ROWS4(4, 1, 2, sml_rw_rows128l)
 
-// The splits of a tile joined, 16 columns a workgroup, 16 lanes a column: the
-// bases of its splits shared out over the lanes, then each lane's dims of every
-// split in turn.
-template <int D>
+// The splits of a tile joined, C columns a workgroup: the bases of a column's splits
+// shared out over its 256 / C lanes, then the splits over each 16 of them, which
+// take a few dims each. Latency bounds it.
+template <int D, int C>
 __device__ __forceinline__ void rows_merge_body(const sml_krows & a) {
-    __shared__ float f[16][RW_SPLITS + 1];
-    const int kh = blockIdx.x, tid = threadIdx.x, c = tid >> 4, l = tid & 15;
-    const int groups = (a.cols + 15) / 16, unit = rows_item();
+    constexpr int LC = 256 / C, SG = LC / 16;         // a column's lanes, and how many splits they take at once
+    __shared__ float f[C][RW_SPLITS + 1];
+    const int kh = blockIdx.x, tid = threadIdx.x, lane = tid & 63, c = tid / LC, lc = tid % LC, l = tid & 15, share = lc / 16;
+    const int groups = a.cols / C, unit = rows_item();
     rows_at p;
-    if (!rows_place<true>(a, unit / groups, tid & 63, p) || p.count == 1) return;
-    const rows_of sq = rows_seq(a, p.b);
-    const int rep = a.n_head / a.pg.n_kv, pc = 16 * (unit % groups) + c, col = p.tile * a.cols + pc;
-    if (16 * (unit % groups) + p.tile * a.cols >= sq.m * rep || p.item + p.count > a.items || p.count > RW_SPLITS) return;
-    const bool mine = col < sq.m * rep;
+    if (!rows_place<true>(a, unit / groups, lane, p) || p.count == 1) return;
+    const int rep = a.n_head / a.pg.n_kv, pc = C * (unit % groups) + c, col = p.tile * a.cols + pc;
+    if (p.item + p.count > a.items || p.count > RW_SPLITS) return;
+    if (p.tile * a.cols + pc - c >= p.sq.m * rep) return;
+    const bool mine = col < p.sq.m * rep;
     const float2 * ml = part_ml(a, kh, p.item, D) + (mine ? pc : 0);
     const float * po = part_o(a, kh, p.item, D) + (size_t) (mine ? pc : 0) * D + 4 * l;
     const size_t step = (size_t) a.part_cols;
     float m = -INFINITY;
-    for (int s = l; s < p.count; s += 16) m = fmaxf(m, ml[s * step].x);
-    m = max16(m);
+    for (int s = lc; s < p.count; s += LC) m = fmaxf(m, ml[s * step].x);
+    m = LC == 64 ? wave_max(m) : max16(m);
     const float mu = m == -INFINITY ? 0.0f : m;
     float sum = 0.0f;
-    for (int s = l; s < p.count; s += 16) {
-        const float2 x = ml[s * step];
-        const float e = __builtin_amdgcn_exp2f(x.x - mu);
-        const bool none = x.x == -INFINITY && x.y == 0.0f;    // what lies there counts for nothing
+    for (int s = lc; s < p.count; s += LC) {
+        const float2 y = ml[s * step];
+        const float e = __builtin_amdgcn_exp2f(y.x - mu);
+        const bool none = y.x == -INFINITY && y.y == 0.0f;    // what lies there counts for nothing
         f[c][s] = none ? -1.0f : e;
-        if (!none) sum += e * x.y;
+        if (!none) sum += e * y.y;
     }
-    sum = sum16(sum);
+    sum = LC == 64 ? wave_sum(sum) : sum16(sum);
     wave_lds();
-    if (!mine) return;
     v4f o[D / 64];
     #pragma unroll
     for (int u = 0; u < D / 64; u++) o[u] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-    #pragma unroll 4
-    for (int s = 0; s < p.count; s++) {
+    #pragma unroll 8
+    for (int s = share; s < p.count; s += SG) {
         const float e = f[c][s];
         #pragma unroll
         for (int u = 0; u < D / 64; u++) {
-            const v4f x = *(const v4f *) (po + s * step * D + 64 * u);
+            const v4f y = *(const v4f *) (po + s * step * D + 64 * u);
             #pragma unroll
-            for (int k = 0; k < 4; k++) o[u][k] = e >= 0.0f || e != e ? __builtin_fmaf(e, x[k], o[u][k]) : o[u][k];
+            for (int k = 0; k < 4; k++) o[u][k] = e >= 0.0f || e != e ? __builtin_fmaf(e, y[k], o[u][k]) : o[u][k];
         }
     }
+    if constexpr (SG > 1) {
+        #pragma unroll
+        for (int u = 0; u < D / 64; u++)
+            #pragma unroll
+            for (int k = 0; k < 4; k++) {
+                o[u][k] += __shfl_xor(o[u][k], 16);
+                o[u][k] += __shfl_xor(o[u][k], 32);
+            }
+    }
+    if (share || !mine) return;
     const int i = col / rep;
-    float * const to = a.out + ((size_t) (sq.s0 + i) * a.n_head + kh * rep + (col - i * rep)) * D + 4 * l;
+    float * const to = a.out + ((size_t) (p.sq.s0 + i) * a.n_head + kh * rep + (col - i * rep)) * D + 4 * l;
     #pragma unroll
     for (int u = 0; u < D / 64; u++) {
-        v4f x;
+        v4f y;
         #pragma unroll
-        for (int k = 0; k < 4; k++) x[k] = sum == 0.0f ? 0.0f : o[u][k] / sum;
-        *(v4fu *) (to + 64 * u) = x;
+        for (int k = 0; k < 4; k++) y[k] = sum == 0.0f ? 0.0f : o[u][k] / sum;
+        *(v4fu *) (to + 64 * u) = y;
     }
 }
-extern "C" __global__ __launch_bounds__(256) void sml_rw_merge(const sml_krows a) { rows_merge_body<128>(a); }
-extern "C" __global__ __launch_bounds__(256) void sml_rw_merge_d64(const sml_krows a) { rows_merge_body<64>(a); }
+#define MERGE(D, C, name) \
+    extern "C" __global__ __launch_bounds__(256) void name(const sml_krows a) { rows_merge_body<D, C>(a); }
+MERGE(128, 4, sml_rw_merge4)
+MERGE(128, 16, sml_rw_merge16)
+MERGE(64, 4, sml_rw_merge4_d64)
+MERGE(64, 16, sml_rw_merge16_d64)
 
 // ---------------------------------------------------------------- layers of a cache
 
