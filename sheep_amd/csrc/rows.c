@@ -58,7 +58,7 @@ static const struct form { const char * name; int cols, cw, pg, per_cu; } forms[
 static void rows_launch(sml_krows * a, int hd, int type, hipStream_t st) {
     const int n_kv = a->pg.n_kv, rep = a->n_head / n_kv, n_seq = a->pg.n_seq;
     const int ncol = a->n_row * rep, some = n_seq < a->n_row ? n_seq : a->n_row;
-    int f = ncol > 64L * some && ((long) ceil_div(ncol, 128) * n_kv >= hx.ncu || (long) ceil_div(ncol, 64) * n_kv < hx.ncu);
+    int f = ncol > 40L * some && ((long) ceil_div(ncol, 128) * n_kv >= hx.ncu || (long) ceil_div(ncol, 64) * n_kv < hx.ncu);
     if (getenv("RWF")) f = atoi(getenv("RWF"));
     const struct form * const fm = forms + f;
     a->cols = fm->cols;
@@ -71,7 +71,7 @@ static void rows_launch(sml_krows * a, int hd, int type, hipStream_t st) {
     long items = split ? tiles + want : tiles;
     a->items = (int) items;
     a->part_cols = ncol < a->cols ? ncol : a->cols;
-    const size_t stages = (size_t) fm->pg * 2 * (4 * 32 * hd + 4 * 32 + 4 * fm->cw) + 16 * fm->cw;
+    const size_t stages = (size_t) fm->pg * 2 * (4 * 32 * hd + 4 * 32 + 4 * fm->cw) + (16 + 20 * 32) * fm->cw;
     const size_t joined = fm->pg > 1 ? (size_t) fm->pg * fm->cols * ((hd + 4) * 4 + 8) : 0;
     char base[24], name[40];
     snprintf(base, sizeof base, "sml_rw_%s%s", fm->name, a->cap > 0.0f || a->slope ? "r" : "");

@@ -168,6 +168,7 @@ struct rows_at { int b, tile, count, split, item; rows_of sq; };  // a tile, its
 template <bool TILES>
 __device__ __forceinline__ bool rows_place(const sml_krows & a, int i, int lane, rows_at & p) {
     const int rep = a.n_head / a.pg.n_kv, cols = a.cols;
+    const bool turned = !a.first && !a.last;          // causal rows: the last tiles see most, and begin
     if (!a.want) {
         int lo = 0, hi = a.pg.n_seq;
         while (hi - lo > 1) {
@@ -180,11 +181,12 @@ __device__ __forceinline__ bool rows_place(const sml_krows & a, int i, int lane,
         }
         p.sq = rows_seq(a, lo);
         p.b = lo;
-        p.tile = i - (p.sq.s0 * rep / cols + lo);
+        const int e = i - (p.sq.s0 * rep / cols + lo), nt = (p.sq.m * rep + cols - 1) / cols;
+        p.tile = turned ? nt - 1 - e : e;
         p.count = 1;
         p.split = 0;
         p.item = i;
-        return p.tile >= 0 && p.tile * cols < p.sq.m * rep;
+        return e >= 0 && e < nt;
     }
     if (a.pg.n_seq == 1) {
         p.sq = rows_seq(a, 0);
@@ -195,7 +197,8 @@ __device__ __forceinline__ bool rows_place(const sml_krows & a, int i, int lane,
         p.tile = TILES || p.count == 1 ? i : i / p.count;
         p.split = TILES ? 0 : i - p.tile * p.count;
         p.item = p.tile * p.count;
-        return p.tile < nt;
+        if (turned) p.tile = nt - 1 - p.tile;
+        return p.item < nt * p.count;
     }
     // The blocks of a split: what makes want of them in all if each tile's came out
     // even, and more until they are no more than that, or a tile's each.
@@ -240,6 +243,7 @@ __device__ __forceinline__ bool rows_place(const sml_krows & a, int i, int lane,
                 p.tile = TILES || p.count == 1 ? e : e / p.count;
                 p.split = TILES ? 0 : e - p.tile * p.count;
                 p.item += __builtin_amdgcn_readlane(items, l) - n * p.count + p.tile * p.count;
+                if (turned) p.tile = n - 1 - p.tile;
                 return true;
             }
             i -= __builtin_amdgcn_readlane(mine, 63);
@@ -331,6 +335,8 @@ __device__ __forceinline__ void rows_body(const sml_krows & a) {
     int * const kpos = (int *) (lds + F::stages) + pgi * 2 * KB;
     uint32_t * const found = (uint32_t *) (lds + F::stages + 4 * PG * 2 * KB) + pgi * 2 * CW;
     int * const red = (int *) (lds + F::stages + 4 * PG * 2 * (KB + CW));
+    int4 * const about = (int4 *) (red + 4 * CW);     // of the columns, for the masks: range, tree's bits
+    int * const owner = (int *) (about + 32 * CW);    // and their rows, -1 for those that attend to nothing
     rows_at p;
     if (!rows_place<false>(a, rows_item(), lane, p)) return;
     const rows_of sq = p.sq;
@@ -372,7 +378,11 @@ __device__ __forceinline__ void rows_body(const sml_krows & a) {
         t_hi = w_hi = most32(w_hi);
         t_flo = f_lo = most32(f_lo);
         t_fhi = f_hi = least32(f_hi);
-        if constexpr (CW > 1) {
+        if (!pgi && !g) {
+            about[32 * cw + c] = some ? make_int4(lo, hi, (int) (uint32_t) tw, (int) (uint32_t) (tw >> 32)) : make_int4(0, 0, 0, 0);
+            owner[32 * cw + c] = some ? r : -1;
+        }
+        {
             if (!lane && !pgi) { red[4 * cw] = w_lo; red[4 * cw + 1] = w_hi; red[4 * cw + 2] = f_lo; red[4 * cw + 3] = f_hi; }
             __syncthreads();
             #pragma unroll
@@ -466,7 +476,11 @@ __device__ __forceinline__ void rows_body(const sml_krows & a) {
     int at_pos = 0;
     auto fetch_pos = [&](int t) {
         if (RULES && a.slope && a.pos && t + pgi * KB + KB > past && cw == 0)
-            at_pos = a.pos[sq.s0 + min(max(t + pgi * KB + lane - past, 0), max(sq.m - 1, 0))];
+        {
+            const int slot = t + pgi * KB + lane, i = min(max(slot - past, 0), max(sq.m - 1, 0));
+            at_pos = a.pos[sq.s0 + i];
+            if (slot < past) at_pos = slot;
+        }
     };
     auto keep_pos = [&](int * kp) {
         if (RULES && a.slope && a.pos && cw == 0 && lane < KB) kp[lane] = at_pos;
@@ -496,6 +510,7 @@ __device__ __forceinline__ void rows_body(const sml_krows & a) {
                 parts_of<BF>(__builtin_amdgcn_ldexpf(x[2 * j + e / 4][e % 4], -ex), __builtin_amdgcn_ldexpf(x[2 * j + e / 4][e % 4 + 1], -ex), q[j], e);
         back = __builtin_amdgcn_ldexpf(a.scale, ex);
     }
+    const int q0 = qpos - 4 * g;                      // the row's position, less where the lane's first score is
     const float slope = RULES && a.slope ? -1.44269504088896341f * a.slope[h] : 0.0f;
     const float f = RULES ? 1.0f : back;              // log2 weights are f times the settled scores
 
@@ -539,19 +554,26 @@ __device__ __forceinline__ void rows_body(const sml_krows & a) {
 
     float m1;
     asm("v_mov_b32 %0, -1.0" : "=v"(m1));
-    // A block's keys in registers; the scores; a tile's dims of 16 positions' values; the sums.
-    auto keys = [&](const uint8_t * st, v8 (&ka)[NJ]) {
+    // The scores, their keys NK ahead; a tile's dims of 16 positions' values; the sums.
+    // (bfloat16's three parts leave few registers.)
+    constexpr int NK = BF ? 4 : NJ, NV = BF ? 2 : E;
+    auto products = [&](const uint8_t * st) {
+        auto key = [&](int e) { return *(const v8 *) (st + krow + 16 * ((2 * e + g) ^ kx)); };
+        v8 ka[NK];
         #pragma unroll
-        for (int e = 0; e < NJ; e++) ka[e] = *(const v8 *) (st + krow + 16 * ((2 * e + g) ^ kx));
-    };
-    auto products = [&](const v8 (&ka)[NJ]) {
+        for (int e = 0; e < NK; e++) ka[e] = key(e);
+        __builtin_amdgcn_sched_barrier(0);
         v16f s;
         #pragma unroll
         for (int e = 0; e < 16; e++) s[e] = 0.0f;
         #pragma unroll
-        for (int e = 0; e < NJ; e++)
+        for (int e = 0; e < NJ; e++) {
             #pragma unroll
-            for (int k = 0; k < NP; k++) s = MM::mul(ka[e], q[e][k], s);
+            for (int k = 0; k < NP; k++) s = MM::mul(ka[e % NK], q[e][k], s);
+            if (e + NK < NJ) ka[e % NK] = key(e + NK);
+            if (NK < NJ) __builtin_amdgcn_sched_barrier(0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
         return s;
     };
     auto value = [&](const uint8_t * st, int u, int k) {
@@ -583,13 +605,15 @@ __device__ __forceinline__ void rows_body(const sml_krows & a) {
                 }
             }
             if (a.slope) {
-                const float d0 = (float) (t + 4 * g - qpos);
+                const float d0 = (float) (t - q0);
                 if (a.pos && t + 32 > past) {
+                    const int4 * const at4 = (const int4 *) kp + g;
                     #pragma unroll
-                    for (int e = 0; e < 16; e++) {
-                        const int y = at(e) + 4 * g;
-                        const float d = t + y >= past ? (float) (kp[y] - qpos) : d0 + (float) at(e);
-                        s[e] = __builtin_fmaf(slope, fabsf(d), s[e]);
+                    for (int k = 0; k < 4; k++) {
+                        const int4 y = at4[2 * k];
+                        const int x4[4] = { y.x, y.y, y.z, y.w };
+                        #pragma unroll
+                        for (int e = 0; e < 4; e++) s[4 * k + e] = __builtin_fmaf(slope, fabsf((float) (x4[e] - 4 * g - q0)), s[4 * k + e]);
                     }
                 } else {
                     #pragma unroll
@@ -598,14 +622,17 @@ __device__ __forceinline__ void rows_body(const sml_krows & a) {
             }
         }
         if (pa < 0 || pb < 0 || t < f_lo || t + 32 > f_hi) {
-            uint32_t vm = bits_range(lo - t, hi - t);
+            const int4 mask = about[32 * cw + c];
+            uint32_t vm = bits_range(mask.x - t, mask.y - t);
             const int j0 = t - past;
             if (nbit && j0 + 32 > 0 && j0 < nbit) {
-                uint64_t y = tw;
+                uint64_t y = (uint64_t) (uint32_t) mask.w << 32 | (uint32_t) mask.z;
                 const int w0 = j0 >> 5;               // bits 32 w0.. of the row, 64 of them
                 if (a.words > 2) {
-                    const uint32_t * const bits = a.tree + (size_t) r * a.words;
+                    const int row = owner[32 * cw + c];
+                    const uint32_t * const bits = a.tree + (size_t) max(row, 0) * a.words;
                     y = (uint64_t) (w0 + 1 >= 0 && w0 + 1 < a.words ? bits[w0 + 1] : 0u) << 32 | (w0 >= 0 && w0 < a.words ? bits[w0] : 0u);
+                    if (row < 0) y = 0;
                 } else if (w0) {
                     y = w0 == -1 ? y << 32 : w0 == 1 ? y >> 32 : 0;
                 }
@@ -614,7 +641,6 @@ __device__ __forceinline__ void rows_body(const sml_krows & a) {
             vm &= bits_range(0, sq.n - t);
             if (pa < 0) vm &= 0xFFFF0000u;
             if (pb < 0) vm &= 0x0000FFFFu;
-            if (!some) vm = 0;
             if (vm & bad) l = NAN;
             vm >>= 4 * g;
             #pragma unroll
@@ -648,8 +674,6 @@ __device__ __forceinline__ void rows_body(const sml_krows & a) {
             weights_of<BF>(w0, w1, m1, w[e >> 3], e & 7);
         }
     };
-    v16f s;
-    v8 ka[NJ], w[2][NP];
     rows_block b1 = locate(seek(b0.t + STEP));        // the next block; b2: the one behind it
     // Two stages, one in use and one that is filled.
     int i0 = 0;
@@ -671,13 +695,10 @@ __device__ __forceinline__ void rows_body(const sml_krows & a) {
         }
         const rows_block b2 = b1.t < t_end ? locate(seek(b1.t + STEP)) : b1;
         if (cur < t_end && cur < w_hi && cur + KB > w_lo) {
-            keys(st, ka);
-            __builtin_amdgcn_sched_barrier(0);
-            s = products(ka);
-            __builtin_amdgcn_sched_barrier(0);
-            v8 vv[E];
+            v16f s = products(st);
+            v8 w[2][NP], vv[NV];
             #pragma unroll
-            for (int u = 0; u < E; u++) vv[u] = value(st, u, 0);
+            for (int u = 0; u < NV; u++) vv[u] = value(st, u % E, u / E);
             __builtin_amdgcn_sched_barrier(0);
             uint32_t bad = 0;
             if (differ) {
@@ -688,8 +709,9 @@ __device__ __forceinline__ void rows_body(const sml_krows & a) {
             weights(s, w);
             #pragma unroll
             for (int u = 0; u < 2 * E; u++) {
-                sums(vv[u % E], u % E, w[u / E]);
-                if (u < E) vv[u] = value(st, u, 1);
+                sums(vv[u % NV], u % E, w[u / E]);
+                if (u + NV < 2 * E) vv[u % NV] = value(st, (u + NV) % E, (u + NV) / E);
+                if (NV < E) __builtin_amdgcn_sched_barrier(0);
             }
         }
         b0 = b1;
@@ -699,29 +721,7 @@ __device__ __forceinline__ void rows_body(const sml_krows & a) {
 
     l += __shfl_xor(l, 32);
     if (!some) { base = -INFINITY; l = 0.0f; }
-    if constexpr (PG == 1) {
-        if (!mine) return;
-        if (p.count == 1) {
-            float * const to = a.out + ((size_t) r * a.n_head + h) * D + 4 * g;
-            #pragma unroll
-            for (int u = 0; u < E; u++)
-                #pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    v4f y;
-                    #pragma unroll
-                    for (int e = 0; e < 4; e++) y[e] = l != 0.0f ? o[u][4 * k + e] / l : 0.0f;
-                    *(v4fu *) (to + 32 * u + 8 * k) = y;
-                }
-        } else {
-            const int pc = 32 * cw + c;
-            if (!g) part_ml(a, kh, p.item + p.split, D)[pc] = make_float2(base, l);
-            float * const to = part_o(a, kh, p.item + p.split, D) + (size_t) pc * D + 4 * g;
-            #pragma unroll
-            for (int u = 0; u < E; u++)
-                #pragma unroll
-                for (int k = 0; k < 4; k++) *(v4f *) (to + 32 * u + 8 * k) = v4f{o[u][4 * k], o[u][4 * k + 1], o[u][4 * k + 2], o[u][4 * k + 3]};
-        }
-    } else {
+    {
         // The groups joined: their sums over the stages, rows of D + 4 floats on
         // different banks, their bases and weights' sums behind.
         constexpr int QT = 32 * CW, LD = D + 4;
