@@ -562,6 +562,7 @@ typedef struct {
     float scale, sign;            // |scale| times log2(e), or over the cap; the scale's sign
     float cap;                    // times log2(e)
     int n_head, n_row, max_len, words;
+    uint32_t over;                // 2^32 / rep rounded up (0: rep is 1)
     int cols;                     // columns of a tile
     int want, least;              // splits wanted in all (0: none), blocks of one at least
     int items, part_cols;         // the partials' items a KV head, and the columns of one

@@ -62,6 +62,7 @@ static void rows_launch(sml_krows * a, int hd, int type, hipStream_t st) {
     if (getenv("RWF")) f = atoi(getenv("RWF"));
     const struct form * const fm = forms + f;
     a->cols = fm->cols;
+    a->over = rep > 1 ? (uint32_t) (((1ull << 32) + (unsigned) rep - 1) / (unsigned) rep) : 0;
     // workgroups that run at once; not split where the tiles are as many
     const int want = ceil_div((hx.ncu < 256 ? hx.ncu : 256) * fm->per_cu, n_kv);
     a->least = getenv("RWL") ? atoi(getenv("RWL")) : 2;

@@ -132,6 +132,10 @@ __device__ __forceinline__ void copy_lds16(const void * base, uint32_t off, cons
 }
 #pragma clang diagnostic pop
 
+// col / rep: rep is at most 16 and col below 2^21, so that the high word of a
+// product with 2^32 / rep, rounded up, is it.
+__device__ __forceinline__ int rows_over(const sml_krows & a, int col) { return a.over ? (int) __umulhi((unsigned) col, a.over) : col; }
+
 struct rows_of { int s0, m, n; };                     // a sequence's first row, its rows and its positions
 __device__ __forceinline__ rows_of rows_seq(const sml_krows & a, int b) {
     rows_of x;
@@ -345,12 +349,11 @@ __device__ __forceinline__ void rows_body(const sml_krows & a) {
     const int32_t * const tab = a.pg.table + (size_t) p.b * a.pg.seq_pages;
 
     // the lane's column: its row's range, its tree's bits (if they are no more than 64) and its position
-    const int col = p.tile * a.cols + 32 * cw + c, in_seq = min(col, ncol - 1) / rep;
+    const int col0 = p.tile * a.cols, col = col0 + 32 * cw + c, in_seq = rows_over(a, min(col, ncol - 1));
     const bool mine = col < ncol;
     const int r = sq.s0 + in_seq, h = kh * rep + (min(col, ncol - 1) - in_seq * rep);
     const int lo = a.first ? max(a.first[r], 0) : 0;
     const int hi = min(a.last ? a.last[r] : a.tree ? past : past + in_seq + 1, sq.n);
-    const int qpos = a.pos ? a.pos[r] : past + in_seq;
     const int nbit = a.tree ? min(sq.m, 32 * a.words) : 0;
     uint64_t tw = 0;
     if (nbit) {
@@ -358,50 +361,56 @@ __device__ __forceinline__ void rows_body(const sml_krows & a) {
         tw = bits[0];
         if (a.words > 1) tw |= (uint64_t) bits[1] << 32;
     }
-    // the query: lane (c, g) holds dims 16j + 8g.. of column c
-    v4f x[2 * NJ];
-    {
-        const float * qp = a.q + (size_t) r * a.q_stride + (size_t) h * D + 8 * g;
-        #pragma unroll
-        for (int j = 0; j < 2 * NJ; j++) x[j] = *(const v4fu *) (qp + 16 * (j / 2) + 4 * (j % 2));
-    }
-    const bool range = lo < hi, tree = nbit && (tw || a.words > 2);
-    const bool some = mine && (range || tree);        // does it attend to anything
+    const bool range = lo < hi;
     // what any column of the wave, of the tile attends to lies in w_lo..w_hi, t_lo..t_hi;
     // every one that attends to anything has all of f_lo..f_hi (t_flo.. of the tile)
     int w_lo = 0x7fffffff, w_hi = 0, f_lo = 0, f_hi = 0x7fffffff, t_lo, t_hi, t_flo, t_fhi;
-    {
+    const bool any = col0 + 32 * cw < ncol;
+    if (!a.first && !a.last && past >= 0) {
+        // no loads to wait for: a tree's rows all see the past, causal ones more from row to row
+        if (a.tree) {
+            t_lo = 0;
+            t_hi = past + nbit;
+            t_flo = past > 0 ? 0 : 0x7fffffff;
+            t_fhi = past;
+        } else {
+            t_lo = t_flo = 0;
+            t_hi = past + rows_over(a, min(col0 + a.cols, ncol) - 1) + 1;
+            t_fhi = past + rows_over(a, col0) + 1;
+        }
+        if (any) {
+            w_lo = 0;
+            w_hi = a.tree ? t_hi : __builtin_amdgcn_readlane(hi, 31);
+            f_lo = t_flo;
+            f_hi = a.tree ? t_fhi : __builtin_amdgcn_readlane(hi, 0);
+        }
+    } else {
+        const bool tree = nbit && (tw || a.words > 2);
         if (mine && range) { w_lo = lo; w_hi = hi; }
         if (mine && tree && past + nbit > 0) { w_lo = min(w_lo, max(past, 0)); w_hi = max(w_hi, min(past + nbit, sq.n)); }
-        if (some) { f_lo = range ? lo : 0x7fffffff; f_hi = range ? hi : 0; }
+        if (mine && (range || tree)) { f_lo = range ? lo : 0x7fffffff; f_hi = range ? hi : 0; }
         t_lo = w_lo = least32(w_lo);
         t_hi = w_hi = most32(w_hi);
         t_flo = f_lo = most32(f_lo);
         t_fhi = f_hi = least32(f_hi);
-        if (!pgi && !g) {
-            about[32 * cw + c] = some ? make_int4(lo, hi, (int) (uint32_t) tw, (int) (uint32_t) (tw >> 32)) : make_int4(0, 0, 0, 0);
-            owner[32 * cw + c] = some ? r : -1;
+        if (!lane && !pgi) { red[4 * cw] = w_lo; red[4 * cw + 1] = w_hi; red[4 * cw + 2] = f_lo; red[4 * cw + 3] = f_hi; }
+        __syncthreads();
+        #pragma unroll
+        for (int w = 0; w < CW; w++) {
+            t_lo = min(t_lo, red[4 * w]);
+            t_hi = max(t_hi, red[4 * w + 1]);
+            t_flo = max(t_flo, red[4 * w + 2]);
+            t_fhi = min(t_fhi, red[4 * w + 3]);
         }
-        {
-            if (!lane && !pgi) { red[4 * cw] = w_lo; red[4 * cw + 1] = w_hi; red[4 * cw + 2] = f_lo; red[4 * cw + 3] = f_hi; }
-            __syncthreads();
-            #pragma unroll
-            for (int w = 0; w < CW; w++) {
-                t_lo = min(t_lo, red[4 * w]);
-                t_hi = max(t_hi, red[4 * w + 1]);
-                t_flo = max(t_flo, red[4 * w + 2]);
-                t_fhi = min(t_fhi, red[4 * w + 3]);
-            }
-            t_lo = __builtin_amdgcn_readfirstlane(t_lo);
-            t_hi = __builtin_amdgcn_readfirstlane(t_hi);
-            t_flo = __builtin_amdgcn_readfirstlane(t_flo);
-            t_fhi = __builtin_amdgcn_readfirstlane(t_fhi);
-        }
+        t_lo = __builtin_amdgcn_readfirstlane(t_lo);
+        t_hi = __builtin_amdgcn_readfirstlane(t_hi);
+        t_flo = __builtin_amdgcn_readfirstlane(t_flo);
+        t_fhi = __builtin_amdgcn_readfirstlane(t_fhi);
     }
     // this split's blocks
     int t_at = 0, t_end = 0;
     if (t_lo < t_hi) {
-        const int b0 = t_lo / RW_BLOCK, nb = (t_hi + RW_BLOCK - 1) / RW_BLOCK - b0, per = (nb + p.count - 1) / p.count;
+        const int b0 = t_lo / RW_BLOCK, nb = (t_hi + RW_BLOCK - 1) / RW_BLOCK - b0, per = p.count == 1 ? nb : (nb + p.count - 1) / p.count;
         t_at = (b0 + p.split * per) * RW_BLOCK;
         t_end = min((b0 + min(nb, (p.split + 1) * per)) * RW_BLOCK, t_hi);
     }
@@ -414,6 +423,14 @@ __device__ __forceinline__ void rows_body(const sml_krows & a) {
         return e < a.pg.n_pages ? e : -1;
     };
     int t_tab = t_at, ent = look(t_at), next = look(t_at + 1024);
+    // the query: lane (c, g) holds dims 16j + 8g.. of column c
+    v4f x[2 * NJ];
+    {
+        const float * qp = a.q + (size_t) r * a.q_stride + (size_t) h * D + 8 * g;
+        #pragma unroll
+        for (int j = 0; j < 2 * NJ; j++) x[j] = *(const v4fu *) (qp + 16 * (j / 2) + 4 * (j % 2));
+    }
+    const int qpos = RULES && a.pos ? a.pos[r] : past + in_seq;
     uint64_t at_ent;
     auto place = [&]() { at_ent = 2 * ((uint64_t) max(ent, 0) * a.pg.page_stride + (uint64_t) (uint32_t) (((t_tab + 16 * lane) & pmask) * kvd + kh * D)); };
     place();
@@ -492,6 +509,11 @@ __device__ __forceinline__ void rows_body(const sml_krows & a) {
         fetch_pos(b0.t);
     }
 
+    const bool some = mine && (range || (nbit && (tw || a.words > 2)));      // does it attend to anything
+    if (!pgi && !g) {
+        about[32 * cw + c] = some ? make_int4(lo, hi, (int) (uint32_t) tw, (int) (uint32_t) (tw >> 32)) : make_int4(0, 0, 0, 0);
+        owner[32 * cw + c] = some ? r : -1;
+    }
     // the query in parts
     v8 q[NJ][NP];
     float back;                                       // what a product of the scaled q is multiplied by
@@ -500,7 +522,11 @@ __device__ __forceinline__ void rows_body(const sml_krows & a) {
         #pragma unroll
         for (int j = 0; j < 2 * NJ; j++)
             #pragma unroll
-            for (int k = 0; k < 4; k++) { x[j][k] = mine ? x[j][k] * a.sign : 0.0f; mx = fmaxf(mx, fabsf(x[j][k])); }
+            for (int k = 0; k < 4; k++) mx = fmaxf(mx, fabsf(x[j][k]));
+        if (a.sign < 0.0f) {
+            #pragma unroll
+            for (int j = 0; j < 2 * NJ; j++) x[j] = -x[j];
+        }
         mx = fmaxf(mx, __shfl_xor(mx, 32));
         const int ex = BF ? 0 : scale_of(mx);
         #pragma unroll
@@ -738,28 +764,30 @@ __device__ __forceinline__ void rows_body(const sml_krows & a) {
             if (!g) sml[pgi * QT + pc] = make_float2(base, l);
         }
         __syncthreads();
+        #pragma unroll 1
         for (int x = tid; x < QT * (D / 4); x += 64 * W) {
-            const int pc = x / (D / 4), d = 4 * (x % (D / 4)), col = p.tile * a.cols + pc;
+            const int pc = x / (D / 4), d = 4 * (x % (D / 4)), col = col0 + pc;
             if (col >= ncol) break;
-            float m = -INFINITY;
+            float2 ml[PG];
+            v4f v[PG];
             #pragma unroll
-            for (int k = 0; k < PG; k++) m = fmaxf(m, sml[k * QT + pc].x);
+            for (int k = 0; k < PG; k++) { ml[k] = sml[k * QT + pc]; v[k] = *(const v4f *) (so + (size_t) (k * QT + pc) * LD + d); }
+            float m = ml[0].x;
+            #pragma unroll
+            for (int k = 1; k < PG; k++) m = fmaxf(m, ml[k].x);
             const float mu = m == -INFINITY ? 0.0f : m;
             float ls = 0.0f;
             v4f os = v4f{0.0f, 0.0f, 0.0f, 0.0f};
             #pragma unroll
             for (int k = 0; k < PG; k++) {
-                const float2 ml = sml[k * QT + pc];
-                const float f = __builtin_amdgcn_exp2f(ml.x - mu);
-                const v4f v = *(const v4f *) (so + (size_t) (k * QT + pc) * LD + d);
-                if (ml.x != -INFINITY || ml.y != 0.0f) {
-                    ls += f * ml.y;
-                    #pragma unroll
-                    for (int e = 0; e < 4; e++) os[e] = __builtin_fmaf(f, v[e], os[e]);
-                }
+                const bool none = ml[k].x == -INFINITY && ml[k].y == 0.0f;    // what its sums hold counts for nothing
+                const float f = __builtin_amdgcn_exp2f(ml[k].x - mu);
+                ls += none ? 0.0f : f * ml[k].y;
+                #pragma unroll
+                for (int e = 0; e < 4; e++) os[e] = none ? os[e] : __builtin_fmaf(f, v[k][e], os[e]);
             }
             if (p.count == 1) {
-                const int i = col / rep;
+                const int i = rows_over(a, col);
                 #pragma unroll
                 for (int e = 0; e < 4; e++) os[e] = ls != 0.0f ? os[e] / ls : 0.0f;
                 *(v4fu *) (a.out + ((size_t) (sq.s0 + i) * a.n_head + kh * rep + (col - i * rep)) * D + d) = os;
@@ -836,7 +864,7 @@ __device__ __forceinline__ void rows_merge_body(const sml_krows & a) {
             }
     }
     if (share || !mine) return;
-    const int i = col / rep;
+    const int i = rows_over(a, col);
     float * const to = a.out + ((size_t) (p.sq.s0 + i) * a.n_head + kh * rep + (col - i * rep)) * D + 4 * l;
     #pragma unroll
     for (int u = 0; u < D / 64; u++) {
