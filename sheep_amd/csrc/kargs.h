@@ -548,7 +548,7 @@ typedef struct {
     const float * cos_t, * sin_t;
     float * q_out;                // NULL: in place
     int n_rows, n_rope, n_head, n_axis;
-    uint8_t axis[64];             // of each pair; n_axis and above: not rotated
+    uint32_t axis[16];            // a byte each pair; n_axis and above: not rotated
 } sml_kaxes;
 
 typedef struct {

@@ -5,7 +5,6 @@
 
 #include <math.h>
 #include <stdio.h>
-#include <stdlib.h>
 #include <string.h>
 
 int sml_hip_paged_append_axes(const sml_hip_pages * pg, float * qkv, size_t qkv_stride, int n_rows, const int32_t * seq,
@@ -52,34 +51,44 @@ static void items_launch(const char * name, int n_kv, long items, unsigned threa
     hx_launch3(name, (unsigned) n_kv, (unsigned) y, (unsigned) ((items + y - 1) / y), threads, lds, st, a);
 }
 
-static const struct form { const char * name; int cols, cw, pg, per_cu; } forms[] = {
-    { "rows64", 64, 2, 4, 1 }, { "rows128", 128, 4, 2, 1 },
-};
+// The two forms of the kernel: columns of a tile, waves beside each other, groups
+// of them over the positions.
+static const struct form { const char * name; int cols, cw, pg; } forms[] = { { "rows64", 64, 2, 4 }, { "rows128", 128, 4, 2 } };
+
 static void rows_launch(sml_krows * a, int hd, int type, hipStream_t st) {
     const int n_kv = a->pg.n_kv, rep = a->n_head / n_kv, n_seq = a->pg.n_seq;
     const int ncol = a->n_row * rep, some = n_seq < a->n_row ? n_seq : a->n_row;
-    int f = ncol > 40L * some && ((long) ceil_div(ncol, 128) * n_kv >= hx.ncu || (long) ceil_div(ncol, 64) * n_kv < hx.ncu);
-    if (getenv("RWF")) f = atoi(getenv("RWF"));
-    const struct form * const fm = forms + f;
-    a->cols = fm->cols;
+    // Tiles of 128 columns read the cache less often; those of 64 waste less of a
+    // few and make more workgroups. 128 from 40 columns a sequence on, unless 64
+    // alone make a workgroup for every CU (us a call at 64 / 128, 32 heads over 8 of
+    // 128, fp16; rows x sequences at positions: 8 x 48 to 4000 77 / 97, 16 x 4 to 3000
+    // 24.0 / 21.6, 26 x 16 to 8192 53 / 47, 200 x 1 at 1000 29.9 / 27, 509 at 2040
+    // 47 / 53, 1024 at 1024 50 / 45, 2047 at 4001 284 / 240).
+    const struct form * const f = forms + (ncol > 40L * some && ((long) ceil_div(ncol, 128) * n_kv >= hx.ncu || (long) ceil_div(ncol, 64) * n_kv < hx.ncu));
+    a->cols = f->cols;
     a->over = rep > 1 ? (uint32_t) (((1ull << 32) + (unsigned) rep - 1) / (unsigned) rep) : 0;
-    // workgroups that run at once; not split where the tiles are as many
-    const int want = ceil_div((hx.ncu < 256 ? hx.ncu : 256) * fm->per_cu, n_kv);
-    a->least = getenv("RWL") ? atoi(getenv("RWL")) : 2;
+    // One workgroup runs a CU: splits that make as many of them, of 128 positions at
+    // least; none where the tiles are half as many (1024 rows at 1024, 128 columns a
+    // tile, 33 tiles for 32 a KV head: 44.6 us so, 48.1 with the splits' launch).
+    const int want = ceil_div(hx.ncu < 256 ? hx.ncu : 256, n_kv);
+    a->least = 2;
     const int split = n_seq <= AT_SHARED && 2 * ceil_div(ncol, a->cols) <= want && a->max_len > RW_BLOCK * a->least;
     a->want = split ? want : 0;
-    long tiles = (long) ncol / a->cols + (split ? some : n_seq);
-    long items = split ? tiles + want : tiles;
+    const long tiles = (long) ncol / a->cols + (split ? some : n_seq), items = split ? tiles + want : tiles;
     a->items = (int) items;
     a->part_cols = ncol < a->cols ? ncol : a->cols;
-    const size_t stages = (size_t) fm->pg * 2 * (4 * 32 * hd + 4 * 32 + 4 * fm->cw) + (16 + 20 * 32) * fm->cw;
-    const size_t joined = fm->pg > 1 ? (size_t) fm->pg * fm->cols * ((hd + 4) * 4 + 8) : 0;
+    // LDS: two stages a group, their positions and what they hold that is not finite, and the
+    // columns' ranges; at the end the groups' sums
+    const size_t stages = (size_t) f->pg * 2 * (4 * 32 * hd + 4 * 32 + 4 * f->cw) + (16 + 20 * 32) * f->cw;
+    const size_t joined = (size_t) f->pg * f->cols * ((hd + 4) * 4 + 8);
     char base[24], name[40];
-    snprintf(base, sizeof base, "sml_rw_%s%s", fm->name, a->cap > 0.0f || a->slope ? "r" : "");
+    snprintf(base, sizeof base, "sml_rw_%s%s", f->name, a->cap > 0.0f || a->slope ? "r" : "");
     sv_name(name, sizeof name, base, hd, type);
-    items_launch(name, n_kv, items, 64 * (unsigned) (fm->cw * fm->pg), stages > joined ? stages : joined, st, a);
+    items_launch(name, n_kv, items, 64 * (unsigned) (f->cw * f->pg), stages > joined ? stages : joined, st, a);
     if (split) {
-        // a wave a column while that makes at most two workgroups a CU
+        // a wave a column while that makes at most two workgroups a CU (us of the
+        // merge at 4 / 16 columns a workgroup: one tile of 32 columns, 32 splits 4.0 /
+        // 5.5, 16 sequences of 36 to 104 columns 10.6 / 5.9)
         const int per = tiles * (a->cols / 4) * n_kv <= 2L * hx.ncu ? 4 : 16;
         snprintf(name, sizeof name, "sml_rw_merge%d%s", per, hd == 64 ? "_d64" : "");
         items_launch(name, n_kv, tiles * (a->cols / per), 256, 0, st, a);
@@ -97,9 +106,11 @@ int sml_hip_paged_attention_rows(const sml_hip_pages * pg, const sml_hip_rows * 
         hx_failf("rows' attention: %d rows, lengths up to %d", rows->n_row, rows->max_len);
     if (rows->tree && (rows->tree_words < 1 || rows->tree_words > 2048))
         hx_failf("rows' attention: %d words of a tree's bits a row (1 to 2048)", rows->tree_words);
-    if (!(rows->cap >= 0.0f) || isinf(rows->cap)) hx_failf("rows' attention: scores capped at %g", (double) rows->cap);
     if (n_head < 1 || n_head % pg->n_kv || n_head / pg->n_kv > 16)
         hx_failf("rows' attention: %d heads over %d kv heads (1 to 16 each)", n_head, pg->n_kv);
+    const float sc = scale != 0.0f ? scale : 1.0f / sqrtf((float) pg->hd);
+    if (!(rows->cap >= 0.0f) || isinf(rows->cap) || (rows->cap > 0.0f && isinf(sc / rows->cap)))
+        hx_failf("rows' attention: scores capped at %g", (double) rows->cap);
     if (!q || !part || !out) hx_failf("rows' attention: missing rows, workspace or output");
     if (!al16(part)) hx_failf("rows' attention: workspace off a 16-byte boundary");
     const size_t width = (size_t) n_head * pg->hd;
@@ -109,9 +120,8 @@ int sml_hip_paged_attention_rows(const sml_hip_pages * pg, const sml_hip_rows * 
         a.q = q; a.q_stride = q_stride ? q_stride : width; a.part = part; a.out = out;
         a.start = rows->start; a.len = rows->len; a.first = rows->first; a.last = rows->last; a.pos = rows->pos;
         a.tree = rows->tree; a.words = rows->tree_words; a.slope = rows->slope; a.cap = rows->cap;
-        if (scale == 0.0f) scale = 1.0f / sqrtf((float) pg->hd);
-        a.sign = scale < 0.0f ? -1.0f : 1.0f;
-        a.scale = rows->cap > 0.0f ? fabsf(scale) / rows->cap : fabsf(scale) * LOG2E;
+        a.sign = sc < 0.0f ? -1.0f : 1.0f;
+        a.scale = rows->cap > 0.0f ? fabsf(sc) / rows->cap : fabsf(sc) * LOG2E;
         a.cap = rows->cap * LOG2E;
         a.n_head = n_head; a.n_row = rows->n_row;
         const long cap = (long) pg->seq_pages * pg->page_size;

@@ -36,20 +36,29 @@ __device__ __forceinline__ void axes_body(const sml_kaxes & a) {
     const int h = i / HQ, d = 4 * (i % HQ);
     float * x = row + (size_t) h * D + d;
     const v4f lo = *(const v4fu *) x, hi = *(const v4fu *) (x + D / 2);
-    v4f y0, y1;
-    #pragma unroll
-    for (int e = 0; e < 4; e++) {
-        const int ax = a.axis[d + e];
-        float c = 1.0f, sn = 0.0f;
-        if (ax < a.n_axis) {
-            const size_t o = (size_t) (ax == 0 ? pos[0] : ax == 1 ? pos[1] : ax == 2 ? pos[2] : pos[3]) * (D / 2) + d + e;
-            c = a.cos_t[o];
-            sn = a.sin_t[o];
-            y0[e] = __builtin_fmaf(lo[e], c, -(hi[e] * sn));
-            y1[e] = __builtin_fmaf(lo[e], sn, hi[e] * c);
-        } else {
-            y0[e] = lo[e];
-            y1[e] = hi[e];
+    v4f y0 = lo, y1 = hi;
+    auto of_axis = [&](uint32_t ax) { return (size_t) (ax == 0 ? pos[0] : ax == 1 ? pos[1] : ax == 2 ? pos[2] : pos[3]) * (D / 2) + d; };
+    const uint32_t four = a.axis[d / 4];
+    if (four == (four & 255u) * 0x01010101u) {
+        if ((four & 255u) < (uint32_t) a.n_axis) {
+            const size_t o = of_axis(four & 255u);
+            const v4f c = *(const v4fu *) (a.cos_t + o), sn = *(const v4fu *) (a.sin_t + o);
+            #pragma unroll
+            for (int e = 0; e < 4; e++) {
+                y0[e] = __builtin_fmaf(lo[e], c[e], -(hi[e] * sn[e]));
+                y1[e] = __builtin_fmaf(lo[e], sn[e], hi[e] * c[e]);
+            }
+        }
+    } else {
+        #pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const uint32_t ax = four >> (8 * e) & 255u;
+            if (ax < (uint32_t) a.n_axis) {
+                const size_t o = of_axis(ax) + e;
+                const float c = a.cos_t[o], sn = a.sin_t[o];
+                y0[e] = __builtin_fmaf(lo[e], c, -(hi[e] * sn));
+                y1[e] = __builtin_fmaf(lo[e], sn, hi[e] * c);
+            }
         }
     }
     if (h < a.n_head) {
@@ -78,25 +87,38 @@ AXES(64, 1, sml_rw_append_d64_bf)
 // over the cache with a running base m.
 //
 // The (row, query head) pairs of a sequence and KV head are columns, a row's
-// heads side by side. A workgroup takes a tile of 16 W of them, 16 a wave, and a
-// split of the positions, in blocks of 64 whose keys and values all its waves
-// share in LDS. The matrix cores take S^T = K Q^T and O^T = V^T P^T, columns in
-// the columns. With the lane's c = lane % 16, g = lane / 16:
-// - K is read from LDS as the first operand: lane (c, g) takes position 16j + c's
-//   dims 32i + 8g..; S comes back as positions 16j + 4g + r of column c.
+// heads side by side. A workgroup of eight waves takes a tile of 64 or 128 of them
+// and a split of the positions: CW waves of 32 columns side by side, and PG such
+// groups that take blocks of 32 positions in turn and are joined in LDS at the end.
+// The matrix cores take S^T = K Q^T and O^T = V^T P^T in tiles of 32 x 32, columns
+// in the columns. With the lane's c = lane % 32, g = lane / 32:
+// - K is read from LDS as the first operand: lane (c, g) takes position c's dims
+//   16j + 8g..; score e comes back as position 8 (e / 4) + 4g + e % 4 of column c.
 // - That is just what the second product takes as P^T if its inner index 8g + i
-//   stands for position 4g + i of an even 16 positions (i < 4) or of the next odd
-//   ones: P never crosses lanes.
+//   stands for position 4g + i of 16 (i < 4) or 8 + 4g + i - 4: P never crosses
+//   lanes.
 // - V^T comes by transposing LDS reads (ds_read_b64_tr_b16: 16 lanes read 4 rows
 //   of 16 dims and take a dim's 4 rows each) in the same order, and lane (c, g)
-//   ends with dims 16u + 4g.. of column c: the base's rescaling is a lane's own.
+//   ends with dims 32u + 8 (e / 4) + 4g + e % 4 of column c: the base's rescaling is
+//   a lane's own.
 // q and the weights are split into 16-bit parts, as in sml_sv_attend, whose base
 // and room these are. K and V go from memory to LDS without registers, a block
-// ahead, 16-byte words swizzled by row so that both kinds of read touch each bank
-// as often as any other.
+// ahead, 16-byte words swizzled by row so that both kinds of read spread over the
+// banks; a chunk of the table is a lane's entry each, 1024 positions ahead.
+//
+// What bounds it: of many rows the matrix cores' rate on real data (2048 rows at
+// 16384, 32 heads over 8 of 128: 552 TFLOP/s of the formula, which in fp16's two
+// parts is 1104 of the 1217 that a large library product reaches; bf16 436, which
+// in three parts is 1308 of 1277). The same columns as 16 x 16 tiles took 10 to 20%
+// longer (a matrix instruction keeps the vector unit from issuing for more than
+// half of its time, so fewer and larger ones leave it more), 16 columns a wave
+// twice the LDS reads. A next block's scores made during this one's softmax,
+// with three stages, gained nothing: the two waves of a SIMD do that for each
+// other. Of few rows the chain of latencies bounds it (place, table, rows,
+// products, joining: 8.7 us at 4095 positions), then the cache's stream.
 //
 // Masks cost a block only where it is not whole for all of a wave's columns: each
-// lane then makes its column's 64 bits of the block, of the range, the tree and
+// lane then makes its column's 32 bits of the block, of the range, the tree and
 // the pages that are there. What a column does not attend to has no weight, but
 // 0 times a NaN or an infinity is none either: rows that no column of the tile
 // may see are loaded as zeros, and where columns differ, each wave looks its share
@@ -111,13 +133,13 @@ typedef short v4s __attribute__((ext_vector_type(4)));
 typedef float v16f __attribute__((ext_vector_type(16)));
 
 // What no column may see is read from here.
-__device__ const uint8_t rw_zeros[16] = { 0 };
+__device__ const __align__(16) uint8_t rw_zeros[16] = { 0 };
 
 // 16 bytes a lane straight into LDS, from an address of its own or from base + off,
-// the wave's 64 lanes side by side from dst (a wave-uniform address) on; the caller waits (vmcnt) and then meets the other
-// waves before any of the bytes is read. Written out because the compiler, which
-// cannot tell the buffers apart, otherwise waits for every copy in flight before
-// the next LDS read.
+// the wave's 64 lanes side by side from dst (a wave-uniform address) on; the caller
+// waits (vmcnt) and then meets the other waves before any of the bytes is read.
+// Written out because the compiler, which cannot tell the buffers apart, otherwise
+// waits for every copy in flight before the next LDS read.
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"             // m0 among the clobbers: it is what the statement sets
 __device__ __forceinline__ void copy_lds16(const void * src, const void * dst) {
@@ -747,67 +769,67 @@ __device__ __forceinline__ void rows_body(const sml_krows & a) {
 
     l += __shfl_xor(l, 32);
     if (!some) { base = -INFINITY; l = 0.0f; }
+    // The groups joined: their sums over the stages, rows of D + 4 floats on
+    // different banks, their bases and weights' sums behind.
+    constexpr int QT = 32 * CW, LD = D + 4;
+    float * const so = (float *) lds;
+    float2 * const sml = (float2 *) (lds + F::joined);
+    __syncthreads();                                  // all are done with the stages
     {
-        // The groups joined: their sums over the stages, rows of D + 4 floats on
-        // different banks, their bases and weights' sums behind.
-        constexpr int QT = 32 * CW, LD = D + 4;
-        float * const so = (float *) lds;
-        float2 * const sml = (float2 *) (lds + F::joined);
-        __syncthreads();                              // all are done with the stages
-        {
-            const int pc = 32 * cw + c;
-            float * const to = so + (size_t) (pgi * QT + pc) * LD + 4 * g;
+        const int pc = 32 * cw + c;
+        float * const to = so + (size_t) (pgi * QT + pc) * LD + 4 * g;
+        #pragma unroll
+        for (int u = 0; u < E; u++)
             #pragma unroll
-            for (int u = 0; u < E; u++)
-                #pragma unroll
-                for (int k = 0; k < 4; k++) *(v4f *) (to + 32 * u + 8 * k) = v4f{o[u][4 * k], o[u][4 * k + 1], o[u][4 * k + 2], o[u][4 * k + 3]};
-            if (!g) sml[pgi * QT + pc] = make_float2(base, l);
+            for (int k = 0; k < 4; k++) *(v4f *) (to + 32 * u + 8 * k) = v4f{o[u][4 * k], o[u][4 * k + 1], o[u][4 * k + 2], o[u][4 * k + 3]};
+        if (!g) sml[pgi * QT + pc] = make_float2(base, l);
+    }
+    __syncthreads();
+    #pragma unroll 1
+    for (int x = tid; x < QT * (D / 4); x += 64 * W) {
+        const int pc = x / (D / 4), d = 4 * (x % (D / 4)), col = col0 + pc;
+        if (col >= ncol) break;
+        float2 ml[PG];
+        v4f v[PG];
+        #pragma unroll
+        for (int k = 0; k < PG; k++) { ml[k] = sml[k * QT + pc]; v[k] = *(const v4f *) (so + (size_t) (k * QT + pc) * LD + d); }
+        float m = ml[0].x;
+        #pragma unroll
+        for (int k = 1; k < PG; k++) m = fmaxf(m, ml[k].x);
+        const float mu = m == -INFINITY ? 0.0f : m;
+        float ls = 0.0f;
+        v4f os = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+        #pragma unroll
+        for (int k = 0; k < PG; k++) {
+            const bool none = ml[k].x == -INFINITY && ml[k].y == 0.0f;    // what its sums hold counts for nothing
+            const float f = __builtin_amdgcn_exp2f(ml[k].x - mu);
+            ls += none ? 0.0f : f * ml[k].y;
+            #pragma unroll
+            for (int e = 0; e < 4; e++) os[e] = none ? os[e] : __builtin_fmaf(f, v[k][e], os[e]);
         }
-        __syncthreads();
-        #pragma unroll 1
-        for (int x = tid; x < QT * (D / 4); x += 64 * W) {
-            const int pc = x / (D / 4), d = 4 * (x % (D / 4)), col = col0 + pc;
-            if (col >= ncol) break;
-            float2 ml[PG];
-            v4f v[PG];
+        if (p.count == 1) {
+            const int i = rows_over(a, col);
             #pragma unroll
-            for (int k = 0; k < PG; k++) { ml[k] = sml[k * QT + pc]; v[k] = *(const v4f *) (so + (size_t) (k * QT + pc) * LD + d); }
-            float m = ml[0].x;
-            #pragma unroll
-            for (int k = 1; k < PG; k++) m = fmaxf(m, ml[k].x);
-            const float mu = m == -INFINITY ? 0.0f : m;
-            float ls = 0.0f;
-            v4f os = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-            #pragma unroll
-            for (int k = 0; k < PG; k++) {
-                const bool none = ml[k].x == -INFINITY && ml[k].y == 0.0f;    // what its sums hold counts for nothing
-                const float f = __builtin_amdgcn_exp2f(ml[k].x - mu);
-                ls += none ? 0.0f : f * ml[k].y;
-                #pragma unroll
-                for (int e = 0; e < 4; e++) os[e] = none ? os[e] : __builtin_fmaf(f, v[k][e], os[e]);
-            }
-            if (p.count == 1) {
-                const int i = rows_over(a, col);
-                #pragma unroll
-                for (int e = 0; e < 4; e++) os[e] = ls != 0.0f ? os[e] / ls : 0.0f;
-                *(v4fu *) (a.out + ((size_t) (sq.s0 + i) * a.n_head + kh * rep + (col - i * rep)) * D + d) = os;
-            } else {
-                if (!d) part_ml(a, kh, p.item + p.split, D)[pc] = make_float2(m, ls);
-                *(v4f *) (part_o(a, kh, p.item + p.split, D) + (size_t) pc * D + d) = os;
-            }
+            for (int e = 0; e < 4; e++) os[e] = ls != 0.0f ? os[e] / ls : 0.0f;
+            *(v4fu *) (a.out + ((size_t) (sq.s0 + i) * a.n_head + kh * rep + (col - i * rep)) * D + d) = os;
+        } else {
+            if (!d) part_ml(a, kh, p.item + p.split, D)[pc] = make_float2(m, ls);
+            *(v4f *) (part_o(a, kh, p.item + p.split, D) + (size_t) pc * D + d) = os;
         }
     }
 }
-#define ROWS(D, BF, CW, PG, EU, name, sfx) \
-    extern "C" __global__ __launch_bounds__(64 * CW * PG, EU) void name##sfx(const sml_krows a) { rows_body<D, BF, CW, PG, false>(a); } \
-    extern "C" __global__ __launch_bounds__(64 * CW * PG, EU) void name##r##sfx(const sml_krows a) { rows_body<D, BF, CW, PG, true>(a); }
-#define ROWS4(CW, PG, E, name) \
-    ROWS(128, 0, CW, PG, 2, name, ) \
-    ROWS(128, 1, CW, PG, 2, name, _bf) \
-    ROWS(64, 0, CW, PG, E, name, _d64) \
-    ROWS(64, 1, CW, PG, E, name, _d64_bf)
-ROWS4(2, 4, 2, sml_rw_rows64)
-ROWS4(4, 2, 2, sml_rw_rows128)
+// Two waves a SIMD: at three or four, heads of 64 spill (509 rows at 2040 30.7 us
+// so, 37.5 with two workgroups a CU).
+#define ROWS(D, BF, CW, PG, name, sfx) \
+    extern "C" __global__ __launch_bounds__(64 * CW * PG, 2) void name##sfx(const sml_krows a) { rows_body<D, BF, CW, PG, false>(a); } \
+    extern "C" __global__ __launch_bounds__(64 * CW * PG, 2) void name##r##sfx(const sml_krows a) { rows_body<D, BF, CW, PG, true>(a); }
+#define ROWS4(CW, PG, name) \
+    ROWS(128, 0, CW, PG, name, ) \
+    ROWS(128, 1, CW, PG, name, _bf) \
+    ROWS(64, 0, CW, PG, name, _d64) \
+    ROWS(64, 1, CW, PG, name, _d64_bf)
+ROWS4(2, 4, sml_rw_rows64)
+ROWS4(4, 2, sml_rw_rows128)
 
 // The splits of a tile joined, C columns a workgroup: the bases of a column's splits
 // shared out over its 256 / C lanes, then the splits over each 16 of them, which
