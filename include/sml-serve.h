@@ -127,7 +127,8 @@ typedef struct {
     // (NULL: its slot); an earlier slot's is its number.
     const int32_t * pos;          // [n_row], at most 2^30 in size
     const float * slope;          // [n_head], NULL: no bias
-    float cap;                    // a score s becomes cap * tanh(s / cap) before the bias; 0: it stays
+    float cap;                    // a score s becomes cap * tanh(s / cap) before the bias; 0: it stays.
+                                  //   Within a factor of 2^100 of |scale|
     int tree_words;
     int n_row;                    // 0..65535
     int max_len;                  // (host) bounds every length, as above

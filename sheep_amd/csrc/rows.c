@@ -109,7 +109,8 @@ int sml_hip_paged_attention_rows(const sml_hip_pages * pg, const sml_hip_rows * 
     if (n_head < 1 || n_head % pg->n_kv || n_head / pg->n_kv > 16)
         hx_failf("rows' attention: %d heads over %d kv heads (1 to 16 each)", n_head, pg->n_kv);
     const float sc = scale != 0.0f ? scale : 1.0f / sqrtf((float) pg->hd);
-    if (!(rows->cap >= 0.0f) || isinf(rows->cap) || (rows->cap > 0.0f && isinf(sc / rows->cap)))
+    if (!(rows->cap >= 0.0f) || isinf(rows->cap * LOG2E) ||
+        (rows->cap > 0.0f && !(fabsf(sc) <= 0x1p100f * rows->cap && rows->cap <= 0x1p100f * fabsf(sc))))
         hx_failf("rows' attention: scores capped at %g", (double) rows->cap);
     if (!q || !part || !out) hx_failf("rows' attention: missing rows, workspace or output");
     if (!al16(part)) hx_failf("rows' attention: workspace off a 16-byte boundary");

@@ -375,7 +375,7 @@ __device__ __forceinline__ void rows_body(const sml_krows & a) {
     const bool mine = col < ncol;
     const int r = sq.s0 + in_seq, h = kh * rep + (min(col, ncol - 1) - in_seq * rep);
     const int lo = a.first ? max(a.first[r], 0) : 0;
-    const int hi = min(a.last ? a.last[r] : a.tree ? past : past + in_seq + 1, sq.n);
+    const int hi = max(min(a.last ? a.last[r] : a.tree ? past : past + in_seq + 1, sq.n), 0);
     const int nbit = a.tree ? min(sq.m, 32 * a.words) : 0;
     uint64_t tw = 0;
     if (nbit) {

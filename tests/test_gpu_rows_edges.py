@@ -148,6 +148,27 @@ def test_trees_of_many_rows(dtype, m, words):
     rows_case([m, 2], [m + 77, 500], 6, 2, 64, dtype, 16, seed=m, mask="tree", idle=0.1, bad_slots={0: [80, 77 + m // 2]})
 
 
+@pytest.mark.parametrize("hd", [64, 128])
+def test_ranges_of_any_numbers(hd):
+    """Ranges past both ends of int32's room, alone and beside a tree's bits."""
+    rng = np.random.default_rng(12)
+    n, m = 200, 40
+    k, v = (so.to_bits(rng.standard_normal((1, n, 1, hd)), "f16") for _ in range(2))
+    q = rng.standard_normal((m, hd)).astype(np.float32)
+    least, most = -2 ** 31, 2 ** 31 - 1
+    first = np.array([least, most, 0, -1, 100, most, least, 150] * 5)
+    last = np.array([most, least, least, most, least, most, least, -7] * 5)
+    tree = ro.ancestors([-1] + list(range(m - 1)))
+    tree[::3] = False
+    for bits in (None, sa.DevBuf.of(ro.words(tree, 2))):
+        see = (np.arange(n) >= first[:, None]) & (np.arange(n) < last[:, None])
+        if bits:
+            see[:, n - m:] |= tree
+        got = attend(q, k, v, "f16", [0, m], [n], 1, first=ints(first), last=ints(last), tree=bits, tree_words=2 if bits else 0)
+        want, tol = ro.attend(q, so.from_bits(k[0, :, 0], "f16"), so.from_bits(v[0, :, 0], "f16"), hd ** -0.5, see)
+        within(got[:, 0], want, tol)
+
+
 def test_positions_far_apart():
     """A bias of distances past 2^24, which fp32 rounds by half a step, and of 0."""
     rng = np.random.default_rng(8)

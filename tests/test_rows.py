@@ -55,7 +55,8 @@ def test_append_axes_refusals(args, kw, match):
     (dict(start=None), {}, {}, "missing starts"), (dict(lens=None), {}, {}, "missing starts"), (dict(n_row=-1), {}, {}, "-1 rows"),
     (dict(n_row=65536), {}, {}, "65536 rows"), (dict(max_len=-1), {}, {}, "up to -1"), (dict(tree=A), {}, {}, "0 words"),
     (dict(tree=A, tree_words=2049), {}, {}, "2049 words"), (dict(cap=-1.0), {}, {}, "capped at -1"),
-    (dict(cap=1e-44), {}, {}, "capped"), (dict(cap=float("nan")), {}, {}, "capped"), (dict(cap=float("inf")), {}, {}, "capped"),
+    (dict(cap=1e-44), {}, {}, "capped"), (dict(cap=1e37), {}, {}, "capped"),
+    (dict(cap=3e38), {}, dict(scale=1e20), "capped"), (dict(cap=float("nan")), {}, {}, "capped"), (dict(cap=float("inf")), {}, {}, "capped"),
     ({}, dict(n_head=3), {}, "3 heads over 2"), ({}, dict(n_head=34), {}, "34 heads"), ({}, dict(q=None), {}, "missing rows"),
     ({}, dict(part=None), {}, "missing rows"), ({}, dict(out=None), {}, "missing rows"),
     ({}, dict(part=At(C.ptr + 8)), {}, "16-byte"), ({}, {}, dict(q_stride=511), "511 apart"),
