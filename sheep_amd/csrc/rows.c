@@ -51,28 +51,45 @@ static void items_launch(const char * name, int n_kv, long items, unsigned threa
     hx_launch3(name, (unsigned) n_kv, (unsigned) y, (unsigned) ((items + y - 1) / y), threads, lds, st, a);
 }
 
-// The two forms of the kernel: columns of a tile, waves beside each other, groups
-// of them over the positions.
-static const struct form { const char * name; int cols, cw, pg; } forms[] = { { "rows64", 64, 2, 4 }, { "rows128", 128, 4, 2 } };
+// The forms of the kernel: columns of a tile, waves beside each other, groups of
+// them over the positions. Eight waves have a CU to themselves; of four, two
+// workgroups share one, so that a short tile waits for no long one and one's
+// products run beside the other's softmax.
+static const struct form { const char * name; int cols, cw, pg; } forms[] = {
+    { "rows64", 64, 2, 4 }, { "rows64h", 64, 2, 2 }, { "rows128", 128, 4, 2 }, { "rows128h", 128, 4, 1 }
+};
+
+// Tiles of 128 columns read the cache less often; those of 64 waste less of a few
+// and make more workgroups. Measured as us a call, 32 heads over 8 of 128, fp16,
+// rows x sequences at positions.
+static const struct form * form_of(long ncol, long some, int n_kv) {
+    const long ncu = hx.ncu, t64 = (ncol + 63) / 64 * n_kv, t128 = (ncol + 127) / 128 * n_kv;
+    // long prompts, tiles for both places of every CU and more (128 / 128h / 64h: 4096 at 4096 295 / 291 / 299,
+    // 8192 at 8192 1073 / 1023 / 1105, 2000 x 2 at 2000 122 / 103 / 121; but 2600 at 8000 594 / 629 / 626)
+    if (t128 > 2 * ncu && ncol >= 2048 * some) return forms + 3;
+    // a tile and a half a CU (2048 at 16384 953 / 971 / 1018; 2047 of packed documents, 28 heads over 4, 97 / 152 / 116)
+    if (2 * t128 >= 3 * ncu && ncol >= 4096 * some) return forms + 2;
+    // four sequences, or more tiles of 64 than CUs (64 / 64h / 128: 8 x 16 to 3000 47 / 36 / 53, 26 x 16 to 8192
+    // 49 / 44 / 44, 8 x 48 to 4000 125 / 109 / 144, 33 x 200 to 600 213 / 130 / 164, 560 at 3000 98 / 85 / 89)
+    if (some >= 4 || 16 * t64 > 17 * ncu) return forms + 1;
+    // fewer (60 at 6000 28.9 / 31.3 / 30.6, 200 at 6000 61 / 62 / 58, 400 at 3000 56 / 61 / 58, 300 x 3 to 3000 70 /
+    // 76 / 88)
+    return forms;
+}
 
 static void rows_launch(sml_krows * a, int hd, int type, hipStream_t st) {
     const int n_kv = a->pg.n_kv, rep = a->n_head / n_kv, n_seq = a->pg.n_seq;
     const int ncol = a->n_row * rep, some = n_seq < a->n_row ? n_seq : a->n_row;
-    // Tiles of 128 columns read the cache less often; those of 64 waste less of a
-    // few and make more workgroups. 128 from 40 columns a sequence on, unless 64
-    // alone make a workgroup for every CU (us a call at 64 / 128, 32 heads over 8 of
-    // 128, fp16; rows x sequences at positions: 8 x 48 to 4000 77 / 97, 16 x 4 to 3000
-    // 24.0 / 21.6, 26 x 16 to 8192 53 / 47, 200 x 1 at 1000 29.9 / 27, 509 at 2040
-    // 47 / 53, 1024 at 1024 50 / 45, 2047 at 4001 284 / 240).
-    const struct form * const f = forms + (ncol > 40L * some && ((long) ceil_div(ncol, 128) * n_kv >= hx.ncu || (long) ceil_div(ncol, 64) * n_kv < hx.ncu));
+    const struct form * const f = form_of(ncol, some, n_kv);
     a->cols = f->cols;
     a->over = rep > 1 ? (uint32_t) (((1ull << 32) + (unsigned) rep - 1) / (unsigned) rep) : 0;
-    // One workgroup runs a CU: splits that make as many of them, of 128 positions at
-    // least; none where the tiles are half as many (1024 rows at 1024, 128 columns a
-    // tile, 33 tiles for 32 a KV head: 44.6 us so, 48.1 with the splits' launch).
-    const int want = ceil_div(hx.ncu < 256 ? hx.ncu : 256, n_kv);
+    // Splits make a workgroup for every place on the card, of 128 positions at least;
+    // none where the tiles are half as many (1024 rows at 1024, 128 columns a tile, 33
+    // tiles for 32 places a KV head: 44.6 us so, 48.1 with the splits' launch), or a
+    // place's sequences one each.
+    const int want = ceil_div((f->cw * f->pg == 8 ? 1 : 2) * (hx.ncu < 256 ? hx.ncu : 256), n_kv);
     a->least = 2;
-    const int split = n_seq <= AT_SHARED && 2 * ceil_div(ncol, a->cols) <= want && a->max_len > RW_BLOCK * a->least;
+    const int split = n_seq <= AT_SHARED && some < want && 2 * ceil_div(ncol, a->cols) <= want && a->max_len > RW_BLOCK * a->least;
     a->want = split ? want : 0;
     const long tiles = (long) ncol / a->cols + (split ? some : n_seq), items = split ? tiles + want : tiles;
     a->items = (int) items;

@@ -90,9 +90,10 @@ AXES(64, 1, sml_rw_append_d64_bf)
 // over the cache with a running base m.
 //
 // The (row, query head) pairs of a sequence and KV head are columns, a row's
-// heads side by side. A workgroup of eight waves takes a tile of 64 or 128 of them
-// and a split of the positions: CW waves of 32 columns side by side, and PG such
-// groups that take blocks of 32 positions in turn and are joined in LDS at the end.
+// heads side by side. A workgroup of eight or four waves takes a tile of
+// 64 or 128 of them and a split of the positions: CW waves of 32 columns side by
+// side, and PG such groups that take blocks of 32 positions in turn and are joined
+// in LDS at the end.
 // The matrix cores take S^T = K Q^T and O^T = V^T P^T in tiles of 32 x 32, columns
 // in the columns. With the lane's c = lane % 32, g = lane / 32:
 // - K is read from LDS as the first operand: lane (c, g) takes position c's dims
@@ -247,7 +248,7 @@ __device__ __forceinline__ bool rows_place(const sml_krows & a, int i, int lane,
         }
     sum = wave_total(sum);
     int chunk = max(a.least, (int) (sum * 1.0001f / (float) a.want) + 1);
-    for (int tries = 0; tries < 3; tries++) {
+    for (int tries = 0; tries < 8; tries++) {
         float made = 0.0f;
         #pragma unroll
         for (int k = 0; k < AT_SHARED / 64; k++)
@@ -835,6 +836,8 @@ __device__ __forceinline__ void rows_body(const sml_krows & a) {
     ROWS(64, 1, CW, PG, name, _d64_bf)
 ROWS4(2, 4, sml_rw_rows64)
 ROWS4(4, 2, sml_rw_rows128)
+ROWS4(2, 2, sml_rw_rows64h)
+ROWS4(4, 1, sml_rw_rows128h)
 
 // The splits of a tile joined, C columns a workgroup: the bases of a column's splits
 // shared out over its 256 / C lanes, then the splits over each 16 of them, which

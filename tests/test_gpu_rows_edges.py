@@ -356,6 +356,44 @@ def test_a_path_as_long_as_may_be_kept():
         np.testing.assert_array_equal(b.read(np.uint16).reshape(-1, hd), want)
 
 
+@pytest.mark.parametrize("rules", [False, True])
+@pytest.mark.parametrize("m, n", [(1601, 1700), (2100, 2100)])
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_long_prompts(hd, dtype, m, n, rules):
+    """Tiles enough for a CU and a half, and for two workgroups of every CU: 32
+    heads over 8, two of them looked at in all rows. With rules, windows, a tree, rows of
+    padding, a cap and the bias of distance; infinities where only some rows look."""
+    rng = np.random.default_rng(m + hd)
+    k, v = (so.to_bits(rng.standard_normal((1, n, 8, hd)), dtype) for _ in range(2))
+    q = rng.standard_normal((m, 32, hd)).astype(np.float32)
+    row, past = np.arange(m), n - m
+    see = np.arange(n)[None] <= past + row[:, None]
+    kw = {}
+    if rules:
+        first = np.where(row % 7 == 3, n, np.maximum(0, row - 300))
+        last = np.where(row % 5 == 1, 0, past + row // 2)
+        tree = rng.random((m, m)) < 0.05
+        tree[row % 11 == 2] = False
+        bits = np.packbits(np.pad(tree, ((0, 0), (0, -m % 32))), axis=1, bitorder="little").view(np.uint32)
+        see = (np.arange(n) >= first[:, None]) & (np.arange(n) < last[:, None])
+        see[:, past:] |= tree
+        slope = rng.uniform(0, 0.02, 32).astype(np.float32)
+        pos = past + rng.permutation(m)
+        kw = dict(first=ints(first), last=ints(last), tree=sa.DevBuf.of(bits), tree_words=bits.shape[1], slope=sa.DevBuf.of(slope), pos=ints(pos),
+                  cap=20.0)
+        far = np.abs(pos[:, None] - np.concatenate([np.arange(past), pos])[None]).astype(np.float64)
+        v[0, [5, 600], :, 1] = 0x7C00 if dtype == "f16" else 0x7F80
+    got = attend(q.reshape(m, -1), k, v, dtype, [0, m], [n], 32, **kw)
+    for h in (5, 30):
+        kk, vv = (so.from_bits(x[0, :, h // 4], dtype) for x in (k, v))
+        bad = see[:, [5, 600]].any(1) if rules else np.zeros(m, bool)
+        assert np.isnan(got[bad, h]).any(1).all()
+        want, tol = ro.attend(q[:, h], kk, np.where(np.isfinite(vv), vv, 0), hd ** -0.5, see, *((20.0, float(slope[h]) * far) if rules else ()))
+        within(got[~bad, h], want[~bad], tol[~bad], f"head {h}")
+        assert not rules or (0 < bad.sum() < m and (got[~see.any(1), h] == 0).all() and (~see.any(1)).any())
+
+
 # ------------------------------------------------------------ streams and graphs
 
 def step_state(seed, ms=(9, 1, 30, 4), most=8):
