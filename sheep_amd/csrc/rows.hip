@@ -118,8 +118,8 @@ AXES(64, 1, sml_rw_append_d64_bf)
 // half of its time, so fewer and larger ones leave it more), 16 columns a wave
 // twice the LDS reads. A next block's scores made during this one's softmax,
 // with three stages, gained nothing: the two waves of a SIMD do that for each
-// other. Neither did a third stage alone (16 x 26 rows 45 us for 46, 2047 rows of
-// packed documents in bfloat16 155 for 151) nor a wave's priority raised in its
+// other. Neither did a third stage alone (of 128 columns and eight waves, 16 x 26
+// rows 45 us for 46, 2047 rows of packed documents in bfloat16 155 for 151) nor a wave's priority raised in its
 // products or its softmax. Of few rows the chain of latencies bounds it (place, table, rows,
 // products, joining: 8.7 us at 4095 positions), then the cache's stream.
 //
