@@ -91,7 +91,8 @@ static void rows_launch(sml_krows * a, int hd, int type, hipStream_t st) {
     a->least = 2;
     const int split = n_seq <= AT_SHARED && some < want && 2 * ceil_div(ncol, a->cols) <= want && a->max_len > RW_BLOCK * a->least;
     a->want = split ? want : 0;
-    const long tiles = (long) ncol / a->cols + (split ? some : n_seq), items = split ? tiles + want : tiles;
+    const long tiles = n_seq == 1 ? ceil_div(ncol, a->cols) : (long) ncol / a->cols + (split ? some : n_seq);
+    const long items = split && tiles < want ? want : tiles;
     a->items = (int) items;
     a->part_cols = ncol < a->cols ? ncol : a->cols;
     // LDS: two stages a group, their positions and what they hold that is not finite, and the

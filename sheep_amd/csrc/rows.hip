@@ -119,9 +119,10 @@ AXES(64, 1, sml_rw_append_d64_bf)
 // twice the LDS reads. A next block's scores made during this one's softmax,
 // with three stages, gained nothing: the two waves of a SIMD do that for each
 // other. Neither did a third stage alone (of 128 columns and eight waves, 16 x 26
-// rows 45 us for 46, 2047 rows of packed documents in bfloat16 155 for 151) nor a wave's priority raised in its
-// products or its softmax. Of few rows the chain of latencies bounds it (place, table, rows,
-// products, joining: 8.7 us at 4095 positions), then the cache's stream.
+// rows 45 us for 46, 2047 rows of packed documents in bfloat16 155 for 151) nor a
+// wave's priority raised in its products or its softmax. Of few rows the chain of
+// latencies bounds it (place, table, rows, products, joining: 8.7 us at 4095
+// positions), then the cache's stream.
 //
 // Masks cost a block only where it is not whole for all of a wave's columns: each
 // lane then makes its column's 32 bits of the block, of the range, the tree and
@@ -133,8 +134,8 @@ AXES(64, 1, sml_rw_append_d64_bf)
 //
 // Lengths and counts are ragged and on the device: every wave sums them up and
 // finds its workgroup's tile and split (rows_place), splits of one size for all
-// but cut to what a tile's rows see. Calls with tiles enough are not split, and
-// sequences past AT_SHARED neither; those tiles are found by halving.
+// but cut to what a tile's rows see. Calls with tiles enough are not split, nor
+// sequences past AT_SHARED, whose tiles are found by halving.
 typedef short v4s __attribute__((ext_vector_type(4)));
 typedef float v16f __attribute__((ext_vector_type(16)));
 
@@ -194,14 +195,17 @@ __device__ __forceinline__ int most32(int v) {
 
 struct rows_block { int t, pa, pb; uint64_t aa, ab; };  // a step's start, a group's block's two pages and their places in a pool
 struct rows_at { int b, tile, count, split, item; rows_of sq; };  // a tile, its splits, this one's number, the first's among all items
-// Item i's (or, of TILES, tile i's) place; false past the last. Without splits
-// (want 0) sequence b's tiles are numbered from start[b] * rep / cols + b on, which
-// leaves each as many numbers as it has tiles, and the number says whose it is.
+// Item i's (or, of TILES, tile i's) place; false past the last. Numbers run through
+// the items without a gap, so that workgroups that run at once lie evenly (64
+// sequences of up to 8 rows to 2000 in 75 us, 91 with gaps). Of more sequences than
+// AT_SHARED, which are not split, b's tiles are numbered from start[b] * rep / cols +
+// b on, which leaves each as many numbers as it has tiles, and the number says whose
+// it is.
 template <bool TILES>
 __device__ __forceinline__ bool rows_place(const sml_krows & a, int i, int lane, rows_at & p) {
     const int rep = a.n_head / a.pg.n_kv, cols = a.cols;
     const bool turned = !a.first && !a.last;          // causal rows: the last tiles see most, and begin
-    if (!a.want) {
+    if (a.pg.n_seq > AT_SHARED) {
         int lo = 0, hi = a.pg.n_seq;
         while (hi - lo > 1) {
             const int step = (hi - lo + 63) / 64, at = lo + lane * step;
@@ -232,8 +236,8 @@ __device__ __forceinline__ bool rows_place(const sml_krows & a, int i, int lane,
         if (turned) p.tile = nt - 1 - p.tile;
         return p.item < nt * p.count;
     }
-    // The blocks of a split: what makes want of them in all if each tile's came out
-    // even, and more until they are no more than that, or a tile's each.
+    // The blocks of a split (want 0: all): what makes want of them in all if each tile's came out
+    // even, and more until they are no more than that; else a tile's each.
     rows_of x[AT_SHARED / 64];
     int nb[AT_SHARED / 64], nt[AT_SHARED / 64];
     float sum = 0.0f;
@@ -247,15 +251,15 @@ __device__ __forceinline__ bool rows_place(const sml_krows & a, int i, int lane,
             sum += (float) nt[k] * (float) nb[k];
         }
     sum = wave_total(sum);
-    int chunk = max(a.least, (int) (sum * 1.0001f / (float) a.want) + 1);
-    for (int tries = 0; tries < 8; tries++) {
+    int chunk = a.want ? max(a.least, (int) (sum * 1.0001f / (float) a.want) + 1) : 1 << 30;
+    for (int tries = 0; a.want && tries < 8; tries++) {
         float made = 0.0f;
         #pragma unroll
         for (int k = 0; k < AT_SHARED / 64; k++)
             if (k == 0 || 64 * k < a.pg.n_seq) made += (float) (nt[k] * max((nb[k] + chunk - 1) / chunk, 1));
         made = wave_total(made);
         if (made <= (float) a.want) break;
-        chunk += (int) ((float) chunk * (made / (float) a.want - 1.0f)) + 1;
+        chunk = tries < 6 ? chunk + (int) ((float) chunk * (made / (float) a.want - 1.0f)) + 1 : 1 << 30;
     }
     p.item = 0;
     #pragma unroll
