@@ -203,13 +203,13 @@ struct rows_at { int b, tile, count, split, item; rows_of sq; };  // a tile, its
 // it is.
 template <bool TILES>
 __device__ __forceinline__ bool rows_place(const sml_krows & a, int i, int lane, rows_at & p) {
-    const int rep = a.n_head / a.pg.n_kv, cols = a.cols;
+    const int rep = a.n_head / a.pg.n_kv, cols = a.cols, cl = __builtin_ctz(a.cols);
     const bool turned = !a.first && !a.last;          // causal rows: the last tiles see most, and begin
     if (a.pg.n_seq > AT_SHARED) {
         int lo = 0, hi = a.pg.n_seq;
         while (hi - lo > 1) {
             const int step = (hi - lo + 63) / 64, at = lo + lane * step;
-            const bool in = at < hi && min(max(a.start[at], 0), a.n_row) * rep / cols + at <= i;
+            const bool in = at < hi && (min(max(a.start[at], 0), a.n_row) * rep >> cl) + at <= i;
             const unsigned long long hit = __ballot(in);
             const int k = hit ? 63 - __builtin_clzll(hit) : 0;
             lo += k * step;
@@ -217,7 +217,7 @@ __device__ __forceinline__ bool rows_place(const sml_krows & a, int i, int lane,
         }
         p.sq = rows_seq(a, lo);
         p.b = lo;
-        const int e = i - (p.sq.s0 * rep / cols + lo), nt = (p.sq.m * rep + cols - 1) / cols;
+        const int e = i - ((p.sq.s0 * rep >> cl) + lo), nt = (p.sq.m * rep + cols - 1) >> cl;
         p.tile = turned ? nt - 1 - e : e;
         p.count = 1;
         p.split = 0;
@@ -226,7 +226,7 @@ __device__ __forceinline__ bool rows_place(const sml_krows & a, int i, int lane,
     }
     if (a.pg.n_seq == 1) {
         p.sq = rows_seq(a, 0);
-        const int nb = (p.sq.n + RW_BLOCK - 1) / RW_BLOCK, nt = (p.sq.m * rep + cols - 1) / cols, most = max(a.want / max(nt, 1), 1);
+        const int nb = (p.sq.n + RW_BLOCK - 1) / RW_BLOCK, nt = (p.sq.m * rep + cols - 1) >> cl, most = max(a.want / max(nt, 1), 1);
         const int chunk = max(a.least, (nb + most - 1) / most);
         p.b = 0;
         p.count = max((nb + chunk - 1) / chunk, 1);
@@ -236,8 +236,10 @@ __device__ __forceinline__ bool rows_place(const sml_krows & a, int i, int lane,
         if (turned) p.tile = nt - 1 - p.tile;
         return p.item < nt * p.count;
     }
-    // The blocks of a split (want 0: all): what makes want of them in all if each tile's came out
-    // even, and more until they are no more than that; else a tile's each.
+    // The blocks of a split (want 0: all): what makes want of them in all if each
+    // tile's came out even, and more until they are no more than that; else a tile's
+    // each. How many that makes of a tile's blocks need not be exact, but the same
+    // everywhere: a product with the reciprocal, rounded up.
     rows_of x[AT_SHARED / 64];
     int nb[AT_SHARED / 64], nt[AT_SHARED / 64];
     float sum = 0.0f;
@@ -246,26 +248,29 @@ __device__ __forceinline__ bool rows_place(const sml_krows & a, int i, int lane,
         if (k == 0 || 64 * k < a.pg.n_seq) {
             x[k] = rows_of{0, 0, 0};
             if (64 * k + lane < a.pg.n_seq) x[k] = rows_seq(a, 64 * k + lane);
-            nt[k] = (x[k].m * rep + cols - 1) / cols;
+            nt[k] = (x[k].m * rep + cols - 1) >> cl;
             nb[k] = (x[k].n + RW_BLOCK - 1) / RW_BLOCK;
             sum += (float) nt[k] * (float) nb[k];
         }
     sum = wave_total(sum);
     int chunk = a.want ? max(a.least, (int) (sum * 1.0001f / (float) a.want) + 1) : 1 << 30;
+    float per = __builtin_amdgcn_rcpf((float) chunk);
+    auto splits = [&](int blocks) { return max((int) __builtin_ceilf((float) blocks * per), 1); };
     for (int tries = 0; a.want && tries < 8; tries++) {
         float made = 0.0f;
         #pragma unroll
         for (int k = 0; k < AT_SHARED / 64; k++)
-            if (k == 0 || 64 * k < a.pg.n_seq) made += (float) (nt[k] * max((nb[k] + chunk - 1) / chunk, 1));
+            if (k == 0 || 64 * k < a.pg.n_seq) made += (float) (nt[k] * splits(nb[k]));
         made = wave_total(made);
         if (made <= (float) a.want) break;
         chunk = tries < 6 ? chunk + (int) ((float) chunk * (made / (float) a.want - 1.0f)) + 1 : 1 << 30;
+        per = __builtin_amdgcn_rcpf((float) chunk);
     }
     p.item = 0;
     #pragma unroll
     for (int k = 0; k < AT_SHARED / 64; k++)
         if (k == 0 || 64 * k < a.pg.n_seq) {
-            const int count = max((nb[k] + chunk - 1) / chunk, 1);
+            const int count = splits(nb[k]);
             const int items = wave_scan(nt[k] * count), mine = TILES ? wave_scan(nt[k]) : items;
             const unsigned long long hit = __ballot(mine > i);
             if (hit) {
