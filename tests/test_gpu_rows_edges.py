@@ -356,6 +356,23 @@ def test_a_path_as_long_as_may_be_kept():
         np.testing.assert_array_equal(b.read(np.uint16).reshape(-1, hd), want)
 
 
+@pytest.mark.parametrize("kv", [257, 4096])
+def test_as_many_heads_as_there_may_be(kv):
+    """More KV heads than there are CUs, some of them looked at."""
+    rng = np.random.default_rng(kv)
+    n, ms = 150, [2, 0, 5, 1, 3]
+    k, v = (so.to_bits(rng.standard_normal((5, n, kv, 64)), "f16") for _ in range(2))
+    start = np.concatenate([[0], np.cumsum(ms)])
+    q = rng.standard_normal((11, kv, 64)).astype(np.float32)
+    got = attend(q.reshape(11, -1), k, v, "f16", start, [n, 5, 70, 129, 3], kv)
+    for h in (0, 1, 200, kv - 1):
+        for b, (m, ln) in enumerate(zip(ms, [n, 5, 70, 129, 3])):
+            see = np.arange(ln)[None] <= ln - m + np.arange(m)[:, None]
+            rows = slice(start[b], start[b + 1])
+            want, tol = ro.attend(q[rows, h], so.from_bits(k[b, :ln, h], "f16"), so.from_bits(v[b, :ln, h], "f16"), 0.125, see)
+            within(got[rows, h], want, tol, f"sequence {b}, head {h}")
+
+
 @pytest.mark.parametrize("rules", [False, True])
 @pytest.mark.parametrize("m, n", [(1601, 1700), (2100, 2100)])
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
