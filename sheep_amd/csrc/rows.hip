@@ -931,11 +931,13 @@ __device__ __forceinline__ uint16_t * pool_of(const sml_kpages & pg, size_t laye
 //
 // Every workgroup walks its sequence's tree for itself: a step is the first row
 // behind the present one that follows it with its pick, 64 rows looked at a time
-// by one wave. A thread then moves 16 bytes of a position in one pool, the
-// path's rows in order: a row's new place lies before every later row's old one,
-// so nothing is overwritten that is still to be read. Latency bounds it, the walk's
-// chain of loads and then the path's copies: 3.8 us for 8 rows in 32 layers, 4.8
-// for 16 sequences of up to 26 in 28.
+// by one wave (up to 64 in all are loaded once, a lane each). A thread then moves 16
+// bytes of a position in one pool, a few of the path's rows at a time, in order: a
+// row's new place lies before every later row's old one, so nothing is overwritten
+// that is still to be read. Latency bounds it, the walk's chain of loads and then the
+// path's copies: 3.7 us for 8 rows in 32 layers, 4.6 for 16 sequences of up to 26 in
+// 28 (3.9 and 4.8 with a load a step of the walk and a row's copy at a time).
+#define AC_AHEAD 4
 extern "C" __global__ __launch_bounds__(256) void sml_rw_accept(const sml_kaccept a) {
     __shared__ int path[AC_MOST], count;
     const int b = blockIdx.y, tid = threadIdx.x, lane = tid & 63;
@@ -946,6 +948,19 @@ extern "C" __global__ __launch_bounds__(256) void sml_rw_accept(const sml_kaccep
         if (m > 0) {
             if (!lane) path[0] = 0;
             k = 1;
+        }
+        if (m > 0 && m <= 64) {                       // a row a lane
+            const bool in = lane < m;
+            const int up = in ? a.parent[s0 + lane] : -1, tok = in ? a.tok[s0 + lane] : 0, pick = in ? a.pick[s0 + lane] : -1;
+            while (k < a.most) {
+                const int want = __builtin_amdgcn_readlane(pick, at);
+                const unsigned long long hit = __ballot(want >= 0 && lane > at && up == at && tok == want);
+                if (!hit) break;
+                at = __builtin_ctzll(hit);
+                if (!lane) path[k] = at;
+                k++;
+            }
+        } else if (m > 0) {
             while (k < a.most) {
                 const int want = a.pick[s0 + at];
                 if (want < 0) break;
@@ -976,17 +991,26 @@ extern "C" __global__ __launch_bounds__(256) void sml_rw_accept(const sml_kaccep
         }
     }
     const int row = a.pg.n_kv * a.pg.hd / 8;          // 16-byte units of a position
-    const long u = (long) blockIdx.x * 256 + tid;
-    if (u >= (long) 2 * a.n_layer * row) return;
-    uint16_t * const pool = pool_of(a.pg, a.layer_stride, (int) (u / row)) + 8 * (u % row);
+    const uint32_t u = blockIdx.x * 256 + tid, z = u / (uint32_t) row;    // 2^31 units at most
+    if (u >= 2u * (uint32_t) a.n_layer * (uint32_t) row) return;
+    uint16_t * const pool = pool_of(a.pg, a.layer_stride, (int) z) + 8 * (u - z * (uint32_t) row);
     const int sh = a.pg.page_shift, pmask = (1 << sh) - 1;
-    for (int j = 1; j < k; j++) {
-        const int from = past + path[j], to = past + j;
-        if (from == to || to < 0) continue;
-        const int pf = page_of(a.pg, b, from >> sh), pt = page_of(a.pg, b, to >> sh);
-        if (pf < 0 || pt < 0) continue;
-        const v4u w = *(const v4u *) (pool + (size_t) pf * a.pg.page_stride + (size_t) (from & pmask) * 8 * row);
-        *(v4u *) (pool + (size_t) pt * a.pg.page_stride + (size_t) (to & pmask) * 8 * row) = w;
+    for (int j0 = 1; j0 < k; j0 += AC_AHEAD) {
+        v4u w[AC_AHEAD];
+        v4u * to[AC_AHEAD];
+        #pragma unroll
+        for (int e = 0; e < AC_AHEAD; e++) {
+            const int j = j0 + e, from = past + (j < k ? path[j] : j), at = past + j;
+            to[e] = NULL;
+            if (from == at || at < 0) continue;
+            const int pf = page_of(a.pg, b, from >> sh), pt = page_of(a.pg, b, at >> sh);
+            if (pf < 0 || pt < 0) continue;
+            w[e] = *(const v4u *) (pool + (size_t) pf * a.pg.page_stride + (size_t) (from & pmask) * 8 * row);
+            to[e] = (v4u *) (pool + (size_t) pt * a.pg.page_stride + (size_t) (at & pmask) * 8 * row);
+        }
+        #pragma unroll
+        for (int e = 0; e < AC_AHEAD; e++)
+            if (to[e]) *to[e] = w[e];
     }
 }
 
