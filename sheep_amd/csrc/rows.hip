@@ -575,7 +575,10 @@ __device__ __forceinline__ void rows_body(const sml_krows & a) {
     }
     const int q0 = qpos - 4 * g;                      // the row's position, less where the lane's first score is
     const float slope = RULES && a.slope ? -1.44269504088896341f * a.slope[h] : 0.0f;
-    const float f = RULES ? 1.0f : back;              // log2 weights are f times the settled scores
+    // log2 weights are f times the settled scores. Masked ones are -infinity, of which
+    // 0 would make NaN: a factor that fp32 does not hold (a row of q below 2^-137, or
+    // a scale as small) becomes its least, and scores stay below 2^-115.
+    const float f = RULES ? 1.0f : fmaxf(back, 0x1p-149f);
 
     v16f o[E];
     #pragma unroll
