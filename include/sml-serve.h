@@ -83,11 +83,12 @@ size_t sml_hip_paged_part_floats(int n_seq, int n_head, int hd, int max_len);
 // cache in the matrix cores as sums of 16-bit parts that together hold them to
 // fp32's accuracy. Finite queries, keys and values give finite outputs wherever
 // fp32 holds q * scale, the sums of |q_d k_d|, twice those times |scale|, and
-// the sums of weight * |value|, the largest weight 1; an infinite key or value
-// that a sequence does attend over makes its KV head's outputs NaN, an infinite
-// query its own head's. How the positions are split follows all of the lengths:
-// a sequence's sums depend on the others by their rounding alone, and equal
-// calls give equal bits.
+// the sums of weight * |value|, the largest weight 1; an infinite or NaN value that
+// a sequence does attend over makes its dim of its KV head's outputs infinite or
+// NaN, however small its weight, and no other; an infinite key makes its KV head's
+// outputs NaN, an infinite query its own head's. How the positions are split
+// follows all of the lengths: a sequence's sums depend on the others by their
+// rounding alone, and equal calls give equal bits.
 int sml_hip_paged_attention(const sml_hip_pages * pg, const float * q, size_t q_stride, const int32_t * len,
                             int max_len, int n_head, float scale, float * part, float * out, void * stream);
 

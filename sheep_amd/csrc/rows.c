@@ -96,13 +96,13 @@ static void rows_launch(sml_krows * a, int hd, int type, hipStream_t st) {
     a->items = (int) items;
     a->part_cols = ncol < a->cols ? ncol : a->cols;
     // LDS: two stages a group, their positions and what they hold that is not finite, and the
-    // columns' ranges; at the end the groups' sums
-    const size_t stages = (size_t) f->pg * 2 * (4 * 32 * hd + 4 * 32 + 4 * f->cw) + (16 + 20 * 32) * f->cw;
+    // columns' ranges; at the end the groups' sums; behind both a bit for each column's dims
+    const size_t stages = (size_t) f->pg * 2 * (4 * 32 * hd + 4 * 32 + 4 * f->cw + 4 * hd) + (16 + 20 * 32 + 4 * 32 * f->pg) * f->cw;
     const size_t joined = (size_t) f->pg * f->cols * ((hd + 4) * 4 + 8);
     char base[24], name[40];
     snprintf(base, sizeof base, "sml_rw_%s%s", f->name, a->cap > 0.0f || a->slope ? "r" : "");
     sv_name(name, sizeof name, base, hd, type);
-    items_launch(name, n_kv, items, 64 * (unsigned) (f->cw * f->pg), stages > joined ? stages : joined, st, a);
+    items_launch(name, n_kv, items, 64 * (unsigned) (f->cw * f->pg), (stages > joined ? stages : joined) + (size_t) f->cols * hd / 8, st, a);
     if (split) {
         // a wave a column while that makes at most two workgroups a CU (us of the
         // merge at 4 / 16 columns a workgroup: one tile of 32 columns, 32 splits 4.0 /

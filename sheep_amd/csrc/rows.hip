@@ -130,7 +130,8 @@ AXES(64, 1, sml_rw_append_d64_bf)
 // 0 times a NaN or an infinity is none either: rows that no column of the tile
 // may see are loaded as zeros, and where columns differ, each wave looks its share
 // of the values through on its arrival, puts zeros for those that are not finite
-// and notes their positions: a column that attends to one gets NaN.
+// and notes their positions: a column that attends to one gets NaN in its dim
+// (spoiled), as the products leave an infinity or NaN there where columns agree.
 //
 // Lengths and counts are ragged and on the device: every wave sums them up and
 // finds its workgroup's tile and split (rows_place), splits of one size for all
@@ -343,11 +344,13 @@ __device__ __forceinline__ uint32_t bits_range(int lo, int hi) {
 }
 
 // A form of the rows' attention: CW waves of 32 columns beside each other, PG
-// groups of them; two stages of 32 positions a group, and where the groups'
-// joined sums end.
+// groups of them; two stages of 32 positions a group, where the groups' joined
+// sums end, and the dims that are no longer finite, behind both.
 template <int D, int CW, int PG> struct RowsForm {
     static constexpr int stages = PG * 2 * 4 * 32 * D;
     static constexpr int joined = PG * 32 * CW * (D + 4) * 4;
+    static constexpr int filled = stages + PG * 2 * 4 * (32 + CW + D) + (16 + 20 * 32 + 4 * 32 * PG) * CW, joining = joined + PG * 32 * CW * 8;
+    static constexpr int spoiled = filled > joining ? filled : joining;
 };
 
 template <int BF> struct Mx32;
@@ -378,6 +381,9 @@ __device__ __forceinline__ void rows_body(const sml_krows & a) {
     int * const red = (int *) (lds + F::stages + 4 * PG * 2 * (KB + CW));
     int4 * const about = (int4 *) (red + 4 * CW);     // of the columns, for the masks: range, tree's bits
     int * const owner = (int *) (about + 32 * CW);    // and their rows, -1 for those that attend to nothing
+    uint8_t * const dims = (uint8_t *) (owner + 32 * CW) + pgi * 2 * KB * (D / 8);   // those of the positions found, a bit each
+    uint32_t * const hits = (uint32_t *) ((uint8_t *) (owner + 32 * CW) + PG * 2 * KB * (D / 8)) + 32 * wave;   // which of them a column attends to
+    uint32_t * const spoiled = (uint32_t *) (lds + F::spoiled);   // [column][E] and of the columns that attend to them
     rows_at p;
     if (!rows_place<false>(a, rows_item(), lane, p)) return;
     const rows_of sq = p.sq;
@@ -551,6 +557,7 @@ __device__ __forceinline__ void rows_body(const sml_krows & a) {
         about[32 * cw + c] = some ? make_int4(lo, hi, (int) (uint32_t) tw, (int) (uint32_t) (tw >> 32)) : make_int4(0, 0, 0, 0);
         owner[32 * cw + c] = some ? r : -1;
     }
+    for (int x = tid; x < 32 * CW * E; x += 64 * W) spoiled[x] = 0;
     // the query in parts
     v8 q[NJ][NP];
     float back;                                       // what a product of the scaled q is multiplied by
@@ -592,24 +599,31 @@ __device__ __forceinline__ void rows_body(const sml_krows & a) {
     const int vrow = 4 * g + ((lane & 15) >> 2), q16 = (lane >> 4) & 1;
     const int vx = D == 128 ? vrow : g, vat = POOL + vrow * RB + (D == 128 ? 8 * (lane & 3) : 16 * (((lane >> 1) & 1) ^ ((lane >> 3) & 1)) + 8 * (lane & 1));
     // Values that are not finite among those that this wave has fetched, where columns
-    // differ: zeros in their place; their positions in the block.
-    auto screen = [&](uint8_t * st) {
+    // differ: zeros in their place; their positions in the block and, a byte a lane, dims.
+    auto screen = [&](uint8_t * st, uint8_t * of) {
         uint32_t bad = 0;
         #pragma unroll 1
         for (int e = 0; e < NC; e++) {
             const int row0 = RC * (CW * e + cw);
             v4u * const at = (v4u *) (st + POOL + row0 * RB + 16 * lane);
             v4u x = *at;
-            uint32_t any = 0;
-            #pragma unroll
-            for (int k = 0; k < 4; k++) {             // an exponent of all ones carries into the top bit
-                const uint32_t up = BF ? ((x[k] & 0x7F807F80u) + 0x00800080u) & 0x80008000u : ((x[k] & 0x7C007C00u) + 0x04000400u) & 0x80008000u;
-                x[k] &= ~((up >> 15) * 0xFFFFu);
-                any |= up;
-            }
-            const uint64_t hit = __ballot(any != 0);
+            auto ones = [&](int k) {                  // an exponent of all ones carries into the top bit
+                return BF ? ((x[k] & 0x7F807F80u) + 0x00800080u) & 0x80008000u : ((x[k] & 0x7C007C00u) + 0x04000400u) & 0x80008000u;
+            };
+            const uint64_t hit = __ballot((ones(0) | ones(1) | ones(2) | ones(3)) != 0);
             if (hit) {
+                int ln = lane;                        // so that no register is kept for what follows from it
+                asm volatile("" : "+v"(ln));
+                const int row = row0 + ln / (RB / 16);
+                uint32_t mark = 0;
+                #pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    const uint32_t up = ones(k);
+                    x[k] &= ~((up >> 15) * 0xFFFFu);
+                    mark |= (up >> 15 & 1u | up >> 30) << (2 * k);
+                }
                 *at = x;
+                of[row * (D / 8) + (ln % (RB / 16) ^ swz_v(row))] = (uint8_t) mark;
                 #pragma unroll 1
                 for (int k = 0; k < RC; k++)
                     if (hit >> (64 / RC * k) & ((1ull << (64 / RC)) - 1)) bad |= 1u << (row0 + k);
@@ -652,6 +666,19 @@ __device__ __forceinline__ void rows_body(const sml_krows & a) {
     auto sums = [&](const v8 & vv, int u, const v8 (&w)[NP]) {
         #pragma unroll
         for (int y = 0; y < NP; y++) o[u] = MM::mul(vv, w[y], o[u]);
+    };
+    // The dims of the positions found in a block marked for the columns that attend to them.
+    auto spoil = [&](const uint8_t * of, uint32_t bad) {
+        int ln = lane;                                // so that no register is kept for what follows from it
+        asm volatile("" : "+v"(ln));
+        const uint32_t hit = hits[ln & 31];
+        #pragma unroll 1
+        for (; bad; bad &= bad - 1) {
+            const int y = __builtin_ctz(bad);
+            if (hit >> y & 1)
+                #pragma unroll 1
+                for (int u = ln >> 5; u < E; u += 2) atomicOr(&spoiled[(32 * cw + (ln & 31)) * E + u], ((const uint32_t *) of)[y * E + u]);
+        }
     };
     // Scores of positions t.., whose pages are pa and pb, under the rules and the
     // masks; the base that their weights have. Score e is position at(e) + 4g.
@@ -707,12 +734,12 @@ __device__ __forceinline__ void rows_body(const sml_krows & a) {
             vm &= bits_range(0, sq.n - t);
             if (pa < 0) vm &= 0xFFFF0000u;
             if (pb < 0) vm &= 0x0000FFFFu;
-            if (vm & bad) l = NAN;
+            if (bad) hits[c] = vm;
             vm >>= 4 * g;
             #pragma unroll
             for (int e = 0; e < 16; e++) s[e] = (vm >> at(e)) & 1 ? s[e] : -INFINITY;
         } else if (bad) {
-            l = NAN;
+            hits[c] = some ? ~0u : 0u;
         }
         float mx = -INFINITY;
         #pragma unroll
@@ -750,7 +777,7 @@ __device__ __forceinline__ void rows_body(const sml_krows & a) {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         keep_pos(kpos + i0 * KB);
         if (differ) {
-            const uint32_t bad = screen(st);
+            const uint32_t bad = screen(st, dims + i0 * KB * (D / 8));
             if (!lane) found[i0 * CW + cw] = bad;
         }
         __syncthreads();                          // the block is whole, and nobody reads the last one
@@ -770,6 +797,7 @@ __device__ __forceinline__ void rows_body(const sml_krows & a) {
             if (differ) {
                 #pragma unroll
                 for (int y = 0; y < CW; y++) bad |= found[i0 * CW + y];
+                bad = (uint32_t) __builtin_amdgcn_readfirstlane((int) bad);
             }
             settle(s, kpos + i0 * KB, cur, b0.pa, b0.pb, bad);
             weights(s, w);
@@ -779,6 +807,7 @@ __device__ __forceinline__ void rows_body(const sml_krows & a) {
                 if (u + NV < 2 * E) vv[u % NV] = value(st, (u + NV) % E, (u + NV) / E);
                 if (NV < E) __builtin_amdgcn_sched_barrier(0);
             }
+            if (bad) spoil(dims + i0 * KB * (D / 8), bad);
         }
         b0 = b1;
         b1 = b2;
@@ -825,6 +854,9 @@ __device__ __forceinline__ void rows_body(const sml_krows & a) {
             #pragma unroll
             for (int e = 0; e < 4; e++) os[e] = none ? os[e] : __builtin_fmaf(f, v[k][e], os[e]);
         }
+        const uint32_t dims = spoiled[pc * E + d / 32] >> (d & 31);
+        #pragma unroll
+        for (int e = 0; e < 4; e++) os[e] = dims >> e & 1 ? NAN : os[e];
         if (p.count == 1) {
             const int i = rows_over(a, col);
             #pragma unroll

@@ -3,8 +3,12 @@ range, and over values and keys that are not finite."""
 import numpy as np
 import pytest
 
+import rows_oracle as ro
+import serving_oracle as so
 import sheep_amd as sa
-from test_gpu_rows import rows_case
+from sheep_amd import serving
+from test_gpu_rows import ints, rows_case, within
+from test_gpu_rows_edges import attend
 
 pytestmark = pytest.mark.gpu
 
@@ -24,3 +28,73 @@ def test_scores_near_nothing(dtype, heads, kv, hd, mask, q_exp, scale):
     """Scores of some 2^-137 and less, beside masked ones and absent pages: a row is
     the mean of what it attends to, in the general bounds."""
     rows_case([40, 3, 9], [150, 3, 700], heads, kv, hd, dtype, 16, seed=hd, mask=mask, q_exp=q_exp, scale=scale, gone={2: [1, 20]})
+
+
+# ------------------------------------------------------------ values that are not finite
+
+BAD = {"f16": [0x7E00, 0x7C00, 0xFC00], "bf16": [0x7FC0, 0x7F80, 0xFF80]}
+# one sequence in splits and in one piece, several (tiles of four waves), prompts (tiles of 128 columns of eight
+# and of four waves): the new rows, their positions, heads and KV heads
+SHAPES = [([40], [300], 4, 2), ([40], [90], 4, 2), ([9, 40, 1, 30, 3], [300, 190, 210, 230, 90], 4, 2), ([1601], [1650], 32, 8), ([2100], [2100], 32, 8)]
+
+
+@pytest.mark.parametrize("cap", [0.0, 20.0])
+@pytest.mark.parametrize("ms, lens, heads, kv", SHAPES)
+@pytest.mark.parametrize("hd, dtype", [(128, "f16"), (64, "bf16"), (128, "bf16"), (64, "f16")])
+def test_values_that_are_not_finite_reach_their_dims(ms, lens, heads, kv, hd, dtype, cap):
+    """Single values that are NaN or infinite: rows that attend to them have no
+    finite output in these dims and the right one in the others, whether every other
+    row of the call attends to them too, some do or none but the rows with tree bits do."""
+    rng = np.random.default_rng(len(ms) + hd)
+    n_seq, n, g = len(ms), max(lens), heads // kv
+    k, v = (so.to_bits(rng.standard_normal((n_seq, n, kv, hd)), dtype) for _ in range(2))
+    spots = [(5, 3), (17, 3), (70, hd - 1), (71, 40), (85, 0), (n - 2, 33)]
+    for i, (slot, dim) in enumerate(spots):
+        v[:, slot, kv - 1, dim] = BAD[dtype][i % 3]
+    start = np.concatenate([[0], np.cumsum(ms)])
+    q = rng.standard_normal((sum(ms), heads, hd)).astype(np.float32)
+    row = np.concatenate([np.arange(m) for m in ms])
+    top = np.repeat(lens, ms)
+    whole = (np.zeros(sum(ms), int), top)
+    mixed = (np.where(row % 2, 18, 0), np.where(row % 2, 65, np.where(row % 4, 80, top)))     # odd rows see none of them
+    past = np.maximum(0, top - np.repeat(ms, ms) - 6)
+    for what, (first, last), bits in (("whole", whole, None), ("mixed", mixed, None), ("tree", (np.minimum(20, past), np.where(row % 3, past, 0)), 0.3)):
+        tree = np.zeros((sum(ms), max(ms)), bool)
+        if bits:
+            tree = (rng.random(tree.shape) < bits) & (row % 5 != 1)[:, None]
+        words = -(-max(ms) // 32)
+        packed = np.packbits(np.pad(tree, ((0, 0), (0, 32 * words - max(ms)))), axis=1, bitorder="little").view(np.uint32)
+        kw = dict(tree=sa.DevBuf.of(packed), tree_words=words) if bits else {}
+        got = attend(q.reshape(sum(ms), -1), k, v, dtype, start, lens, heads, first=ints(first), last=ints(last), cap=cap, **kw)
+        for b, (m, ln) in enumerate(zip(ms, lens)):
+            mine = slice(start[b], start[b + 1])
+            see = (np.arange(ln) >= first[mine, None]) & (np.arange(ln) < last[mine, None])
+            see[:, ln - m:] |= tree[mine, :m]
+            for h in (0, heads - g, heads - 1):
+                kk, vv = (so.from_bits(x[b, :ln, h // g], dtype) for x in (k, v))
+                hit = see.astype(float) @ ~np.isfinite(vv) > 0
+                want, tol = ro.attend(q[mine, h], kk, np.where(np.isfinite(vv), vv, 0), hd ** -0.5, see, cap)
+                assert not np.isfinite(got[mine, h][hit]).any(), what
+                within(np.where(hit, 0, got[mine, h]), np.where(hit, 0, want), tol, f"{what}, sequence {b}, head {h}")
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("n", [40, 90, 700])
+def test_values_that_are_not_finite_of_one_token(n, dtype):
+    """The attention of one token a sequence keeps them to their dims as well."""
+    rng = np.random.default_rng(n)
+    hd, page, pages = 64, 16, 44
+    kb, vb = (so.to_bits(rng.standard_normal((pages, page, 2, hd)), dtype) for _ in range(2))
+    for i, (slot, dim) in enumerate([(5, 3), (17, 3), (31, 40), (n - 1, 63)]):
+        vb[slot // page, slot % page, 1, dim] = BAD[dtype][i % 3]
+    q = rng.standard_normal((1, 6, hd)).astype(np.float32)
+    out, part = sa.DevBuf(4 * 6 * hd), sa.DevBuf(4 * serving.part_floats(1, 6, hd, n))
+    pg = serving.Pages(sa.DevBuf.of(kb), sa.DevBuf.of(vb), ints([np.arange(pages)]), pages, page, 1, pages, 2, hd, dtype)
+    serving.attention(pg, sa.DevBuf.of(q), ints([n]), n, 6, part, out)
+    got = out.read(np.float32).reshape(6, hd)
+    for h in range(6):
+        kk, vv = (so.from_bits(x.reshape(-1, 2, hd)[:n, h // 3], dtype) for x in (kb, vb))
+        hit = ~np.isfinite(vv).all(0)
+        want, tol = ro.attend(q[:, h], kk, np.where(np.isfinite(vv), vv, 0), hd ** -0.5, np.ones((1, n), bool))
+        assert not np.isfinite(got[h][hit]).any()
+        within(np.where(hit, 0, got[h]), np.where(hit, 0, want[0]), tol[0], f"head {h}")
