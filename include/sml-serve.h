@@ -85,10 +85,12 @@ size_t sml_hip_paged_part_floats(int n_seq, int n_head, int hd, int max_len);
 // fp32 holds q * scale, the sums of |q_d k_d|, twice those times |scale|, and
 // the sums of weight * |value|, the largest weight 1; an infinite or NaN value that
 // a sequence does attend over makes its dim of its KV head's outputs infinite or
-// NaN, however small its weight, and no other; an infinite key makes its KV head's
-// outputs NaN, an infinite query its own head's. How the positions are split
-// follows all of the lengths: a sequence's sums depend on the others by their
-// rounding alone, and equal calls give equal bits.
+// NaN, however small its weight, and no other; an infinite or NaN query makes its
+// own head's outputs NaN. So does a key of its KV head's, unless the score is
+// -infinity: that has no weight (such a position's values that are not finite may
+// count or not). How the positions are split follows all of the lengths: a
+// sequence's sums depend on the others by their rounding alone, and equal calls
+// give equal bits.
 int sml_hip_paged_attention(const sml_hip_pages * pg, const float * q, size_t q_stride, const int32_t * len,
                             int max_len, int n_head, float scale, float * part, float * out, void * stream);
 
@@ -148,7 +150,8 @@ size_t sml_hip_paged_rows_floats(int n_seq, int n_row, int n_kv, int n_head, int
 // also where other rows of the call do attend to it; a row with no slot left, or
 // with no score above -infinity, gets zeros. Rows outside every sequence's are
 // left as they were. Precision, ranges and infinities are
-// sml_hip_paged_attention's; the cap and the bias are fp32. How the positions are
+// sml_hip_paged_attention's; the cap and the bias are fp32, and a key's infinite
+// score may be the cap's, with its sign. How the positions are
 // split follows all of the lengths: a row's sums depend on the other rows by
 // their rounding alone, and equal calls give equal bits.
 int sml_hip_paged_attention_rows(const sml_hip_pages * pg, const sml_hip_rows * rows, const float * q, size_t q_stride,

@@ -98,3 +98,71 @@ def test_values_that_are_not_finite_of_one_token(n, dtype):
         want, tol = ro.attend(q[:, h], kk, np.where(np.isfinite(vv), vv, 0), hd ** -0.5, np.ones((1, n), bool))
         assert not np.isfinite(got[h][hit]).any()
         within(np.where(hit, 0, got[h]), np.where(hit, 0, want[0]), tol[0], f"head {h}")
+
+
+# ------------------------------------------------------------ keys that are not finite
+
+def key_rule(got, want, tol, other, other_tol, see, up, capped, what):
+    """Rows of one head, of which those that see a slot with an infinite key have a
+    score that is infinite there (up: upwards) or, of its parts, NaN. NaN and, without a
+    cap, an infinity upwards leave nothing but NaN; else the row is `other`."""
+    for i in range(len(got)):
+        if not see[i]:
+            within(got[i], want[i], tol[i], f"{what}, row {i}")
+        elif not np.isnan(got[i]).all():
+            assert capped or not up[i], f"{what}, row {i}"
+            within(got[i], other[i], other_tol[i], f"{what}, row {i}")
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("cap", [0.0, 20.0])
+@pytest.mark.parametrize("n", [60, 300])
+def test_keys_that_are_not_finite(n, cap, hd, dtype):
+    """A key with one infinite dim: rows that do not attend to it know nothing of it,
+    of those that do, a score of -infinity has no weight and a capped one is +-cap."""
+    rng = np.random.default_rng(hd + n)
+    m, heads, g, slot, dim = 40, 4, 2, 30, 7
+    k, v = (so.to_bits(rng.standard_normal((1, n, 2, hd)), dtype) for _ in range(2))
+    k[0, slot, 1, dim] = BAD[dtype][1]
+    q = rng.standard_normal((m, heads, hd)).astype(np.float32)
+    first = np.where(np.arange(m) % 3 == 1, 31, 5)
+    first[6], last = 30, np.full(m, n)
+    last[6] = 31                                              # that slot alone
+    got = attend(q.reshape(m, -1), k, v, dtype, [0, m], [n], heads, first=ints(first), last=ints(last), cap=cap)
+    see = (np.arange(n) >= first[:, None]) & (np.arange(n) < last[:, None])
+    for h in range(heads):
+        kk, vv = (so.from_bits(x[0, :, h // g], dtype).copy() for x in (k, v))
+        up, bad = q[:, h, dim] > 0, see[:, slot] if h // g else np.zeros(m, bool)
+        kk[slot] = np.where(np.isfinite(kk[slot]), kk[slot], 0)
+        want, tol = ro.attend(q[:, h], kk, vv, hd ** -0.5, see, cap)
+        kk[slot] = 0
+        at, rest = np.zeros((m, n)), see.copy()
+        at[:, slot] = np.where(up, -cap, cap)
+        rest[:, slot] &= cap > 0
+        other, other_tol = ro.attend(q[:, h], kk, vv, hd ** -0.5, rest, cap, at)
+        key_rule(got[:, h], want, tol, other, other_tol, bad, up, cap > 0, f"head {h}")
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("n", [31, 90, 700])
+def test_keys_that_are_not_finite_of_one_token(n, dtype):
+    rng = np.random.default_rng(n)
+    hd, page, pages, rows, slot, dim = 64, 16, 44, 24, 30, 7
+    kb, vb = (so.to_bits(rng.standard_normal((pages, page, 2, hd)), dtype) for _ in range(2))
+    kb[slot // page, slot % page, 1, dim] = BAD[dtype][2]
+    q = rng.standard_normal((rows, 4, hd)).astype(np.float32)
+    out, part = sa.DevBuf(4 * rows * 4 * hd), sa.DevBuf(4 * serving.part_floats(rows, 4, hd, n))
+    pg = serving.Pages(sa.DevBuf.of(kb), sa.DevBuf.of(vb), ints(np.tile(np.arange(pages), (rows, 1))), pages, page, rows, pages, 2, hd, dtype)
+    lens = np.where(np.arange(rows) % 4 == 1, slot, n)
+    serving.attention(pg, sa.DevBuf.of(q), ints(lens), n, 4, part, out)
+    got = out.read(np.float32).reshape(rows, 4, hd)
+    see = np.arange(n) < lens[:, None]
+    for h in range(4):
+        kk, vv = (so.from_bits(x.reshape(-1, 2, hd)[:n, h // 2], dtype).copy() for x in (kb, vb))
+        kk[slot] = np.where(np.isfinite(kk[slot]), kk[slot], 0)
+        want, tol = ro.attend(q[:, h], kk, vv, hd ** -0.5, see)
+        rest = see.copy()
+        rest[:, slot] = False
+        other, other_tol = ro.attend(q[:, h], kk, vv, hd ** -0.5, rest)
+        key_rule(got[:, h], want, tol, other, other_tol, see[:, slot] if h // 2 else np.zeros(rows, bool), q[:, h, dim] < 0, False, f"head {h}")
