@@ -561,6 +561,7 @@ __device__ __forceinline__ void rows_body(const sml_krows & a) {
     // the query in parts
     v8 q[NJ][NP];
     float back;                                       // what a product of the scaled q is multiplied by
+    int ex;
     {
         float mx = 0.0f;
         #pragma unroll
@@ -572,13 +573,22 @@ __device__ __forceinline__ void rows_body(const sml_krows & a) {
             for (int j = 0; j < 2 * NJ; j++) x[j] = -x[j];
         }
         mx = fmaxf(mx, __shfl_xor(mx, 32));
-        const int ex = BF ? 0 : scale_of(mx);
+        ex = BF ? 0 : scale_of(mx);
         #pragma unroll
         for (int j = 0; j < NJ; j++)
             #pragma unroll
             for (int e = 0; e < 8; e += 2)
                 parts_of<BF>(__builtin_amdgcn_ldexpf(x[2 * j + e / 4][e % 4], -ex), __builtin_amdgcn_ldexpf(x[2 * j + e / 4][e % 4 + 1], -ex), q[j], e);
         back = __builtin_amdgcn_ldexpf(a.scale, ex);
+    }
+    // Over the cap, the factor may leave fp32's room where scores or the cap do not.
+    // Below 2^-110 (products are below 2^34) a tanh is its argument, also one 2^60 as
+    // large: the cap gives these up. Past the largest, scores are 0 or the cap.
+    float cap = a.cap;
+    if (RULES && !BF && a.cap > 0.0f) {
+        const bool far = back < 0x1p-110f;
+        back = fminf(far ? __builtin_amdgcn_ldexpf(a.scale, ex + 60) : back, 0x1.fffffep127f);
+        cap = far ? __builtin_amdgcn_ldexpf(cap, -60) : cap;
     }
     const int q0 = qpos - 4 * g;                      // the row's position, less where the lane's first score is
     const float slope = RULES && a.slope ? -1.44269504088896341f * a.slope[h] : 0.0f;
@@ -691,10 +701,10 @@ __device__ __forceinline__ void rows_body(const sml_krows & a) {
             if (a.cap > 0.0f) {
                 if (__any(!(top <= 0.625f))) {
                     #pragma unroll
-                    for (int e = 0; e < 16; e++) s[e] = a.cap * tanh_any(s[e]);
+                    for (int e = 0; e < 16; e++) s[e] = cap * tanh_any(s[e]);
                 } else {
                     #pragma unroll
-                    for (int e = 0; e < 16; e++) s[e] = a.cap * tanh_small(s[e]);
+                    for (int e = 0; e < 16; e++) s[e] = cap * tanh_small(s[e]);
                 }
             }
             if (a.slope) {

@@ -30,6 +30,35 @@ def test_scores_near_nothing(dtype, heads, kv, hd, mask, q_exp, scale):
     rows_case([40, 3, 9], [150, 3, 700], heads, kv, hd, dtype, 16, seed=hd, mask=mask, q_exp=q_exp, scale=scale, gone={2: [1, 20]})
 
 
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("bias", [False, True])
+@pytest.mark.parametrize("cap, scale, q_exp, kv_size", [
+    (2.0 ** 114, 2.0 ** 15, -38, 9000.0), (2.0 ** 120, -2.0 ** 22, -45, 9000.0), (2.0 ** 90, 0.0, 0, 1.0), (2.0 ** 96, 0.0, -12, 1000.0),
+    (2.0 ** 126, 2.0 ** 40, -62, 9000.0), (2.0 ** -40, 2.0 ** -60, 0, 1.0), (2.0 ** -126, 2.0 ** -60, 0, 1.0)])
+def test_caps_far_from_their_scores(dtype, hd, bias, cap, scale, q_exp, kv_size):
+    """Caps that no score comes near, up to 2^100 times the scale, leave the scores as
+    they are, and caps next to nothing leave nothing of them, in the general bounds."""
+    rows_case([40, 9], [150, 300], 4, 2, hd, dtype, 16, seed=hd, cap=cap, scale=scale, q_exp=q_exp, kv_size=kv_size, bias=bias)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("cap, scale, q_exp", [(2.0 ** -40, 0.0, 100), (2.0 ** -100, 1.0, 40), (2.0 ** -100, 1.0, 100), (1.0, 2.0 ** 60, 60)])
+def test_keys_of_zeros_under_small_caps(dtype, hd, cap, scale, q_exp):
+    """Scores of exactly 0, however large the query is over the cap."""
+    rng = np.random.default_rng(hd)
+    n, m = 150, 40
+    k = np.zeros((1, n, 2, hd), np.uint16)
+    v = so.to_bits(rng.standard_normal((1, n, 2, hd)), dtype)
+    q = (rng.standard_normal((m, 4, hd)) * 2.0 ** q_exp).astype(np.float32)
+    got = attend(q.reshape(m, -1), k, v, dtype, [0, m], [n], 4, cap=cap, scale=scale)
+    see = np.arange(n) <= n - m + np.arange(m)[:, None]
+    for h in range(4):
+        want, tol = ro.attend(q[:, h], so.from_bits(k[0, :, 0], dtype), so.from_bits(v[0, :, h // 2], dtype), 1.0, see)
+        within(got[:, h], want, tol, f"head {h}")
+
+
 # ------------------------------------------------------------ values that are not finite
 
 BAD = {"f16": [0x7E00, 0x7C00, 0xFC00], "bf16": [0x7FC0, 0x7F80, 0xFF80]}
