@@ -172,9 +172,10 @@ int sml_hip_paged_attention_rows(const sml_hip_pages * pg, const sml_hip_rows * 
 // rows are kept. Out: n_kept[b]; kept[b][j], the path's rows by number; next[b][j],
 // the tokens that follow them (row j's pick; the last is the next step's root);
 // both [n_seq][max_kept], -1 behind; len_out[b] = len[b] - m + n_kept[b] (apart
-// from len). Keys and values of the path's rows move to slots h, h + 1 and on, in all
-// layers; n_layer 0 moves nothing. Any of the outputs may be NULL. A sequence of
-// no rows keeps none. The slots of new rows belong to one sequence alone.
+// from len; a negative len[b] is 0). Keys and values of the path's rows move to
+// slots h, h + 1 and on, in all layers, where both slots have pages; n_layer 0 moves
+// nothing. Any of the outputs may be NULL. A sequence of no rows keeps none. The
+// slots of new rows belong to one sequence alone.
 int sml_hip_draft_accept(const sml_hip_pages * pg, int n_layer, size_t layer_stride, int n_row, const int32_t * start,
                          const int32_t * len, const int32_t * tok, const int32_t * parent, const int32_t * pick,
                          int max_kept, int32_t * n_kept, int32_t * kept, int32_t * next, int32_t * len_out,

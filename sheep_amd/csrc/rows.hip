@@ -987,7 +987,7 @@ extern "C" __global__ __launch_bounds__(256) void sml_rw_accept(const sml_kaccep
     __shared__ int path[AC_MOST], count;
     const int b = blockIdx.y, tid = threadIdx.x, lane = tid & 63;
     const int s0 = min(max(a.start[b], 0), a.n_row), s1 = min(max(a.start[b + 1], s0), a.n_row), m = s1 - s0;
-    const int cap = a.pg.seq_pages << a.pg.page_shift, n = min(max(a.len[b], 0), cap), past = n - m;
+    const int cap = a.pg.seq_pages << a.pg.page_shift, past = max(a.len[b], 0) - m;
     if (tid < 64) {
         int k = 0, at = 0;
         if (m > 0) {
@@ -1045,9 +1045,11 @@ extern "C" __global__ __launch_bounds__(256) void sml_rw_accept(const sml_kaccep
         v4u * to[AC_AHEAD];
         #pragma unroll
         for (int e = 0; e < AC_AHEAD; e++) {
-            const int j = j0 + e, from = past + (j < k ? path[j] : j), at = past + j;
+            const int j = j0 + e;
             to[e] = NULL;
-            if (from == at || at < 0) continue;
+            if (j >= k) continue;
+            const int from = past + path[j], at = past + j;
+            if (from == at || at < 0 || from >= cap) continue;
             const int pf = page_of(a.pg, b, from >> sh), pt = page_of(a.pg, b, at >> sh);
             if (pf < 0 || pt < 0) continue;
             w[e] = *(const v4u *) (pool + (size_t) pf * a.pg.page_stride + (size_t) (from & pmask) * 8 * row);
