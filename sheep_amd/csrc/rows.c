@@ -61,7 +61,8 @@ static const struct form { const char * name; int cols, cw, pg; } forms[] = {
 
 // Tiles of 128 columns read the cache less often; those of 64 waste less of a few
 // and make more workgroups. Measured as us a call, 32 heads over 8 of 128, fp16,
-// rows x sequences at positions.
+// rows x sequences at positions; bfloat16 and heads of 64 go by the same counts,
+// which were not measured for them.
 static const struct form * form_of(long ncol, long some, int n_kv) {
     const long ncu = hx.ncu, t64 = (ncol + 63) / 64 * n_kv, t128 = (ncol + 127) / 128 * n_kv;
     // long prompts, tiles for both places of every CU and more (128 / 128h / 64h: 4096 at 4096 295 / 291 / 299,
@@ -84,9 +85,13 @@ static void rows_launch(sml_krows * a, int hd, int type, hipStream_t st) {
     a->cols = f->cols;
     a->over = rep > 1 ? (uint32_t) (((1ull << 32) + (unsigned) rep - 1) / (unsigned) rep) : 0;
     // Splits make a workgroup for every place on the card, of 128 positions at least;
-    // none where the tiles are half as many (1024 rows at 1024, 128 columns a tile, 33
-    // tiles for 32 places a KV head: 44.6 us so, 48.1 with the splits' launch), or a
-    // place's sequences one each.
+    // none where the tiles are more than half as many, of which each could only be one,
+    // or as many sequences have rows (32 heads over 8 of 128, fp16, 32 places a KV head, none / split: 256 rows, 16
+    // tiles, at 1024 25.5 / 23.9 us, at 8192 117 / 82; 272 rows, 17 tiles, 26.0 / 28.1 and
+    // 120 / 123; bfloat16 at 8192 149 / 99 and, 320 rows, 153 / 155). That holds for
+    // tiles as long as each other: 8 sequences of up to 128 rows at 500 to 4000 take 94 us
+    // for 51 with splits, and a long sequence of one row beside a prompt's 256 rows is walked by
+    // one workgroup a KV head (at 65536 774 us, apart 19 and 46).
     const int want = ceil_div((f->cw * f->pg == 8 ? 1 : 2) * (hx.ncu < 256 ? hx.ncu : 256), n_kv);
     a->least = 2;
     const int split = n_seq <= AT_SHARED && some < want && 2 * ceil_div(ncol, a->cols) <= want && a->max_len > RW_BLOCK * a->least;

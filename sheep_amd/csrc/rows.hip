@@ -7,9 +7,10 @@
 //
 // The rotation of sml_sv_append with a position for each pair: a thread's four
 // pairs look up their axis (in the arguments) and its position, and their angles
-// come in one load where the axis is one. Latency bounds 128 rows (3.8 us, 2.7 MB),
-// the stream 1369 (6.4 us, 22 MB, 12 heads over 2 of 128 with three axes; 6.6 with
-// an angle a load). A row as one workgroup of 512 threads was no faster.
+// come in one load where the axis is one. Latency bounds 59 rows (3.8 us, 2.7 MB, 32
+// heads over 8 of 128), the stream 1369 (6.4 us, 22 MB, 12 heads over 2 of 128 with
+// three axes, whose 288 items a row are 512 threads; 6.6 with an angle a load). A row
+// as one workgroup of 512 threads was no faster.
 template <int D, int BF>
 __device__ __forceinline__ void axes_body(const sml_kaxes & a) {
     constexpr int HQ = D / 8;                         // threads of a rotated head
@@ -108,7 +109,9 @@ AXES(64, 1, sml_rw_append_d64_bf)
 // q and the weights are split into 16-bit parts, as in sml_sv_attend, whose base
 // and room these are. K and V go from memory to LDS without registers, a block
 // ahead, 16-byte words swizzled by row so that both kinds of read spread over the
-// banks; a chunk of the table is a lane's entry each, 1024 positions ahead.
+// banks; a chunk of the table is a lane's entry each, looked up 1024 positions ahead.
+// (An entry is compared with n_pages where it is loaded, so every 1024 positions the
+// wave waits for it and for the copies in flight.)
 //
 // What bounds it: of many rows the matrix cores' rate on real data (2048 rows at
 // 16384, 32 heads over 8 of 128: 552 TFLOP/s of the formula, which in fp16's two
@@ -302,9 +305,10 @@ __device__ __forceinline__ float2 * part_ml(const sml_krows & a, int kh, int ite
     return (float2 *) (a.part + (size_t) a.pg.n_kv * a.items * a.part_cols * d) + ((size_t) kh * a.items + item) * a.part_cols;
 }
 
-// tanh(y) for |y| up to 0.625: y times a polynomial of y^2 (least relative error
-// on that range, 4e-9; 1.1e-7 as evaluated). Past it 1 - 2 / (e^2y + 1), whose
-// cancellation costs less than a bit there.
+// tanh(y) for |y| up to 0.625: y times a polynomial of y^2, fitted to the relative
+// error on that range (1.1e-8 as its coefficients are rounded, 1.1e-7 as evaluated;
+// five unrounded ones reach 4.4e-9). Past it 1 - 2 / (e^2y + 1), whose cancellation
+// costs less than a bit there. (The Cephes library's tanhf has the same two ranges.)
 __device__ __forceinline__ float tanh_small(float y) {
     const float z = y * y;
     float p = __builtin_fmaf(-0.0056599886f, z, 0.020590989f);
@@ -532,7 +536,8 @@ __device__ __forceinline__ void rows_body(const sml_krows & a) {
             }
         }
     };
-    // The positions of a block's new rows, on their way; they are in LDS with the block.
+    // The positions of a block's new rows; they are in LDS with the block. (Chosen from
+    // as they are loaded: the wave waits for them, behind the copies that it has begun.)
     int at_pos = 0;
     auto fetch_pos = [&](int t) {
         if (RULES && a.slope && a.pos && t + pgi * KB + KB > past && cw == 0)
@@ -732,7 +737,7 @@ __device__ __forceinline__ void rows_body(const sml_krows & a) {
                 uint64_t y = (uint64_t) (uint32_t) mask.w << 32 | (uint32_t) mask.z;
                 const int w0 = j0 >> 5;               // bits 32 w0.. of the row, 64 of them
                 if (a.words > 2) {
-                    const int row = owner[32 * cw + c];
+                    const int row = owner[32 * cw + c];   // the bits' load waits for the copies in flight, too
                     const uint32_t * const bits = a.tree + (size_t) max(row, 0) * a.words;
                     y = (uint64_t) (w0 + 1 >= 0 && w0 + 1 < a.words ? bits[w0 + 1] : 0u) << 32 | (w0 >= 0 && w0 < a.words ? bits[w0] : 0u);
                     if (row < 0) y = 0;
@@ -980,7 +985,7 @@ __device__ __forceinline__ uint16_t * pool_of(const sml_kpages & pg, size_t laye
 // bytes of a position in one pool, a few of the path's rows at a time, in order: a
 // row's new place lies before every later row's old one, so nothing is overwritten
 // that is still to be read. Latency bounds it, the walk's chain of loads and then the
-// path's copies: 3.7 us for 8 rows in 32 layers, 4.6 for 16 sequences of up to 26 in
+// path's copies: 3.6 us for 8 rows in 32 layers, 4.3 for 16 sequences of up to 26 in
 // 28 (3.9 and 4.8 with a load a step of the walk and a row's copy at a time).
 #define AC_AHEAD 4
 extern "C" __global__ __launch_bounds__(256) void sml_rw_accept(const sml_kaccept a) {
@@ -1102,7 +1107,7 @@ extern "C" __global__ __launch_bounds__(256) void sml_rw_fork(const sml_kfork a)
 //
 // A workgroup copies 16 KB of a page in one pool; behind the moves' workgroups
 // (y) come those that rename the table's entries, each found among the
-// ascending sources by halving. The stream bounds it: 190 pages' 444 MB, read and
+// ascending sources by halving. The stream bounds it: 121 pages' 444 MB, read and
 // written, 90 us, as a large copy would take 86; 9 pages 6.4.
 extern "C" __global__ __launch_bounds__(256) void sml_rw_compact(const sml_kcompact a) {
     const int tid = threadIdx.x;
